@@ -56,6 +56,21 @@ class LayerWeight(ctypes.Structure):
     ]
 
 
+class Pages(ctypes.Structure):
+    """btl_pages_t: the page pools of one layer's cache."""
+
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_exp", ctypes.c_void_p),
+        ("v_exp", ctypes.c_void_p),
+        ("num_pages", ctypes.c_int64),
+        ("num_kv_heads", ctypes.c_int64),
+        ("page_size", ctypes.c_int64),
+        ("head_dim", ctypes.c_int64),
+    ]
+
+
 def layer_weight(w, gamma) -> LayerWeight:
     """LayerWeight of a PackedTernaryWeight and the RMSNorm gain of its input."""
     n = len(w.segment_scales)
@@ -72,6 +87,7 @@ def layer_weight(w, gamma) -> LayerWeight:
 
 
 _LWP = ctypes.POINTER(LayerWeight)
+_PGP = ctypes.POINTER(Pages)
 
 # name -> (argtypes, restype); the exported C ABI, one entry per declaration.
 EXPORTS = {
@@ -129,6 +145,24 @@ EXPORTS = {
     "btl_decode_attention_split_bytes": ([_I64, _I64, _I64], _I64),
     "btl_decode_attention_split": ([_P, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _I, _F, _P, _P, _P, _P, _SZ, _P,
                                     _SZ, _P], _I),
+    "btl_rope_write": (
+        [_P, _I64, _I64, _I64, _I64, _I64, _P, _P, _I64, _I64, _I, _P, _P, _I64, _P, _I64, _P, _I64, _PGP, _P, _I64,
+         _P, _P],
+        _I,
+    ),
+    "btl_read_pages": ([_PGP, _P, _I64, _I64, _P, _I64, _P, _P, _P, _P], _I),
+    "btl_prompt_attention": (
+        [_P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _F, _I64, _P, _I64, _P, _P],
+        _I,
+    ),
+    "btl_paged_attention_scratch_bytes": ([_I64, _I64, _I64, _I64, _I64, _I64, _I64], _I64),
+    "btl_paged_attention": (
+        [_P, _I64, _I64, _I64, _PGP, _P, _I64, _P, _P, _I64, _F, _I64, _I64, _P, _I64, _P, _SZ, _P, _P],
+        _I,
+    ),
+    "btl_page_row": ([_I64, _I64, _I64, _I64, _I64, _I64], _I64),
+    "btl_clamp_seq": ([_I64, _I64, _I64, _I64, _I64, _P], _I),
+    "btl_row_exponent": ([_F], _I),
     "btl_decode_attention": ([_P, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _I, _F, _P, _P, _P, _P, _SZ, _P], _I),
 }
 
@@ -446,8 +480,8 @@ def check_errors(device=None) -> None:
     torch.cuda.synchronize(dev)
     what = ", ".join(f"{k[0]} workspace (stream {k[2]:#x}) word at byte {off} = {w}" for k, off, w in bad)
     raise RuntimeError(
-        f"a kernel on {dev} set its error word ({what}): a bounded wait ran out, or a decode-attention position "
-        "was out of range; the outputs of the calls since the last check are invalid, and the workspaces have "
+        f"a kernel on {dev} set its error word ({what}): a bounded wait ran out, a decode-attention position "
+        "was out of range, or a batch over pages was not well formed; the outputs of the calls since the last check are invalid, and the workspaces have "
         "been reset"
     )
 

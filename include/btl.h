@@ -407,6 +407,100 @@ int btl_decode_attention_split(const uint16_t* qkv, int64_t B, int64_t H, int64_
                                float scale, uint16_t* k_cache, uint16_t* v_cache, uint16_t* out, void* workspace,
                                size_t workspace_bytes, void* split, size_t split_bytes, btl_stream_t stream);
 
+/* ---- prompts and the paged key-value cache -----------------------------
+ * The reference's prompt path is src/bitnet_tt/layers/attention.py:1348-1507 (head
+ * split, RoPE, cache fill, causal SDPA) with its KVCache (:115-458).
+ *
+ * Pages: k, v [num_pages, num_kv_heads, page_size, head_dim], bf16 where k_exp
+ * and v_exp are NULL, else e4m3 codes (OCP) with one exponent byte per row in
+ * k_exp, v_exp [num_pages, num_kv_heads, page_size]: a value is code x
+ * 2^(byte - 127).  page_size a multiple of 16 up to 2^20, head_dim 64 or 128.
+ * Position p of sequence b is row p % page_size of page
+ * page_table[b][p / page_size] (int32 [B][max_pages], device).  A contiguous
+ * cache [B, Hkv, S, D] is pages of S rows.
+ *
+ * A batch: T packed rows, sequence b's being cu_q[b] .. cu_q[b+1] - 1 (int32
+ * [B+1], device): its newest tokens, at positions kv_len[b] - n_b ..
+ * kv_len[b] - 1 (int32 [B], device; kv_len counts the new tokens).  Rows with a
+ * negative position (kv_len[b] < n_b: padding) attend to nothing: their outputs are zero
+ * and nothing is written for them.  Rows outside [cu_q[0], cu_q[B]) are left
+ * as they were.
+ *
+ * error_word: a device int32 the caller owns, zero at first; a kernel that
+ * meets a cu_q that decreases or leaves [0, T], a kv_len that is negative or
+ * behind the page table's (or the angle tables') last position, or a page
+ * outside the pool stores a non-zero value and the outputs are invalid; no
+ * access leaves its buffer.  Calls may share it. */
+typedef struct {
+  void* k;
+  void* v;
+  uint8_t* k_exp;
+  uint8_t* v_exp;
+  int64_t num_pages;
+  int64_t num_kv_heads;
+  int64_t page_size;
+  int64_t head_dim;
+} btl_pages_t;
+
+/* Rotates the q and k heads of fused QKV rows (qkv [T, (H + 2 Hkv) D] bf16, row
+ * stride ldx) at their positions over the first R dims of each head (R a
+ * multiple of 16; pairs (2i, 2i+1) when rope_adjacent, else (i, i + R/2);
+ * rope_cos / rope_sin [S, R/2] fp32, 16-byte aligned) and writes q to q_out (row
+ * stride ldq), k to k_out if given (row stride ldk) and k and v to their pages
+ * if pages is given (k from the fp32 rotation, rounded once).  8-bit pages: per row the least exponent e >= -126
+ * with max|x| <= 448 * 2^e and the codes e4m3(x / 2^e); a row with a value
+ * that is not finite reads as NaN.  kv_len NULL: the rows are whole prompts
+ * (positions from 0).  q_out and k_out may be the q and k parts of qkv
+ * itself.  Without pages, page_table is ignored. */
+int btl_rope_write(const uint16_t* qkv, int64_t T, int64_t ldx, int64_t H, int64_t Hkv, int64_t D,
+                   const float* rope_cos, const float* rope_sin, int64_t R, int64_t S, int rope_adjacent,
+                   const int32_t* cu_q, const int32_t* kv_len, int64_t B, uint16_t* q_out, int64_t ldq,
+                   uint16_t* k_out, int64_t ldk, const btl_pages_t* pages, const int32_t* page_table,
+                   int64_t max_pages, int32_t* error_word, btl_stream_t stream);
+
+/* k, v [B, Hkv, S, D] bf16 (the contiguous caches of btl_decode_attention and
+ * btl_decode_step_full): rows [0, kv_len[b]) of sequence b from its pages; the
+ * rows behind stay as they were. */
+int btl_read_pages(const btl_pages_t* pages, const int32_t* page_table, int64_t B, int64_t max_pages,
+                   const int32_t* kv_len, int64_t S, uint16_t* k, uint16_t* v, int32_t* error_word,
+                   btl_stream_t stream);
+
+/* Causal attention within packed sequences: out[i] = sum_j softmax_j(scale
+ * q_i.k_j) v_j over the rows j <= i of i's sequence, query head h reading
+ * key-value head h / (H / Hkv).  q, k, v bf16, element (t, h, d) at
+ * t * ld + h * D + d (parts of a QKV row, say); out [T, H, D] with row stride
+ * ldo.  scale > 0.  H / Hkv <= 64.  max_q: an upper bound of the sequences' lengths where
+ * known, else T (a hint: results do not depend on it beyond rounding). */
+int btl_prompt_attention(const uint16_t* q, int64_t ldq, const uint16_t* k, int64_t ldk, const uint16_t* v,
+                         int64_t ldv, int64_t T, int64_t H, int64_t Hkv, int64_t D, const int32_t* cu_q, int64_t B,
+                         float scale, int64_t max_q, uint16_t* out, int64_t ldo, int32_t* error_word,
+                         btl_stream_t stream);
+
+/* Attention of the newest tokens over the pages: the row at position p attends
+ * to positions [0, p].  max_q and max_kv: upper bounds of the new tokens and
+ * of kv_len of any sequence where known, else T and max_pages * page_size
+ * (hints, as above).  Long contexts of few rows are split over workgroups,
+ * whose partials are merged in a fixed order by a second launch: scratch, 16-byte aligned, of
+ * btl_paged_attention_scratch_bytes with the same arguments (0: not split) on the same
+ * device; its content is neither read nor kept, and calls that may run at once
+ * need one each. */
+int64_t btl_paged_attention_scratch_bytes(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t B, int64_t max_q,
+                                          int64_t max_kv);
+int btl_paged_attention(const uint16_t* q, int64_t ldq, int64_t T, int64_t H, const btl_pages_t* pages,
+                        const int32_t* page_table, int64_t max_pages, const int32_t* cu_q, const int32_t* kv_len,
+                        int64_t B, float scale, int64_t max_q, int64_t max_kv, uint16_t* out, int64_t ldo,
+                        void* scratch, size_t scratch_bytes, int32_t* error_word, btl_stream_t stream);
+
+/* Test hooks, host only: the functions that the kernels call.  btl_page_row:
+ * the index of a position's (page, head, row), -1 for a page outside the pool.
+ * btl_clamp_seq: {first row, rows, positions} of a sequence (cu_q entries lo
+ * and hi) after clamping; 1 if nothing had to be.  btl_row_exponent: e of an 8-bit
+ * row whose largest magnitude is given. */
+int64_t btl_page_row(int64_t page, int64_t num_pages, int64_t num_kv_heads, int64_t kv_head, int64_t page_size,
+                     int64_t position);
+int btl_clamp_seq(int64_t lo, int64_t hi, int64_t len, int64_t T, int64_t cap, int64_t* seq);
+int btl_row_exponent(float largest);
+
 #ifdef __cplusplus
 }
 #endif
