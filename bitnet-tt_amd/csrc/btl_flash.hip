@@ -16,11 +16,12 @@
 // the order is made up for where V is read (transposing LDS reads of row
 // groups in the same order).
 //
-// Softmax in base 2: p = 2^(c' s - c' m), c' = c log2(e), in fp32; m is a running
-// maximum that is only raised, and the output rescaled, where a row's maximum
-// grew by more than 2^kLazy (p then stays below 2^kLazy, which costs an fp32 sum
-// nothing).  p is rounded to bf16 for the second product, the matrix units'
-// operand type; the sum takes p unrounded.
+// Softmax in base 2: p = 2^(c' s - m), c' = c log2(e), in fp32; m, a whole number,
+// is raised to the running maximum's ceiling only where that is more than kLazy
+// above it (p then stays below 2^kLazy, which costs an fp32 sum nothing), and the
+// factors that this puts on what has been summed are powers of two: exact.  p is rounded to bf16 for the second product, the matrix units'
+// operand type, and the sum takes the same rounded values, so the weights that
+// are used sum to one.
 //
 // Rows of V behind the last position read as zero (whatever lies there), and a
 // value that is not finite at a position that some of the tile's rows may not see is added
@@ -32,6 +33,7 @@
 #include "btl_common.h"
 #include "btl_fp8.h"
 #include "btl_paged.h"
+#include <stdlib.h>
 
 namespace btl {
 
@@ -45,6 +47,7 @@ typedef __attribute__((address_space(3))) uint8_t lds8;
 enum { kDense = 0, kPagedBf16 = 1, kPagedFp8 = 2 };
 
 constexpr float kLazy = 8.0f;
+constexpr float kWhole = -1.0f;
 constexpr float kNegInf = -__builtin_inff();
 
 struct FlashArgs {
@@ -60,13 +63,21 @@ struct FlashArgs {
   uint16_t* out;
   int32_t* error;
   // splits > 1: workgroup z takes positions [z chunk, (z + 1) chunk), the last
-  // split the rest, and leaves a partial per row
+  // split the rest, and leaves a partial per row; a sequence of at most chunk
+  // positions is workgroup 0's alone, which writes the output and marks the row
+  // (the sum of its first partial is kWhole)
   int splits, chunk;
   float* part_o;    // [splits][T][H][D]
-  float2* part_ml;  // [splits][T][H]: maximum (in score units), sum
+  float2* part_ml;  // [splits][T][H]: exponents' offset, sum
 };
 
 __device__ const uint4 g_zero_row[16] = {};  // 256 bytes that read as zero
+
+// l plus both bf16 values of a pair, in 32 bits (one instruction).
+__device__ __forceinline__ float sum_pair(uint32_t two, float l) {
+  typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, two), __builtin_bit_cast(v2bf, 0x3f803f80u), l, false);
+}
 
 // No score of a row so far (a NaN score leaves the maximum alone, not the sum).
 __device__ __forceinline__ bool empty(float m, float l) { return m == kNegInf && l == 0.0f; }
@@ -93,6 +104,21 @@ __device__ __forceinline__ uint4 mem_ld128(const uint8_t* p) {
 }
 __device__ __forceinline__ uint32_t mem_ld8(const uint8_t* p) { return *(const __attribute__((address_space(1))) uint8_t*)p; }
 
+// Loads through a buffer resource of `bytes` bytes at a scalar address; a piece behind them reads as zero.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buf_rsrc(const uint8_t* p, uint32_t bytes) {
+  const uint64_t at = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = (uint32_t)uni((int)(uint32_t)at), hi = (uint32_t)uni((int)(at >> 32));
+  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(((uint64_t)hi << 32) | lo), (short)0,
+                                           uni((int)bytes), 0x00020000);
+}
+__device__ __forceinline__ uint4 buf_ld128(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+  const auto v = __builtin_amdgcn_raw_buffer_load_b128(r, (int)off, 0, 0);
+  return make_uint4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ uint32_t buf_ld8(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+  return (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(r, (int)off, 0, 0);
+}
+
 __device__ __forceinline__ uint4 lds_ld128(const lds8* p) {
   typedef uint32_t v4u __attribute__((ext_vector_type(4)));
   const v4u v = *(const __attribute__((address_space(3))) v4u*)p;
@@ -118,47 +144,61 @@ __device__ __forceinline__ v4s lds_tr16(const lds8* p) {
 // ======================================================================
 // Tiles of 128 rows: 4 waves of 32 rows each, 64 positions a step.
 //
-// Keys and values go to LDS as bf16, two stages of each: 64 KiB at D = 128, so two
-// workgroups share a CU and one's softmax runs under the other's MFMAs.  A step's
-// loads are issued one step ahead of their use; one barrier a step.  16-byte pieces of a row are
-// stored at piece ^ f(row): for K, f = row, so that 8 lanes that read the same
-// piece of 8 rows hit different banks; for V, f = 2 row, so that the 4 rows x 32
-// bytes of a transposing read do.
+// Keys and values are in LDS as bf16, two stages of each: 64 KiB at D = 128, so two
+// workgroups share a CU.  Loads go to LDS directly (8-bit pages: through
+// registers, converted), one barrier a step.  The scores run one step ahead: the
+// MFMAs of step j + 1's scores are independent of step j's exponentials, so
+// that a wave's vector work runs under its own matrix work, and not only under the other
+// workgroup's.  (The second product one step behind as well, so that nothing
+// in a step depends on anything else in it: the same speed, and 30 registers more than there are.)
+//
+// 16-byte pieces of a row are stored at piece ^ f(row), for the LDS's 64 banks:
+// the 16 rows that 16 lanes read a piece of, and the 4 rows x 64 bytes that 32 lanes
+// of a transposing read cover, lie in different banks.
 // ======================================================================
 constexpr int kTileRows = 128;
 constexpr int kStep = 64;
 
 template <int D>
 struct Tile {
-  static constexpr int kPieces = D / 8;                // 16-byte pieces of a bf16 row
   static constexpr int kBytes = kStep * D * 2;         // one stage of K, or of V
-  static constexpr int kLoads = kBytes / (256 * 16);   // 16-byte loads of a thread for it
-  static constexpr int kRowsLoad = 256 / kPieces;      // rows that one load of every thread covers
-  static __device__ __forceinline__ int k_swz(int row) { return row & (kPieces - 1); }
-  static __device__ __forceinline__ int v_swz(int row) { return (2 * row) & (kPieces - 1); }
+  static constexpr int kLoads = kBytes / (256 * 16);   // 16-byte pieces of a thread for it
+  static __device__ __forceinline__ int k_swz(int row) { return D == 128 ? row & 15 : (row >> 1) & 7; }
+  static __device__ __forceinline__ int v_swz(int row) { return D == 128 ? (row & 3) << 2 : (row & 2) << 1; }
 };
 
 // Where a step's rows come from: the sequence's packed rows, or its pages.
-// A thread's rows of a step are i * RPL + tid / TPR for its loads i (TPR threads
-// to a row); each run of 16 rows is in one page.
+// A thread's rows of a step are i * kRpl + tid / kTpr for its loads i (kTpr threads
+// to a row); a wave's rows of one load are in one run of 16 positions, and so in
+// one page.  An address is a buffer resource at a scalar address plus a 32-bit
+// offset that a thread keeps: no vector arithmetic per load (64-bit row addresses
+// per load took half as many vector cycles again as the softmax).  Rows behind the
+// end, and rows in no page, are out of the resource's range: they read as zeros.
 template <int D, int KV>
 struct Source {
   static constexpr int kRowBytes = KV == kPagedFp8 ? D : 2 * D;
   static constexpr int kTpr = kRowBytes / 16;      // threads of a row
   static constexpr int kRpl = 256 / kTpr;          // rows of a load
   static constexpr int kN = kStep / kRpl;          // loads of a thread
-  int32_t page[kN];                                // pages of the next step's row runs
-  const uint8_t* k;
+  const uint8_t* k;                                // dense: the sequence's first row
   const uint8_t* v;
-  int64_t ldk, ldv;   // bytes
+  int64_t ldk, ldv;                                // dense: bytes of a row
   const int32_t* table;
-  int hk, kv_end;
+  int hk, kv_end, row0, my_row;                    // the wave's first row and the thread's row in the first load
+  uint32_t off_k[kN], off_v[kN];                   // of the thread's pieces, from the step's first row
+  bool one;                                        // pages of whole steps
+  int32_t page_k[kN], page_v[kN];                  // pages of the runs of the keys and of the values to be loaded next
   bool bad;
+  uint4 rk[kN], rv[kN];                            // 8-bit pages: a step on its way
+  uint32_t ek[kN], ev[kN];
 
   __device__ __forceinline__ void init(const FlashArgs& p, const Seq& s, int b, int hk_, int kv_end_) {
+    const int tid = threadIdx.x;
     hk = hk_;
     kv_end = kv_end_;
     bad = false;
+    row0 = uni(tid) / kTpr;
+    my_row = tid / kTpr;
     if (KV == kDense) {
       ldk = p.ldk * 2;
       ldv = p.ldv * 2;
@@ -166,154 +206,187 @@ struct Source {
       v = reinterpret_cast<const uint8_t*>(p.v + (int64_t)s.row0 * p.ldv + hk * D);
     } else {
       table = p.bt.table + (int64_t)b * p.bt.max_pages;
+      one = p.pg.ps.d % kStep == 0;
+    }
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      // pieces land in LDS in the order of the lanes: the order f makes is made here
+      const int row = i * kRpl + tid / kTpr, c = tid % kTpr;
+      off_k[i] = row * (KV == kDense ? (uint32_t)ldk : kRowBytes) + 16 * (KV == kPagedFp8 ? c : c ^ Tile<D>::k_swz(row));
+      off_v[i] = row * (KV == kDense ? (uint32_t)ldv : kRowBytes) + 16 * (KV == kPagedFp8 ? c : c ^ Tile<D>::v_swz(row));
     }
   }
-  // Run of 16 rows that this wave's rows of load i lie in.
-  __device__ __forceinline__ int run(int kv, int i) const {
-    return kv + i * kRpl + (uni(threadIdx.x) / kTpr & ~15);
-  }
-  __device__ __forceinline__ void fetch_pages(const FlashArgs& p, int kv) {
+  // The run of 16 rows that the wave's rows of load i are in.
+  __device__ __forceinline__ int run_of(int i) const { return (i * kRpl + row0) & ~15; }
+  __device__ __forceinline__ void fetch_pages(const FlashArgs& p, int kv, int32_t (&page)[kN]) const {
     if (KV == kDense) return;
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
-      const int at = run(kv, i);
+      const int at = one ? kv : kv + run_of(i);
       page[i] = 0;
-      if (at < kv_end) page[i] = scalar_load(table, div_by(at, p.pg.ps));
+      if (at < kv_end && (i == 0 || !one)) page[i] = scalar_load(table, div_by(at, p.pg.ps));
     }
   }
-  // The row of load i as (address of its first byte in k, in v, exponent index);
-  // a row behind the end or in no page reads zeros.
-  __device__ __forceinline__ void row(const FlashArgs& p, int kv, int i, const uint8_t*& rk, const uint8_t*& rv,
-                                      int64_t& at) {
-    const int pos = kv + i * kRpl + (int)threadIdx.x / kTpr;
-    at = -1;
+  // The values follow the keys by a step; the keys' next pages, of the step at kv, are fetched.
+  __device__ __forceinline__ void turn_pages(const FlashArgs& p, int kv) {
+    if (KV == kDense) return;
+#pragma unroll
+    for (int i = 0; i < kN; ++i) page_v[i] = page_k[i];
+    fetch_pages(p, kv, page_k);
+  }
+  // Page row of the step's position `at`, and how many of up to `most` rows from there there are.
+  __device__ __forceinline__ int64_t rows_at(const FlashArgs& p, int at, int32_t page, int most, uint32_t& n) {
+    n = (uint32_t)clampi(kv_end - at, 0, most);
+    const bool none = (uint32_t)page >= (uint32_t)p.pg.P;
+    bad |= none & (n > 0);
+    n = none ? 0 : n;
+    return page_row(none ? 0 : page, p.pg.P, p.pg.Hkv, hk, p.pg.ps.d, at - (int)div_by(at, p.pg.ps) * (int)p.pg.ps.d);
+  }
+  // The step's keys (VAL: values) to LDS (8-bit pages: to registers).
+  template <bool VAL>
+  __device__ __forceinline__ void load(const FlashArgs& p, int kv, lds8* at) {
+    lds8* const dst = at + uni(threadIdx.x >> 6) * 1024;
     if (KV == kDense) {
-      rk = k + (int64_t)pos * ldk;
-      rv = v + (int64_t)pos * ldv;
-    } else {
-      const int r0 = run(kv, i);
-      const int32_t id = page[i];
-      const int64_t base = page_row(id, p.pg.P, p.pg.Hkv, hk, p.pg.ps.d,
-                                    r0 - (int)div_by(r0, p.pg.ps) * (int)p.pg.ps.d);
-      if (base < 0 && r0 < kv_end) bad = true;
-      at = base < 0 ? -1 : base + (pos - r0);
-      rk = at < 0 ? reinterpret_cast<const uint8_t*>(g_zero_row) : p.pg.k + at * kRowBytes;
-      rv = at < 0 ? reinterpret_cast<const uint8_t*>(g_zero_row) : p.pg.v + at * kRowBytes;
-    }
-    if (pos >= kv_end) {
-      rk = rv = reinterpret_cast<const uint8_t*>(g_zero_row);
-      at = -1;
-    }
-  }
-};
-
-// A step's rows on their way from memory to LDS.  (Through registers: loads
-// into LDS directly would cost none, but the compiler takes every LDS read
-// to depend on them, and would wait for the next step's rows before reading this one's.)
-template <int N>
-struct Staged {
-  uint4 k[N], v[N];
-  uint32_t ke[N], ve[N];  // exponent bytes (8-bit pages)
-};
-
-template <int D, int KV>
-__device__ __forceinline__ void load_step(const FlashArgs& p, Source<D, KV>& src, int kv,
-                                          Staged<Source<D, KV>::kN>& st) {
-  using S = Source<D, KV>;
-  const int c = threadIdx.x % S::kTpr;
+      const uint32_t ld = (uint32_t)(VAL ? ldv : ldk);
+      const auto r = buf_rsrc((VAL ? v : k) + kv * (VAL ? ldv : ldk), (uint32_t)min(kv_end - kv, kStep) * ld);
 #pragma unroll
-  for (int i = 0; i < S::kN; ++i) {
-    const uint8_t *rk, *rv;
-    int64_t at;
-    src.row(p, kv, i, rk, rv, at);
-    st.k[i] = mem_ld128(rk + 16 * c);
-    st.v[i] = mem_ld128(rv + 16 * c);
-    if (KV == kPagedFp8) {
-      st.ke[i] = st.ve[i] = 127;
-      if (at >= 0) {
-        st.ke[i] = mem_ld8(p.pg.ke + at);
-        st.ve[i] = mem_ld8(p.pg.ve + at);
+      for (int i = 0; i < kN; ++i) piece<VAL>(r, i, dst);
+      return;
+    }
+    const uint8_t* const pool = VAL ? p.pg.v : p.pg.k;
+    const uint8_t* const exps = VAL ? p.pg.ve : p.pg.ke;
+    if (one) {
+      uint32_t n;
+      const int64_t row = rows_at(p, kv, VAL ? page_v[0] : page_k[0], kStep, n);
+      const auto r = buf_rsrc(pool + row * kRowBytes, n * kRowBytes);
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        piece<VAL>(r, i, dst);
+        if (KV == kPagedFp8) (VAL ? ev : ek)[i] = buf_ld8(buf_rsrc(exps + row, n), i * kRpl + my_row);
       }
+      return;
     }
-  }
-}
-
-template <int D, int KV>
-__device__ __forceinline__ void store_step(lds8* ks, lds8* vs, const Staged<Source<D, KV>::kN>& st) {
-  using S = Source<D, KV>;
-  const int c = threadIdx.x % S::kTpr;
 #pragma unroll
-  for (int i = 0; i < S::kN; ++i) {
-    const int r = i * S::kRpl + threadIdx.x / S::kTpr;
-    lds8 *const k = ks + r * 2 * D, *const v = vs + r * 2 * D;
-    if (KV == kPagedFp8) {
-      const float fk = exp_scale(st.ke[i]), fv = exp_scale(st.ve[i]);
-      const int k0 = 2 * c ^ Tile<D>::k_swz(r), v0 = 2 * c ^ Tile<D>::v_swz(r);
-      lds_st128(k + k0 * 16, from_e4m3(make_uint2(st.k[i].x, st.k[i].y), fk));
-      lds_st128(k + (k0 ^ 1) * 16, from_e4m3(make_uint2(st.k[i].z, st.k[i].w), fk));
-      lds_st128(v + v0 * 16, from_e4m3(make_uint2(st.v[i].x, st.v[i].y), fv));
-      lds_st128(v + (v0 ^ 1) * 16, from_e4m3(make_uint2(st.v[i].z, st.v[i].w), fv));
-    } else {
-      lds_st128(k + (c ^ Tile<D>::k_swz(r)) * 16, st.k[i]);
-      lds_st128(v + (c ^ Tile<D>::v_swz(r)) * 16, st.v[i]);
+    for (int i = 0; i < kN; ++i) {
+      // a run's rows, by their offsets from the step's first
+      uint32_t n;
+      const int r0 = run_of(i);
+      const int64_t row = rows_at(p, kv + r0, VAL ? page_v[i] : page_k[i], 16, n) - r0;
+      n = n ? n + r0 : 0;
+      piece<VAL>(buf_rsrc(pool + row * kRowBytes, n * kRowBytes), i, dst);
+      if (KV == kPagedFp8) (VAL ? ev : ek)[i] = buf_ld8(buf_rsrc(exps + row, n), i * kRpl + my_row);
     }
   }
-}
+  template <bool VAL>
+  __device__ __forceinline__ void piece(__amdgpu_buffer_rsrc_t r, int i, lds8* dst) {
+    const uint32_t off = VAL ? off_v[i] : off_k[i];
+    if (KV == kPagedFp8)
+      (VAL ? rv : rk)[i] = buf_ld128(r, off);
+    else
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, dst + i * 4096, 16, (int)off, 0, 0, 0);
+  }
+  // 8-bit pages: what load() brought, converted, to LDS.
+  template <bool VAL>
+  __device__ __forceinline__ void store(lds8* at) const {
+    if (KV != kPagedFp8) return;
+    const int c = threadIdx.x % kTpr;
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const int row = i * kRpl + threadIdx.x / kTpr;
+      const uint4 w = (VAL ? rv : rk)[i];
+      const float f = exp_scale((VAL ? ev : ek)[i]);
+      const int c0 = 2 * c ^ (VAL ? Tile<D>::v_swz(row) : Tile<D>::k_swz(row));
+      lds_st128(at + row * 2 * D + c0 * 16, from_e4m3(make_uint2(w.x, w.y), f));
+      lds_st128(at + row * 2 * D + (c0 ^ 1) * 16, from_e4m3(make_uint2(w.z, w.w), f));
+    }
+  }
+};
 
 template <int D>
 struct TileState {
   v8bf q[D / 16];   // B operands: this lane's query row, dims 16 ks + 8 h ..
-  v16f o[D / 32];   // O^T: element r of o[t] is dim 32 t + acc_row(r) of the lane's row
-  float m, l;       // running maximum (score units), this lane's share of the sum
+  v16f o[D / 32];   // O^T: element r of o[t] is dim 32 t + c_row(r) of the lane's row
+  float m, l[2];    // the exponents' offset (a whole number; -inf: no score yet), this lane's share of the sum
   int limit;        // the last position that the lane's row sees, -1: none
   int lo, hi;       // of the wave's rows: least limit, greatest
 };
 
 __device__ __forceinline__ int c_row(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }
 
-// Scores of the step, softmax, and the probabilities as operands.
-template <int D, bool MASK>
-__device__ __forceinline__ void step_scores(const lds8* ks, TileState<D>& s, float c, int kv, v8bf (&pb)[4]) {
+// The larger of the two halves' values.
+__device__ __forceinline__ float half_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// Key operands of a step: positions 32 t + r32, dims 16 k + 8 h .. + 7.
+template <int D>
+__device__ __forceinline__ v8bf tile_key(const lds8* ks, int t, int k) {
   const int lane = __lane_id(), h = lane >> 5, r32 = lane & 31;
-  v16f sc[2];
+  return lds_ld_bf8(ks + (32 * t + r32) * 2 * D + ((Tile<D>::k_swz(r32) ^ h ^ (2 * k)) * 16));
+}
+// The first of them, which are read ahead of whatever is issued before the products.
+constexpr int kAhead = 2;
+typedef v8bf TileKeys[kAhead][2];
+template <int D>
+__device__ __forceinline__ void tile_keys(const lds8* ks, TileKeys& a) {
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k)
+#pragma unroll
+    for (int t = 0; t < 2; ++t) a[k][t] = tile_key<D>(ks, t, k);
+}
+// Scores of a step: element r of sc[t] is position 32 t + c_row(r).
+template <int D>
+__device__ __forceinline__ void tile_scores(const lds8* ks, TileKeys& a, const TileState<D>& s, v16f (&sc)[2]) {
 #pragma unroll
   for (int t = 0; t < 2; ++t)
 #pragma unroll
     for (int r = 0; r < 16; ++r) sc[t][r] = 0.0f;
-  const lds8* row = ks + r32 * 2 * D;
-  const int x = Tile<D>::k_swz(r32) ^ h;
 #pragma unroll
-  for (int k = 0; k < D / 16; ++k) {
+  for (int k = 0; k < D / 16; ++k)
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const v8bf a = lds_ld_bf8(row + t * 32 * 2 * D + ((x ^ (2 * k)) * 16));
-      sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, s.q[k], sc[t], 0, 0, 0);
+      sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[k % kAhead][t], s.q[k], sc[t], 0, 0, 0);
+      if (k + kAhead < D / 16) a[k % kAhead][t] = tile_key<D>(ks, t, k + kAhead);
     }
-  }
-  if (MASK) {
+}
+
+template <int D>
+__device__ __forceinline__ void tile_mask(const TileState<D>& s, int kv, v16f (&sc)[2]) {
+  const int h = __lane_id() >> 5;
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+  for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if (kv + 32 * t + c_row(r, h) > s.limit) sc[t][r] = kNegInf;
-  }
+    for (int r = 0; r < 16; ++r)
+      if (kv + 32 * t + c_row(r, h) > s.limit) sc[t][r] = kNegInf;
+}
+
+// Raises the offset where the scores of the next step need it.
+template <int D>
+__device__ __forceinline__ void tile_raise(TileState<D>& s, float c, const v16f (&sc)[2]) {
   float mx = sc[0][0];
 #pragma unroll
   for (int i = 1; i < 32; ++i) mx = fmaxf(mx, sc[i >> 4][i & 15]);
-  mx = fmaxf(mx, xor_partner<32>(mx));
-  if (__any(mx > s.m && (mx - s.m) * c > kLazy)) {  // (m = -inf: any score is more)
-    const float mn = fmaxf(s.m, mx);
-    const float a = s.m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f((s.m - mn) * c);
+  mx = half_max(mx) * c;
+  if (__any(mx - s.m > kLazy)) {  // (from -inf: any score is more)
+    const float mn = fmaxf(s.m, __builtin_ceilf(mx));
+    const float a = s.m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(s.m - mn);
     s.m = mn;
-    s.l *= a;
+    s.l[0] *= a;
+    s.l[1] *= a;
 #pragma unroll
     for (int t = 0; t < D / 32; ++t)
 #pragma unroll
       for (int r = 0; r < 16; ++r) s.o[t][r] *= a;
   }
-  const float mc = s.m == kNegInf ? 0.0f : -s.m * c;
+}
+
+// The probabilities of a step's scores, as operands.
+template <int D>
+__device__ __forceinline__ void tile_exp(TileState<D>& s, float c, const v16f (&sc)[2], v8bf (&pb)[4]) {
+  const float mc = s.m == kNegInf ? 0.0f : -s.m;
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
+  for (int t = 0; t < 2; ++t)
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       uint32_t w[4];
@@ -321,16 +394,17 @@ __device__ __forceinline__ void step_scores(const lds8* ks, TileState<D>& s, flo
       for (int j = 0; j < 4; ++j) {
         const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][8 * k + 2 * j], c, mc));
         const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][8 * k + 2 * j + 1], c, mc));
-        s.l += e0 + e1;
         w[j] = f2bf_pair(e0, e1);
+        s.l[k] = sum_pair(w[j], s.l[k]);
       }
       pb[2 * t + k] = __builtin_bit_cast(v8bf, make_uint4(w[0], w[1], w[2], w[3]));
     }
-  }
 }
 
+// (__restrict__: a transposing read carries no alias information of its own, and the compiler
+// would wait for every load into LDS that is on its way before one.)
 template <int D>
-__device__ __forceinline__ void step_values(const lds8* vs, TileState<D>& s, const v8bf (&pb)[4]) {
+__device__ __forceinline__ void tile_values(const lds8* __restrict__ vs, TileState<D>& s, const v8bf (&pb)[4]) {
   const int lane = __lane_id(), h = lane >> 5, g1 = (lane >> 4) & 1, rr = (lane & 15) >> 2, qq = lane & 3;
   const int row = 4 * h + rr;
   const lds8* base = vs + row * 2 * D + (qq & 1) * 8;
@@ -352,7 +426,7 @@ __device__ __forceinline__ void step_values(const lds8* vs, TileState<D>& s, con
 // values that are not finite: those are added to the rows that see them, and
 // then cleared for the product.
 template <int D>
-__device__ __forceinline__ void add_not_finite(lds8* vs, TileState<D>& s, int kv) {
+__device__ __forceinline__ void add_not_finite(const lds8* vs, TileState<D>& s, int kv) {
   const int h = __lane_id() >> 5;
 #pragma unroll 1
   for (int j = 0; j < kStep; ++j) {
@@ -376,18 +450,20 @@ __device__ __forceinline__ void add_not_finite(lds8* vs, TileState<D>& s, int kv
 
 template <int D, int KV>
 __global__ __launch_bounds__(256, 2) void k_flash_tile(FlashArgs p) {
-  __shared__ __attribute__((aligned(16))) uint8_t smem[4 * Tile<D>::kBytes];
-  __shared__ int s_flag[4];
+  constexpr int kB = Tile<D>::kBytes;
+  // Keys: stages 0 and 1, values: 2 and 3; a flag per wave.  (One LDS object: the
+  // accesses to several get alias scopes, and reads then wait for the loads into LDS that are on their way.)
+  __shared__ __attribute__((aligned(16))) uint8_t smem[4 * kB + 16];
+  int* const s_flag = reinterpret_cast<int*>(smem + 4 * kB);
   const int tid = threadIdx.x, wv = uni(tid >> 6), lane = tid & 63, h = lane >> 5;
-  const int hk = blockIdx.x % p.Hkv, split = blockIdx.y;
+  const int hk = uni(blockIdx.x % p.Hkv), split = blockIdx.y;
   Item it;
   if (!find_item(p.bt, p.G, kTileRows, blockIdx.x / p.Hkv, it)) return;
-  const int64_t cap = (int64_t)p.bt.max_pages * p.pg.ps.d;
-  const Seq sq = load_seq(p.bt, it.b, cap);
+  const Seq sq = load_seq(p.bt, it.b, (int64_t)p.bt.max_pages * p.pg.ps.d);
   if (!sq.ok && tid == 0) flag_error(p.error);
   const int rows = sq.n * p.G, first = sq.len - sq.n;  // position of the first token
   const int r0 = (it.count - 1 - it.i) * kTileRows;     // the longest tiles first
-  const int t_last = row_token(min(r0 + kTileRows, rows) - 1, p);
+  const int t_last = uni(row_token(min(r0 + kTileRows, rows) - 1, p));
 
   TileState<D> s;
   const int r = r0 + 32 * wv + (lane & 31);
@@ -407,82 +483,134 @@ __global__ __launch_bounds__(256, 2) void k_flash_tile(FlashArgs p) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) s.o[t][i] = 0.0f;
   s.m = kNegInf;
-  s.l = 0.0f;
+  s.l[0] = s.l[1] = 0.0f;
 
-  const int wg_lo = max(-1, first + row_token(r0, p));
+  const int wg_lo = max(-1, first + uni(row_token(r0, p)));
   int kv_end = max(0, first + t_last + 1);
   int kv0 = 0;
-  if (p.splits > 1) {
+  const bool whole = p.splits == 1 || sq.len <= p.chunk;
+  if (whole && split > 0) return;
+  if (!whole) {
     kv0 = split * p.chunk;
     if (split + 1 < p.splits) kv_end = min(kv_end, kv0 + p.chunk);
   }
   if (kv0 < kv_end) {
     lds8* const sm = (lds8*)smem;
     Source<D, KV> src;
-    Staged<Source<D, KV>::kN> st;
     src.init(p, sq, it.b, hk, kv_end);
-    src.fetch_pages(p, kv0);
-    load_step<D, KV>(p, src, kv0, st);
-    src.fetch_pages(p, kv0 + kStep);
-    store_step<D, KV>(sm, sm + Tile<D>::kBytes, st);
-    int kv = kv0, at = 0;  // the step's rows are in stage `at` (keys, then values), the next step's go to the other
-    // steps that every row of the tile sees whole
-    for (; kv < kv_end && kv + kStep - 1 <= wg_lo; kv += kStep, at ^= 1) {
-      lds8* const ks = sm + at * 2 * Tile<D>::kBytes;
-      lds8* const kn = sm + (at ^ 1) * 2 * Tile<D>::kBytes;
-      lds_barrier();  // the step's rows are in LDS, and the other stage is free
-      const bool more = kv + kStep < kv_end;
-      if (more) {
-        load_step<D, KV>(p, src, kv + kStep, st);
-        src.fetch_pages(p, kv + 2 * kStep);
-      }
+    const int whole_end = min(kv_end, wg_lo + 1);  // every row of the tile sees the positions before it
+    int kv = kv0, at = 0;  // step j at position kv; at: j's parity
+    auto arrived = [&] {
+      __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this thread's loads
+      lds_barrier();                       // everyone's; and what the last step read is free
+    };
+    // the keys of two steps ahead, the values of the next
+    auto load_ahead = [&](lds8* k_free, lds8* v_free) {
+      if (kv + 2 * kStep < kv_end) src.template load<false>(p, kv + 2 * kStep, k_free);
+      if (kv + kStep < kv_end) src.template load<true>(p, kv + kStep, v_free);
+      src.turn_pages(p, kv + 3 * kStep);
+    };
+    auto store_ahead = [&](lds8* k_free, lds8* v_free) {
+      if (kv + 2 * kStep < kv_end) src.template store<false>(k_free);
+      if (kv + kStep < kv_end) src.template store<true>(v_free);
+    };
+
+    src.fetch_pages(p, kv0, src.page_k);
+    src.template load<false>(p, kv0, sm);
+    src.template store<false>(sm);
+    src.turn_pages(p, kv0 + kStep);
+    src.template load<true>(p, kv0, sm + 2 * kB);
+    src.template store<true>(sm + 2 * kB);
+    if (kv0 + kStep < kv_end) {
+      src.template load<false>(p, kv0 + kStep, sm + kB);
+      src.template store<false>(sm + kB);
+    }
+    src.turn_pages(p, kv0 + 2 * kStep);
+    arrived();
+    TileKeys keys;
+    v16f sa[2], sb[2];
+    if (kv0 <= s.hi) {
+      tile_keys<D>(sm, keys);
+      tile_scores<D>(sm, keys, s, sa);
+      if (kv0 + kStep - 1 > s.lo) tile_mask<D>(s, kv0, sa);
+      tile_raise<D>(s, p.c, sa);
+    }
+    lds_barrier();  // the first keys are read: their stage is free
+
+    // steps whose successor every row of the tile sees whole; a copy for each
+    // parity, so that LDS addresses are constants and scores stay in their registers
+    auto hot = [&](const lds8* ks, const lds8* vs, lds8* k_free, lds8* v_free, const v16f(&cur)[2], v16f(&nxt)[2]) {
+      arrived();
+      tile_keys<D>(ks, keys);
+      load_ahead(k_free, v_free);
       v8bf pb[4];
-      step_scores<D, false>(ks, s, p.c, kv, pb);
-      step_values<D>(ks + Tile<D>::kBytes, s, pb);
-      if (more) store_step<D, KV>(kn, kn + Tile<D>::kBytes, st);
+      tile_scores<D>(ks, keys, s, nxt);
+      tile_exp<D>(s, p.c, cur, pb);
+      tile_values<D>(vs, s, pb);
+      tile_raise<D>(s, p.c, nxt);
+      store_ahead(k_free, v_free);
+      kv += kStep;
+    };
+    while (kv + 2 * kStep <= whole_end) {
+      hot(sm + kB, sm + 2 * kB, sm, sm + 3 * kB, sa, sb);
+      if (kv + 2 * kStep > whole_end) {
+        at = 1;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) sa[t] = sb[t];
+        break;
+      }
+      hot(sm, sm + 3 * kB, sm + kB, sm + 2 * kB, sb, sa);
     }
     for (; kv < kv_end; kv += kStep, at ^= 1) {
-      lds8* const ks = sm + at * 2 * Tile<D>::kBytes;
-      lds8* const vs = ks + Tile<D>::kBytes;
-      lds8* const kn = sm + (at ^ 1) * 2 * Tile<D>::kBytes;
-      lds_barrier();
-      const bool more = kv + kStep < kv_end;
-      if (more) {
-        load_step<D, KV>(p, src, kv + kStep, st);
-        src.fetch_pages(p, kv + 2 * kStep);
-      }
-      bool nf = false;
+      const lds8* const ks = sm + (at ^ 1) * kB;
+      lds8* const vs = sm + (2 + at) * kB;
+      lds8 *const k_free = sm + at * kB, *const v_free = sm + (2 + (at ^ 1)) * kB;
+      arrived();
+      load_ahead(k_free, v_free);
+      const bool mine = kv <= s.hi, next = kv + kStep < kv_end && kv + kStep <= s.hi;  // some of the wave's rows see some of it
+      bool special = false;
+      if (kv + kStep - 1 > wg_lo) {  // some of the tile's rows do not see all of it
+        bool nf = false;
 #pragma unroll
-      for (int i = 0; i < Tile<D>::kLoads; ++i) nf |= any_not_finite(lds_ld128(vs + (i * 256 + tid) * 16));
-      const bool any = __any(nf);
-      if (lane == 0) s_flag[wv] = any;
-      lds_barrier();
-      const bool special = s_flag[0] | s_flag[1] | s_flag[2] | s_flag[3];
-      const bool mine = kv <= s.hi;  // some of the wave's rows see some of it
-      v8bf pb[4];
-      if (mine) step_scores<D, true>(ks, s, p.c, kv, pb);
+        for (int i = 0; i < Tile<D>::kLoads; ++i) nf |= any_not_finite(lds_ld128(vs + (i * 256 + tid) * 16));
+        const bool any = __any(nf);
+        if (lane == 0) s_flag[wv] = any;
+        lds_barrier();
+        special = s_flag[0] | s_flag[1] | s_flag[2] | s_flag[3];
+      }
       if (special) {
         if (mine) add_not_finite<D>(vs, s, kv);
         lds_barrier();
 #pragma unroll
         for (int i = 0; i < Tile<D>::kLoads; ++i) {
-          lds8* const at = vs + (i * 256 + tid) * 16;
-          const uint4 x = lds_ld128(at);
-          lds_st128(at, make_uint4(drop_not_finite(x.x), drop_not_finite(x.y), drop_not_finite(x.z),
-                                   drop_not_finite(x.w)));
+          lds8* const piece = vs + (i * 256 + tid) * 16;
+          const uint4 x = lds_ld128(piece);
+          lds_st128(piece, make_uint4(drop_not_finite(x.x), drop_not_finite(x.y), drop_not_finite(x.z),
+                                      drop_not_finite(x.w)));
         }
         lds_barrier();
       }
-      if (mine) step_values<D>(vs, s, pb);
-      if (more) store_step<D, KV>(kn, kn + Tile<D>::kBytes, st);
+      if (mine) {
+        v8bf pb[4];
+        tile_exp<D>(s, p.c, sa, pb);
+        tile_values<D>(vs, s, pb);
+      }
+      if (next) {
+        tile_keys<D>(ks, keys);
+        tile_scores<D>(ks, keys, s, sa);
+        if (kv + 2 * kStep - 1 > s.lo) tile_mask<D>(s, kv + kStep, sa);
+        tile_raise<D>(s, p.c, sa);
+      }
+      store_ahead(k_free, v_free);
     }
     if (KV != kDense && src.bad) flag_error(p.error);
   }
 
-  const float l = s.l + xor_partner<32>(s.l);
+  const float l0 = s.l[0] + s.l[1], l = l0 + xor_partner<32>(l0);
   if (r >= rows) return;
   const int64_t row = sq.row0 + tok;
-  if (p.splits > 1) {
+  if (whole && p.splits > 1 && h == 0) p.part_ml[row * p.H + head] = make_float2(0.0f, kWhole);
+  if (!whole) {
     const int64_t at = ((int64_t)split * p.bt.T + row) * p.H + head;
     if (h == 0) p.part_ml[at] = make_float2(s.m, l);
     if (empty(s.m, l)) return;
@@ -509,104 +637,174 @@ __global__ __launch_bounds__(256, 2) void k_flash_tile(FlashArgs p) {
 // ======================================================================
 // Few rows (up to 16 to a sequence and key-value head: single tokens, short
 // drafts): bound by the bytes of keys and values.  8 waves share a context,
-// 32 positions each a round; a wave's keys go straight from memory to the MFMA's
-// registers, its values through its own 8 KiB of LDS, and the next round's
-// loads are issued before this one is computed, so 256 KiB a CU are on their way.
-// The waves' partials meet in LDS.
+// a round of kPos positions each; a wave's keys go straight from memory to the
+// MFMA's registers, its values through its own 8 KiB of LDS.  The next round's
+// loads are issued as soon as this one's registers are free (unconditionally:
+// behind the end they are out of the resource's range and read nothing), so 16 KiB a
+// wave, 128 KiB a CU, are on their way nearly all the time.  Page table entries are
+// fetched a round ahead of that.  The waves' partials meet in LDS.
 // ======================================================================
 constexpr int kFewRows = 16;
 constexpr int kFewWaves = 8;
-constexpr int kFewPos = 32;  // positions of a wave and round
+
+// Pieces of a value row in LDS are at piece ^ few_swz(row): the 8 rows x 32 bytes
+// that 32 lanes of a transposing read cover are in different banks.
+template <int D>
+__device__ __forceinline__ int few_swz(int row) {
+  return D == 128 ? (2 * row) & 15 : row & 6;
+}
 
 template <int D>
 struct FewShared {
   union {
-    uint8_t v[kFewWaves][kFewPos * 2 * D];
-    float o[kFewWaves][kFewRows][D];  // after the last round
+    uint8_t v[kFewWaves][32 * 2 * D];       // 32 value rows of a wave
+    float o[kFewWaves][kFewRows][D];        // after the last round
   };
   float ml[kFewWaves][kFewRows][2];
 };
 
 template <int D, int KV>
-struct FewRound {
+struct Few {
   static constexpr int kRowBytes = KV == kPagedFp8 ? D : 2 * D;
-  static constexpr int kK = kRowBytes / 64;                 // key loads of a lane per 16 rows
-  static constexpr int kV = kFewPos * kRowBytes / 1024;     // value loads of a lane
-  uint4 k[2][kK];
-  uint4 v[kV];
-  uint32_t ke[2], ve[kV];
-};
+  static constexpr int kRuns = KV == kPagedFp8 ? 4 : 2;     // runs of 16 positions of a wave and round
+  static constexpr int kPos = 16 * kRuns;
+  static constexpr int kK = kRowBytes / 64;                 // key loads of a lane for a run
+  static constexpr int kV = kRowBytes / 64;                 // value loads of a lane for a run
+  static constexpr int kTpr = kRowBytes / 16;               // lanes of a value row
+  uint4 k[kRuns][kK];
+  uint4 v[kRuns][kV];
+  uint32_t ke[kRuns], ve[kRuns][kV];
+  int32_t page[kRuns];  // of the round to be loaded next
 
-template <int D, int KV>
-__device__ __forceinline__ void few_load(const FlashArgs& p, const int32_t* table, int hk, int kv, int kv_end,
-                                         FewRound<D, KV>& r, bool& bad) {
-  using R = FewRound<D, KV>;
-  const int lane = __lane_id();
-  int64_t base[2];  // page row of each run of 16 positions
+  // Page table entries of the round from position kv (any up to the table's end).
+  __device__ __forceinline__ void fetch_pages(const FlashArgs& p, const int32_t* table, int kv) {
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < kRuns; ++t)
+      page[t] = scalar_load(table, min(div_by(kv + 16 * t, p.pg.ps), (uint32_t)p.bt.max_pages - 1));
+  }
+  // First page row of run t, and how many of its rows are there (0: none, or no page).
+  __device__ __forceinline__ int64_t run(const FlashArgs& p, int hk, int kv, int kv_end, int t, uint32_t& n,
+                                         bool& bad) const {
     const int at = kv + 16 * t;
-    base[t] = -1;
-    if (at < kv_end) {
-      const uint32_t pi = div_by(at, p.pg.ps);
-      base[t] = page_row(scalar_load(table, pi), p.pg.P, p.pg.Hkv, hk, p.pg.ps.d, at - (int)pi * (int)p.pg.ps.d);
-      if (base[t] < 0) bad = true;
+    n = (uint32_t)clampi(kv_end - at, 0, 16);
+    const bool none = (uint32_t)page[t] >= (uint32_t)p.pg.P;
+    bad |= none & (n > 0);
+    n = none ? 0 : n;
+    return page_row(none ? 0 : page[t], p.pg.P, p.pg.Hkv, hk, p.pg.ps.d, at - (int)div_by(at, p.pg.ps) * (int)p.pg.ps.d);
+  }
+  __device__ __forceinline__ void load_keys(const FlashArgs& p, int hk, int kv, int kv_end, bool& bad) {
+    const int lane = __lane_id(), row = lane & 15;
+#pragma unroll
+    for (int t = 0; t < kRuns; ++t) {
+      uint32_t n;
+      const int64_t r = run(p, hk, kv, kv_end, t, n, bad);
+      const auto rs = buf_rsrc(p.pg.k + r * kRowBytes, n * kRowBytes);
+#pragma unroll
+      for (int i = 0; i < kK; ++i) k[t][i] = buf_ld128(rs, row * kRowBytes + 64 * i + 16 * (lane >> 4));
+      if (KV == kPagedFp8) ke[t] = buf_ld8(buf_rsrc(p.pg.ke + r, n), row);
     }
   }
-  const uint8_t* const zero = reinterpret_cast<const uint8_t*>(g_zero_row);
+  __device__ __forceinline__ void load_values(const FlashArgs& p, int hk, int kv, int kv_end, bool& bad) {
+    const int lane = __lane_id();
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const int row = lane & 15;
-    const bool ok = base[t] >= 0 && kv + 16 * t + row < kv_end;
-    const int64_t at = base[t] + row;
-    const uint8_t* a = ok ? p.pg.k + at * R::kRowBytes : zero;
+    for (int t = 0; t < kRuns; ++t) {
+      uint32_t n;
+      const int64_t r = run(p, hk, kv, kv_end, t, n, bad);
+      const auto rs = buf_rsrc(p.pg.v + r * kRowBytes, n * kRowBytes);
 #pragma unroll
-    for (int i = 0; i < R::kK; ++i) r.k[t][i] = mem_ld128(a + 64 * i + 16 * (lane >> 4));
-    r.ke[t] = 127;
-    if (KV == kPagedFp8 && ok) r.ke[t] = mem_ld8(p.pg.ke + at);
+      for (int i = 0; i < kV; ++i) {
+        v[t][i] = buf_ld128(rs, 1024 * i + 16 * lane);
+        if (KV == kPagedFp8) ve[t][i] = buf_ld8(buf_rsrc(p.pg.ve + r, n), (64 / kTpr) * i + lane / kTpr);
+      }
+    }
   }
-  constexpr int TPR = R::kRowBytes / 16, RPL = 64 / TPR;
-#pragma unroll
-  for (int i = 0; i < R::kV; ++i) {
-    const int row = i * RPL + lane / TPR, t = (i * RPL) / 16;  // RPL <= 16: a load's rows are in one run
-    const bool ok = base[t] >= 0 && kv + row < kv_end;
-    const int64_t at = base[t] + row - 16 * t;
-    const uint8_t* a = ok ? p.pg.v + at * R::kRowBytes : zero;
-    r.v[i] = mem_ld128(a + 16 * (lane % TPR));
-    r.ve[i] = 127;
-    if (KV == kPagedFp8 && ok) r.ve[i] = mem_ld8(p.pg.ve + at);
+  // Key operand of run t, dims 32 k ..: 8-bit keys give a lane 16 dims of each 64.
+  __device__ __forceinline__ v8bf key(int t, int i) const {
+    if (KV != kPagedFp8) return __builtin_bit_cast(v8bf, k[t][i]);
+    const uint4 w = k[t][i / 2];
+    return __builtin_bit_cast(v8bf, from_e4m3(i & 1 ? make_uint2(w.z, w.w) : make_uint2(w.x, w.y), exp_scale(ke[t])));
   }
+  // Value rows of runs t and t + 1 to the wave's LDS.
+  __device__ __forceinline__ void store_values(lds8* vs, int t0) const {
+    const int lane = __lane_id(), c = lane % kTpr;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < kV; ++i) {
+        const int row = 16 * t + (64 / kTpr) * i + lane / kTpr;
+        lds8* const at = vs + row * 2 * D;
+        const uint4 w = v[t0 + t][i];
+        if (KV == kPagedFp8) {
+          const float f = exp_scale(ve[t0 + t][i]);
+          const int c0 = 2 * c ^ few_swz<D>(row);
+          lds_st128(at + c0 * 16, from_e4m3(make_uint2(w.x, w.y), f));
+          lds_st128(at + (c0 ^ 1) * 16, from_e4m3(make_uint2(w.z, w.w), f));
+        } else {
+          lds_st128(at + (c ^ few_swz<D>(row)) * 16, w);
+        }
+      }
+  }
+};
+
+// 32 value rows in LDS some of which some of the rows may not see: as
+// add_not_finite, for this kernel's layout (lane r16: a query, its dims 16 t +
+// 4 grp ..).
+template <int D>
+__device__ __forceinline__ void few_not_finite(lds8* vs, v4f (&o)[D / 16], int at, int limit) {
+  const int lane = __lane_id(), grp = lane >> 4;
+  bool nf = false;
+  for (int i = lane; i < 32 * D / 8; i += 64) nf |= any_not_finite(lds_ld128(vs + i * 16));
+  if (!__any(nf)) return;
+#pragma unroll 1
+  for (int j = 0; j < 32; ++j)
+#pragma unroll
+    for (int t = 0; t < D / 16; ++t) {
+      const uint2 x = lds_ld64(vs + j * 2 * D + ((2 * t + (grp >> 1)) ^ few_swz<D>(j)) * 16 + 8 * (grp & 1));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint16_t y = (uint16_t)((i < 2 ? x.x : x.y) >> (16 * (i & 1)));
+        if ((y & 0x7f80u) == 0x7f80u && at + j <= limit) o[t][i] += bf2f(y);
+      }
+    }
+  __builtin_amdgcn_wave_barrier();
+  for (int i = lane; i < 32 * D / 8; i += 64) {
+    const uint4 x = lds_ld128(vs + i * 16);
+    lds_st128(vs + i * 16, make_uint4(drop_not_finite(x.x), drop_not_finite(x.y), drop_not_finite(x.z),
+                                      drop_not_finite(x.w)));
+  }
+  __builtin_amdgcn_wave_barrier();
 }
 
 template <int D, int KV>
 __global__ __launch_bounds__(64 * kFewWaves, 2) void k_flash_few(FlashArgs p) {
-  using R = FewRound<D, KV>;
+  using F = Few<D, KV>;
+  constexpr int kRound = F::kPos * kFewWaves;
   __shared__ __attribute__((aligned(16))) FewShared<D> s;
   const int tid = threadIdx.x, wv = uni(tid >> 6), lane = tid & 63, r16 = lane & 15, grp = lane >> 4;
   const int hk = blockIdx.x, b = blockIdx.y, split = blockIdx.z;
+  const int32_t* const table = p.bt.table + (int64_t)b * p.bt.max_pages;
+  const int kv0 = p.splits > 1 ? split * p.chunk : 0, kv_first = kv0 + F::kPos * wv;
+  F f;
+  f.fetch_pages(p, table, kv_first);  // (does not wait for the lengths)
   const Seq sq = load_seq(p.bt, b, (int64_t)p.bt.max_pages * p.pg.ps.d);
   if (!sq.ok && tid == 0) flag_error(p.error);
   const int rows = sq.n * p.G, first = sq.len - sq.n;
-  const int32_t* const table = p.bt.table + (int64_t)b * p.bt.max_pages;
-  int seq_end = sq.len, kv0 = 0;
-  if (p.splits > 1) {
-    kv0 = split * p.chunk;
-    if (split + 1 < p.splits) seq_end = min(seq_end, kv0 + p.chunk);
-  }
-  constexpr int PC = D / 8;  // 16-byte pieces of a bf16 row
+  const bool whole = p.splits == 1 || sq.len <= p.chunk;
+  if (whole && split > 0) return;
+  const int seq_end = whole || split + 1 == p.splits ? sq.len : min(sq.len, kv0 + p.chunk);
   bool bad = false;
   // one pass unless there are more rows than the caller said
   for (int r0 = 0; r0 < rows; r0 += kFewRows) {
     const int r = r0 + r16, rc = min(r, rows - 1);
     const int tok = row_token(rc, p), head = hk * p.G + rc - tok * p.G;
     const int limit = r < rows ? max(-1, first + tok) : -1;
-    const int lo = max(-1, first + row_token(r0, p));
-    const int kv_end = min(seq_end, max(0, first + row_token(min(r0 + kFewRows, rows) - 1, p) + 1));
-    FewRound<D, KV> cur;
-    int kv = kv0 + kFewPos * wv;
-    if (kv < kv_end) few_load<D, KV>(p, table, hk, kv, kv_end, cur, bad);
-    // B operands: bf16 keys give a lane 8 dims of each 32, 8-bit keys 16 of each 64
-    v8bf q[D / 32];
+    const int lo = uni(max(-1, first + row_token(r0, p)));
+    const int kv_end = uni(min(seq_end, max(0, first + row_token(min(r0 + kFewRows, rows) - 1, p) + 1)));
+    if (r0 > 0) f.fetch_pages(p, table, kv_first);
+    f.load_keys(p, hk, kv_first, kv_end, bad);
+    f.load_values(p, hk, kv_first, kv_end, bad);
+    f.fetch_pages(p, table, kv_first + kRound);
+    v8bf q[D / 32];  // B operands, in the order of the keys' dims
     {
       const uint16_t* a = p.q + (int64_t)(sq.row0 + tok) * p.ldq + head * D;
 #pragma unroll
@@ -621,110 +819,69 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void k_flash_few(FlashArgs p) {
     float m = kNegInf, l = 0.0f;
     lds8* const vs = (lds8*)&s.v[wv][0];
 
-    for (; kv < kv_end; kv += kFewPos * kFewWaves) {
+    for (int kv = kv_first; kv < kv_end; kv += kRound) {
       // scores: positions 16 t + 4 grp + i of query r16
-      v4f sc[2];
+      v4f sc[F::kRuns];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
+      for (int t = 0; t < F::kRuns; ++t) {
         sc[t] = (v4f){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < D / 32; ++k) {
-          uint4 a;
-          if (KV == kPagedFp8) {
-            const uint4 w = cur.k[t][k / 2];
-            a = from_e4m3(k & 1 ? make_uint2(w.z, w.w) : make_uint2(w.x, w.y), exp_scale(cur.ke[t]));
-          } else {
-            a = cur.k[t][k];
-          }
-          sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), q[k], sc[t], 0, 0, 0);
-        }
+        for (int k = 0; k < D / 32; ++k)
+          sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.key(t, k), q[k], sc[t], 0, 0, 0);
       }
-      // this round's value rows to LDS (pieces at piece ^ 2 row, for the transposing reads)
-      bool nf = false;
-      {
-        constexpr int TPR = R::kRowBytes / 16, RPL = 64 / TPR;
-#pragma unroll
-        for (int i = 0; i < R::kV; ++i) {
-          const int row = i * RPL + lane / TPR, c = lane % TPR;
-          if (KV == kPagedFp8) {
-            const float f = exp_scale(cur.ve[i]);
-            const uint4 a = from_e4m3(make_uint2(cur.v[i].x, cur.v[i].y), f);
-            const uint4 e = from_e4m3(make_uint2(cur.v[i].z, cur.v[i].w), f);
-            const int c0 = 2 * c ^ Tile<D>::v_swz(row);
-            lds_st128(vs + row * 2 * D + c0 * 16, a);
-            lds_st128(vs + row * 2 * D + (c0 ^ 1) * 16, e);
-            nf |= any_not_finite(a) | any_not_finite(e);
-          } else {
-            lds_st128(vs + row * 2 * D + (c ^ Tile<D>::v_swz(row)) * 16, cur.v[i]);
-            nf |= any_not_finite(cur.v[i]);
-          }
-        }
-      }
-      const int at = kv;
-      if (kv + kFewPos * kFewWaves < kv_end)
-        few_load<D, KV>(p, table, hk, kv + kFewPos * kFewWaves, kv_end, cur, bad);
+      f.load_keys(p, hk, kv + kRound, kv_end, bad);
 
       float mx = kNegInf;
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < F::kRuns; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          if (at + 16 * t + 4 * grp + i > limit) sc[t][i] = kNegInf;
+          if (kv + 16 * t + 4 * grp + i > limit) sc[t][i] = kNegInf;
           mx = fmaxf(mx, sc[t][i]);
         }
       mx = fmaxf(mx, xor_partner<16>(mx));
-      mx = fmaxf(mx, xor_partner<32>(mx));
-      if (__any(mx > m)) {
-        const float mn = fmaxf(m, mx);
-        const float a = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * p.c);
+      mx = fmaxf(mx, xor_partner<32>(mx)) * p.c;
+      if (__any(mx - m > kLazy)) {
+        const float mn = fmaxf(m, __builtin_ceilf(mx));
+        const float a = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
         m = mn;
         l *= a;
 #pragma unroll
         for (int t = 0; t < D / 16; ++t) o[t] *= a;
       }
-      const float mc = m == kNegInf ? 0.0f : -m * p.c;
-      uint32_t w[4];
+      const float mc = m == kNegInf ? 0.0f : -m;
+      uint32_t w[F::kRuns][2];
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < F::kRuns; ++t)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][2 * i], p.c, mc));
           const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][2 * i + 1], p.c, mc));
-          l += e0 + e1;
-          w[2 * t + i] = f2bf_pair(e0, e1);
+          w[t][i] = f2bf_pair(e0, e1);
+          l = sum_pair(w[t][i], l);
         }
-      const v8bf pb = __builtin_bit_cast(v8bf, make_uint4(w[0], w[1], w[2], w[3]));
-      __builtin_amdgcn_wave_barrier();  // the wave's LDS rows are read back by other lanes
-      if (at + kFewPos - 1 > lo && __any(nf)) {
-        for (int j = 0; j < kFewPos; ++j)
 #pragma unroll
-          for (int t = 0; t < D / 16; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int d = 16 * t + 4 * grp + i;
-              const uint16_t x = *(const __attribute__((address_space(3))) uint16_t*)(
-                  vs + j * 2 * D + ((d / 8) ^ Tile<D>::v_swz(j)) * 16 + (d % 8) * 2);
-              if ((x & 0x7f80u) == 0x7f80u && at + j <= limit) o[t][i] += bf2f(x);
-            }
-        __builtin_amdgcn_wave_barrier();
-        for (int i = lane; i < kFewPos * PC; i += 64) {
-          const uint4 x = lds_ld128(vs + i * 16);
-          lds_st128(vs + i * 16, make_uint4(drop_not_finite(x.x), drop_not_finite(x.y), drop_not_finite(x.z),
-                                            drop_not_finite(x.w)));
+      for (int t0 = 0; t0 < F::kRuns; t0 += 2) {
+        __builtin_amdgcn_wave_barrier();  // reads done before the rows are written again
+        f.store_values(vs, t0);
+        if (t0 + 2 == F::kRuns) {
+          f.load_values(p, hk, kv + kRound, kv_end, bad);
+          f.fetch_pages(p, table, kv + 2 * kRound);
         }
-        __builtin_amdgcn_wave_barrier();
-      }
-      // O^T += V^T P^T: dim 16 t + r16 of positions {4 grp .., 16 + 4 grp ..}
-      const int rr = r16 >> 2, qq = r16 & 3, row = 4 * grp + rr;
-      const lds8* const vb = vs + row * 2 * D + (qq & 1) * 8;
+        __builtin_amdgcn_wave_barrier();  // the wave's LDS rows are read back by other lanes
+        if (kv + 16 * t0 + 31 > lo) few_not_finite<D>(vs, o, kv + 16 * t0, limit);
+        const v8bf pb = __builtin_bit_cast(v8bf, make_uint4(w[t0][0], w[t0][1], w[t0 + 1][0], w[t0 + 1][1]));
+        // O^T += V^T P^T: dim 16 t + r16 of positions {4 grp .., 16 + 4 grp ..}
+        const int rr = r16 >> 2, qq = r16 & 3, row = 4 * grp + rr;
+        const lds8* const vb = vs + row * 2 * D + (qq & 1) * 8;
 #pragma unroll
-      for (int t = 0; t < D / 16; ++t) {
-        const lds8* a = vb + (((2 * t + (qq >> 1)) ^ Tile<D>::v_swz(row)) * 16);
-        const v4s x = lds_tr16(a), y = lds_tr16(a + 16 * 2 * D);
-        const v8bf va = __builtin_bit_cast(v8bf, (v8s){x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w});
-        o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pb, o[t], 0, 0, 0);
+        for (int t = 0; t < D / 16; ++t) {
+          const lds8* a = vb + (((2 * t + (qq >> 1)) ^ few_swz<D>(row)) * 16);
+          const v4s x = lds_tr16(a), y = lds_tr16(a + 16 * 2 * D);
+          const v8bf va = __builtin_bit_cast(v8bf, (v8s){x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w});
+          o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pb, o[t], 0, 0, 0);
+        }
       }
-      __builtin_amdgcn_wave_barrier();  // reads done before the rows are written again
     }
 
     // the waves' partials, in wave order
@@ -750,19 +907,23 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void k_flash_few(FlashArgs p) {
 #pragma unroll
       for (int w = 0; w < kFewWaves; ++w) {
         const float mw = s.ml[w][x][0], lw = s.ml[w][x][1];
+        const float4 ow = *reinterpret_cast<const float4*>(&s.o[w][x][d]);
         if (empty(mw, lw)) continue;
-        const float f = __builtin_amdgcn_exp2f((mw - M) * p.c);
-        L += f * lw;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) O[j] += f * s.o[w][x][d + j];
+        const float e = __builtin_amdgcn_exp2f(mw - M);
+        L += e * lw;
+        O[0] += e * ow.x;
+        O[1] += e * ow.y;
+        O[2] += e * ow.z;
+        O[3] += e * ow.w;
       }
       const int tk = row_token(r0 + x, p), hd = hk * p.G + r0 + x - tk * p.G;
       const int64_t row = sq.row0 + tk;
-      if (p.splits > 1) {
+      if (!whole) {
         const int64_t at = ((int64_t)split * p.bt.T + row) * p.H + hd;
         if (d == 0) p.part_ml[at] = make_float2(M, L);
         if (!empty(M, L)) *reinterpret_cast<float4*>(p.part_o + at * D + d) = make_float4(O[0], O[1], O[2], O[3]);
       } else {
+        if (p.splits > 1 && d == 0) p.part_ml[row * p.H + hd] = make_float2(0.0f, kWhole);
         const float inv = empty(M, L) ? 0.0f : 1.0f / L;
         *reinterpret_cast<uint2*>(p.out + row * p.ldo + hd * D + d) =
             make_uint2(f2bf_pair(O[0] * inv, O[1] * inv), f2bf_pair(O[2] * inv, O[3] * inv));
@@ -773,31 +934,54 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void k_flash_few(FlashArgs p) {
   if (bad) flag_error(p.error);
 }
 
-// The splits' partials of a row, in split order; D / 4 threads a row.
+// The splits' partials of a row, in an order that the number of splits fixes:
+// a group of D / 4 threads sums every `groups`-th split of a row, then the first of a
+// row's groups sums the groups.
 template <int D>
-__global__ __launch_bounds__(256) void k_flash_merge(FlashArgs p) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / (D / 4);  // row: (token, head)
-  const int d = 4 * (int)(i % (D / 4));
+__global__ __launch_bounds__(256) void k_flash_merge(FlashArgs p, int groups) {
+  constexpr int TG = D / 4, NG = 256 / TG;
+  __shared__ float4 s_o[NG][TG];
+  __shared__ float s_l[NG];
+  const int t = threadIdx.x % TG, g = threadIdx.x / TG, z0 = g % groups;
+  const int64_t n = (int64_t)p.bt.T * p.H, row = (int64_t)blockIdx.x * (NG / groups) + g / groups;  // (token, head)
   const int tok = (int)(row / p.H), head = (int)(row - (int64_t)tok * p.H);
-  if (tok < max(0, p.bt.cu[0]) || tok >= min(p.bt.T, p.bt.cu[p.bt.B])) return;
-  const int64_t n = (int64_t)p.bt.T * p.H;
-  float M = kNegInf;
-  for (int z = 0; z < p.splits; ++z) M = fmaxf(M, p.part_ml[z * n + row].x);
-  float L = 0.0f;
+  const bool live = tok >= max(0, p.bt.cu[0]) && tok < min(p.bt.T, p.bt.cu[p.bt.B]) && p.part_ml[row].y != kWhole;
+  float M = kNegInf, L = 0.0f;
   v4f O = (v4f){0.f, 0.f, 0.f, 0.f};
-  for (int z = 0; z < p.splits; ++z) {
-    const float2 ml = p.part_ml[z * n + row];
-    if (empty(ml.x, ml.y)) continue;
-    const float f = __builtin_amdgcn_exp2f((ml.x - M) * p.c);
-    const float4 o = *reinterpret_cast<const float4*>(p.part_o + (z * n + row) * D + d);
-    L += f * ml.y;
-    O[0] += f * o.x;
-    O[1] += f * o.y;
-    O[2] += f * o.z;
-    O[3] += f * o.w;
+  if (live) {
+    for (int z = t; z < p.splits; z += TG) M = fmaxf(M, p.part_ml[z * n + row].x);
+    if (TG == 32) M = fmaxf(M, xor_partner<16>(M));
+    M = fmaxf(M, xor_partner<8>(M));
+    M = fmaxf(M, xor_partner<4>(M));
+    M = fmaxf(M, xor_partner<2>(M));
+    M = fmaxf(M, xor_partner<1>(M));
+#pragma unroll 4
+    for (int z = z0; z < p.splits; z += groups) {
+      const float2 ml = p.part_ml[z * n + row];
+      if (empty(ml.x, ml.y)) continue;
+      const float f = __builtin_amdgcn_exp2f(ml.x - M);
+      const float4 o = *reinterpret_cast<const float4*>(p.part_o + (z * n + row) * D + 4 * t);
+      L += f * ml.y;
+      O[0] += f * o.x;
+      O[1] += f * o.y;
+      O[2] += f * o.z;
+      O[3] += f * o.w;
+    }
+  }
+  s_o[g][t] = make_float4(O[0], O[1], O[2], O[3]);
+  if (t == 0) s_l[g] = L;
+  __syncthreads();
+  if (!live || z0 != 0) return;
+  for (int i = 1; i < groups; ++i) {
+    const float4 o = s_o[g + i][t];
+    O[0] += o.x;
+    O[1] += o.y;
+    O[2] += o.z;
+    O[3] += o.w;
+    L += s_l[g + i];
   }
   const float inv = empty(M, L) ? 0.0f : 1.0f / L;
-  *reinterpret_cast<uint2*>(p.out + tok * p.ldo + head * D + d) =
+  *reinterpret_cast<uint2*>(p.out + tok * p.ldo + head * D + 4 * t) =
       make_uint2(f2bf_pair(O[0] * inv, O[1] * inv), f2bf_pair(O[2] * inv, O[3] * inv));
 }
 
@@ -821,8 +1005,9 @@ inline FlashPlan flash_plan(int64_t T, int64_t H, int64_t Hkv, int64_t B, int64_
   f.splits = 1;
   f.chunk = round_up(max_kv > 0 ? max_kv : 1, 256);
   const int64_t slots = (int64_t)device_cus() * (f.few ? 1 : 2);
-  if (paged && 2 * f.tiles <= slots && max_kv > kMinChunk) {
-    int64_t n = slots / f.tiles;
+  const char* e = getenv("BTL_X_SPLITS");
+  if (paged && max_kv > kMinChunk) {
+    int64_t n = e ? atoi(e) : slots / f.tiles;
     if (n > max_kv / kMinChunk) n = max_kv / kMinChunk;
     if (n > kMaxSplits) n = kMaxSplits;
     if (n > 1) {
@@ -885,6 +1070,8 @@ int btl_prompt_attention(const uint16_t* q, int64_t ldq, const uint16_t* k, int6
   if (T == 0) return BTL_OK;
   if (!k || !v) return set_error(BTL_ERR_NULL, "%s: NULL pointer", who);
   if (ldk < Hkv * D || ldv < Hkv * D) return set_error(BTL_ERR_SHAPE, "%s: row stride smaller than a row", who);
+  if (ldk > (1 << 24) || ldv > (1 << 24))  // a step's rows within a 32-bit range
+    return set_error(BTL_ERR_SHAPE, "%s: row stride over %d elements", who, 1 << 24);
   if (!aligned(k, 16) || !aligned(v, 16) || ldk % 8 || ldv % 8)
     return set_error(BTL_ERR_ALIGN, "%s: misaligned buffer or row stride", who);
   a.k = k;
@@ -954,11 +1141,15 @@ int btl_paged_attention(const uint16_t* q, int64_t ldq, int64_t T, int64_t H, co
   if (f.splits > 1) {
     rc = check_launch("paged attention");
     if (rc != BTL_OK) return rc;
-    const dim3 grid((unsigned)((T * H * (D / 4) + 255) / 256));
+    // up to four splits for a group of threads
+    const int ng = D == 128 ? 8 : 16;
+    int groups = 1;
+    while (groups < ng && 4 * groups < f.splits) groups *= 2;
+    const dim3 grid((unsigned)((T * H * groups + ng - 1) / ng));
     if (D == 128)
-      hipLaunchKernelGGL(k_flash_merge<128>, grid, dim3(256), 0, (hipStream_t)stream, a);
+      hipLaunchKernelGGL(k_flash_merge<128>, grid, dim3(256), 0, (hipStream_t)stream, a, groups);
     else
-      hipLaunchKernelGGL(k_flash_merge<64>, grid, dim3(256), 0, (hipStream_t)stream, a);
+      hipLaunchKernelGGL(k_flash_merge<64>, grid, dim3(256), 0, (hipStream_t)stream, a, groups);
   }
   return check_launch("paged attention");
 }

@@ -100,8 +100,12 @@ __device__ __forceinline__ int32_t scalar_load(const int32_t* p, uint32_t i) {
 }
 
 __device__ __forceinline__ Seq load_seq(const Batch& bt, int b, int64_t cap) {
-  const int lo = bt.cu[b], hi = bt.cu[b + 1];
-  return clamp_seq(lo, hi, bt.len ? bt.len[b] : hi - lo, bt.T, bt.len ? cap : bt.T);
+  const int lo = scalar_load(bt.cu, b), hi = scalar_load(bt.cu, b + 1);
+  Seq s = clamp_seq(lo, hi, bt.len ? scalar_load(bt.len, b) : hi - lo, bt.T, bt.len ? cap : bt.T);
+  s.row0 = uni(s.row0);
+  s.n = uni(s.n);
+  s.len = uni(s.len);
+  return s;
 }
 
 // Item x of the sequences' items, sequence b having ceil(n_b * per / of): the
@@ -127,9 +131,9 @@ __device__ __forceinline__ bool find_item(const Batch& bt, int per, int of, int 
     const int total = __builtin_amdgcn_readlane(inc, 63);
     if (x < base + total) {
       const int l = __builtin_ctzll(__ballot(base + inc > x));
-      it.b = c + l;
+      it.b = uni(c + l);
       it.count = __builtin_amdgcn_readlane(cnt, l);
-      it.i = x - base - (__builtin_amdgcn_readlane(inc, l) - it.count);
+      it.i = uni(x - base - (__builtin_amdgcn_readlane(inc, l) - it.count));
       return true;
     }
     base += total;
