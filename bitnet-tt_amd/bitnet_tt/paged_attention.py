@@ -30,6 +30,7 @@ from . import _native as N
 
 _BF16 = torch.bfloat16
 _ERROR_BYTES = 256
+_ERROR_KIND = "paged"
 
 
 class PagedKVCache:
@@ -37,35 +38,43 @@ class PagedKVCache:
     kv_heads, page_size, head_dim] bf16, or float8_e4m3fn with one exponent byte
     per row in ``key_exp`` and ``value_exp`` [num_pages, kv_heads, page_size]
     uint8 (a value is code x 2^(byte - 127)).  page_size is a multiple of 16;
-    head_dim 64 or 128.  The contiguous caches of DecodeAttention are pages
-    of max_seq_len rows: :meth:`of_cache`."""
+    head_dim 64 or 128.  The pools are written in place, never replaced.  The
+    contiguous caches of DecodeAttention are pages of max_seq_len rows: :meth:`of_cache`."""
+
+    __slots__ = ("_tensors", "_pages", "shape", "index")
 
     def __init__(self, key_pages, value_pages, key_exp=None, value_exp=None) -> None:
-        fp8 = key_exp is not None
-        if key_pages.dim() != 4 or key_pages.shape != value_pages.shape:
+        shape = key_pages.shape
+        if len(shape) != 4 or value_pages.shape != shape:
             raise ValueError("key_pages and value_pages must be [num_pages, kv_heads, page_size, head_dim], alike")
+        P, H, S, D = shape
+        fp8 = key_exp is not None
         if (value_exp is not None) != fp8:
             raise ValueError("key_exp and value_exp come together")
         dtype = torch.float8_e4m3fn if fp8 else _BF16
-        if key_pages.dtype != dtype or value_pages.dtype != dtype:
+        if key_pages.dtype is not dtype or value_pages.dtype is not dtype:
             raise ValueError(f"pages must be {dtype} {'with' if fp8 else 'without'} exponent bytes")
-        P, H, S, D = key_pages.shape
         if S < 16 or S % 16:
             raise ValueError(f"page_size {S} is not a multiple of 16")
-        if D not in (64, 128):
+        if D != 128 and D != 64:
             raise ValueError(f"head_dim {D}: 64 and 128 are supported")
         N.require_cuda(key_pages, "key_pages")
         N.require_cuda(value_pages, "value_pages")
+        index = key_pages.get_device()
         if fp8:
             for t, name in ((key_exp, "key_exp"), (value_exp, "value_exp")):
                 N.require_cuda(t, name)
-                if t.dtype != torch.uint8 or t.shape != (P, H, S):
+                if t.dtype is not torch.uint8 or t.shape != shape[:3]:
                     raise ValueError(f"{name} must be uint8 [num_pages, kv_heads, page_size]")
-        for t in (value_pages, key_exp, value_exp):
-            if t is not None and t.device != key_pages.device:
-                raise ValueError("the pools are on different devices")
-        self.key_pages, self.value_pages = key_pages, value_pages
-        self.key_exp, self.value_exp = key_exp, value_exp
+                if t.get_device() != index:
+                    raise ValueError("the pools are on different devices")
+        if value_pages.get_device() != index:
+            raise ValueError("the pools are on different devices")
+        self._tensors = (key_pages, value_pages, key_exp, value_exp)
+        self._pages = N.Pages(key_pages.data_ptr(), value_pages.data_ptr(), key_exp.data_ptr() if fp8 else None,
+                              value_exp.data_ptr() if fp8 else None, P, H, S, D)
+        self.shape = shape
+        self.index = index
 
     @classmethod
     def allocate(cls, num_pages: int, num_kv_heads: int, head_dim: int, device, page_size: int = 64,
@@ -85,98 +94,77 @@ class PagedKVCache:
         sequence b's, so its page table is arange(batch)[:, None]."""
         return cls(kv_cache.key_cache, kv_cache.value_cache)
 
-    @property
-    def num_pages(self) -> int:
-        return self.key_pages.shape[0]
-
-    @property
-    def num_kv_heads(self) -> int:
-        return self.key_pages.shape[1]
-
-    @property
-    def page_size(self) -> int:
-        return self.key_pages.shape[2]
-
-    @property
-    def head_dim(self) -> int:
-        return self.key_pages.shape[3]
-
-    @property
-    def device(self):
-        return self.key_pages.device
-
-    def _struct(self) -> N.Pages:
-        P, H, S, D = self.key_pages.shape
-        fp8 = self.key_exp is not None
-        return N.Pages(self.key_pages.data_ptr(), self.value_pages.data_ptr(),
-                       self.key_exp.data_ptr() if fp8 else None, self.value_exp.data_ptr() if fp8 else None, P, H, S, D)
+    key_pages = property(lambda self: self._tensors[0])
+    value_pages = property(lambda self: self._tensors[1])
+    key_exp = property(lambda self: self._tensors[2])
+    value_exp = property(lambda self: self._tensors[3])
+    num_pages = property(lambda self: self.shape[0])
+    num_kv_heads = property(lambda self: self.shape[1])
+    page_size = property(lambda self: self.shape[2])
+    head_dim = property(lambda self: self.shape[3])
+    device = property(lambda self: self._tensors[0].device)
 
 
-def _on(t, device, name):
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, the call's tensors on {device}")
-
-
-def _int32(t, device, shape, name):
-    if t.dtype != torch.int32 or not t.is_contiguous() or tuple(t.shape) != shape:
+def _int32(t, index, shape, name):
+    if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor {list(shape)}")
-    _on(t, device, name)
+    if t.get_device() != index:
+        raise ValueError(f"{name} is on {t.device}, the call's tensors on cuda:{index}")
 
 
-def _batch(cu_q, kv_len, page_table, device):
-    """(B, max_pages) after checks of the host-visible side."""
-    B = cu_q.shape[0] - 1 if cu_q.dim() == 1 else -1
-    if B < 1:
+def _sequences(cu_q, index):
+    """B, of cu_q [B + 1]."""
+    shape = cu_q.shape
+    if len(shape) != 1 or shape[0] < 2:
         raise ValueError("cu_q must be int32 [B + 1] of at least one sequence")
-    _int32(cu_q, device, (B + 1,), "cu_q")
-    if kv_len is not None:
-        _int32(kv_len, device, (B,), "kv_len")
-    if page_table is None:
-        return B, 0
-    if page_table.dim() != 2 or page_table.shape[1] < 1:
-        raise ValueError("page_table must be int32 [B, max_pages]")
-    _int32(page_table, device, (B, page_table.shape[1]), "page_table")
-    return B, page_table.shape[1]
+    _int32(cu_q, index, shape, "cu_q")
+    return shape[0] - 1
 
 
-def _rows(t, heads, dim, name, device=None):
+def _table(page_table, index, B):
+    """max_pages, of page_table [B, max_pages]."""
+    shape = page_table.shape
+    if len(shape) != 2 or shape[0] != B or shape[1] < 1:
+        raise ValueError(f"page_table must be int32 [{B}, max_pages]")
+    _int32(page_table, index, shape, "page_table")
+    return shape[1]
+
+
+def _rows(t, T, heads, dim, name, index):
     """Row stride of a packed bf16 tensor [T, heads, dim] whose rows are dense."""
-    if not t.is_cuda:
-        raise ValueError(f"{name} must be a tensor on a ROCm GPU device; this path runs only through the gfx950 kernels")
-    if t.dtype != _BF16 or t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim:
-        raise ValueError(f"{name} must be bf16 [T, {heads}, {dim}]")
-    if device is not None:
-        _on(t, device, name)
-    st = t.stride()
-    if st[2] != 1 or (st[1] != dim and heads > 1):
+    shape = t.shape
+    if t.dtype is not _BF16 or len(shape) != 3 or shape[0] != T or shape[1] != heads or shape[2] != dim:
+        raise ValueError(f"{name} must be bf16 [{T}, {heads}, {dim}]")
+    if t.get_device() != index:
+        raise ValueError(f"{name} is on {t.device}, the call's tensors on cuda:{index}")
+    ld, sh, sd = t.stride()
+    if sd != 1 or (sh != dim and heads > 1):
         raise ValueError(f"{name}: the heads of a row must be dense")
-    ld = st[0] if t.shape[0] > 1 else max(st[0], heads * dim)
+    if T <= 1 and ld < heads * dim:
+        ld = heads * dim
     if ld < heads * dim or ld % 8 or t.data_ptr() % 16:
         raise ValueError(f"{name}: rows must be 16-byte aligned and not overlap")
     return ld
 
 
-def _error_word(device, stream):
-    if not N.has_workspace(device, _ERROR_BYTES, "paged") and torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("run one eager call on this stream before capturing it in a graph")
-    return N.workspace_ptr(device.index, _ERROR_BYTES, "paged", 0, stream)[0]
+def _gpu(t, name):
+    index = t.get_device()
+    if index < 0:
+        raise ValueError(f"{name} must be a tensor on a ROCm GPU device; this path runs only through the gfx950 kernels")
+    return index
 
 
-def _on_device(fn):
-    """Runs fn with its first argument's device current: a launch belongs there."""
-
-    @functools.wraps(fn)
-    def call(first, *args, **kwargs):
-        index = first.device.index
-        if not torch.cuda.is_available() or index is None or index == torch.cuda.current_device():
-            return fn(first, *args, **kwargs)
-        with torch.cuda.device(index):
-            return fn(first, *args, **kwargs)
-
-    return call
+def _error_word(index, stream):
+    """Address of the stream's error word."""
+    hit = N._fast.get((_ERROR_KIND, index, stream, 0, 0))
+    if hit is None:
+        device = torch.device("cuda", index)
+        if not N.has_workspace(device, _ERROR_BYTES, _ERROR_KIND) and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("run one eager call on this stream before capturing it in a graph")
+        hit = N.workspace_ptr(index, _ERROR_BYTES, _ERROR_KIND, 0, stream)
+    return hit[0]
 
 
-@_on_device
 def rope_write(qkv, rope_cos, rope_sin, cu_q, kv_len, num_heads: int, num_kv_heads: int, cache: PagedKVCache | None = None,
                page_table=None, rope_adjacent: bool = False, q_out=None, k_out=None):
     """Rotates the q and k heads of fused QKV rows and writes k and v to their pages.
@@ -184,158 +172,174 @@ def rope_write(qkv, rope_cos, rope_sin, cu_q, kv_len, num_heads: int, num_kv_hea
     qkv: bf16 [T, (H + 2 Hkv) D].  rope_cos / rope_sin: fp32 [S, R / 2], the
     angles of the first R dims of a head (pairs (i, i + R/2), or (2i, 2i+1) with
     ``rope_adjacent``); see utils.rope.rope_tables.  kv_len None: whole prompts,
-    positions from 0.  Without ``cache`` nothing but q (and k_out) is written.  An 8-bit
-    row keeps the least exponent e with max|x| <= 448 * 2^e and is rounded once,
-    from the fp32 rotation; a row with a value that is not finite reads back as NaN.  Returns q [T, H, D] (``q_out``, which may
-    be the q part of qkv itself, as ``k_out`` [T, Hkv, D] may be its k part)."""
+    positions from 0.  Without ``cache`` nothing but q (and k_out) is written.  An
+    8-bit row keeps the least exponent e with max|x| <= 448 * 2^e and is rounded
+    once, from the fp32 rotation; a row with a value that is not finite reads
+    back as NaN.  Returns q [T, H, D] (``q_out``, which may be the q part of qkv
+    itself, as ``k_out`` [T, Hkv, D] may be its k part)."""
+    index = _gpu(qkv, "qkv")
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return rope_write(qkv, rope_cos, rope_sin, cu_q, kv_len, num_heads, num_kv_heads, cache, page_table,
+                              rope_adjacent, q_out, k_out)
     H, Hkv = int(num_heads), int(num_kv_heads)
-    N.require_cuda(qkv, "qkv")
-    if qkv.dtype != _BF16 or qkv.dim() != 2 or H < 1 or Hkv < 1 or qkv.shape[1] % (H + 2 * Hkv):
-        raise ValueError(f"qkv must be bf16 [T, ({H} + 2 * {Hkv}) * head_dim]")
-    T, D = qkv.shape[0], qkv.shape[1] // (H + 2 * Hkv)
-    dev = qkv.device
+    shape, heads = qkv.shape, H + 2 * Hkv
+    if qkv.dtype is not _BF16 or len(shape) != 2 or H < 1 or Hkv < 1 or shape[1] % heads or not qkv.is_contiguous():
+        raise ValueError(f"qkv must be contiguous bf16 [T, ({H} + 2 * {Hkv}) * head_dim]")
+    T, D = shape[0], shape[1] // heads
+    angles = rope_cos.shape
     for t, name in ((rope_cos, "rope_cos"), (rope_sin, "rope_sin")):
-        if t.dtype != torch.float32 or t.dim() != 2 or not t.is_contiguous() or t.shape != rope_cos.shape:
+        if t.dtype is not torch.float32 or len(angles) != 2 or t.shape != angles or not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous fp32 [positions, rotated dims / 2]")
-        _on(t, dev, name)
-    B, max_pages = _batch(cu_q, kv_len, page_table if cache is not None else None, dev)
+        if t.get_device() != index:
+            raise ValueError(f"{name} is on {t.device}, qkv on {qkv.device}")
+    B = _sequences(cu_q, index)
+    if kv_len is not None:
+        _int32(kv_len, index, (B,), "kv_len")
+    pages = table = None
+    max_pages = 0
     if cache is not None:
         if page_table is None:
             raise ValueError("a cache needs a page table")
-        if cache.num_kv_heads != Hkv or cache.head_dim != D:
-            raise ValueError(f"cache of {cache.num_kv_heads} heads of {cache.head_dim}, rows of {Hkv} of {D}")
-        _on(cache.key_pages, dev, "cache")
+        if cache.shape[1] != Hkv or cache.shape[3] != D:
+            raise ValueError(f"cache of {cache.shape[1]} heads of {cache.shape[3]}, rows of {Hkv} of {D}")
+        if cache.index != index:
+            raise ValueError(f"cache is on cuda:{cache.index}, qkv on {qkv.device}")
+        max_pages = _table(page_table, index, B)
+        pages, table = cache._pages, page_table.data_ptr()
     if q_out is None:
-        q_out = torch.empty((T, H, D), dtype=_BF16, device=dev)
-    elif q_out.shape[0] != T:
-        raise ValueError(f"q_out must have {T} rows")
-    ldq = _rows(q_out, H, D, "q_out", dev)
-    ldk = 0
-    if k_out is not None:
-        if k_out.shape[0] != T:
-            raise ValueError(f"k_out must have {T} rows")
-        ldk = _rows(k_out, Hkv, D, "k_out", dev)
-    stream = N.raw_stream(dev.index)
+        q_out = torch.empty((T, H, D), dtype=_BF16, device=qkv.device)
+        ldq = H * D
+    else:
+        ldq = _rows(q_out, T, H, D, "q_out", index)
+    ldk = 0 if k_out is None else _rows(k_out, T, Hkv, D, "k_out", index)
+    stream = N.raw_stream(index)
     rc = N.lib().btl_rope_write(
-        qkv.data_ptr(), T, (H + 2 * Hkv) * D, H, Hkv, D, rope_cos.data_ptr(), rope_sin.data_ptr(),
-        2 * rope_cos.shape[1], rope_cos.shape[0], int(bool(rope_adjacent)), cu_q.data_ptr(),
-        None if kv_len is None else kv_len.data_ptr(), B, q_out.data_ptr(), ldq,
-        None if k_out is None else k_out.data_ptr(), ldk, None if cache is None else cache._struct(),
-        None if cache is None else page_table.data_ptr(), max_pages, _error_word(dev, stream), stream)
+        qkv.data_ptr(), T, heads * D, H, Hkv, D, rope_cos.data_ptr(), rope_sin.data_ptr(), 2 * angles[1], angles[0],
+        1 if rope_adjacent else 0, cu_q.data_ptr(), None if kv_len is None else kv_len.data_ptr(), B, q_out.data_ptr(),
+        ldq, None if k_out is None else k_out.data_ptr(), ldk, pages, table, max_pages, _error_word(index, stream),
+        stream)
     if rc != N.BTL_OK:
         N.check(rc, "btl_rope_write")
     return q_out
 
 
-@_on_device
 def read_pages(cache: PagedKVCache, page_table, kv_len, key_cache, value_cache) -> None:
     """Copies rows [0, kv_len[b]) of every sequence from its pages into the
     contiguous bf16 caches [B, Hkv, S, D] (those of layers.attention.KVCache, which
     the decode steps read); the rows behind stay as they were."""
-    dev = cache.device
-    if page_table.dim() != 2 or page_table.shape[0] < 1 or page_table.shape[1] < 1:
-        raise ValueError("page_table must be int32 [B, max_pages]")
-    B, max_pages = page_table.shape
-    _int32(page_table, dev, (B, max_pages), "page_table")
-    _int32(kv_len, dev, (B,), "kv_len")
+    index = cache.index
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return read_pages(cache, page_table, kv_len, key_cache, value_cache)
+    B = page_table.shape[0]
+    if B < 1:
+        raise ValueError("page_table must be int32 [B, max_pages] of at least one sequence")
+    max_pages = _table(page_table, index, B)
+    _int32(kv_len, index, (B,), "kv_len")
+    shape, (_, Hkv, _, D) = key_cache.shape, cache.shape
     for t, name in ((key_cache, "key_cache"), (value_cache, "value_cache")):
-        N.require_cuda(t, name)
-        _on(t, dev, name)
-        if (t.dtype != _BF16 or t.dim() != 4 or t.shape[:2] != (B, cache.num_kv_heads) or t.shape[3] != cache.head_dim
-                or t.shape != key_cache.shape):
-            raise ValueError(f"{name} must be bf16 [{B}, {cache.num_kv_heads}, positions, {cache.head_dim}]")
-    stream = N.raw_stream(dev.index)
-    rc = N.lib().btl_read_pages(cache._struct(), page_table.data_ptr(), B, max_pages, kv_len.data_ptr(),
-                                key_cache.shape[2], key_cache.data_ptr(), value_cache.data_ptr(),
-                                _error_word(dev, stream), stream)
+        if (t.dtype is not _BF16 or len(shape) != 4 or t.shape != shape or shape[0] != B or shape[1] != Hkv
+                or shape[3] != D or not t.is_contiguous()):
+            raise ValueError(f"{name} must be contiguous bf16 [{B}, {Hkv}, positions, {D}]")
+        if t.get_device() != index:
+            raise ValueError(f"{name} is on {t.device}, the pages on cuda:{index}")
+    stream = N.raw_stream(index)
+    rc = N.lib().btl_read_pages(cache._pages, page_table.data_ptr(), B, max_pages, kv_len.data_ptr(), shape[2],
+                                key_cache.data_ptr(), value_cache.data_ptr(), _error_word(index, stream), stream)
     if rc != N.BTL_OK:
         N.check(rc, "btl_read_pages")
 
 
-def _scale(scale, D):
-    return 1.0 / math.sqrt(D) if scale is None else float(scale)
-
-
-@_on_device
 def prompt_attention(q, k, v, cu_seqlens, scale: float | None = None, max_q: int | None = None, out=None):
     """Causal attention within packed sequences: row i attends to the rows up to
     itself of its own sequence, query head h to key-value head h // (H / Hkv).
 
     q bf16 [T, H, D], k and v [T, Hkv, D] (parts of a QKV row will do: rows may
-    be strided); cu_seqlens int32 [B + 1]; scale defaults to 1/sqrt(D); max_q, where known, is the longest
-    sequence (a hint).  Returns bf16 [T, H, D] (``out``, which must not overlap the inputs)."""
-    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3 or k.shape[0] != q.shape[0] or v.shape != k.shape:
+    be strided); cu_seqlens int32 [B + 1]; scale, positive, defaults to 1/sqrt(D); max_q,
+    where known, is the longest sequence (a hint).  Returns bf16 [T, H, D]
+    (``out``, which must not overlap the inputs)."""
+    index = _gpu(q, "q")
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return prompt_attention(q, k, v, cu_seqlens, scale, max_q, out)
+    if q.dim() != 3 or k.dim() != 3:
         raise ValueError("q must be [T, H, D], k and v [T, Hkv, D]")
     T, H, D = q.shape
     Hkv = k.shape[1]
-    if Hkv < 1 or H % Hkv:
+    if Hkv < 1 or H < 1 or H % Hkv:
         raise ValueError(f"{H} query heads over {Hkv} key-value heads")
-    ldq = _rows(q, H, D, "q")
-    dev = q.device
-    ldk, ldv = _rows(k, Hkv, D, "k", dev), _rows(v, Hkv, D, "v", dev)
-    B, _ = _batch(cu_seqlens, None, None, dev)
+    ldq = _rows(q, T, H, D, "q", index)
+    ldk, ldv = _rows(k, T, Hkv, D, "k", index), _rows(v, T, Hkv, D, "v", index)
+    B = _sequences(cu_seqlens, index)
     if out is None:
-        out = torch.empty((T, H, D), dtype=_BF16, device=dev)
-    elif out.shape[0] != T:
-        raise ValueError(f"out must have {T} rows")
-    ldo = _rows(out, H, D, "out", dev)
-    stream = N.raw_stream(dev.index)
+        out = torch.empty((T, H, D), dtype=_BF16, device=q.device)
+        ldo = H * D
+    else:
+        ldo = _rows(out, T, H, D, "out", index)
+    stream = N.raw_stream(index)
     rc = N.lib().btl_prompt_attention(
         q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, T, H, Hkv, D, cu_seqlens.data_ptr(), B,
-        _scale(scale, D), T if max_q is None else int(max_q), out.data_ptr(), ldo, _error_word(dev, stream), stream)
+        1.0 / math.sqrt(D) if scale is None else scale, T if max_q is None else max_q, out.data_ptr(), ldo,
+        _error_word(index, stream), stream)
     if rc != N.BTL_OK:
         N.check(rc, "btl_prompt_attention")
     return out
 
 
-@_on_device
 def paged_attention(q, cache: PagedKVCache, page_table, cu_q, kv_len, scale: float | None = None,
                     max_q: int | None = None, max_kv: int | None = None, out=None):
     """Attention of each sequence's newest tokens over its pages: the row at
     position p attends to positions [0, p], which have been written before.
 
     q bf16 [T, H, D], rotated.  max_q and max_kv, where known, are the most new
-    tokens and the longest kv_len of any sequence: they choose the kernel and how a long
-    context is split over workgroups, and a wrong one costs time only.  Single-token
-    steps should pass max_q=1.  Returns bf16 [T, H, D] (``out``, not overlapping q)."""
+    tokens and the longest kv_len of any sequence: they choose the kernel and how
+    a long context is split over workgroups, and a wrong one costs time only.
+    Single-token steps should pass max_q=1.  Returns bf16 [T, H, D] (``out``,
+    which must not overlap q)."""
+    index = cache.index
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return paged_attention(q, cache, page_table, cu_q, kv_len, scale, max_q, max_kv, out)
     if q.dim() != 3:
         raise ValueError("q must be [T, H, D]")
     T, H, D = q.shape
-    ldq = _rows(q, H, cache.head_dim, "q", cache.device)
-    if H % cache.num_kv_heads:
-        raise ValueError(f"{H} query heads over {cache.num_kv_heads} key-value heads")
-    dev = q.device
-    if page_table is None or kv_len is None:
-        raise ValueError("paged attention needs a page table and kv_len")
-    B, max_pages = _batch(cu_q, kv_len, page_table, dev)
-    cap = max_pages * cache.page_size
-    mq = T if max_q is None else min(int(max_q), T)
-    mkv = cap if max_kv is None else min(int(max_kv), cap)
+    _, Hkv, page_size, dim = cache.shape
+    ldq = _rows(q, T, H, dim, "q", index)
+    if H < 1 or H % Hkv:
+        raise ValueError(f"{H} query heads over {Hkv} key-value heads")
+    B = _sequences(cu_q, index)
+    _int32(kv_len, index, (B,), "kv_len")
+    max_pages = _table(page_table, index, B)
+    most = max_pages * page_size
+    max_q = T if max_q is None or max_q > T else max_q
+    max_kv = most if max_kv is None or max_kv > most else max_kv
     if out is None:
-        out = torch.empty((T, H, D), dtype=_BF16, device=dev)
-    elif out.shape[0] != T:
-        raise ValueError(f"out must have {T} rows")
-    ldo = _rows(out, H, D, "out", dev)
+        out = torch.empty((T, H, D), dtype=_BF16, device=q.device)
+        ldo = H * D
+    else:
+        ldo = _rows(out, T, H, D, "out", index)
     if T == 0:
         return out
-    if mq < 1 or mkv < 1:
+    if max_q < 1 or max_kv < 1:
         raise ValueError(f"max_q {max_q} and max_kv {max_kv} must be at least 1")
-    stream = N.raw_stream(dev.index)
-    nbytes = _scratch_bytes(dev.index, T, H, cache.num_kv_heads, D, B, mq, mkv)
+    stream = N.raw_stream(index)
+    nbytes = _scratch_bytes(index, T, H, Hkv, D, B, max_q, max_kv, cache._tensors[2] is not None)
     # the call's own, from the stream-ordered allocator: calls that overlap share nothing
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
     rc = N.lib().btl_paged_attention(
-        q.data_ptr(), ldq, T, H, cache._struct(), page_table.data_ptr(), max_pages, cu_q.data_ptr(), kv_len.data_ptr(),
-        B, _scale(scale, D), mq, mkv, out.data_ptr(), ldo, None if scratch is None else scratch.data_ptr(), nbytes,
-        _error_word(dev, stream), stream)
+        q.data_ptr(), ldq, T, H, cache._pages, page_table.data_ptr(), max_pages, cu_q.data_ptr(), kv_len.data_ptr(), B,
+        1.0 / math.sqrt(D) if scale is None else scale, max_q, max_kv, out.data_ptr(), ldo,
+        None if scratch is None else scratch.data_ptr(), nbytes, _error_word(index, stream), stream)
     if rc != N.BTL_OK:
         N.check(rc, "btl_paged_attention")
     return out
 
 
 @functools.lru_cache(maxsize=4096)
-def _scratch_bytes(index: int, T: int, H: int, Hkv: int, D: int, B: int, max_q: int, max_kv: int) -> int:
-    return int(N.lib().btl_paged_attention_scratch_bytes(T, H, Hkv, D, B, max_q, max_kv))
+def _scratch_bytes(index: int, T: int, H: int, Hkv: int, D: int, B: int, max_q: int, max_kv: int,
+                   fp8: bool = False) -> int:
+    return int(N.lib().btl_paged_attention_scratch_bytes(T, H, Hkv, D, B, max_q, max_kv, int(fp8)))
 
 
 def check(device=None) -> None:

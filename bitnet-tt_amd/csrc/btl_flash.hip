@@ -33,7 +33,6 @@
 #include "btl_common.h"
 #include "btl_fp8.h"
 #include "btl_paged.h"
-#include <stdlib.h>
 
 namespace btl {
 
@@ -645,7 +644,7 @@ __global__ __launch_bounds__(256, 2) void k_flash_tile(FlashArgs p) {
 // fetched a round ahead of that.  The waves' partials meet in LDS.
 // ======================================================================
 constexpr int kFewRows = 16;
-constexpr int kFewWaves = 8;
+constexpr int kFewWaves = 4;
 
 // Pieces of a value row in LDS are at piece ^ few_swz(row): the 8 rows x 32 bytes
 // that 32 lanes of a transposing read cover are in different banks.
@@ -666,7 +665,7 @@ struct FewShared {
 template <int D, int KV>
 struct Few {
   static constexpr int kRowBytes = KV == kPagedFp8 ? D : 2 * D;
-  static constexpr int kRuns = KV == kPagedFp8 ? 4 : 2;     // runs of 16 positions of a wave and round
+  static constexpr int kRuns = 2;                           // runs of 16 positions of a wave and round
   static constexpr int kPos = 16 * kRuns;
   static constexpr int kK = kRowBytes / 64;                 // key loads of a lane for a run
   static constexpr int kV = kRowBytes / 64;                 // value loads of a lane for a run
@@ -675,47 +674,54 @@ struct Few {
   uint4 v[kRuns][kV];
   uint32_t ke[kRuns], ve[kRuns][kV];
   int32_t page[kRuns];  // of the round to be loaded next
+  bool one;             // pages of whole rounds
 
   // Page table entries of the round from position kv (any up to the table's end).
   __device__ __forceinline__ void fetch_pages(const FlashArgs& p, const int32_t* table, int kv) {
 #pragma unroll
     for (int t = 0; t < kRuns; ++t)
-      page[t] = scalar_load(table, min(div_by(kv + 16 * t, p.pg.ps), (uint32_t)p.bt.max_pages - 1));
+      if (t == 0 || !one)
+        page[t] = scalar_load(table, min(div_by(kv + 16 * t, p.pg.ps), (uint32_t)p.bt.max_pages - 1));
   }
-  // First page row of run t, and how many of its rows are there (0: none, or no page).
-  __device__ __forceinline__ int64_t run(const FlashArgs& p, int hk, int kv, int kv_end, int t, uint32_t& n,
-                                         bool& bad) const {
-    const int at = kv + 16 * t;
-    n = (uint32_t)clampi(kv_end - at, 0, 16);
-    const bool none = (uint32_t)page[t] >= (uint32_t)p.pg.P;
+  // Page row of position `at`, and how many of up to `most` rows from there there are.
+  __device__ __forceinline__ int64_t rows_at(const FlashArgs& p, int hk, int at, int kv_end, int32_t pg, int most,
+                                             uint32_t& n, bool& bad) const {
+    n = (uint32_t)clampi(kv_end - at, 0, most);
+    const bool none = (uint32_t)pg >= (uint32_t)p.pg.P;
     bad |= none & (n > 0);
     n = none ? 0 : n;
-    return page_row(none ? 0 : page[t], p.pg.P, p.pg.Hkv, hk, p.pg.ps.d, at - (int)div_by(at, p.pg.ps) * (int)p.pg.ps.d);
+    return page_row(none ? 0 : pg, p.pg.P, p.pg.Hkv, hk, p.pg.ps.d, at - (int)div_by(at, p.pg.ps) * (int)p.pg.ps.d);
   }
-  __device__ __forceinline__ void load_keys(const FlashArgs& p, int hk, int kv, int kv_end, bool& bad) {
-    const int lane = __lane_id(), row = lane & 15;
+  // Run t's keys, from row `from` of n page rows at `row`.
+  __device__ __forceinline__ void run_keys(const FlashArgs& p, int t, int64_t row, uint32_t n, int from) {
+    const int lane = __lane_id(), r = from + (lane & 15);
+    const auto rs = buf_rsrc(p.pg.k + row * kRowBytes, n * kRowBytes);
 #pragma unroll
-    for (int t = 0; t < kRuns; ++t) {
-      uint32_t n;
-      const int64_t r = run(p, hk, kv, kv_end, t, n, bad);
-      const auto rs = buf_rsrc(p.pg.k + r * kRowBytes, n * kRowBytes);
+    for (int i = 0; i < kK; ++i) k[t][i] = buf_ld128(rs, r * kRowBytes + 64 * i + 16 * (lane >> 4));
+    if (KV == kPagedFp8) ke[t] = buf_ld8(buf_rsrc(p.pg.ke + row, n), r);
+  }
+  __device__ __forceinline__ void run_values(const FlashArgs& p, int t, int64_t row, uint32_t n, int from) {
+    const int lane = __lane_id();
+    const auto rs = buf_rsrc(p.pg.v + row * kRowBytes, n * kRowBytes);
 #pragma unroll
-      for (int i = 0; i < kK; ++i) k[t][i] = buf_ld128(rs, row * kRowBytes + 64 * i + 16 * (lane >> 4));
-      if (KV == kPagedFp8) ke[t] = buf_ld8(buf_rsrc(p.pg.ke + r, n), row);
+    for (int i = 0; i < kV; ++i) {
+      v[t][i] = buf_ld128(rs, from * kRowBytes + 1024 * i + 16 * lane);
+      if (KV == kPagedFp8) ve[t][i] = buf_ld8(buf_rsrc(p.pg.ve + row, n), from + (64 / kTpr) * i + lane / kTpr);
     }
   }
-  __device__ __forceinline__ void load_values(const FlashArgs& p, int hk, int kv, int kv_end, bool& bad) {
-    const int lane = __lane_id();
+  // The round's keys (VAL: values) from position kv.
+  template <bool VAL>
+  __device__ __forceinline__ void load(const FlashArgs& p, int hk, int kv, int kv_end, bool& bad) {
+    uint32_t n;
+    int64_t row;
+    if (one) row = rows_at(p, hk, kv, kv_end, page[0], kPos, n, bad);
 #pragma unroll
     for (int t = 0; t < kRuns; ++t) {
-      uint32_t n;
-      const int64_t r = run(p, hk, kv, kv_end, t, n, bad);
-      const auto rs = buf_rsrc(p.pg.v + r * kRowBytes, n * kRowBytes);
-#pragma unroll
-      for (int i = 0; i < kV; ++i) {
-        v[t][i] = buf_ld128(rs, 1024 * i + 16 * lane);
-        if (KV == kPagedFp8) ve[t][i] = buf_ld8(buf_rsrc(p.pg.ve + r, n), (64 / kTpr) * i + lane / kTpr);
-      }
+      if (!one) row = rows_at(p, hk, kv + 16 * t, kv_end, page[t], 16, n, bad);
+      if (VAL)
+        run_values(p, t, row, n, one ? 16 * t : 0);
+      else
+        run_keys(p, t, row, n, one ? 16 * t : 0);
     }
   }
   // Key operand of run t, dims 32 k ..: 8-bit keys give a lane 16 dims of each 64.
@@ -776,7 +782,7 @@ __device__ __forceinline__ void few_not_finite(lds8* vs, v4f (&o)[D / 16], int a
 }
 
 template <int D, int KV>
-__global__ __launch_bounds__(64 * kFewWaves, 2) void k_flash_few(FlashArgs p) {
+__global__ __launch_bounds__(64 * kFewWaves, KV == kPagedFp8 ? 3 : 2) void k_flash_few(FlashArgs p) {
   using F = Few<D, KV>;
   constexpr int kRound = F::kPos * kFewWaves;
   __shared__ __attribute__((aligned(16))) FewShared<D> s;
@@ -785,6 +791,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void k_flash_few(FlashArgs p) {
   const int32_t* const table = p.bt.table + (int64_t)b * p.bt.max_pages;
   const int kv0 = p.splits > 1 ? split * p.chunk : 0, kv_first = kv0 + F::kPos * wv;
   F f;
+  f.one = p.pg.ps.d % F::kPos == 0;
   f.fetch_pages(p, table, kv_first);  // (does not wait for the lengths)
   const Seq sq = load_seq(p.bt, b, (int64_t)p.bt.max_pages * p.pg.ps.d);
   if (!sq.ok && tid == 0) flag_error(p.error);
@@ -801,9 +808,6 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void k_flash_few(FlashArgs p) {
     const int lo = uni(max(-1, first + row_token(r0, p)));
     const int kv_end = uni(min(seq_end, max(0, first + row_token(min(r0 + kFewRows, rows) - 1, p) + 1)));
     if (r0 > 0) f.fetch_pages(p, table, kv_first);
-    f.load_keys(p, hk, kv_first, kv_end, bad);
-    f.load_values(p, hk, kv_first, kv_end, bad);
-    f.fetch_pages(p, table, kv_first + kRound);
     v8bf q[D / 32];  // B operands, in the order of the keys' dims
     {
       const uint16_t* a = p.q + (int64_t)(sq.row0 + tok) * p.ldq + head * D;
@@ -813,6 +817,9 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void k_flash_few(FlashArgs p) {
         q[k] = __builtin_bit_cast(v8bf, *reinterpret_cast<const uint4*>(a + d));
       }
     }
+    f.template load<false>(p, hk, kv_first, kv_end, bad);
+    f.template load<true>(p, hk, kv_first, kv_end, bad);
+    f.fetch_pages(p, table, kv_first + kRound);
     v4f o[D / 16];
 #pragma unroll
     for (int t = 0; t < D / 16; ++t) o[t] = (v4f){0.f, 0.f, 0.f, 0.f};
@@ -829,7 +836,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void k_flash_few(FlashArgs p) {
         for (int k = 0; k < D / 32; ++k)
           sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.key(t, k), q[k], sc[t], 0, 0, 0);
       }
-      f.load_keys(p, hk, kv + kRound, kv_end, bad);
+      f.template load<false>(p, hk, kv + kRound, kv_end, bad);
 
       float mx = kNegInf;
 #pragma unroll
@@ -865,7 +872,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void k_flash_few(FlashArgs p) {
         __builtin_amdgcn_wave_barrier();  // reads done before the rows are written again
         f.store_values(vs, t0);
         if (t0 + 2 == F::kRuns) {
-          f.load_values(p, hk, kv + kRound, kv_end, bad);
+          f.template load<true>(p, hk, kv + kRound, kv_end, bad);
           f.fetch_pages(p, table, kv + 2 * kRound);
         }
         __builtin_amdgcn_wave_barrier();  // the wave's LDS rows are read back by other lanes
@@ -992,28 +999,45 @@ struct FlashPlan {
   int splits;
   int64_t chunk;
 };
-// Few rows: the kernel of single tokens where a sequence's rows fit one of its
-// tiles.  Splits: enough workgroups for the chip where the rows alone give
-// too few, each of at least kMinChunk positions.
-constexpr int64_t kMinChunk = 512;
+// Few rows: the kernel of single tokens where a sequence's rows fit one of its tiles.
+//
+// Splits, by the workgroups that the rows alone give (`tiles`) and the longest
+// context, measured on 256 CUs, 20 / 5 heads of 128, us a call; a chunk is at
+// least kMinChunk positions and 256 of them a round.
+//  - Tiles: two workgroups fit a CU, and a call's tiles are mostly of unlike
+//    length, so as many as come nearest to two a CU.  1000 rows of one sequence at 9000
+//    positions (160 workgroups), 1 / 2 / 3 / 4 splits: 173, 128, 110, 123; 4 x 320 at
+//    8192 (220): 167, 141, 160, 150; 4 x 512 at 8192 (340): 234, 229, 224, 220.
+//  - Few rows: bound by memory, which one workgroup a CU saturates: as many
+//    as there are CUs, from 1024 positions on.  bf16, 1 user at 16384, 16 / 25 / 51 / 102
+//    splits: 20.1, 17.8, 16.5, 20.6; 8 users at 4096, 3 / 6 / 8: 24.3, 21.2, 24.6; 32 users
+//    at 4096, 1 / 2 / 3: 60, 78, 70; 1 user at 1024, 1 / 4: 13.2, 11.2.
+//    8-bit pages need half the bytes and three workgroups fit a CU: where whole
+//    contexts leave 3/8 of the CUs idle three splits are better if the contexts
+//    differ (32 users up to 4096: 40.5, 39.0, 32.8), a little worse if not (38.9, 45.6, 41.8).
+constexpr int64_t kMinChunk = 256;
 constexpr int64_t kMaxSplits = 256;
-inline FlashPlan flash_plan(int64_t T, int64_t H, int64_t Hkv, int64_t B, int64_t max_q, int64_t max_kv, bool paged) {
+inline FlashPlan flash_plan(int64_t T, int64_t H, int64_t Hkv, int64_t B, int64_t max_q, int64_t max_kv, bool paged,
+                            bool fp8) {
   FlashPlan f{};
-  const int64_t G = H / Hkv;
+  const int64_t G = H / Hkv, cus = device_cus();
   f.few = paged && max_q * G <= kFewRows;
   f.tiles = (f.few ? B : T * G / kTileRows + (B < T ? B : T)) * Hkv;
   f.splits = 1;
-  f.chunk = round_up(max_kv > 0 ? max_kv : 1, 256);
-  const int64_t slots = (int64_t)device_cus() * (f.few ? 1 : 2);
-  const char* e = getenv("BTL_X_SPLITS");
-  if (paged && max_kv > kMinChunk) {
-    int64_t n = e ? atoi(e) : slots / f.tiles;
-    if (n > max_kv / kMinChunk) n = max_kv / kMinChunk;
-    if (n > kMaxSplits) n = kMaxSplits;
-    if (n > 1) {
-      f.chunk = round_up((max_kv + n - 1) / n, 256);
-      f.splits = (int)((max_kv + f.chunk - 1) / f.chunk);
-    }
+  f.chunk = round_up(max_kv > 0 ? max_kv : 1, kMinChunk);
+  if (!paged || max_kv < (f.few ? 4 : 2) * kMinChunk) return f;
+  int64_t n;
+  if (f.few) {
+    n = cus / f.tiles;
+    if (n == 1 && fp8 && 8 * f.tiles <= 5 * cus) n = 3;
+  } else {
+    n = (4 * cus + f.tiles) / (2 * f.tiles);
+  }
+  if (n > max_kv / kMinChunk) n = max_kv / kMinChunk;
+  if (n > kMaxSplits) n = kMaxSplits;
+  if (n > 1) {
+    f.chunk = round_up((max_kv + n - 1) / n, kMinChunk);
+    f.splits = (int)((max_kv + f.chunk - 1) / f.chunk);
   }
   return f;
 }
@@ -1079,7 +1103,7 @@ int btl_prompt_attention(const uint16_t* q, int64_t ldq, const uint16_t* k, int6
   a.ldk = ldk;
   a.ldv = ldv;
   a.splits = 1;
-  const FlashPlan f = flash_plan(T, H, Hkv, B, T, T, false);
+  const FlashPlan f = flash_plan(T, H, Hkv, B, T, T, false, false);
   const dim3 grid((unsigned)f.tiles);
   if (D == 128)
     hipLaunchKernelGGL((k_flash_tile<128, kDense>), grid, dim3(256), 0, (hipStream_t)stream, a);
@@ -1089,9 +1113,9 @@ int btl_prompt_attention(const uint16_t* q, int64_t ldq, const uint16_t* k, int6
 }
 
 int64_t btl_paged_attention_scratch_bytes(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t B, int64_t max_q,
-                                          int64_t max_kv) {
+                                          int64_t max_kv, int fp8) {
   if (T <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || B <= 0 || max_q <= 0 || max_kv <= 0) return 0;
-  return flash_scratch(flash_plan(T, H, Hkv, B, max_q, max_kv, true), T, H, D);
+  return flash_scratch(flash_plan(T, H, Hkv, B, max_q, max_kv, true, fp8 != 0), T, H, D);
 }
 
 int btl_paged_attention(const uint16_t* q, int64_t ldq, int64_t T, int64_t H, const btl_pages_t* pages,
@@ -1113,7 +1137,8 @@ int btl_paged_attention(const uint16_t* q, int64_t ldq, int64_t T, int64_t H, co
                      (long long)max_kv, (long long)max_pages);
   if (T == 0) return BTL_OK;
   if (!page_table || !kv_len) return set_error(BTL_ERR_NULL, "%s: NULL pointer", who);
-  const FlashPlan f = flash_plan(T, H, Hkv, B, max_q, max_kv, true);
+  const bool fp8 = pages->k_exp != nullptr;
+  const FlashPlan f = flash_plan(T, H, Hkv, B, max_q, max_kv, true, fp8);
   if (f.few && B > 65535) return set_error(BTL_ERR_SHAPE, "%s: %lld sequences", who, (long long)B);
   const int64_t need = flash_scratch(f, T, H, D);
   if (need > 0) {
@@ -1126,7 +1151,6 @@ int btl_paged_attention(const uint16_t* q, int64_t ldq, int64_t T, int64_t H, co
   a.chunk = (int)f.chunk;
   a.part_o = static_cast<float*>(scratch);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + (f.splits > 1 ? (int64_t)f.splits * T * H * D : 0));
-  const bool fp8 = pages->k_exp != nullptr;
   if (f.few) {
     const dim3 grid((unsigned)Hkv, (unsigned)B, (unsigned)f.splits);
     auto* kern = D == 128 ? (fp8 ? k_flash_few<128, kPagedFp8> : k_flash_few<128, kPagedBf16>)
