@@ -32,6 +32,10 @@ layer's QKV and o_proj (150 launches per 30-layer step).
 
 All buffers are allocated once, so :meth:`BitLinearDecodeStep.step` is
 allocation-free and can be captured in a HIP graph.
+
+Prompts and chunks: after ``alloc_paged``, ``forward_rows`` runs the layers on
+any number of rows of any users over a paged cache, and ``load_contiguous`` hands
+what is cached to the contiguous caches of the decode step.
 """
 
 from __future__ import annotations
@@ -316,6 +320,56 @@ class BitLinearDecodeStep:
         for i in range(len(self.layers)):
             self.layer_full(i)
         return self.hidden
+
+    # -- prompts and chunks over a paged cache --------------------------------
+    def alloc_paged(self, num_pages: int, max_seq_len: int, page_size: int = 64, dtype: str = "bf16",
+                    use_fused_rope: bool = False, rope_scaling: dict | None = None):
+        """Page pools of every layer for ``forward_rows``: num_pages pages of
+        page_size rows, dtype "bf16" or "fp8", positions up to max_seq_len."""
+        from .layers.attention import PagedAttention
+
+        c = self.config
+        self.paged = PagedAttention(c.num_attention_heads, c.num_kv_heads, c.head_dim, max_seq_len, self.device,
+                                    rope_theta=c.rope_theta, use_fused_rope=use_fused_rope, rope_scaling=rope_scaling,
+                                    max_position=c.max_position_embeddings)
+        self.pages = [self.paged.new_cache(num_pages, page_size, dtype) for _ in self.layers]
+        return self
+
+    def forward_rows(self, hidden, page_table, cu_q, kv_len, max_q: int | None = None, max_kv: int | None = None):
+        """The layers on any rows of any users: hidden bf16 [T, hidden], in place.
+        Sequence b's rows are ``cu_q[b] .. cu_q[b + 1] - 1``, its newest tokens; their
+        keys and values are cached, and kv_len counts them (bitnet_tt.paged_attention).
+        Whole prompts, chunks of them and single tokens may share a call.  Needs
+        alloc_paged()."""
+        import torch
+
+        if getattr(self, "paged", None) is None:
+            raise RuntimeError("forward_rows needs alloc_paged() first")
+        c = self.config
+        T = hidden.shape[0]
+        dev = hidden.device
+        qkv = torch.empty((T, c.qkv_dim), dtype=torch.bfloat16, device=dev)
+        attn = torch.empty((T, c.num_attention_heads * c.head_dim), dtype=torch.bfloat16, device=dev)
+        ffn = torch.empty((T, c.intermediate_size), dtype=torch.bfloat16, device=dev)
+        for w, pages in zip(self.layers, self.pages):
+            ternary_matmul_into(hidden, w.qkv, qkv, norm_weight=w.input_layernorm, norm_epsilon=self.eps)
+            self.paged(qkv, pages, page_table, cu_q, kv_len, max_q=max_q, max_kv=max_kv, out=attn)
+            ternary_matmul_into(attn, w.o_proj, hidden, norm_weight=w.attn_sub_norm, norm_epsilon=self.eps,
+                                residual=hidden)
+            ternary_matmul_into(hidden, w.gate_up, ffn, norm_weight=w.post_attention_layernorm, norm_epsilon=self.eps,
+                                epilogue="relu2_mul")
+            ternary_matmul_into(ffn, w.down, hidden, norm_weight=w.ffn_sub_norm, norm_epsilon=self.eps, residual=hidden)
+        return hidden
+
+    def load_contiguous(self, page_table, kv_len) -> None:
+        """What the pages hold, into the contiguous caches of ``alloc_attention``
+        (rows [0, kv_len[b]) of user b), for the one-launch step to go on from."""
+        from .paged_attention import read_pages
+
+        if getattr(self, "paged", None) is None or getattr(self, "kv", None) is None:
+            raise RuntimeError("load_contiguous needs alloc_paged() and alloc_attention() first")
+        for kv, pages in zip(self.kv, self.pages):
+            read_pages(pages, page_table, kv_len, kv.key_cache, kv.value_cache)
 
     # -- the step ----------------------------------------------------------
     def layer(self, i: int, hidden, attn_out, qkv_out, ffn_h):

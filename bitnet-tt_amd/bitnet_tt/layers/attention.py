@@ -4,7 +4,9 @@ prologue, and the o_proj projection (API pieces of bitnet-tt's
 
 ``DecodeAttention`` is the decode attention between the QKV projection and
 o_proj (attention.py:1040-1262): RoPE, KV-cache update and SDPA over the
-cached positions, one gfx950 launch per layer.
+cached positions, one gfx950 launch per layer.  ``PagedAttention`` is the
+same for any number of rows a user: prompts, chunks and single tokens over a
+paged cache, bf16 or 8-bit.
 
 Fused QKV: q, k and v are quantised separately (three absmean scales), the
 Q and K column blocks are optionally permuted from HF half-split to
@@ -210,3 +212,83 @@ class DecodeAttention:
         ws = N.workspace(self.device if device is None else device, 0, kind="attention")
         off = int(L.btl_decode_attention_error_offset(B, self.num_kv_heads))
         return int(ws[off:off + 4].view(__import__("torch").int32).item())
+
+
+class PagedAttention:
+    """The attention of one layer for prompts, chunks and single tokens over a
+    paged cache (the reference's prompt path, attention.py:1348-1507, and its caches,
+    :115-458): RoPE, page writes and causal GQA SDPA of any number of packed rows.
+
+    One object serves every layer of a model; each layer has its own
+    PagedKVCache, all of them one page table.  Rows and the device arrays cu_q,
+    kv_len and page_table: see bitnet_tt.paged_attention.  ``rotary_dim`` (a multiple
+    of 16, default head_dim) rotates part of a head; ``rope_scaling`` is a model
+    config's dict (utils.rope.scaled_frequencies).  Without scaling the angles are those of
+    DecodeAttention.  ``scale`` as for DecodeAttention."""
+
+    def __init__(self, num_heads: int, num_kv_heads: int, head_dim: int, max_seq_len: int, device=None,
+                 rope_theta: float = 500000.0, use_fused_rope: bool = False, scale: float | None = None,
+                 rotary_dim: int | None = None, rope_scaling: dict | None = None, max_position: int = 4096) -> None:
+        import math
+
+        import torch
+
+        from ..utils.rope import long_rope_tables, rope_tables
+
+        rotary_dim = head_dim if rotary_dim is None else rotary_dim
+        if head_dim not in (64, 128) or num_heads % num_kv_heads or num_heads // num_kv_heads > 64:
+            raise ValueError("the paged attention kernels take head_dim 64 or 128 and up to 64 query heads per KV head")
+        if rotary_dim < 16 or rotary_dim % 16 or rotary_dim > head_dim:
+            raise ValueError(f"rotary_dim {rotary_dim}: a multiple of 16 up to head_dim")
+        self.num_heads = num_heads
+        self.num_kv_heads = num_kv_heads
+        self.head_dim = head_dim
+        self.max_seq_len = max_seq_len
+        self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        self.use_fused_rope = use_fused_rope
+        self.scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
+        if rope_scaling is None:
+            cos, sin = (torch.from_numpy(t) for t in rope_tables(rotary_dim, max_seq_len, rope_theta))
+        else:
+            cos, sin = long_rope_tables(rotary_dim, max_seq_len, rope_theta, rope_scaling, max_position, self.device)
+        self.rope_cos, self.rope_sin = cos.to(self.device), sin.to(self.device)
+
+    def new_cache(self, num_pages: int, page_size: int = 64, dtype: str = "bf16"):
+        """A layer's page pools; dtype "bf16" or "fp8"."""
+        from ..paged_attention import PagedKVCache
+
+        return PagedKVCache.allocate(num_pages, self.num_kv_heads, self.head_dim, self.device, page_size, dtype)
+
+    def __call__(self, qkv, cache, page_table, cu_q, kv_len, max_q: int | None = None, max_kv: int | None = None,
+                 out=None):
+        """qkv bf16 [T, (H + 2 Hkv) D]: writes its keys and values to their pages,
+        then attends over everything cached; bf16 [T, H D]."""
+        from ..paged_attention import paged_attention, rope_write
+
+        H, D = self.num_heads, self.head_dim
+        q = rope_write(qkv, self.rope_cos, self.rope_sin, cu_q, kv_len, H, self.num_kv_heads, cache=cache,
+                       page_table=page_table, rope_adjacent=self.use_fused_rope)
+        o = paged_attention(q, cache, page_table, cu_q, kv_len, scale=self.scale, max_q=max_q, max_kv=max_kv,
+                            out=None if out is None else out.view(-1, H, D))
+        return o.view(-1, H * D)
+
+    def prompt(self, qkv, cu_seqlens, cache=None, page_table=None, kv_len=None, max_q: int | None = None, out=None):
+        """Whole prompts: attention within the packed rows themselves, whose keys
+        and values need not be cached, and are not rounded to 8 bits where they are.
+        With ``cache``: page_table too; kv_len, if given, must be the prompts' lengths."""
+        import torch
+
+        from ..paged_attention import prompt_attention, rope_write
+
+        H, Hkv, D = self.num_heads, self.num_kv_heads, self.head_dim
+        k = torch.empty((qkv.shape[0], Hkv, D), dtype=torch.bfloat16, device=qkv.device)
+        q = rope_write(qkv, self.rope_cos, self.rope_sin, cu_seqlens, kv_len, H, Hkv, cache=cache,
+                       page_table=page_table, rope_adjacent=self.use_fused_rope, k_out=k)
+        v = qkv.view(-1, H + 2 * Hkv, D)[:, H + Hkv:]
+        o = prompt_attention(q, k, v, cu_seqlens, scale=self.scale, max_q=max_q,
+                             out=None if out is None else out.view(-1, H, D))
+        return o.view(-1, H * D)
+
+    def check(self) -> None:
+        """As DecodeAttention.check: a batch that was not well formed raises."""
+        N.check_errors(self.device)

@@ -27,3 +27,61 @@ def rope_tables(dim: int, max_seq_len: int, theta: float = 10000.0):
     decode-attention kernel reads these."""
     cos, sin = precompute_freqs_cis(dim, max_seq_len, theta)
     return np.ascontiguousarray(cos[0, 0, :, 0::2]), np.ascontiguousarray(sin[0, 0, :, 0::2])
+
+
+def scaled_frequencies(dim: int, theta: float = 10000.0, scaling: dict | None = None, max_position: int = 4096):
+    """(float64 frequencies [dim/2], factor of cos and sin) for contexts longer
+    than the model was trained on.  ``scaling`` as in a model's config
+    ("rope_type" or "type"):
+
+    - None, "default": theta^(-2i/dim).
+    - "linear" (factor): every frequency / factor.
+    - "llama3" (factor, low_freq_factor, high_freq_factor,
+      original_max_position_embeddings): wavelengths below original / high keep
+      their frequency, those above original / low get it / factor, and between
+      the two the mix goes linearly with original / wavelength.
+    - "yarn" (factor, beta_fast 32, beta_slow 1, attention_factor,
+      original_max_position_embeddings): a ramp between the dims that turn
+      beta_fast and beta_slow times within the original context; cos and sin
+      times attention_factor (0.1 ln(factor) + 1).
+
+    original_max_position_embeddings defaults to ``max_position``."""
+    i = np.arange(0, dim, 2, dtype=np.float64)
+    freq = float(theta) ** (-i / dim)
+    kind = "default" if scaling is None else scaling.get("rope_type", scaling.get("type", "default"))
+    if kind == "default":
+        return freq, 1.0
+    if kind not in ("linear", "llama3", "yarn"):
+        raise ValueError(f"rope scaling {kind!r}: default, linear, llama3 and yarn are supported")
+    factor = float(scaling["factor"])
+    if not factor >= 1.0:
+        raise ValueError(f"rope scaling factor {factor} must be at least 1")
+    if kind == "linear":
+        return freq / factor, 1.0
+    original = float(scaling.get("original_max_position_embeddings", max_position))
+    if kind == "llama3":
+        low, high = float(scaling.get("low_freq_factor", 1.0)), float(scaling.get("high_freq_factor", 4.0))
+        turns = original * freq / (2.0 * np.pi)  # original / wavelength
+        mix = np.clip((turns - low) / (high - low), 0.0, 1.0)
+        return freq * (mix + (1.0 - mix) / factor), 1.0
+    fast, slow = float(scaling.get("beta_fast", 32.0)), float(scaling.get("beta_slow", 1.0))
+
+    def dim_of(turns):  # the dim pair that turns this often within the original context
+        return dim * np.log(original / (turns * 2.0 * np.pi)) / (2.0 * np.log(float(theta)))
+
+    first, last = max(np.floor(dim_of(fast)), 0.0), min(np.ceil(dim_of(slow)), dim - 1.0)
+    ramp = np.clip((np.arange(dim // 2) - first) / max(last - first, 0.001), 0.0, 1.0)
+    attention = scaling.get("attention_factor")
+    return freq * (1.0 - ramp) + freq / factor * ramp, 0.1 * np.log(factor) + 1.0 if attention is None else float(attention)
+
+
+def long_rope_tables(dim: int, max_seq_len: int, theta: float = 10000.0, scaling: dict | None = None,
+                     max_position: int = 4096, device="cpu"):
+    """(cos, sin) torch tensors [max_seq_len, dim/2] fp32 of scaled_frequencies,
+    angles in float64: at position 100000 a float32 angle is off by up to 0.004,
+    half a step of bf16; rope_tables keeps the reference's float32 angles."""
+    import torch
+
+    freq, factor = scaled_frequencies(dim, theta, scaling, max_position)
+    angle = torch.arange(max_seq_len, dtype=torch.float64, device=device)[:, None] * torch.from_numpy(freq).to(device)
+    return (angle.cos() * factor).float(), (angle.sin() * factor).float()

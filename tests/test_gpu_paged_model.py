@@ -1,0 +1,202 @@
+"""Prompts, chunks and single tokens through the layers of a model over a paged
+cache: the operators together, as a program uses them."""
+
+import numpy as np
+import pytest
+import torch
+
+from paged_helpers import attend64, check_close, cu_of, dev, ints, normal
+
+from bitnet_tt import paged_attention as pa
+from bitnet_tt.config import BitNetMiniConfig
+from bitnet_tt.decode import BitLinearDecodeStep
+from bitnet_tt.layers.attention import DecodeAttention, PagedAttention
+from bitnet_tt.ternary_matmul import ternary_matmul
+from bitnet_tt.utils.rope import long_rope_tables, rope_tables, scaled_frequencies
+
+
+def rotate64(x, cos, sin, adjacent):
+    """x [n, heads, D] in 64 bits, whole heads."""
+    c, s = cos[:, None].double(), sin[:, None].double()
+    if adjacent:
+        a, b = x[..., 0::2], x[..., 1::2]
+        return torch.stack((a * c - b * s, b * c + a * s), -1).flatten(-2)
+    h = x.shape[-1] // 2
+    a, b = x[..., :h], x[..., h:]
+    return torch.cat((a * c - b * s, b * c + a * s), -1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp8"])
+@pytest.mark.parametrize("adjacent", [False, True])
+def test_prompt_then_chunk_then_tokens(dtype, adjacent):
+    """Two users: a prompt each, a chunk of one beside a token of the other, tokens.
+    Every attention output against 64 bits over what the pages hold."""
+    H, Hkv, D, page = 4, 2, 64, 16
+    att = PagedAttention(H, Hkv, D, 128, dev(), use_fused_rope=adjacent)
+    cache = att.new_cache(20, page, dtype)
+    table = torch.arange(20, dtype=torch.int32).view(2, 10).flip(1).contiguous()
+    length = [0, 0]
+    for i, new in enumerate(([37, 20], [9, 1], [1, 1], [1, 1], [0, 1])):
+        length = [a + b for a, b in zip(length, new)]
+        qkv = normal((sum(new), (H + 2 * Hkv) * D), 50 + i).to(torch.bfloat16)
+        out = att(qkv.to(dev()), cache, table.to(dev()), cu_of(new), ints(length), max_q=max(new))
+        att.check()
+        k = torch.zeros((2, Hkv, 160, D), dtype=torch.bfloat16, device=dev())
+        v = torch.zeros_like(k)
+        pa.read_pages(cache, table.to(dev()), ints(length), k, v)
+        # the rotated queries as the write gives them (its own tests hold them to 64 bits)
+        q = pa.rope_write(qkv.to(dev()), att.rope_cos, att.rope_sin, cu_of(new), ints(length), H, Hkv,
+                          rope_adjacent=adjacent).double().cpu()
+        at, x = 0, qkv.double().view(-1, H + 2 * Hkv, D)
+        for b in range(2):
+            n, m = new[b], length[b]
+            pos = torch.arange(m - n, m)
+            turned = rotate64(x[at:at + n, :H], att.rope_cos.cpu()[pos], att.rope_sin.cpu()[pos], adjacent)
+            assert n == 0 or float((q[at:at + n] - turned).abs().max()) <= 2.0 ** -7 * float(turned.abs().max())
+            want, tol = attend64(q[at:at + n], k[b, :, :m].double().cpu(), v[b, :, :m].double().cpu())
+            check_close(out[at:at + n].view(n, H, D), want, tol)
+            at += n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp8"])
+def test_prompt_of_packed_rows_and_its_pages(dtype):
+    """prompt() attends to the rows themselves and caches them; the cached chunk call over
+    the same pages is the same up to what 8 bits cost."""
+    H, Hkv, D = 8, 2, 128
+    att = PagedAttention(H, Hkv, D, 128, dev())
+    lens = [33, 70]
+    qkv = normal((sum(lens), (H + 2 * Hkv) * D), 9).to(torch.bfloat16).to(dev())
+    cu, table = cu_of(lens), torch.arange(8, dtype=torch.int32, device=dev()).view(2, 4)
+    cache = att.new_cache(8, 32, dtype)
+    o = att.prompt(qkv, cu, cache, table)
+    again = att.prompt(qkv, cu)
+    assert torch.equal(o, again)
+    fresh = att.new_cache(8, 32, dtype)
+    paged = att(qkv, fresh, table, cu, ints(lens))
+    att.check()
+    assert torch.equal(fresh.key_pages.view(torch.uint8), cache.key_pages.view(torch.uint8))
+    assert torch.equal(fresh.value_pages.view(torch.uint8), cache.value_pages.view(torch.uint8))
+    if dtype == "bf16":
+        assert torch.equal(o, paged)  # the same kernel arithmetic on the same values
+
+
+@pytest.mark.gpu
+def test_forward_rows_is_the_layers_chain():
+    """Each layer of forward_rows: the BitLinears are the calls of the rest of the package on
+    the same rows (bits), the attention is PagedAttention's."""
+    cfg = BitNetMiniConfig()
+    step = BitLinearDecodeStep.random_init(cfg, dev(), seed=3, batch=2, num_layers=2)
+    step.alloc_paged(16, 256, page_size=32)
+    new, total = [50, 7], [50, 7]
+    table = torch.arange(16, dtype=torch.int32, device=dev()).view(2, 8)
+    hidden = normal((57, cfg.hidden_size), 4).to(torch.bfloat16).to(dev())
+    h = hidden.clone()
+    got = step.forward_rows(hidden, table, cu_of(new), ints(total))
+    step.check()
+    assert got is hidden
+    att = PagedAttention(cfg.num_attention_heads, cfg.num_kv_heads, cfg.head_dim, 256, dev(), rope_theta=cfg.rope_theta)
+    for w in step.layers:
+        qkv = ternary_matmul(h, w.qkv, norm_weight=w.input_layernorm, norm_epsilon=step.eps)
+        a = att(qkv, att.new_cache(16, 32), table, cu_of(new), ints(total))
+        h = ternary_matmul(a, w.o_proj, norm_weight=w.attn_sub_norm, norm_epsilon=step.eps, residual=h)
+        f = ternary_matmul(h, w.gate_up, norm_weight=w.post_attention_layernorm, norm_epsilon=step.eps,
+                           epilogue="relu2_mul")
+        h = ternary_matmul(f, w.down, norm_weight=w.ffn_sub_norm, norm_epsilon=step.eps, residual=h)
+    assert torch.equal(got, h)
+
+
+@pytest.mark.gpu
+def test_pages_to_the_contiguous_step():
+    """A prompt over pages, then decode steps on the contiguous caches: the attention of the
+    first step sees what the pages held."""
+    from bitnet_tt.config import BitNetConfig
+
+    cfg = BitNetConfig(hidden_size=512, num_layers=2, num_attention_heads=4, num_key_value_heads=1,
+                       intermediate_size=1024, vocab_size=1000, max_position_embeddings=256)
+    step = BitLinearDecodeStep.random_init(cfg, dev(), seed=5, batch=3)
+    step.alloc_buffers().alloc_attention(max_seq_len=128, pos=0)
+    step.alloc_paged(12, 128, page_size=32)
+    lens = [40, 1, 90]
+    table = torch.randperm(12, generator=torch.Generator().manual_seed(1)).to(torch.int32).view(3, 4).to(dev())
+    step.forward_rows(normal((sum(lens), 512), 6).to(torch.bfloat16).to(dev()), table, cu_of(lens), ints(lens), max_kv=90)
+    step.load_contiguous(table, ints(lens))
+    for i in range(2):
+        k, v = step.kv[i].key_cache, step.kv[i].value_cache
+        for b, n in enumerate(lens):
+            ids = table[b, : -(-n // 32)].long()
+            assert torch.equal(k[b, 0, :n], step.pages[i].key_pages[ids, 0].flatten(0, 1)[:n])
+            assert torch.equal(v[b, 0, :n], step.pages[i].value_pages[ids, 0].flatten(0, 1)[:n])
+    # one more token each, both ways
+    step.pos.copy_(ints(lens))
+    step.reset_hidden()
+    rows = step.hidden.clone()
+    step.step_full()
+    step.forward_rows(rows, table, cu_of([1, 1, 1]), ints([n + 1 for n in lens]), max_q=1)
+    step.check()
+    a, b = step.hidden.double(), rows.double()
+    # two attention kernels that round differently, then int8 codes: normwise
+    assert float((a - b).norm() / a.norm()) < 0.05
+    with pytest.raises(RuntimeError, match="alloc_paged"):
+        BitLinearDecodeStep(cfg, dev()).forward_rows(rows, table, cu_of([1]), ints([1]))
+
+
+# ---- angle tables (host) --------------------------------------------------
+
+
+def test_long_tables_without_scaling_are_the_plain_angles():
+    cos, sin = long_rope_tables(64, 300, 10000.0)
+    c, s = rope_tables(64, 300, 10000.0)
+    # float32 angles of up to 300: off by 300 x 2^-24 and the frequency's own half step
+    assert float((cos - torch.from_numpy(c)).abs().max()) < 300 * 2.0 ** -23 + 2.0 ** -23
+    assert float((sin - torch.from_numpy(s)).abs().max()) < 300 * 2.0 ** -23 + 2.0 ** -23
+    far, _ = long_rope_tables(16, 100001, 10000.0)
+    want = np.cos(100000.0 * 10000.0 ** (-np.arange(0, 16, 2) / 16.0))
+    assert np.abs(far[100000].double().numpy() - want).max() <= 2.0 ** -24
+
+
+def test_linear_and_llama3_frequencies():
+    plain, one = scaled_frequencies(128, 500000.0)
+    f, a = scaled_frequencies(128, 500000.0, {"type": "linear", "factor": 4})
+    assert one == a == 1.0 and np.allclose(f * 4, plain, rtol=1e-15)
+    cfg = {"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0,
+           "original_max_position_embeddings": 8192}
+    f, a = scaled_frequencies(128, 500000.0, cfg)
+    for x, y in zip(plain, f):  # dim by dim
+        wave = 2 * np.pi / x
+        if wave < 8192 / 4:
+            want = x
+        elif wave > 8192:
+            want = x / 8
+        else:
+            t = (8192 / wave - 1.0) / 3.0
+            want = (1 - t) * x / 8 + t * x
+        assert abs(y - want) <= 1e-14 * want
+    assert a == 1.0 and f[0] == plain[0] and abs(f[-1] * 8 / plain[-1] - 1) < 1e-14
+
+
+def test_yarn_frequencies():
+    cfg = {"rope_type": "yarn", "factor": 16.0, "original_max_position_embeddings": 4096}
+    plain, _ = scaled_frequencies(64, 10000.0)
+    f, a = scaled_frequencies(64, 10000.0, cfg)
+    assert abs(a - (0.1 * np.log(16.0) + 1.0)) < 1e-15
+    turns = 4096 * plain / (2 * np.pi)
+    assert np.allclose(f[turns > 40], plain[turns > 40], rtol=1e-15)
+    assert np.allclose(f[turns < 0.5] * 16, plain[turns < 0.5], rtol=1e-15)
+    assert (np.diff(f) < 0).all() and (f <= plain).all() and (f >= plain / 16 * (1 - 1e-15)).all()
+    assert scaled_frequencies(64, 10000.0, {**cfg, "attention_factor": 1.5})[1] == 1.5
+
+
+@pytest.mark.parametrize("bad", [{"type": "dynamic", "factor": 2.0}, {"type": "linear", "factor": 0.5}])
+def test_scalings_refused(bad):
+    with pytest.raises(ValueError):
+        scaled_frequencies(64, 10000.0, bad)
+
+
+def test_layer_refuses():
+    for kw in (dict(head_dim=96), dict(num_kv_heads=3), dict(rotary_dim=24), dict(rotary_dim=128)):
+        a = dict(num_heads=4, num_kv_heads=2, head_dim=64, max_seq_len=32, device="cpu")
+        a.update(kw)
+        with pytest.raises(ValueError):
+            PagedAttention(**a)
