@@ -151,6 +151,13 @@ __device__ __forceinline__ v4s lds_tr16(const lds8* p) {
 // workgroup's.  (The second product one step behind as well, so that nothing
 // in a step depends on anything else in it: the same speed, and 30 registers more than there are.)
 //
+// Bound by the matrix units' and the vector units' issue: at 16001 tokens of 20 / 5 heads of
+// 128, 405 us, 1000 TFLOP/s (a large library product reaches 1360), the matrix units are
+// busy 51% of the cycles and the vector units 41%, and the LDS 26%.  Over pages, 8192 tokens: 1005
+// TFLOP/s; 8-bit pages, which are converted on the way, 955.  Measured beside it: 64 rows a
+// wave, 795 (one wave a SIMD: nothing runs under a wait); 32 positions a step and
+// three workgroups a CU, 963; keys and values through registers to LDS, 843.
+//
 // 16-byte pieces of a row are stored at piece ^ f(row), for the LDS's 64 banks:
 // the 16 rows that 16 lanes read a piece of, and the 4 rows x 64 bytes that 32 lanes
 // of a transposing read cover, lie in different banks.
@@ -233,14 +240,6 @@ struct Source {
     for (int i = 0; i < kN; ++i) page_v[i] = page_k[i];
     fetch_pages(p, kv, page_k);
   }
-  // Page row of the step's position `at`, and how many of up to `most` rows from there there are.
-  __device__ __forceinline__ int64_t rows_at(const FlashArgs& p, int at, int32_t page, int most, uint32_t& n) {
-    n = (uint32_t)clampi(kv_end - at, 0, most);
-    const bool none = (uint32_t)page >= (uint32_t)p.pg.P;
-    bad |= none & (n > 0);
-    n = none ? 0 : n;
-    return page_row(none ? 0 : page, p.pg.P, p.pg.Hkv, hk, p.pg.ps.d, at - (int)div_by(at, p.pg.ps) * (int)p.pg.ps.d);
-  }
   // The step's keys (VAL: values) to LDS (8-bit pages: to registers).
   template <bool VAL>
   __device__ __forceinline__ void load(const FlashArgs& p, int kv, lds8* at) {
@@ -255,23 +254,22 @@ struct Source {
     const uint8_t* const pool = VAL ? p.pg.v : p.pg.k;
     const uint8_t* const exps = VAL ? p.pg.ve : p.pg.ke;
     if (one) {
-      uint32_t n;
-      const int64_t row = rows_at(p, kv, VAL ? page_v[0] : page_k[0], kStep, n);
-      const auto r = buf_rsrc(pool + row * kRowBytes, n * kRowBytes);
+      const Run run = run_at(p.pg, hk, kv, kv_end, VAL ? page_v[0] : page_k[0], kStep, bad);
+      const auto r = buf_rsrc(pool + run.row * kRowBytes, run.n * kRowBytes);
 #pragma unroll
       for (int i = 0; i < kN; ++i) {
         piece<VAL>(r, i, dst);
-        if (KV == kPagedFp8) (VAL ? ev : ek)[i] = buf_ld8(buf_rsrc(exps + row, n), i * kRpl + my_row);
+        if (KV == kPagedFp8) (VAL ? ev : ek)[i] = buf_ld8(buf_rsrc(exps + run.row, run.n), i * kRpl + my_row);
       }
       return;
     }
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
       // a run's rows, by their offsets from the step's first
-      uint32_t n;
       const int r0 = run_of(i);
-      const int64_t row = rows_at(p, kv + r0, VAL ? page_v[i] : page_k[i], 16, n) - r0;
-      n = n ? n + r0 : 0;
+      const Run run = run_at(p.pg, hk, kv + r0, kv_end, VAL ? page_v[i] : page_k[i], 16, bad);
+      const int64_t row = run.row - r0;
+      const uint32_t n = run.n ? run.n + r0 : 0;
       piece<VAL>(buf_rsrc(pool + row * kRowBytes, n * kRowBytes), i, dst);
       if (KV == kPagedFp8) (VAL ? ev : ek)[i] = buf_ld8(buf_rsrc(exps + row, n), i * kRpl + my_row);
     }
@@ -550,6 +548,13 @@ __global__ __launch_bounds__(256, 2) void k_flash_tile(FlashArgs p) {
       store_ahead(k_free, v_free);
       kv += kStep;
     };
+    if (wr >= rows) {  // a wave without rows only loads (67 tokens at 40000 positions: 68.5 us, 65.5 so)
+      for (; kv + 2 * kStep <= whole_end; kv += kStep, at ^= 1) {
+        arrived();
+        load_ahead(sm + at * kB, sm + (3 - at) * kB);
+        store_ahead(sm + at * kB, sm + (3 - at) * kB);
+      }
+    }
     while (kv + 2 * kStep <= whole_end) {
       hot(sm + kB, sm + 2 * kB, sm, sm + 3 * kB, sa, sb);
       if (kv + 2 * kStep > whole_end) {
@@ -635,13 +640,18 @@ __global__ __launch_bounds__(256, 2) void k_flash_tile(FlashArgs p) {
 
 // ======================================================================
 // Few rows (up to 16 to a sequence and key-value head: single tokens, short
-// drafts): bound by the bytes of keys and values.  8 waves share a context,
-// a round of kPos positions each; a wave's keys go straight from memory to the
-// MFMA's registers, its values through its own 8 KiB of LDS.  The next round's
-// loads are issued as soon as this one's registers are free (unconditionally:
-// behind the end they are out of the resource's range and read nothing), so 16 KiB a
-// wave, 128 KiB a CU, are on their way nearly all the time.  Page table entries are
+// drafts): bound by the bytes of keys and values.  4 waves share a context, a
+// round of kPos positions each; a wave's keys go straight from memory to the
+// MFMA's registers, its values through its own LDS.  The next round's loads are
+// issued as soon as this one's registers are free (unconditionally: behind the end
+// they are out of the resource's range and read nothing), so 16 KiB a wave (8 KiB of
+// 8-bit pages) are on their way nearly all the time.  Page table entries are
 // fetched a round ahead of that.  The waves' partials meet in LDS.
+//
+// 5 heads of 128: one user at 131001 positions 67 us (5.0 TB/s, merge included), 48 users
+// at 4096 90 us (5.6 TB/s); 8-bit pages 48 us (5.3).  8 / 4 / 2 waves a workgroup, each
+// at its best number of splits, 32 users of mixed lengths up to 4096, 8-bit pages: 38.5, 36.9,
+// 36.2 us; one user at 512 positions: 10.7, 9.7, 13.0.
 // ======================================================================
 constexpr int kFewRows = 16;
 constexpr int kFewWaves = 4;
@@ -683,15 +693,6 @@ struct Few {
       if (t == 0 || !one)
         page[t] = scalar_load(table, min(div_by(kv + 16 * t, p.pg.ps), (uint32_t)p.bt.max_pages - 1));
   }
-  // Page row of position `at`, and how many of up to `most` rows from there there are.
-  __device__ __forceinline__ int64_t rows_at(const FlashArgs& p, int hk, int at, int kv_end, int32_t pg, int most,
-                                             uint32_t& n, bool& bad) const {
-    n = (uint32_t)clampi(kv_end - at, 0, most);
-    const bool none = (uint32_t)pg >= (uint32_t)p.pg.P;
-    bad |= none & (n > 0);
-    n = none ? 0 : n;
-    return page_row(none ? 0 : pg, p.pg.P, p.pg.Hkv, hk, p.pg.ps.d, at - (int)div_by(at, p.pg.ps) * (int)p.pg.ps.d);
-  }
   // Run t's keys, from row `from` of n page rows at `row`.
   __device__ __forceinline__ void run_keys(const FlashArgs& p, int t, int64_t row, uint32_t n, int from) {
     const int lane = __lane_id(), r = from + (lane & 15);
@@ -712,16 +713,15 @@ struct Few {
   // The round's keys (VAL: values) from position kv.
   template <bool VAL>
   __device__ __forceinline__ void load(const FlashArgs& p, int hk, int kv, int kv_end, bool& bad) {
-    uint32_t n;
-    int64_t row;
-    if (one) row = rows_at(p, hk, kv, kv_end, page[0], kPos, n, bad);
+    Run run;
+    if (one) run = run_at(p.pg, hk, kv, kv_end, page[0], kPos, bad);
 #pragma unroll
     for (int t = 0; t < kRuns; ++t) {
-      if (!one) row = rows_at(p, hk, kv + 16 * t, kv_end, page[t], 16, n, bad);
+      if (!one) run = run_at(p.pg, hk, kv + 16 * t, kv_end, page[t], 16, bad);
       if (VAL)
-        run_values(p, t, row, n, one ? 16 * t : 0);
+        run_values(p, t, run.row, run.n, one ? 16 * t : 0);
       else
-        run_keys(p, t, row, n, one ? 16 * t : 0);
+        run_keys(p, t, run.row, run.n, one ? 16 * t : 0);
     }
   }
   // Key operand of run t, dims 32 k ..: 8-bit keys give a lane 16 dims of each 64.
@@ -1014,7 +1014,8 @@ struct FlashPlan {
 //    at 4096, 1 / 2 / 3: 60, 78, 70; 1 user at 1024, 1 / 4: 13.2, 11.2.
 //    8-bit pages need half the bytes and three workgroups fit a CU: where whole
 //    contexts leave 3/8 of the CUs idle three splits are better if the contexts
-//    differ (32 users up to 4096: 40.5, 39.0, 32.8), a little worse if not (38.9, 45.6, 41.8).
+//    differ (32 users up to 4096: 40.5, 39.0, 32.8), a little worse if not (38.9, 45.6, 41.8);
+//    from 2048 positions on (32 users at 1024, 1 / 3: 13.2, 18.4; at 2048: 24.6, 24.6).
 constexpr int64_t kMinChunk = 256;
 constexpr int64_t kMaxSplits = 256;
 inline FlashPlan flash_plan(int64_t T, int64_t H, int64_t Hkv, int64_t B, int64_t max_q, int64_t max_kv, bool paged,
@@ -1029,7 +1030,7 @@ inline FlashPlan flash_plan(int64_t T, int64_t H, int64_t Hkv, int64_t B, int64_
   int64_t n;
   if (f.few) {
     n = cus / f.tiles;
-    if (n == 1 && fp8 && 8 * f.tiles <= 5 * cus) n = 3;
+    if (n == 1 && fp8 && 8 * f.tiles <= 5 * cus && max_kv >= 8 * kMinChunk) n = 3;
   } else {
     n = (4 * cus + f.tiles) / (2 * f.tiles);
   }

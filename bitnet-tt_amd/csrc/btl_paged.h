@@ -74,6 +74,21 @@ __host__ __device__ __forceinline__ int64_t page_row(int32_t page, int P, int Hk
   return (page < 0 || page >= P) ? -1 : ((int64_t)page * Hkv + hk) * ps + row;
 }
 
+// A run of rows in a pool: index of the first, how many there are (none behind
+// kv_end, none in a page outside the pool).  Scalars, without a branch.
+struct Run {
+  int64_t row;
+  uint32_t n;
+};
+__device__ __forceinline__ Run run_at(const Pages& pg, int hk, int at, int kv_end, int32_t page, int most, bool& bad) {
+  const int left = clampi(kv_end - at, 0, most);
+  const bool none = (uint32_t)page >= (uint32_t)pg.P;
+  bad |= none & (left > 0);
+  const uint32_t id = none ? 0u : (uint32_t)page, ps = pg.ps.d;
+  const uint32_t in_page = (uint32_t)at - div_by((uint32_t)at, pg.ps) * ps;
+  return {(int64_t)((uint64_t)id * (uint32_t)(pg.Hkv * ps)) + (uint32_t)(hk * ps + in_page), none ? 0u : (uint32_t)left};
+}
+
 // ---- e4m3 rows with a power of two ---------------------------------------
 // Exponent of a row with largest magnitude a > 0: the least e >= -126 with
 // a <= 448 * 2^e (448 = 1.75 * 2^8 is the largest code).  Scaling by a power
