@@ -347,6 +347,8 @@ class BitLinearDecodeStep:
             raise RuntimeError("forward_rows needs alloc_paged() first")
         c = self.config
         T = hidden.shape[0]
+        if T == 0:
+            return hidden
         dev = hidden.device
         qkv = torch.empty((T, c.qkv_dim), dtype=torch.bfloat16, device=dev)
         attn = torch.empty((T, c.num_attention_heads * c.head_dim), dtype=torch.bfloat16, device=dev)

@@ -14,6 +14,9 @@ and the other ``check()`` methods read, and its outputs are invalid.  Rows with 
 negative position (kv_len below the number of rows: padding) give zeros and
 write nothing; rows outside [cu_q[0], cu_q[B]) are left as they were.
 
+Sequences may share pages that they only read; two rows of one call that are
+written must not be the same row of the same page, nor may outputs overlap pages.
+
 Calls are ordered on the current stream of their tensors' device.  Calls that
 write one cache, and calls that read what another writes, must be ordered by the caller;
 calls that only read it may overlap (each has its own scratch).
@@ -140,7 +143,7 @@ def _rows(t, T, heads, dim, name, index):
     ld, sh, sd = t.stride()
     if sd != 1 or (sh != dim and heads > 1):
         raise ValueError(f"{name}: the heads of a row must be dense")
-    if T <= 1 and ld < heads * dim:
+    if T <= 1:  # its stride says nothing
         ld = heads * dim
     if ld < heads * dim or ld % 8 or t.data_ptr() % 16:
         raise ValueError(f"{name}: rows must be 16-byte aligned and not overlap")

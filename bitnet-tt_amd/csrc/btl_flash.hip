@@ -455,7 +455,7 @@ __global__ __launch_bounds__(256, 2) void k_flash_tile(FlashArgs p) {
   const int tid = threadIdx.x, wv = uni(tid >> 6), lane = tid & 63, h = lane >> 5;
   const int hk = uni(blockIdx.x % p.Hkv), split = blockIdx.y;
   Item it;
-  if (!find_item(p.bt, p.G, kTileRows, blockIdx.x / p.Hkv, it)) return;
+  if (!find_item(p.bt, p.G, kTileRows, blockIdx.x / p.Hkv, it, p.error)) return;
   const Seq sq = load_seq(p.bt, it.b, (int64_t)p.bt.max_pages * p.pg.ps.d);
   if (!sq.ok && tid == 0) flag_error(p.error);
   const int rows = sq.n * p.G, first = sq.len - sq.n;  // position of the first token

@@ -125,17 +125,22 @@ __device__ __forceinline__ Seq load_seq(const Batch& bt, int b, int64_t cap) {
 
 // Item x of the sequences' items, sequence b having ceil(n_b * per / of): the
 // sequence and the item's number in it.  Every wave searches by itself, 64
-// sequences a step.  False where there are fewer items.
+// sequences a step.  False where there are fewer items.  A workgroup checks the sequences
+// that it passes, item 0's all of them: one that gives no item has no other reader.
 struct Item {
   int b, i, count;
 };
-__device__ __forceinline__ bool find_item(const Batch& bt, int per, int of, int x, Item& it) {
+__device__ __forceinline__ bool find_item(const Batch& bt, int per, int of, int x, Item& it, int32_t* error) {
   const int lane = __lane_id();
   int base = 0;
+  bool found = false, ok = true;
   for (int c = 0; c < bt.B; c += 64) {
     const int b = c + lane;
-    int n = 0;
-    if (b < bt.B) n = clamp_seq(bt.cu[b], bt.cu[b + 1], 0, bt.T, 0).n;
+    Seq s{0, 0, 0, true};
+    if (b < bt.B) s = clamp_seq(bt.cu[b], bt.cu[b + 1], 0, bt.T, 0);
+    ok &= s.ok;
+    if (found) continue;
+    const int n = s.n;
     const int cnt = (n * per + of - 1) / of;
     int inc = cnt;
 #pragma unroll
@@ -149,11 +154,13 @@ __device__ __forceinline__ bool find_item(const Batch& bt, int per, int of, int 
       it.b = uni(c + l);
       it.count = __builtin_amdgcn_readlane(cnt, l);
       it.i = uni(x - base - (__builtin_amdgcn_readlane(inc, l) - it.count));
-      return true;
+      found = true;
+      if (x > 0) break;
     }
     base += total;
   }
-  return false;
+  if (!ok) flag_error(error);
+  return found;
 }
 #endif
 

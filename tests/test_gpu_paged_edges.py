@@ -1,0 +1,147 @@
+"""Prompts and the paged cache on the GPU where a call is allowed and rare:
+shared pages, pools past 32-bit offsets, captured calls at once, entries of
+cu_q that no row reads, rows in wide buffers."""
+
+import math
+
+import pytest
+import torch
+
+from paged_helpers import PagedBatch, attend64, check_close, cu_of, dev, ints, normal, quantise, values_of
+
+from bitnet_tt import paged_attention as pa
+from bitnet_tt.utils.rope import rope_tables
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def no_error_left():
+    yield
+    pa.check("cuda:0")
+
+
+def expect_error():
+    with pytest.raises(RuntimeError, match="paged workspace"):
+        pa.check("cuda:0")
+
+
+@pytest.mark.parametrize("B", [3, 65, 130])
+@pytest.mark.parametrize("bad", [[1, 0], [2, 1], [1, -1]])
+def test_a_last_sequence_that_ends_before_it_begins(B, bad):
+    """One row, many empty sequences, and a last entry that is wrong: no row is in it."""
+    cu = ints([0] + [bad[0]] * (B - 1) + [bad[1]])
+    x = normal((1, 8, 64), 1).to(torch.bfloat16).to(dev())
+    pa.prompt_attention(x[:, :4], x[:, 4:6], x[:, 6:], cu)
+    expect_error()
+    cache = pa.PagedKVCache.allocate(2, 2, 64, dev(), page_size=16)
+    table, lens = torch.zeros((B, 1), dtype=torch.int32, device=dev()), ints([1] + [0] * (B - 1))
+    for max_q in (1, 40):
+        pa.paged_attention(x[:, :4].contiguous(), cache, table, cu, lens, max_q=max_q)
+        expect_error()
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+@pytest.mark.parametrize("max_q", [1, 40])
+def test_sequences_that_share_pages(kv, max_q):
+    """The same pages in every row of the table, lengths that end in different places of them."""
+    pb = PagedBatch([1], [100], 4, 2, 64, 16, kv, seed=4)
+    lens = [100, 1, 64, 17, 100]
+    q = normal((len(lens), 4, 64), 8, 1.5).to(torch.bfloat16)
+    table = pb.table.expand(len(lens), -1).contiguous()
+    out = pa.paged_attention(q.to(dev()), pb.cache, table, cu_of([1] * len(lens)), ints(lens), max_q=max_q)
+    k, v = pb.rows(pb.k64, 0), pb.rows(pb.v64, 0)
+    for b, n in enumerate(lens):
+        want, tol = attend64(q[b:b + 1].double(), k[:, :n], v[:, :n])
+        check_close(out[b:b + 1], want, tol)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+def test_pools_past_32_bit_offsets(kv):
+    """Pages whose rows lie more than 2^32 bytes (2^31 elements, where a row has two bytes) into the pool."""
+    H, Hkv, D, page = 4, 2, 128, 64
+    each = Hkv * page * D * (2 if kv == "bf16" else 1)
+    P = 2 ** 32 // each + 40
+    cache = pa.PagedKVCache.allocate(P, Hkv, D, dev(), page_size=page, dtype=kv)
+    near, far = 3, P - 2  # the last one's rows begin behind 2^32 bytes
+    assert far * each > 2 ** 32
+    ids = [far, near, far + 1]
+    table = torch.tensor([ids], dtype=torch.int32, device=dev())
+    n = 2 * page + 9
+    qkv = normal((n, (H + 2 * Hkv) * D), 5).to(torch.bfloat16)
+    cos, sin = (torch.from_numpy(t) for t in rope_tables(D, n, 1e4))
+    pa.rope_write(qkv.to(dev()), cos.to(dev()), sin.to(dev()), cu_of([n]), None, H, Hkv, cache=cache, page_table=table)
+    k = torch.empty((1, Hkv, n, D), dtype=torch.bfloat16, device=dev())
+    v = torch.empty_like(k)
+    pa.read_pages(cache, table, ints([n]), k, v)
+    want_v = qkv.view(n, H + 2 * Hkv, D)[:, H + Hkv:].float()
+    if kv == "fp8":
+        want_v = values_of(*quantise(want_v)).float()
+    assert torch.equal(v[0].cpu().float().transpose(0, 1), want_v)
+    for pool in (cache.key_pages, cache.value_pages):  # nothing landed where a wrapped offset would be
+        raw = pool.view(torch.uint8)
+        assert not bool(raw[:near].any()) and not bool(raw[near + 1: near + 40].any())
+    k64, v64 = k[0].double().cpu(), v[0].double().cpu()
+    for new, max_q in ((1, 1), (40, 40)):
+        q = normal((new, H, D), 7, 1.5).to(torch.bfloat16)
+        want, tol = attend64(q.double(), k64, v64)
+        out = pa.paged_attention(q.to(dev()), cache, table, cu_of([new]), ints([n]), max_q=max_q)
+        check_close(out, want, tol)
+
+
+def test_two_graphs_with_split_contexts_at_once():
+    """Each captured call has its own partials: replays on two streams, with eager work between."""
+    pbs = [PagedBatch([1], [5000], 4, 2, 64, 64, "bf16", seed=s) for s in (1, 2)]
+    runs = []
+    for pb in pbs:
+        args = (pb.q_dev, pb.cache, pb.table, pb.cu, pb.len)
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            want = pa.paged_attention(*args, max_q=1)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                out = pa.paged_attention(*args, max_q=1)
+        runs.append((stream, graph, out, want, args))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for _, _, out, _, _ in runs:
+            out.fill_(9.0)
+        torch.cuda.synchronize()
+        for stream, graph, _, _, _ in runs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        eager = [pa.paged_attention(*args, max_q=1) for _, _, _, _, args in runs]
+        torch.cuda.synchronize()
+        for (_, _, out, want, _), e in zip(runs, eager):
+            assert torch.equal(out, want) and torch.equal(e, want)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_rows_in_wide_buffers(D):
+    """Row strides of a million elements: a tile's rows span more than 2^27 bytes."""
+    n, H, Hkv, ld = 70, 2, 1, 1 << 20
+    x = normal((n, H + 2 * Hkv, D), 3, 1.2).to(torch.bfloat16)
+    wide = torch.full((n, ld), math.nan, dtype=torch.bfloat16, device=dev())
+    wide[:, : (H + 2 * Hkv) * D] = x.view(n, -1).to(dev())
+    w = wide[:, : (H + 2 * Hkv) * D].unflatten(1, (H + 2 * Hkv, D))
+    out = wide[:, -H * D:].unflatten(1, (H, D))
+    pa.prompt_attention(w[:, :H], w[:, H:H + Hkv], w[:, H + Hkv:], cu_of([n]), out=out)
+    want, tol = attend64(x[:, :H].double(), x[:, H:H + Hkv].double().transpose(0, 1),
+                         x[:, H + Hkv:].double().transpose(0, 1))
+    check_close(out, want, tol)
+    assert bool(wide[:, (H + 2 * Hkv) * D: ld - H * D].isnan().all())
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+def test_read_of_lengths_around_a_workgroups_rows(D, kv):
+    total = [0, 1, 15, 16, 17, 31, 32, 33, 47, 48]
+    pb = PagedBatch([0] * len(total), total, 2, 1, D, 16, kv)
+    k = torch.full((len(total), 1, 48, D), 3.0, dtype=torch.bfloat16, device=dev())
+    v = k.clone()
+    pa.read_pages(pb.cache, pb.table, pb.len, k, v)
+    for got, pool in ((k, pb.k64), (v, pb.v64)):
+        got = got.cpu()
+        for b, n in enumerate(total):
+            assert torch.equal(got[b, :, :n].double(), pb.rows(pool, b))
+            assert bool((got[b, :, n:] == 3.0).all())
