@@ -28,6 +28,9 @@
 // to the rows that do see it and multiplied with none: 0 x inf is NaN.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+#include <cmath>
+
 #include "btl.h"
 #include "btl_act_row.h"
 #include "btl_common.h"
@@ -1007,7 +1010,14 @@ struct FlashPlan {
 //  - Tiles: two workgroups fit a CU, and a call's tiles are mostly of unlike
 //    length, so as many as come nearest to two a CU.  1000 rows of one sequence at 9000
 //    positions (160 workgroups), 1 / 2 / 3 / 4 splits: 173, 128, 110, 123; 4 x 320 at
-//    8192 (220): 167, 141, 160, 150; 4 x 512 at 8192 (340): 234, 229, 224, 220.
+//    8192 (220): 167, 141, 160, 150; 4 x 512 at 8192 (340): 234, 229, 224, 220; 2047 rows of
+//    4 contexts of unlike length up to 8000 (339), 1 / 2: 172, 138.
+//    But a split costs the merge's launch (4 us) and the writing and reading of its
+//    partials, part = T H D 8 bytes at 4.8 TB/s each, and saves its share of the
+//    longest workgroup's steps, whole = 0.75 us per 64 positions: the least of whole / n + n part is
+//    at n = sqrt(whole / part), and n = 1 is better where that saves less than it costs.
+//    Without this, with it: 2 x 512 rows at 512: 27.4, 17.8; 4 x 256 at 1024: 36.0, 26.8;
+//    1000 at 1000: 28.9, 26.6; 512 at 2048: 34.9, 31.0; 256 at 1024: 23.2, 24.2.
 //  - Few rows: bound by memory, which one workgroup a CU saturates: as many
 //    as there are CUs, from 1024 positions on.  bf16, 1 user at 16384, 16 / 25 / 51 / 102
 //    splits: 20.1, 17.8, 16.5, 20.6; 8 users at 4096, 3 / 6 / 8: 24.3, 21.2, 24.6; 32 users
@@ -1018,8 +1028,8 @@ struct FlashPlan {
 //    from 2048 positions on (32 users at 1024, 1 / 3: 13.2, 18.4; at 2048: 24.6, 24.6).
 constexpr int64_t kMinChunk = 256;
 constexpr int64_t kMaxSplits = 256;
-inline FlashPlan flash_plan(int64_t T, int64_t H, int64_t Hkv, int64_t B, int64_t max_q, int64_t max_kv, bool paged,
-                            bool fp8) {
+inline FlashPlan flash_plan(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t B, int64_t max_q, int64_t max_kv,
+                            bool paged, bool fp8) {
   FlashPlan f{};
   const int64_t G = H / Hkv, cus = device_cus();
   f.few = paged && max_q * G <= kFewRows;
@@ -1033,6 +1043,9 @@ inline FlashPlan flash_plan(int64_t T, int64_t H, int64_t Hkv, int64_t B, int64_
     if (n == 1 && fp8 && 8 * f.tiles <= 5 * cus && max_kv >= 8 * kMinChunk) n = 3;
   } else {
     n = (4 * cus + f.tiles) / (2 * f.tiles);
+    const double whole = 0.0117 * (double)max_kv, part = 1.67e-6 * (double)(T * H * D);  // us
+    n = std::min(n, (int64_t)(std::sqrt(whole / part) + 0.5));
+    if (n > 1 && whole - whole / (double)n <= 4.0 + part * (double)n) n = 1;
   }
   if (n > max_kv / kMinChunk) n = max_kv / kMinChunk;
   if (n > kMaxSplits) n = kMaxSplits;
@@ -1104,7 +1117,7 @@ int btl_prompt_attention(const uint16_t* q, int64_t ldq, const uint16_t* k, int6
   a.ldk = ldk;
   a.ldv = ldv;
   a.splits = 1;
-  const FlashPlan f = flash_plan(T, H, Hkv, B, T, T, false, false);
+  const FlashPlan f = flash_plan(T, H, Hkv, D, B, T, T, false, false);
   const dim3 grid((unsigned)f.tiles);
   if (D == 128)
     hipLaunchKernelGGL((k_flash_tile<128, kDense>), grid, dim3(256), 0, (hipStream_t)stream, a);
@@ -1116,7 +1129,7 @@ int btl_prompt_attention(const uint16_t* q, int64_t ldq, const uint16_t* k, int6
 int64_t btl_paged_attention_scratch_bytes(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t B, int64_t max_q,
                                           int64_t max_kv, int fp8) {
   if (T <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || B <= 0 || max_q <= 0 || max_kv <= 0) return 0;
-  return flash_scratch(flash_plan(T, H, Hkv, B, max_q, max_kv, true, fp8 != 0), T, H, D);
+  return flash_scratch(flash_plan(T, H, Hkv, D, B, max_q, max_kv, true, fp8 != 0), T, H, D);
 }
 
 int btl_paged_attention(const uint16_t* q, int64_t ldq, int64_t T, int64_t H, const btl_pages_t* pages,
@@ -1139,7 +1152,7 @@ int btl_paged_attention(const uint16_t* q, int64_t ldq, int64_t T, int64_t H, co
   if (T == 0) return BTL_OK;
   if (!page_table || !kv_len) return set_error(BTL_ERR_NULL, "%s: NULL pointer", who);
   const bool fp8 = pages->k_exp != nullptr;
-  const FlashPlan f = flash_plan(T, H, Hkv, B, max_q, max_kv, true, fp8);
+  const FlashPlan f = flash_plan(T, H, Hkv, D, B, max_q, max_kv, true, fp8);
   if (f.few && B > 65535) return set_error(BTL_ERR_SHAPE, "%s: %lld sequences", who, (long long)B);
   const int64_t need = flash_scratch(f, T, H, D);
   if (need > 0) {
