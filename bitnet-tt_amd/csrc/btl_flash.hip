@@ -154,12 +154,15 @@ __device__ __forceinline__ v4s lds_tr16(const lds8* p) {
 // workgroup's.  (The second product one step behind as well, so that nothing
 // in a step depends on anything else in it: the same speed, and 30 registers more than there are.)
 //
-// Bound by the matrix units' and the vector units' issue: at 16001 tokens of 20 / 5 heads of
-// 128, 405 us, 1000 TFLOP/s (a large library product reaches 1360), the matrix units are
-// busy 51% of the cycles and the vector units 41%, and the LDS 26%.  Over pages, 8192 tokens: 1005
-// TFLOP/s; 8-bit pages, which are converted on the way, 955.  Measured beside it: 64 rows a
-// wave, 795 (one wave a SIMD: nothing runs under a wait); 32 positions a step and
-// three workgroups a CU, 963; keys and values through registers to LDS, 843.
+// Bound by how far one wave's matrix work covers the other's vector work on a SIMD: at
+// 16001 tokens of 20 / 5 heads of 128, 390-415 us, 980-1045 TFLOP/s (a large library
+// product reaches 1360), the matrix units are busy 58% of the cycles and the vector units 47%;
+// reading LDS alone would take 155 us.  Over pages, 8192 tokens: 1005 TFLOP/s; 8-bit
+// pages, which are converted on the way, 955.  Measured beside it, in TFLOP/s: 64 rows a wave
+// and one wave a SIMD, which halves the reading of LDS, 904 with 32 positions a
+// step and 860 with 64; 32 rows and 32 positions 1018; all products of a step together and all
+// exponentials after them 1003, with a raised priority for the products 980; keys and values
+// through registers to LDS 843.
 //
 // 16-byte pieces of a row are stored at piece ^ f(row), for the LDS's 64 banks:
 // the 16 rows that 16 lanes read a piece of, and the 4 rows x 64 bytes that 32 lanes
@@ -946,53 +949,49 @@ __global__ __launch_bounds__(64 * kFewWaves, KV == kPagedFp8 ? 3 : 2) void k_fla
 
 // The splits' partials of a row, in an order that the number of splits fixes:
 // a group of D / 4 threads sums every `groups`-th split of a row, then the first of a
-// row's groups sums the groups.
+// row's groups sums the groups.  Bound by latency: one pass with a running maximum (a pass
+// for the maximum before it: 20 rows of 47 splits 6.7 us, 4.8 so).
+struct MergeSum {
+  float m = kNegInf, l = 0.0f;
+  v4f o = (v4f){0.f, 0.f, 0.f, 0.f};
+  __device__ __forceinline__ void add(float m2, float l2, float4 o2) {
+    const bool none = empty(m2, l2);
+    const float mn = fmaxf(m, m2), a = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+    const float f = none ? 0.0f : __builtin_amdgcn_exp2f(m2 - mn);
+    m = mn;
+    l = a * l + (none ? 0.0f : f * l2);
+    o[0] = a * o[0] + (none ? 0.0f : f * o2.x);
+    o[1] = a * o[1] + (none ? 0.0f : f * o2.y);
+    o[2] = a * o[2] + (none ? 0.0f : f * o2.z);
+    o[3] = a * o[3] + (none ? 0.0f : f * o2.w);
+  }
+};
 template <int D>
 __global__ __launch_bounds__(256) void k_flash_merge(FlashArgs p, int groups) {
   constexpr int TG = D / 4, NG = 256 / TG;
   __shared__ float4 s_o[NG][TG];
-  __shared__ float s_l[NG];
+  __shared__ float2 s_ml[NG];
   const int t = threadIdx.x % TG, g = threadIdx.x / TG, z0 = g % groups;
-  const int64_t n = (int64_t)p.bt.T * p.H, row = (int64_t)blockIdx.x * (NG / groups) + g / groups;  // (token, head)
-  const int tok = (int)(row / p.H), head = (int)(row - (int64_t)tok * p.H);
+  const int n = p.bt.T * p.H, row = blockIdx.x * (NG / groups) + g / groups;  // (token, head)
+  const int tok = (int)((uint32_t)row / (uint32_t)p.H), head = row - tok * p.H;
   const bool live = tok >= max(0, p.bt.cu[0]) && tok < min(p.bt.T, p.bt.cu[p.bt.B]) && p.part_ml[row].y != kWhole;
-  float M = kNegInf, L = 0.0f;
-  v4f O = (v4f){0.f, 0.f, 0.f, 0.f};
+  MergeSum s;
   if (live) {
-    for (int z = t; z < p.splits; z += TG) M = fmaxf(M, p.part_ml[z * n + row].x);
-    if (TG == 32) M = fmaxf(M, xor_partner<16>(M));
-    M = fmaxf(M, xor_partner<8>(M));
-    M = fmaxf(M, xor_partner<4>(M));
-    M = fmaxf(M, xor_partner<2>(M));
-    M = fmaxf(M, xor_partner<1>(M));
 #pragma unroll 4
-    for (int z = z0; z < p.splits; z += groups) {
-      const float2 ml = p.part_ml[z * n + row];
-      if (empty(ml.x, ml.y)) continue;
-      const float f = __builtin_amdgcn_exp2f(ml.x - M);
-      const float4 o = *reinterpret_cast<const float4*>(p.part_o + (z * n + row) * D + 4 * t);
-      L += f * ml.y;
-      O[0] += f * o.x;
-      O[1] += f * o.y;
-      O[2] += f * o.z;
-      O[3] += f * o.w;
+    for (int z = z0; z < p.splits; z += groups) {  // (an empty split's products are not read: any values)
+      const int64_t at = (int64_t)z * n + row;
+      const float2 ml = p.part_ml[at];
+      s.add(ml.x, ml.y, *reinterpret_cast<const float4*>(p.part_o + at * D + 4 * t));
     }
   }
-  s_o[g][t] = make_float4(O[0], O[1], O[2], O[3]);
-  if (t == 0) s_l[g] = L;
+  s_o[g][t] = make_float4(s.o[0], s.o[1], s.o[2], s.o[3]);
+  if (t == 0) s_ml[g] = make_float2(s.m, s.l);
   __syncthreads();
   if (!live || z0 != 0) return;
-  for (int i = 1; i < groups; ++i) {
-    const float4 o = s_o[g + i][t];
-    O[0] += o.x;
-    O[1] += o.y;
-    O[2] += o.z;
-    O[3] += o.w;
-    L += s_l[g + i];
-  }
-  const float inv = empty(M, L) ? 0.0f : 1.0f / L;
+  for (int i = 1; i < groups; ++i) s.add(s_ml[g + i].x, s_ml[g + i].y, s_o[g + i][t]);
+  const float inv = empty(s.m, s.l) ? 0.0f : 1.0f / s.l;
   *reinterpret_cast<uint2*>(p.out + tok * p.ldo + head * D + 4 * t) =
-      make_uint2(f2bf_pair(O[0] * inv, O[1] * inv), f2bf_pair(O[2] * inv, O[3] * inv));
+      make_uint2(f2bf_pair(s.o[0] * inv, s.o[1] * inv), f2bf_pair(s.o[2] * inv, s.o[3] * inv));
 }
 
 // ---- host ---------------------------------------------------------------
