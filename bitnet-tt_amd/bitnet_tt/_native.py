@@ -155,7 +155,7 @@ EXPORTS = {
         [_P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _F, _I64, _P, _I64, _P, _P],
         _I,
     ),
-    "btl_paged_attention_scratch_bytes": ([_I64, _I64, _I64, _I64, _I64, _I64, _I64, _I], _I64),
+    "btl_paged_attention_scratch_bytes": ([_I64, _I64, _I64, _I64, _I64, _I64, _I64], _I64),
     "btl_paged_attention": (
         [_P, _I64, _I64, _I64, _PGP, _P, _I64, _P, _P, _I64, _F, _I64, _I64, _P, _I64, _P, _SZ, _P, _P],
         _I,

@@ -327,7 +327,7 @@ def paged_attention(q, cache: PagedKVCache, page_table, cu_q, kv_len, scale: flo
     if max_q < 1 or max_kv < 1:
         raise ValueError(f"max_q {max_q} and max_kv {max_kv} must be at least 1")
     stream = N.raw_stream(index)
-    nbytes = _scratch_bytes(index, T, H, Hkv, D, B, max_q, max_kv, cache._tensors[2] is not None)
+    nbytes = _scratch_bytes(index, T, H, Hkv, D, B, max_q, max_kv)
     # the call's own, from the stream-ordered allocator: calls that overlap share nothing
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
     rc = N.lib().btl_paged_attention(
@@ -340,9 +340,8 @@ def paged_attention(q, cache: PagedKVCache, page_table, cu_q, kv_len, scale: flo
 
 
 @functools.lru_cache(maxsize=4096)
-def _scratch_bytes(index: int, T: int, H: int, Hkv: int, D: int, B: int, max_q: int, max_kv: int,
-                   fp8: bool = False) -> int:
-    return int(N.lib().btl_paged_attention_scratch_bytes(T, H, Hkv, D, B, max_q, max_kv, int(fp8)))
+def _scratch_bytes(index: int, T: int, H: int, Hkv: int, D: int, B: int, max_q: int, max_kv: int) -> int:
+    return int(N.lib().btl_paged_attention_scratch_bytes(T, H, Hkv, D, B, max_q, max_kv))
 
 
 def check(device=None) -> None:

@@ -654,8 +654,8 @@ __global__ __launch_bounds__(256, 2) void k_flash_tile(FlashArgs p) {
 // 8-bit pages) are on their way nearly all the time.  Page table entries are
 // fetched a round ahead of that.  The waves' partials meet in LDS.
 //
-// 5 heads of 128: one user at 131001 positions 67 us (5.0 TB/s, merge included), 48 users
-// at 4096 90 us (5.6 TB/s); 8-bit pages 48 us (5.3).  8 / 4 / 2 waves a workgroup, each
+// 5 heads of 128: one user at 131001 positions 59 us (5.7 TB/s) and 5 of the merge, 128
+// users at 2048 124 us (5.4 TB/s); 8-bit pages 69 us (4.9).  8 / 4 / 2 waves a workgroup, each
 // at its best number of splits, 32 users of mixed lengths up to 4096, 8-bit pages: 38.5, 36.9,
 // 36.2 us; one user at 512 positions: 10.7, 9.7, 13.0.
 // ======================================================================
@@ -1021,14 +1021,17 @@ struct FlashPlan {
 //    as there are CUs, from 1024 positions on.  bf16, 1 user at 16384, 16 / 25 / 51 / 102
 //    splits: 20.1, 17.8, 16.5, 20.6; 8 users at 4096, 3 / 6 / 8: 24.3, 21.2, 24.6; 32 users
 //    at 4096, 1 / 2 / 3: 60, 78, 70; 1 user at 1024, 1 / 4: 13.2, 11.2.
-//    8-bit pages need half the bytes and three workgroups fit a CU: where whole
-//    contexts leave 3/8 of the CUs idle three splits are better if the contexts
-//    differ (32 users up to 4096: 40.5, 39.0, 32.8), a little worse if not (38.9, 45.6, 41.8);
-//    from 2048 positions on (32 users at 1024, 1 / 3: 13.2, 18.4; at 2048: 24.6, 24.6).
+//    Up to 9/4 as many workgroups as CUs, some CUs have a long context more than others:
+//    four splits from 2560 positions on.  Contexts of unlike length up to 4000, 1 / 2 / 3 / 4 / 6:
+//    bf16, 36 users 53, 56, 49, 43, 49; 56: 100, 70, 65, 65, 66; 80: 107, 84, 85, 85, 87; 110: 125,
+//    116, 115, 114, 116; 8-bit, 56: 48, 45, 40, 34, 37; 110: 84, 68, 69, 67, 68.  All of 4000,
+//    bf16: 36: 69, 82, 82, 72, 76; 56: 138, 121, 117, 110, 110; 110: 227, 214, 209, 203, 207.  At 2048 positions,
+//    1 / 4, unlike or alike, the gain is gone: bf16, 32 users 25.7, 27.2 or 33.7, 37.5;
+//    140: 86, 86 or 134, 138.
 constexpr int64_t kMinChunk = 256;
 constexpr int64_t kMaxSplits = 256;
 inline FlashPlan flash_plan(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t B, int64_t max_q, int64_t max_kv,
-                            bool paged, bool fp8) {
+                            bool paged) {
   FlashPlan f{};
   const int64_t G = H / Hkv, cus = device_cus();
   f.few = paged && max_q * G <= kFewRows;
@@ -1039,7 +1042,7 @@ inline FlashPlan flash_plan(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_
   int64_t n;
   if (f.few) {
     n = cus / f.tiles;
-    if (n == 1 && fp8 && 8 * f.tiles <= 5 * cus && max_kv >= 8 * kMinChunk) n = 3;
+    if (n <= 1 && 4 * f.tiles <= 9 * cus && max_kv >= 10 * kMinChunk) n = 4;
   } else {
     n = (4 * cus + f.tiles) / (2 * f.tiles);
     const double whole = 0.0117 * (double)max_kv, part = 1.67e-6 * (double)(T * H * D);  // us
@@ -1116,7 +1119,7 @@ int btl_prompt_attention(const uint16_t* q, int64_t ldq, const uint16_t* k, int6
   a.ldk = ldk;
   a.ldv = ldv;
   a.splits = 1;
-  const FlashPlan f = flash_plan(T, H, Hkv, D, B, T, T, false, false);
+  const FlashPlan f = flash_plan(T, H, Hkv, D, B, T, T, false);
   const dim3 grid((unsigned)f.tiles);
   if (D == 128)
     hipLaunchKernelGGL((k_flash_tile<128, kDense>), grid, dim3(256), 0, (hipStream_t)stream, a);
@@ -1126,9 +1129,9 @@ int btl_prompt_attention(const uint16_t* q, int64_t ldq, const uint16_t* k, int6
 }
 
 int64_t btl_paged_attention_scratch_bytes(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t B, int64_t max_q,
-                                          int64_t max_kv, int fp8) {
+                                          int64_t max_kv) {
   if (T <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || B <= 0 || max_q <= 0 || max_kv <= 0) return 0;
-  return flash_scratch(flash_plan(T, H, Hkv, D, B, max_q, max_kv, true, fp8 != 0), T, H, D);
+  return flash_scratch(flash_plan(T, H, Hkv, D, B, max_q, max_kv, true), T, H, D);
 }
 
 int btl_paged_attention(const uint16_t* q, int64_t ldq, int64_t T, int64_t H, const btl_pages_t* pages,
@@ -1151,7 +1154,7 @@ int btl_paged_attention(const uint16_t* q, int64_t ldq, int64_t T, int64_t H, co
   if (T == 0) return BTL_OK;
   if (!page_table || !kv_len) return set_error(BTL_ERR_NULL, "%s: NULL pointer", who);
   const bool fp8 = pages->k_exp != nullptr;
-  const FlashPlan f = flash_plan(T, H, Hkv, D, B, max_q, max_kv, true, fp8);
+  const FlashPlan f = flash_plan(T, H, Hkv, D, B, max_q, max_kv, true);
   if (f.few && B > 65535) return set_error(BTL_ERR_SHAPE, "%s: %lld sequences", who, (long long)B);
   const int64_t need = flash_scratch(f, T, H, D);
   if (need > 0) {

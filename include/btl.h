@@ -481,11 +481,10 @@ int btl_prompt_attention(const uint16_t* q, int64_t ldq, const uint16_t* k, int6
  * of kv_len of any sequence where known, else T and max_pages * page_size
  * (hints, as above).  Long contexts of few rows are split over workgroups,
  * whose partials are merged in a fixed order by a second launch: scratch, 16-byte aligned, of
- * btl_paged_attention_scratch_bytes with the same arguments (fp8: whether the pages are
- * 8-bit; 0: not split) on the same device; its content is neither read nor kept, and calls that may run at once
+ * btl_paged_attention_scratch_bytes with the same arguments (0: not split) on the same device; its content is neither read nor kept, and calls that may run at once
  * need one each. */
 int64_t btl_paged_attention_scratch_bytes(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t B, int64_t max_q,
-                                          int64_t max_kv, int fp8);
+                                          int64_t max_kv);
 int btl_paged_attention(const uint16_t* q, int64_t ldq, int64_t T, int64_t H, const btl_pages_t* pages,
                         const int32_t* page_table, int64_t max_pages, const int32_t* cu_q, const int32_t* kv_len,
                         int64_t B, float scale, int64_t max_q, int64_t max_kv, uint16_t* out, int64_t ldo,

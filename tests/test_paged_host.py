@@ -109,11 +109,11 @@ def test_no_rows_is_no_launch(L):
 
 def test_scratch_bytes(L):
     f = L.btl_paged_attention_scratch_bytes
-    assert f(32, 20, 5, 128, 32, 1, 512, 0) == 0  # a context that is not worth a split
-    n = f(1, 20, 5, 128, 1, 1, 131072, 0)
+    assert f(32, 20, 5, 128, 32, 1, 512) == 0  # a context that is not worth a split
+    n = f(1, 20, 5, 128, 1, 1, 131072)
     assert n > 0 and n % (20 * 130 * 4) == 0
-    assert f(0, 20, 5, 128, 1, 1, 4096, 0) == 0 and f(1, 20, 3, 128, 1, 1, 4096, 0) == 0
-    assert f(32, 20, 5, 128, 32, 1, 4096, 1) > f(32, 20, 5, 128, 32, 1, 4096, 0) == 0  # 160 workgroups, 8-bit pages
+    assert f(0, 20, 5, 128, 1, 1, 4096) == 0 and f(1, 20, 3, 128, 1, 1, 4096) == 0
+    assert f(32, 20, 5, 128, 32, 1, 4096) > f(300, 20, 5, 128, 300, 1, 4096) == 0  # 160 workgroups, 1500
 
 
 def test_page_of_a_position(L):
