@@ -211,7 +211,7 @@ def rope_write(qkv, rope_cos, rope_sin, cu_q, kv_len, num_heads: int, num_kv_hea
         max_pages = _table(page_table, index, B)
         pages, table = cache._pages, page_table.data_ptr()
     if q_out is None:
-        q_out = torch.empty((T, H, D), dtype=_BF16, device=qkv.device)
+        q_out = qkv.new_empty(T, H, D)
         ldq = H * D
     else:
         ldq = _rows(q_out, T, H, D, "q_out", index)
@@ -276,7 +276,7 @@ def prompt_attention(q, k, v, cu_seqlens, scale: float | None = None, max_q: int
     ldk, ldv = _rows(k, T, Hkv, D, "k", index), _rows(v, T, Hkv, D, "v", index)
     B = _sequences(cu_seqlens, index)
     if out is None:
-        out = torch.empty((T, H, D), dtype=_BF16, device=q.device)
+        out = q.new_empty(T, H, D)
         ldo = H * D
     else:
         ldo = _rows(out, T, H, D, "out", index)
@@ -318,7 +318,7 @@ def paged_attention(q, cache: PagedKVCache, page_table, cu_q, kv_len, scale: flo
     max_q = T if max_q is None or max_q > T else max_q
     max_kv = most if max_kv is None or max_kv > most else max_kv
     if out is None:
-        out = torch.empty((T, H, D), dtype=_BF16, device=q.device)
+        out = q.new_empty(T, H, D)
         ldo = H * D
     else:
         ldo = _rows(out, T, H, D, "out", index)
