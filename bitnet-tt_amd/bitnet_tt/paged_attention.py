@@ -260,7 +260,7 @@ def prompt_attention(q, k, v, cu_seqlens, scale: float | None = None, max_q: int
 
     q bf16 [T, H, D], k and v [T, Hkv, D] (parts of a QKV row will do: rows may
     be strided); cu_seqlens int32 [B + 1]; scale, positive, defaults to 1/sqrt(D); max_q,
-    where known, is the longest sequence (a hint).  Returns bf16 [T, H, D]
+    where known, is the longest sequence (a hint that the present kernel has no use for).  Returns bf16 [T, H, D]
     (``out``, which must not overlap the inputs)."""
     index = _gpu(q, "q")
     if index != torch.cuda.current_device():

@@ -19,9 +19,9 @@
 // Softmax in base 2: p = 2^(c' s - m), c' = c log2(e), in fp32; m, a whole number,
 // is raised to the running maximum's ceiling only where that is more than kLazy
 // above it (p then stays below 2^kLazy, which costs an fp32 sum nothing), and the
-// factors that this puts on what has been summed are powers of two: exact.  p is rounded to bf16 for the second product, the matrix units'
-// operand type, and the sum takes the same rounded values, so the weights that
-// are used sum to one.
+// factors that this puts on what has been summed are powers of two: exact.  p is
+// rounded to bf16 for the second product, the matrix units' operand type, and the
+// sum takes the same rounded values, so the weights that are used sum to one.
 //
 // Rows of V behind the last position read as zero (whatever lies there), and a
 // value that is not finite at a position that some of the tile's rows may not see is added

@@ -13,8 +13,8 @@
 // neighbouring lanes and its maximum three lane exchanges.  A workgroup takes
 // whole tokens: one where there are few, so that every row has a workgroup,
 // else 8, which looks the sequences up once for 1920 pieces of the 2B heads.
-// 32 single tokens of 20 / 5 heads of 128 4.0 us; prompts of 8192 tokens to 8-bit pages 27.9 us,
-// 115 MB at 4.1 TB/s.  (Ordinary stores: what is written is read by the attention next.)
+// 32 single tokens of 20 / 5 heads of 128 4.0 us; prompts of 8191 tokens to 8-bit pages 27.8 us,
+// 120 MB at 4.3 TB/s.  (Ordinary stores: what is written is read by the attention next.)
 //
 // k_read_pages: rows of pages -> a contiguous [B, Hkv, S, D] bf16 cache, a copy
 // (or one conversion per two values).  Bound by memory: small workgroups whose

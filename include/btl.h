@@ -469,8 +469,8 @@ int btl_read_pages(const btl_pages_t* pages, const int32_t* page_table, int64_t 
  * q_i.k_j) v_j over the rows j <= i of i's sequence, query head h reading
  * key-value head h / (H / Hkv).  q, k, v bf16, element (t, h, d) at
  * t * ld + h * D + d (parts of a QKV row, say); out [T, H, D] with row stride
- * ldo.  scale > 0.  H / Hkv <= 64.  max_q: an upper bound of the sequences' lengths where
- * known, else T (a hint: results do not depend on it beyond rounding). */
+ * ldo.  scale > 0.  H / Hkv <= 64.  max_q >= 0: an upper bound of the sequences' lengths
+ * where known, else T; a hint that the present kernel has no use for. */
 int btl_prompt_attention(const uint16_t* q, int64_t ldq, const uint16_t* k, int64_t ldk, const uint16_t* v,
                          int64_t ldv, int64_t T, int64_t H, int64_t Hkv, int64_t D, const int32_t* cu_q, int64_t B,
                          float scale, int64_t max_q, uint16_t* out, int64_t ldo, int32_t* error_word,
@@ -479,10 +479,11 @@ int btl_prompt_attention(const uint16_t* q, int64_t ldq, const uint16_t* k, int6
 /* Attention of the newest tokens over the pages: the row at position p attends
  * to positions [0, p].  max_q and max_kv: upper bounds of the new tokens and
  * of kv_len of any sequence where known, else T and max_pages * page_size
- * (hints, as above).  Long contexts of few rows are split over workgroups,
- * whose partials are merged in a fixed order by a second launch: scratch, 16-byte aligned, of
- * btl_paged_attention_scratch_bytes with the same arguments (0: not split) on the same device; its content is neither read nor kept, and calls that may run at once
- * need one each. */
+ * (hints: they choose the kernel and the split, results depend on them in rounding
+ * only).  Long contexts of few rows are split over workgroups, whose partials are
+ * merged in a fixed order by a second launch: scratch, 16-byte aligned, of
+ * btl_paged_attention_scratch_bytes with the same arguments (0: not split) on the same
+ * device; its content is neither read nor kept, and calls that may run at once need one each. */
 int64_t btl_paged_attention_scratch_bytes(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t B, int64_t max_q,
                                           int64_t max_kv);
 int btl_paged_attention(const uint16_t* q, int64_t ldq, int64_t T, int64_t H, const btl_pages_t* pages,
