@@ -40,7 +40,7 @@ class PagedKVCache:
     """One layer's page pools: ``key_pages`` and ``value_pages`` [num_pages,
     kv_heads, page_size, head_dim] bf16, or float8_e4m3fn with one exponent byte
     per row in ``key_exp`` and ``value_exp`` [num_pages, kv_heads, page_size]
-    uint8 (a value is code x 2^(byte - 127)).  page_size is a multiple of 16;
+    uint8 (a value is code x 2^(byte - 127), bytes 1 .. 247).  page_size is a multiple of 16;
     head_dim 64 or 128.  The pools are written in place, never replaced.  The
     contiguous caches of DecodeAttention are pages of max_seq_len rows: :meth:`of_cache`."""
 

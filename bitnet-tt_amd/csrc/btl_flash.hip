@@ -1010,7 +1010,9 @@ struct FlashPlan {
 //    length, so as many as come nearest to two a CU.  1000 rows of one sequence at 9000
 //    positions (160 workgroups), 1 / 2 / 3 / 4 splits: 173, 128, 110, 123; 4 x 320 at
 //    8192 (220): 167, 141, 160, 150; 4 x 512 at 8192 (340): 234, 229, 224, 220; 2047 rows of
-//    4 contexts of unlike length up to 8000 (339), 1 / 2: 172, 138.
+//    4 contexts of unlike length up to 8000 (339), 1 / 2 / 3 / 4: 172, 143, 165, 155.  Up to three
+//    a CU two splits still even out the lengths, 1 / 2 / 3: 8 x 256 up to 8000 (360): 146, 132, 148;
+//    16 x 128 (400): 163, 143, 155; 4000 rows of one at 8000 (630): 290, 271, 286.
 //    But a split costs the merge's launch (4 us) and the writing and reading of its
 //    partials, part = T H D 8 bytes at 4.8 TB/s each, and saves its share of the
 //    longest workgroup's steps, whole = 0.75 us per 64 positions: the least of whole / n + n part is
@@ -1044,7 +1046,7 @@ inline FlashPlan flash_plan(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_
     n = cus / f.tiles;
     if (n <= 1 && 4 * f.tiles <= 9 * cus && max_kv >= 10 * kMinChunk) n = 4;
   } else {
-    n = (4 * cus + f.tiles) / (2 * f.tiles);
+    n = std::max((4 * cus + f.tiles) / (2 * f.tiles), (int64_t)(f.tiles <= 3 * cus ? 2 : 1));
     const double whole = 0.0117 * (double)max_kv, part = 1.67e-6 * (double)(T * H * D);  // us
     n = std::min(n, (int64_t)(std::sqrt(whole / part) + 0.5));
     if (n > 1 && whole - whole / (double)n <= 4.0 + part * (double)n) n = 1;

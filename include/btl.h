@@ -414,7 +414,7 @@ int btl_decode_attention_split(const uint16_t* qkv, int64_t B, int64_t H, int64_
  * Pages: k, v [num_pages, num_kv_heads, page_size, head_dim], bf16 where k_exp
  * and v_exp are NULL, else e4m3 codes (OCP) with one exponent byte per row in
  * k_exp, v_exp [num_pages, num_kv_heads, page_size]: a value is code x
- * 2^(byte - 127).  page_size a multiple of 16 up to 2^20, head_dim 64 or 128.
+ * 2^(byte - 127), bytes 1 .. 247.  page_size a multiple of 16 up to 2^20, head_dim 64 or 128.
  * Position p of sequence b is row p % page_size of page
  * page_table[b][p / page_size] (int32 [B][max_pages], device).  A contiguous
  * cache [B, Hkv, S, D] is pages of S rows.
