@@ -191,11 +191,11 @@ def rope_write(qkv, rope_cos, rope_sin, cu_q, kv_len, num_heads: int, num_kv_hea
         raise ValueError(f"qkv must be contiguous bf16 [T, ({H} + 2 * {Hkv}) * head_dim]")
     T, D = shape[0], shape[1] // heads
     angles = rope_cos.shape
-    for t, name in ((rope_cos, "rope_cos"), (rope_sin, "rope_sin")):
-        if t.dtype is not torch.float32 or len(angles) != 2 or t.shape != angles or not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous fp32 [positions, rotated dims / 2]")
-        if t.get_device() != index:
-            raise ValueError(f"{name} is on {t.device}, qkv on {qkv.device}")
+    if (len(angles) != 2 or rope_sin.shape != angles or rope_cos.dtype is not torch.float32
+            or rope_sin.dtype is not torch.float32 or not rope_cos.is_contiguous() or not rope_sin.is_contiguous()):
+        raise ValueError("rope_cos and rope_sin must be contiguous fp32 [positions, rotated dims / 2], alike")
+    if rope_cos.get_device() != index or rope_sin.get_device() != index:
+        raise ValueError(f"rope_cos is on {rope_cos.device}, rope_sin on {rope_sin.device}, qkv on {qkv.device}")
     B = _sequences(cu_q, index)
     if kv_len is not None:
         _int32(kv_len, index, (B,), "kv_len")
