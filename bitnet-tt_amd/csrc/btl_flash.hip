@@ -21,7 +21,8 @@
 // above it (p then stays below 2^kLazy, which costs an fp32 sum nothing), and the
 // factors that this puts on what has been summed are powers of two: exact.  p is
 // rounded to bf16 for the second product, the matrix units' operand type, and the
-// sum takes the same rounded values, so the weights that are used sum to one.
+// sum takes the same rounded values, so the weights that are used sum to one (few rows over bf16
+// pages: 16 bits of p).
 //
 // Rows of V behind the last position read as zero (whatever lies there), and a
 // value that is not finite at a position that some of the tile's rows may not see is added
@@ -656,6 +657,11 @@ __global__ __launch_bounds__(256, 2) void k_flash_tile(FlashArgs p) {
 // 8-bit pages) are on their way nearly all the time.  Page table entries are
 // fetched a round ahead of that.  The waves' partials meet in LDS.
 //
+// Over bf16 pages p is two bf16 values, itself rounded and what that leaves, so 16 bits of it
+// are used: the matrix units have the time (one user at 131001 positions 66.0 us, 66.2 so; 128 users at 2048
+// 121 and 120), and the error against 64 bits is that of the output's own rounding.  8-bit
+// pages, whose values have 4 bits, cost 1 to 8% for it and have one.
+//
 // 5 heads of 128: one user at 131001 positions 59 us (5.7 TB/s) and 5 of the merge, 128
 // users at 2048 124 us (5.4 TB/s); 8-bit pages 69 us (4.9).  8 / 4 / 2 waves a workgroup, each
 // at its best number of splits, 32 users of mixed lengths up to 4096, 8-bit pages: 38.5, 36.9,
@@ -688,6 +694,7 @@ struct Few {
   static constexpr int kK = kRowBytes / 64;                 // key loads of a lane for a run
   static constexpr int kV = kRowBytes / 64;                 // value loads of a lane for a run
   static constexpr int kTpr = kRowBytes / 16;               // lanes of a value row
+  static constexpr bool kRest = KV == kPagedBf16;           // p as two bf16 values
   uint4 k[kRuns][kK];
   uint4 v[kRuns][kV];
   uint32_t ke[kRuns], ve[kRuns][kV];
@@ -865,7 +872,7 @@ __global__ __launch_bounds__(64 * kFewWaves, KV == kPagedFp8 ? 3 : 2) void k_fla
         for (int t = 0; t < D / 16; ++t) o[t] *= a;
       }
       const float mc = m == kNegInf ? 0.0f : -m;
-      uint32_t w[F::kRuns][2];
+      uint32_t w[F::kRuns][2], rest[F::kRuns][2];
 #pragma unroll
       for (int t = 0; t < F::kRuns; ++t)
 #pragma unroll
@@ -873,7 +880,12 @@ __global__ __launch_bounds__(64 * kFewWaves, KV == kPagedFp8 ? 3 : 2) void k_fla
           const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][2 * i], p.c, mc));
           const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][2 * i + 1], p.c, mc));
           w[t][i] = f2bf_pair(e0, e1);
-          l = sum_pair(w[t][i], l);
+          if (F::kRest) {
+            rest[t][i] = f2bf_pair(e0 - __uint_as_float(w[t][i] << 16), e1 - __uint_as_float(w[t][i] & 0xffff0000u));
+            l += e0 + e1;
+          } else {
+            l = sum_pair(w[t][i], l);
+          }
         }
 #pragma unroll
       for (int t0 = 0; t0 < F::kRuns; t0 += 2) {
@@ -886,6 +898,8 @@ __global__ __launch_bounds__(64 * kFewWaves, KV == kPagedFp8 ? 3 : 2) void k_fla
         __builtin_amdgcn_wave_barrier();  // the wave's LDS rows are read back by other lanes
         if (kv + 16 * t0 + 31 > lo) few_not_finite<D>(vs, o, kv + 16 * t0, limit);
         const v8bf pb = __builtin_bit_cast(v8bf, make_uint4(w[t0][0], w[t0][1], w[t0 + 1][0], w[t0 + 1][1]));
+        v8bf pr;
+        if (F::kRest) pr = __builtin_bit_cast(v8bf, make_uint4(rest[t0][0], rest[t0][1], rest[t0 + 1][0], rest[t0 + 1][1]));
         // O^T += V^T P^T: dim 16 t + r16 of positions {4 grp .., 16 + 4 grp ..}
         const int rr = r16 >> 2, qq = r16 & 3, row = 4 * grp + rr;
         const lds8* const vb = vs + row * 2 * D + (qq & 1) * 8;
@@ -895,6 +909,7 @@ __global__ __launch_bounds__(64 * kFewWaves, KV == kPagedFp8 ? 3 : 2) void k_fla
           const v4s x = lds_tr16(a), y = lds_tr16(a + 16 * 2 * D);
           const v8bf va = __builtin_bit_cast(v8bf, (v8s){x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w});
           o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pb, o[t], 0, 0, 0);
+          if (F::kRest) o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pr, o[t], 0, 0, 0);
         }
       }
     }
