@@ -74,8 +74,6 @@ struct FlashArgs {
   float2* part_ml;  // [splits][T][H]: exponents' offset, sum
 };
 
-__device__ const uint4 g_zero_row[16] = {};  // 256 bytes that read as zero
-
 // l plus both bf16 values of a pair, in 32 bits (one instruction).
 __device__ __forceinline__ float sum_pair(uint32_t two, float l) {
   typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
@@ -98,14 +96,6 @@ __device__ __forceinline__ uint32_t drop_not_finite(uint32_t x) {
   if ((x & 0x7f800000u) == 0x7f800000u) x &= 0x0000ffffu;
   return x;
 }
-
-// Loads from memory, not from LDS: a flat load would count as both.
-__device__ __forceinline__ uint4 mem_ld128(const uint8_t* p) {
-  typedef uint32_t v4u __attribute__((ext_vector_type(4)));
-  const v4u v = *(const __attribute__((address_space(1))) v4u*)p;
-  return make_uint4(v[0], v[1], v[2], v[3]);
-}
-__device__ __forceinline__ uint32_t mem_ld8(const uint8_t* p) { return *(const __attribute__((address_space(1))) uint8_t*)p; }
 
 // Loads through a buffer resource of `bytes` bytes at a scalar address; a piece behind them reads as zero.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buf_rsrc(const uint8_t* p, uint32_t bytes) {

@@ -110,16 +110,16 @@ class PagedBatch:
         return torch.cat(o), torch.cat(tol)
 
 
-def attend64(q, k, v, scale=None):
+def attend64(q, k, v, scale=None, p_half=BF16_HALF):
     """q [n, H, D], k and v [Hkv, m, D] in 64 bits: rows at positions m - n ..
     m - 1 (negative: zeros).  Returns the output and how far a kernel may be from it.
 
     A kernel's weights are p_j (1 + d_j), the same in the product and in the sum that
     it is divided by, so with o = sum p v / sum p its output is off by
-    sum p_j d_j (v_j - o) / sum p_j (1 + d_j).  |d_j| is half a step of bf16 (the
-    operands of the second product) and what 32 bits make of scores, exponentials
-    and sums; the denominator is within twice half a step of sum p.  The result is rounded once
-    more."""
+    sum p_j d_j (v_j - o) / sum p_j (1 + d_j).  |d_j| is p_half, half a step of bf16 (the
+    operands of the second product; of two bf16 values that make up p the square of that), and
+    what 32 bits make of scores, exponentials and sums; the denominator is within twice p_half
+    of sum p.  The result is rounded to bf16 once more."""
     n, H, D = q.shape
     Hkv, m = k.shape[0], k.shape[1]
     scale = 1.0 / math.sqrt(D) if scale is None else scale
@@ -139,7 +139,7 @@ def attend64(q, k, v, scale=None):
             # 2^-24 of at most `big` (x 2: against the maximum's own error); L a sum of p + 1 terms
             slack = 2 * (D + 4) * F32_HALF * big + (p + 16) * F32_HALF
             spread = w @ (vh - out[i, h]).abs() if torch.isfinite(out[i, h]).all() else w @ vh.abs() + out[i, h].abs()
-            tol[i, h] = (BF16_HALF + 2 * slack) * ((1 + 2 * BF16_HALF) * spread + out[i, h].abs())
+            tol[i, h] = (p_half + 2 * slack) * (1 + 2 * p_half) * spread + (BF16_HALF + 2 * slack) * out[i, h].abs()
     return out, tol + 1e-30
 
 

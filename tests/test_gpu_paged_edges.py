@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from paged_helpers import PagedBatch, attend64, check_close, cu_of, dev, ints, normal, quantise, values_of
+from paged_helpers import BF16_HALF, PagedBatch, attend64, check_close, cu_of, dev, ints, normal, quantise, values_of
 
 from bitnet_tt import paged_attention as pa
 from bitnet_tt.utils.rope import rope_tables
@@ -145,3 +145,27 @@ def test_read_of_lengths_around_a_workgroups_rows(D, kv):
         for b, n in enumerate(total):
             assert torch.equal(got[b, :, :n].double(), pb.rows(pool, b))
             assert bool((got[b, :, n:] == 3.0).all())
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+def test_many_users_of_unlike_lengths(kv):
+    """Contexts that are split beside ones that are not, empty ones and padding."""
+    total = [0, 1, 2600] + [(i * 389) % 2600 for i in range(67)]
+    new = [1] * len(total)
+    pb = PagedBatch(new, total, 4, 2, 64, 32, kv, seed=6)
+    assert pa._scratch_bytes(0, 70, 4, 2, 64, 70, 1, 2600) == 4 * 70 * 4 * 66 * 4  # four splits
+    want, tol = pb.reference()
+    args = (pb.q_dev, pb.cache, pb.table, pb.cu, pb.len)
+    out = pa.paged_attention(*args, max_q=1, max_kv=2600)
+    check_close(out, want, tol)
+    assert bool((out[0] == 0).all())
+    assert torch.equal(out, pa.paged_attention(*args, max_q=1, max_kv=2600))
+
+
+def test_few_rows_over_bf16_pages_use_16_bits_of_p():
+    """Half a step of the output's bf16 is nearly all of the bound that is left."""
+    pb = PagedBatch([1, 1], [300, 77], 4, 2, 128, 16, "bf16", seed=2)
+    out = pa.paged_attention(pb.q_dev, pb.cache, pb.table, pb.cu, pb.len, max_q=1)
+    for b in range(2):
+        want, tol = attend64(pb.q[b:b + 1].double(), pb.rows(pb.k64, b), pb.rows(pb.v64, b), p_half=BF16_HALF ** 2)
+        check_close(out[b:b + 1], want, tol)
