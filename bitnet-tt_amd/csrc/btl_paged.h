@@ -58,13 +58,19 @@ struct Seq {
   bool ok;
 };
 __host__ __device__ __forceinline__ int clampi(int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; }
-// cap: the positions that the page table has room for.
+// cap: the positions that the page table has room for; negative: no lengths are
+// given, the sequence is its rows (as clamped: row0 + len is at most T).
 __host__ __device__ __forceinline__ Seq clamp_seq(int lo, int hi, int len, int T, int64_t cap) {
   Seq s;
   s.row0 = clampi(lo, 0, T);
   s.n = clampi(hi, s.row0, T) - s.row0;
-  s.len = (len < 0 || len > cap) ? 0 : len;  // a length that cannot be: nothing is cached
-  s.ok = s.row0 == lo && s.row0 + s.n == hi && s.len == len;
+  s.ok = s.row0 == lo && s.row0 + s.n == hi;
+  if (cap < 0) {
+    s.len = s.n;
+  } else {
+    s.len = (len < 0 || len > cap) ? 0 : len;  // a length that cannot be: nothing is cached
+    s.ok = s.ok && s.len == len;
+  }
   return s;
 }
 
@@ -116,7 +122,7 @@ __device__ __forceinline__ int32_t scalar_load(const int32_t* p, uint32_t i) {
 
 __device__ __forceinline__ Seq load_seq(const Batch& bt, int b, int64_t cap) {
   const int lo = scalar_load(bt.cu, b), hi = scalar_load(bt.cu, b + 1);
-  Seq s = clamp_seq(lo, hi, bt.len ? scalar_load(bt.len, b) : hi - lo, bt.T, bt.len ? cap : bt.T);
+  Seq s = clamp_seq(lo, hi, bt.len ? scalar_load(bt.len, b) : 0, bt.T, bt.len ? cap : -1);
   s.row0 = uni(s.row0);
   s.n = uni(s.n);
   s.len = uni(s.len);

@@ -494,7 +494,8 @@ int btl_paged_attention(const uint16_t* q, int64_t ldq, int64_t T, int64_t H, co
 /* Test hooks, host only: the functions that the kernels call.  btl_page_row:
  * the index of a position's (page, head, row), -1 for a page outside the pool.
  * btl_clamp_seq: {first row, rows, positions} of a sequence (cu_q entries lo
- * and hi) after clamping; 1 if nothing had to be.  btl_row_exponent: e of an 8-bit
+ * and hi) after clamping; 1 if nothing had to be; cap < 0: no length is given, the
+ * positions are the rows.  btl_row_exponent: e of an 8-bit
  * row whose largest magnitude is given. */
 int64_t btl_page_row(int64_t page, int64_t num_pages, int64_t num_kv_heads, int64_t kv_head, int64_t page_size,
                      int64_t position);

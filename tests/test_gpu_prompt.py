@@ -135,3 +135,18 @@ def test_sequences_not_well_formed(cu):
     pa.prompt_attention(x[:, :4], x[:, 4:6], x[:, 6:], ints(cu))
     with pytest.raises(RuntimeError, match="paged workspace"):
         pa.check("cuda:0")
+
+
+@pytest.mark.parametrize("cu", [[0, 40, 60], [0, 49, 99], [0, 50, 2 ** 31 - 1], [-2 ** 31, 10, 50], [0, 20, 51]])
+def test_offsets_behind_the_rows(cu):
+    """The sequences as clamped, the error word set; the rows behind k and v, here another
+    tensor's, are not read."""
+    x = packed([50], 4, 2, 64, extra=60)  # NaN from row 50 on
+    d = x.to(dev())
+    out = pa.prompt_attention(d[:50, :4], d[:50, 4:6], d[:50, 6:], ints(cu))
+    with pytest.raises(RuntimeError, match="paged workspace"):
+        pa.check("cuda:0")
+    at = [min(max(c, 0), 50) for c in cu]
+    lens = [b - a for a, b in zip(at, at[1:])]
+    want, tol = reference(x[:50, :4], x[:50, 4:6], x[:50, 6:], lens)
+    check_close(out, want, tol)

@@ -149,6 +149,27 @@ def test_clamped_sequences(L):
     assert f(0, 10, -1) == (0, (0, 10, 0))
 
 
+def test_rows_without_lengths_stay_in_their_buffer(L):
+    """Prompts have no lengths: a sequence's positions are its rows as clamped, whatever the offsets say,
+    so that no key or value row from T on is read."""
+    out = (ctypes.c_int64 * 3)()
+
+    def f(lo, hi, T):
+        return L.btl_clamp_seq(lo, hi, 0, T, -1, out), tuple(out)
+
+    assert f(0, 40, 50) == (1, (0, 40, 40)) and f(50, 50, 50) == (1, (50, 0, 0))
+    assert f(40, 60, 50) == (0, (40, 10, 10))
+    assert f(-2 ** 31, 2 ** 31 - 1, 50) == (0, (0, 50, 50))
+    r = random.Random(4)
+    some = [0, 1, -1, 2 ** 31 - 1, -2 ** 31]
+    for _ in range(5000):
+        T = r.choice([0, 1, 50, 1 << 24])
+        lo, hi = (r.choice(some + [T, T + 1, r.randint(-60, 120), r.randint(0, T)]) for _ in range(2))
+        ok, (row0, n, length) = f(lo, hi, T)
+        assert 0 <= row0 <= row0 + n <= T and length == n
+        assert ok == (0 <= lo <= hi <= T)
+
+
 def test_row_exponent(L):
     f = L.btl_row_exponent
     assert f(448.0) == 0 and f(1.75) == -8 and f(1.7500001) == -7 and f(0.0) == -126 and f(1e-40) == -126
