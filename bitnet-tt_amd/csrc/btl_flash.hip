@@ -649,7 +649,8 @@ __global__ __launch_bounds__(256, 2) void k_flash_tile(FlashArgs p) {
 //
 // Over bf16 pages p is two bf16 values, itself rounded and what that leaves, so 16 bits of it
 // are used: the matrix units have the time (one user at 131001 positions 66.0 us, 66.2 so; 128 users at 2048
-// 121 and 120), and the error against 64 bits is that of the output's own rounding.  8-bit
+// 121 and 120).  The rests have a sum of their own (one sum for both: 0.3 us less at 512 positions, but infinite values
+// that a row sees would become NaN), and the error against 64 bits is that of the output's own rounding.  8-bit
 // pages, whose values have 4 bits, cost 1 to 8% for it and have one.
 //
 // 5 heads of 128: one user at 131001 positions 59 us (5.7 TB/s) and 5 of the merge, 128
@@ -825,9 +826,9 @@ __global__ __launch_bounds__(64 * kFewWaves, KV == kPagedFp8 ? 3 : 2) void k_fla
     f.template load<false>(p, hk, kv_first, kv_end, bad);
     f.template load<true>(p, hk, kv_first, kv_end, bad);
     f.fetch_pages(p, table, kv_first + kRound);
-    v4f o[D / 16];
+    v4f o[D / 16], o_rest[D / 16];
 #pragma unroll
-    for (int t = 0; t < D / 16; ++t) o[t] = (v4f){0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; t < D / 16; ++t) o[t] = o_rest[t] = (v4f){0.f, 0.f, 0.f, 0.f};
     float m = kNegInf, l = 0.0f;
     lds8* const vs = (lds8*)&s.v[wv][0];
 
@@ -859,7 +860,10 @@ __global__ __launch_bounds__(64 * kFewWaves, KV == kPagedFp8 ? 3 : 2) void k_fla
         m = mn;
         l *= a;
 #pragma unroll
-        for (int t = 0; t < D / 16; ++t) o[t] *= a;
+        for (int t = 0; t < D / 16; ++t) {
+          o[t] *= a;
+          if (F::kRest) o_rest[t] *= a;
+        }
       }
       const float mc = m == kNegInf ? 0.0f : -m;
       uint32_t w[F::kRuns][2], rest[F::kRuns][2];
@@ -899,9 +903,18 @@ __global__ __launch_bounds__(64 * kFewWaves, KV == kPagedFp8 ? 3 : 2) void k_fla
           const v4s x = lds_tr16(a), y = lds_tr16(a + 16 * 2 * D);
           const v8bf va = __builtin_bit_cast(v8bf, (v8s){x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w});
           o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pb, o[t], 0, 0, 0);
-          if (F::kRest) o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pr, o[t], 0, 0, 0);
+          if (F::kRest) o_rest[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pr, o_rest[t], 0, 0, 0);
         }
       }
+    }
+
+    // What is left of p may be negative or zero, so that its product with an infinite value is no
+    // part of the sum: where the product of the rounded p is not finite, that is the sum.
+    if (F::kRest) {
+#pragma unroll
+      for (int t = 0; t < D / 16; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[t][i] += __builtin_isfinite(o[t][i]) ? o_rest[t][i] : 0.0f;
     }
 
     // the waves' partials, in wave order

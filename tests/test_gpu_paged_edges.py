@@ -169,3 +169,23 @@ def test_few_rows_over_bf16_pages_use_16_bits_of_p():
     for b in range(2):
         want, tol = attend64(pb.q[b:b + 1].double(), pb.rows(pb.k64, b), pb.rows(pb.v64, b), p_half=BF16_HALF ** 2)
         check_close(out[b:b + 1], want, tol)
+
+
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("total,max_kv", [(300, None), (5000, 5000)])
+def test_values_not_finite_early_in_a_context(bad, D, total, max_kv):
+    """A value that every row sees, in the first round, in a later one and in another split:
+    infinite where the weights are positive, whichever kernel max_q chooses."""
+    H, Hkv = 4, 2
+    pb = PagedBatch([1], [total], H, Hkv, D, 32, "bf16", seed=5)
+    if max_kv:
+        assert pa._scratch_bytes(0, 1, H, Hkv, D, 1, 1, max_kv) > 0
+    for dim, where in ((1, 3), (2, 130), (7, total // 2), (D - 1, total - 40)):
+        pid, row = int(pb.table_host[0, where // 32]), where % 32
+        pb.cache.value_pages[pid, :, row, dim] = bad
+        pb.v64[pid, :, row, dim] = bad
+    want, tol = pb.reference()
+    assert int((~torch.isfinite(want)).sum()) == 4 * H
+    for max_q in (1, 40):
+        check_close(pa.paged_attention(pb.q_dev, pb.cache, pb.table, pb.cu, pb.len, max_q=max_q, max_kv=max_kv), want, tol)
