@@ -163,6 +163,7 @@ EXPORTS = {
     "btl_page_row": ([_I64, _I64, _I64, _I64, _I64, _I64], _I64),
     "btl_clamp_seq": ([_I64, _I64, _I64, _I64, _I64, _P], _I),
     "btl_row_exponent": ([_F], _I),
+    "btl_paged_attention_plan": ([_I64, _I64, _I64, _I64, _I64, _I64, _I64, _P], _I),
     "btl_decode_attention": ([_P, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _I, _F, _P, _P, _P, _P, _SZ, _P], _I),
 }
 

@@ -1018,8 +1018,7 @@ __global__ __launch_bounds__(256) void k_flash_merge(FlashArgs p, int groups) {
 struct FlashPlan {
   bool few;
   int64_t tiles;  // workgroups per split
-  int splits;
-  int64_t chunk;
+  int splits, chunk;
 };
 // Few rows: the kernel of single tokens where a sequence's rows fit one of its tiles.
 //
@@ -1052,14 +1051,19 @@ struct FlashPlan {
 //    140: 86, 86 or 134, 138.
 constexpr int64_t kMinChunk = 256;
 constexpr int64_t kMaxSplits = 256;
+// A hint behind this plans for as many positions as a page table may have room for: splits x
+// chunk stays below 2^31, the kernels' positions.
+constexpr int64_t kMaxPositions = INT32_MAX / 2;
 inline FlashPlan flash_plan(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t B, int64_t max_q, int64_t max_kv,
                             bool paged) {
   FlashPlan f{};
   const int64_t G = H / Hkv, cus = device_cus();
+  max_q = std::min(max_q, T);
+  max_kv = std::min(max_kv, kMaxPositions);
   f.few = paged && max_q * G <= kFewRows;
   f.tiles = (f.few ? B : T * G / kTileRows + (B < T ? B : T)) * Hkv;
   f.splits = 1;
-  f.chunk = round_up(max_kv > 0 ? max_kv : 1, kMinChunk);
+  f.chunk = (int)round_up(max_kv > 0 ? max_kv : 1, kMinChunk);
   if (!paged || max_kv < (f.few ? 4 : 2) * kMinChunk) return f;
   int64_t n;
   if (f.few) {
@@ -1074,7 +1078,7 @@ inline FlashPlan flash_plan(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_
   if (n > max_kv / kMinChunk) n = max_kv / kMinChunk;
   if (n > kMaxSplits) n = kMaxSplits;
   if (n > 1) {
-    f.chunk = round_up((max_kv + n - 1) / n, kMinChunk);
+    f.chunk = (int)round_up((max_kv + n - 1) / n, kMinChunk);
     f.splits = (int)((max_kv + f.chunk - 1) / f.chunk);
   }
   return f;
@@ -1156,6 +1160,16 @@ int64_t btl_paged_attention_scratch_bytes(int64_t T, int64_t H, int64_t Hkv, int
   return flash_scratch(flash_plan(T, H, Hkv, D, B, max_q, max_kv, true), T, H, D);
 }
 
+int btl_paged_attention_plan(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t B, int64_t max_q, int64_t max_kv,
+                             int64_t* plan) {
+  if (!plan || T <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || B <= 0 || max_q <= 0 || max_kv <= 0) return 0;
+  const FlashPlan f = flash_plan(T, H, Hkv, D, B, max_q, max_kv, true);
+  plan[0] = f.few;
+  plan[1] = f.splits;
+  plan[2] = f.chunk;
+  return 1;
+}
+
 int btl_paged_attention(const uint16_t* q, int64_t ldq, int64_t T, int64_t H, const btl_pages_t* pages,
                         const int32_t* page_table, int64_t max_pages, const int32_t* cu_q, const int32_t* kv_len,
                         int64_t B, float scale, int64_t max_q, int64_t max_kv, uint16_t* out, int64_t ldo,
@@ -1170,7 +1184,7 @@ int btl_paged_attention(const uint16_t* q, int64_t ldq, int64_t T, int64_t H, co
   if (rc != BTL_OK) return rc;
   rc = flash_args(who, q, ldq, T, H, Hkv, D, scale, out, ldo, error_word, &a);
   if (rc != BTL_OK) return rc;
-  if (max_q <= 0 || max_kv <= 0 || max_pages <= 0 || max_pages * pages->page_size > INT32_MAX / 2)
+  if (max_q <= 0 || max_kv <= 0 || max_pages <= 0 || max_pages * pages->page_size > kMaxPositions)
     return set_error(BTL_ERR_SHAPE, "%s: max_q=%lld max_kv=%lld max_pages=%lld", who, (long long)max_q,
                      (long long)max_kv, (long long)max_pages);
   if (T == 0) return BTL_OK;
@@ -1186,7 +1200,7 @@ int btl_paged_attention(const uint16_t* q, int64_t ldq, int64_t T, int64_t H, co
     if (!aligned(scratch, 16)) return set_error(BTL_ERR_ALIGN, "%s: misaligned scratch", who);
   }
   a.splits = f.splits;
-  a.chunk = (int)f.chunk;
+  a.chunk = f.chunk;
   a.part_o = static_cast<float*>(scratch);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + (f.splits > 1 ? (int64_t)f.splits * T * H * D : 0));
   if (f.few) {

@@ -479,7 +479,7 @@ int btl_prompt_attention(const uint16_t* q, int64_t ldq, const uint16_t* k, int6
 /* Attention of the newest tokens over the pages: the row at position p attends
  * to positions [0, p].  max_q and max_kv: upper bounds of the new tokens and
  * of kv_len of any sequence where known, else T and max_pages * page_size
- * (hints: they choose the kernel and the split, results depend on them in rounding
+ * (hints, any positive number: they choose the kernel and the split, results depend on them in rounding
  * only).  Long contexts of few rows are split over workgroups, whose partials are
  * merged in a fixed order by a second launch: scratch, 16-byte aligned, of
  * btl_paged_attention_scratch_bytes with the same arguments (0: not split) on the same
@@ -496,11 +496,15 @@ int btl_paged_attention(const uint16_t* q, int64_t ldq, int64_t T, int64_t H, co
  * btl_clamp_seq: {first row, rows, positions} of a sequence (cu_q entries lo
  * and hi) after clamping; 1 if nothing had to be; cap < 0: no length is given, the
  * positions are the rows.  btl_row_exponent: e of an 8-bit
- * row whose largest magnitude is given. */
+ * row whose largest magnitude is given.  btl_paged_attention_plan: {1 where the kernel of
+ * few rows runs, splits, positions of a split} of btl_paged_attention; 1, or 0 for sizes
+ * that it refuses. */
 int64_t btl_page_row(int64_t page, int64_t num_pages, int64_t num_kv_heads, int64_t kv_head, int64_t page_size,
                      int64_t position);
 int btl_clamp_seq(int64_t lo, int64_t hi, int64_t len, int64_t T, int64_t cap, int64_t* seq);
 int btl_row_exponent(float largest);
+int btl_paged_attention_plan(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t B, int64_t max_q, int64_t max_kv,
+                             int64_t* plan);
 
 #ifdef __cplusplus
 }

@@ -189,3 +189,26 @@ def test_values_not_finite_early_in_a_context(bad, D, total, max_kv):
     assert int((~torch.isfinite(want)).sum()) == 4 * H
     for max_q in (1, 40):
         check_close(pa.paged_attention(pb.q_dev, pb.cache, pb.table, pb.cu, pb.len, max_q=max_q, max_kv=max_kv), want, tol)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+@pytest.mark.parametrize("max_kv", [2 ** 31 + 7, 3 * 2 ** 31, 2 ** 40, 2 ** 63 - 1])
+@pytest.mark.parametrize("new,max_q", [([1, 1], 1), ([40, 3], 40), ([1, 1], 2 ** 62)])
+def test_hints_of_the_c_entry_behind_the_table(kv, max_kv, new, max_q):
+    """The C entry point with hints far behind the page table's room, in its own scratch: rounding only."""
+    from bitnet_tt import _native as N
+
+    H, Hkv, D = 4, 2, 64
+    pb = PagedBatch(new, [700, 41], H, Hkv, D, 16, kv, seed=3)
+    T, B, L = sum(new), len(new), N.lib()
+    nbytes = L.btl_paged_attention_scratch_bytes(T, H, Hkv, D, B, max_q, max_kv)
+    scratch = torch.empty(max(16, nbytes), dtype=torch.uint8, device=dev())
+    word = torch.zeros(1, dtype=torch.int32, device=dev())
+    out = torch.empty_like(pb.q_dev)
+    rc = L.btl_paged_attention(pb.q_dev.data_ptr(), H * D, T, H, pb.cache._pages, pb.table.data_ptr(), pb.table.shape[1],
+                               pb.cu.data_ptr(), pb.len.data_ptr(), B, D ** -0.5, max_q, max_kv, out.data_ptr(), H * D,
+                               scratch.data_ptr(), nbytes, word.data_ptr(), N.raw_stream(0))
+    assert rc == 0
+    want, tol = pb.reference()
+    check_close(out, want, tol)
+    assert int(word) == 0

@@ -116,6 +116,29 @@ def test_scratch_bytes(L):
     assert f(32, 20, 5, 128, 32, 1, 4096) > f(300, 20, 5, 128, 300, 1, 4096) == 0  # 160 workgroups, 1500
 
 
+def plan(L, *sizes):
+    out = (ctypes.c_int64 * 3)()
+    assert L.btl_paged_attention_plan(*sizes, out) == 1
+    return tuple(out)
+
+
+@pytest.mark.parametrize("T,B,max_q", [(1, 1, 1), (32, 32, 1), (67, 1, 67), (2047, 4, 700), (3, 1, 2 ** 62)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_plan_of_any_hint(L, T, B, max_q, D):
+    """The kernels' positions are 32-bit numbers: the end of the last split stays below 2^31, however far
+    behind the page table's room the hint is, and the scratch is that of the splits that run."""
+    for max_kv in (1, 255, 1024, 40067, 2 ** 30 - 1, 2 ** 30, 2 ** 31 - 1, 2 ** 31, 2 ** 31 + 7, 3 * 2 ** 31, 2 ** 33 + 2 ** 31,
+                   2 ** 40, 2 ** 62, 2 ** 63 - 1):
+        sizes = (T, 20, 5, D, B, max_q, max_kv)
+        few, splits, chunk = plan(L, *sizes)
+        assert 1 <= splits <= 256 and 256 <= chunk <= 2 ** 30 and splits * chunk < 2 ** 31
+        assert splits * chunk >= min(max_kv, 2 ** 30 - 1)
+        assert L.btl_paged_attention_scratch_bytes(*sizes) == (splits * T * 20 * (D + 2) * 4 if splits > 1 else 0)
+        if max_kv >= 2 ** 30:
+            assert (few, splits, chunk) == plan(L, T, 20, 5, D, B, max_q, 2 ** 30 - 1)
+    assert plan(L, T, 20, 5, D, B, max_q, 4096)[0] == (min(max_q, T) * 4 <= 16)
+
+
 def test_page_of_a_position(L):
     """The division by multiplication, and pages outside the pool."""
     r = random.Random(1)
