@@ -1088,12 +1088,21 @@ inline int64_t flash_scratch(const FlashPlan& f, int64_t T, int64_t H, int64_t D
   return f.splits > 1 ? (int64_t)f.splits * T * H * (D + 2) * 4 : 0;
 }
 
+inline bool flash_heads(int64_t T, int64_t H, int64_t Hkv) {
+  return H > 0 && Hkv > 0 && H <= 1024 && H % Hkv == 0 && H / Hkv <= 64 && T <= INT32_MAX / 2 / H;
+}
+// Sizes of calls with rows: those that the entry point takes, so that nothing planned from them overflows.
+inline bool flash_sizes(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t B, int64_t max_q, int64_t max_kv) {
+  return T > 0 && T <= kMaxRows && B > 0 && B <= kMaxSeqs && (D == 64 || D == 128) && flash_heads(T, H, Hkv) &&
+         max_q > 0 && max_kv > 0;
+}
+
 // Checks shared by both entry points; fills what they share.
 int flash_args(const char* who, const uint16_t* q, int64_t ldq, int64_t T, int64_t H, int64_t Hkv, int64_t D,
                float scale, uint16_t* out, int64_t ldo, int32_t* error, FlashArgs* a) {
   if (D != 64 && D != 128)
     return set_error(BTL_ERR_SHAPE, "%s: head dim %lld (64 and 128 supported)", who, (long long)D);
-  if (H <= 0 || Hkv <= 0 || H > 1024 || H % Hkv || H / Hkv > 64 || T * H > INT32_MAX / 2)
+  if (!flash_heads(T, H, Hkv))
     return set_error(BTL_ERR_SHAPE, "%s: T=%lld H=%lld Hkv=%lld (H / Hkv <= 64)", who, (long long)T, (long long)H,
                      (long long)Hkv);
   if (!(scale > 0.0f) || !(scale < __builtin_inff()))
@@ -1156,13 +1165,13 @@ int btl_prompt_attention(const uint16_t* q, int64_t ldq, const uint16_t* k, int6
 
 int64_t btl_paged_attention_scratch_bytes(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t B, int64_t max_q,
                                           int64_t max_kv) {
-  if (T <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || B <= 0 || max_q <= 0 || max_kv <= 0) return 0;
+  if (!flash_sizes(T, H, Hkv, D, B, max_q, max_kv)) return 0;
   return flash_scratch(flash_plan(T, H, Hkv, D, B, max_q, max_kv, true), T, H, D);
 }
 
 int btl_paged_attention_plan(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t B, int64_t max_q, int64_t max_kv,
                              int64_t* plan) {
-  if (!plan || T <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || B <= 0 || max_q <= 0 || max_kv <= 0) return 0;
+  if (!plan || !flash_sizes(T, H, Hkv, D, B, max_q, max_kv)) return 0;
   const FlashPlan f = flash_plan(T, H, Hkv, D, B, max_q, max_kv, true);
   plan[0] = f.few;
   plan[1] = f.splits;

@@ -19,6 +19,8 @@
 namespace btl {
 
 constexpr int kMaxPageSize = 1 << 20;
+constexpr int kMaxRows = 1 << 24;  // packed rows of a batch
+constexpr int kMaxSeqs = 1 << 20;
 
 // n / d for n < 2^31 by a multiplication: m = ceil(2^(31+l) / d), l = ceil(log2 d);
 // the excess e = m d - 2^(31+l) is below d <= 2^l, so n e < 2^(31+l) and the

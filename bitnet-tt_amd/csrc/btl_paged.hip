@@ -299,7 +299,7 @@ int check_pages(const char* who, const btl_pages_t* p, Pages* out) {
 
 int check_batch(const char* who, int64_t B, int64_t T, const int32_t* cu_q, const int32_t* kv_len,
                 const int32_t* page_table, int64_t max_pages, Batch* out) {
-  if (B <= 0 || B > (1 << 20) || T < 0 || T > (1 << 24) || max_pages < 0 || max_pages > (1 << 24))
+  if (B <= 0 || B > kMaxSeqs || T < 0 || T > kMaxRows || max_pages < 0 || max_pages > (1 << 24))
     return set_error(BTL_ERR_SHAPE, "%s: B=%lld T=%lld max_pages=%lld", who, (long long)B, (long long)T,
                      (long long)max_pages);
   if (!cu_q && T > 0) return set_error(BTL_ERR_NULL, "%s: cu_q is NULL", who);

@@ -139,6 +139,16 @@ def test_plan_of_any_hint(L, T, B, max_q, D):
     assert plan(L, T, 20, 5, D, B, max_q, 4096)[0] == (min(max_q, T) * 4 <= 16)
 
 
+@pytest.mark.parametrize("sizes", [
+    (1 << 10, 16, 16, 64, 1 << 60, 1, 4096), (1, 1 << 62, 1 << 62, 128, 4, 1, 1 << 17), (1 << 62, 20, 5, 128, 32, 1, 1 << 17),
+    (1 << 24, 128, 2, 64, 4, 1, 1 << 17), (1, 130, 2, 64, 1, 1, 1 << 17), (1, 20, 5, 96, 1, 1, 1 << 17),
+    (1, 20, 5, 128, (1 << 20) + 1, 1, 1 << 17), (1, 20, 5, 128, 1, -1, 1 << 17), (1, 20, 5, 128, 1, 1, -2 ** 63),
+])
+def test_scratch_of_sizes_that_no_call_takes(L, sizes):
+    assert L.btl_paged_attention_scratch_bytes(*sizes) == 0
+    assert L.btl_paged_attention_plan(*sizes, (ctypes.c_int64 * 3)()) == 0
+
+
 def test_page_of_a_position(L):
     """The division by multiplication, and pages outside the pool."""
     r = random.Random(1)
