@@ -365,11 +365,16 @@ class BitLinearDecodeStep:
 
     def load_contiguous(self, page_table, kv_len) -> None:
         """What the pages hold, into the contiguous caches of ``alloc_attention``
-        (rows [0, kv_len[b]) of user b), for the one-launch step to go on from."""
+        (rows [0, kv_len[b]) of user b), for the one-launch step to go on from.  Its
+        queries are rotated as ``alloc_attention`` says, so
+        ValueError where ``alloc_paged`` rotated the cached keys otherwise."""
         from .paged_attention import read_pages
 
         if getattr(self, "paged", None) is None or getattr(self, "kv", None) is None:
             raise RuntimeError("load_contiguous needs alloc_paged() and alloc_attention() first")
+        if self.paged.rotation != self.attention.rotation:
+            raise ValueError(f"the cached keys are rotated by {self.paged.rotation}, the queries of the decode steps by "
+                             f"{self.attention.rotation}")
         for kv, pages in zip(self.kv, self.pages):
             read_pages(pages, page_table, kv_len, kv.key_cache, kv.value_cache)
 

@@ -123,6 +123,14 @@ class KVCache:
         self.seq_len_cached = 0
 
 
+def _rotation(dim: int, theta: float, adjacent: bool, scaling: dict | None = None, max_position: int = 0) -> dict:
+    """What a layer's rotation is made of: two layers may use one cache where these are equal."""
+    if scaling is not None and scaling.get("rope_type", scaling.get("type", "default")) == "default":
+        scaling = None
+    return {"rotated dims": dim, "theta": float(theta), "pairs": "(2i, 2i+1)" if adjacent else "(i, i + R/2)",
+            "scaling": None if scaling is None else {"original_max_position_embeddings": max_position, **scaling}}
+
+
 class DecodeAttention:
     """Decode attention of one layer (attention.py:1040-1262):
 
@@ -152,6 +160,7 @@ class DecodeAttention:
         self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         self.use_fused_rope = use_fused_rope
         self.scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
+        self.rotation = _rotation(head_dim, rope_theta, use_fused_rope)
         cos, sin = rope_tables(head_dim, max_seq_len, rope_theta)
         self.rope_cos = torch.from_numpy(cos).to(self.device)
         self.rope_sin = torch.from_numpy(sin).to(self.device)
@@ -247,6 +256,7 @@ class PagedAttention:
         self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         self.use_fused_rope = use_fused_rope
         self.scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
+        self.rotation = _rotation(rotary_dim, rope_theta, use_fused_rope, rope_scaling, max_position)
         if rope_scaling is None:
             cos, sin = (torch.from_numpy(t) for t in rope_tables(rotary_dim, max_seq_len, rope_theta))
         else:

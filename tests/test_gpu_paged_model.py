@@ -142,6 +142,29 @@ def test_pages_to_the_contiguous_step():
         BitLinearDecodeStep(cfg, dev()).forward_rows(rows, table, cu_of([1]), ints([1]))
 
 
+def stepping(paged=(), attention=()):
+    """A model of no layers on the host with both kinds of attention."""
+    cfg = BitNetMiniConfig(num_attention_heads=2)
+    step = BitLinearDecodeStep(cfg, torch.device("cpu"), batch=2)
+    step.alloc_attention(max_seq_len=64, **dict(attention))
+    step.paged = PagedAttention(cfg.num_attention_heads, cfg.num_kv_heads, cfg.head_dim,
+                                **{"max_seq_len": 64, "device": "cpu", "rope_theta": cfg.rope_theta, **dict(paged)})
+    step.pages = []
+    return step
+
+
+@pytest.mark.parametrize("paged,attention", [
+    ({"use_fused_rope": True}, {}), ({}, {"use_fused_rope": True}), ({"rope_theta": 10000.0}, {}), ({"rotary_dim": 64}, {}),
+    ({"rope_scaling": {"type": "linear", "factor": 2.0}}, {}),
+    ({"rope_scaling": {"rope_type": "yarn", "factor": 4.0}, "use_fused_rope": True}, {"use_fused_rope": True}),
+])
+def test_keys_that_the_steps_queries_do_not_match(paged, attention):
+    step = stepping(paged, attention)
+    with pytest.raises(ValueError, match="rotated by"):
+        step.load_contiguous(torch.zeros((2, 1), dtype=torch.int32), torch.tensor([5, 7], dtype=torch.int32))
+    assert step.pos.tolist() == [63, 63]
+
+
 # ---- angle tables (host) --------------------------------------------------
 
 
