@@ -365,8 +365,8 @@ class BitLinearDecodeStep:
 
     def load_contiguous(self, page_table, kv_len) -> None:
         """What the pages hold, into the contiguous caches of ``alloc_attention``
-        (rows [0, kv_len[b]) of user b), for the one-launch step to go on from.  Its
-        queries are rotated as ``alloc_attention`` says, so
+        (rows [0, kv_len[b]) of user b), and ``pos`` to kv_len, every user's next position: the
+        decode steps go on from here.  Their queries are rotated as ``alloc_attention`` says, so
         ValueError where ``alloc_paged`` rotated the cached keys otherwise."""
         from .paged_attention import read_pages
 
@@ -377,6 +377,7 @@ class BitLinearDecodeStep:
                              f"{self.attention.rotation}")
         for kv, pages in zip(self.kv, self.pages):
             read_pages(pages, page_table, kv_len, kv.key_cache, kv.value_cache)
+        self.pos.copy_(kv_len)
 
     # -- the step ----------------------------------------------------------
     def layer(self, i: int, hidden, attn_out, qkv_out, ffn_h):

@@ -142,6 +142,31 @@ def test_pages_to_the_contiguous_step():
         BitLinearDecodeStep(cfg, dev()).forward_rows(rows, table, cu_of([1]), ints([1]))
 
 
+@pytest.mark.gpu
+def test_the_step_goes_on_where_the_prompts_end():
+    """As the README has it: alloc_attention's own positions (the last) and random caches, prompts, load_contiguous,
+    and a step: it attends to the prompts and its own token, not to what else the caches hold."""
+    from bitnet_tt.config import BitNetConfig
+
+    cfg = BitNetConfig(hidden_size=512, num_layers=2, num_attention_heads=4, num_key_value_heads=1,
+                       intermediate_size=1024, vocab_size=1000, max_position_embeddings=256)
+    step = BitLinearDecodeStep.random_init(cfg, dev(), seed=5, batch=3)
+    step.alloc_buffers().alloc_attention(max_seq_len=128).alloc_paged(12, 128, page_size=32)
+    lens = [40, 1, 90]
+    table = torch.arange(12, dtype=torch.int32, device=dev()).view(3, 4)
+    step.forward_rows(normal((sum(lens), 512), 6).to(torch.bfloat16).to(dev()), table, cu_of(lens), ints(lens), max_q=90)
+    step.load_contiguous(table, ints(lens))
+    assert step.pos.tolist() == lens
+    step.reset_hidden()
+    rows = step.hidden.clone()
+    step.step_full()
+    step.forward_rows(rows, table, cu_of([1, 1, 1]), ints([n + 1 for n in lens]), max_q=1)
+    step.check()
+    a, b = step.hidden.double(), rows.double()
+    # two attention kernels that round differently, then int8 codes: normwise
+    assert float((a - b).norm() / a.norm()) < 0.05
+
+
 def stepping(paged=(), attention=()):
     """A model of no layers on the host with both kinds of attention."""
     cfg = BitNetMiniConfig(num_attention_heads=2)
@@ -163,6 +188,16 @@ def test_keys_that_the_steps_queries_do_not_match(paged, attention):
     with pytest.raises(ValueError, match="rotated by"):
         step.load_contiguous(torch.zeros((2, 1), dtype=torch.int32), torch.tensor([5, 7], dtype=torch.int32))
     assert step.pos.tolist() == [63, 63]
+
+
+@pytest.mark.parametrize("paged,attention", [
+    ({}, {}), ({"use_fused_rope": True}, {"use_fused_rope": True}), ({"max_seq_len": 32}, {}),
+    ({"rope_scaling": {"rope_type": "default"}}, {}),
+])
+def test_keys_that_match_and_the_next_positions(paged, attention):
+    step = stepping(paged, attention)
+    step.load_contiguous(torch.zeros((2, 1), dtype=torch.int32), torch.tensor([5, 7], dtype=torch.int32))
+    assert step.pos.tolist() == [5, 7]
 
 
 # ---- angle tables (host) --------------------------------------------------
