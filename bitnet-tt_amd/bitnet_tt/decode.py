@@ -367,8 +367,10 @@ class BitLinearDecodeStep:
         """What the pages hold, into the contiguous caches of ``alloc_attention``
         (rows [0, kv_len[b]) of user b), and ``pos`` to kv_len, every user's next position: the
         decode steps go on from here.  Their queries are rotated as ``alloc_attention`` says, so
-        ValueError where ``alloc_paged`` rotated the cached keys otherwise."""
+        ValueError where ``alloc_paged`` rotated the cached keys otherwise; from position 4096 on
+        the steps' angle tables get the rows that the cached keys were rotated by (float64 angles)."""
         from .paged_attention import read_pages
+        from .utils.rope import FLOAT32_POSITIONS
 
         if getattr(self, "paged", None) is None or getattr(self, "kv", None) is None:
             raise RuntimeError("load_contiguous needs alloc_paged() and alloc_attention() first")
@@ -377,6 +379,10 @@ class BitLinearDecodeStep:
                              f"{self.attention.rotation}")
         for kv, pages in zip(self.kv, self.pages):
             read_pages(pages, page_table, kv_len, kv.key_cache, kv.value_cache)
+        far = slice(FLOAT32_POSITIONS, min(self.paged.max_seq_len, self.attention.max_seq_len))
+        if far.stop > far.start:
+            self.attention.rope_cos[far].copy_(self.paged.rope_cos[far])
+            self.attention.rope_sin[far].copy_(self.paged.rope_sin[far])
         self.pos.copy_(kv_len)
 
     # -- the step ----------------------------------------------------------

@@ -125,10 +125,10 @@ class KVCache:
 
 def _rotation(dim: int, theta: float, adjacent: bool, scaling: dict | None = None, max_position: int = 0) -> dict:
     """What a layer's rotation is made of: two layers may use one cache where these are equal."""
-    if scaling is not None and scaling.get("rope_type", scaling.get("type", "default")) == "default":
-        scaling = None
+    from ..utils.rope import is_scaled
+
     return {"rotated dims": dim, "theta": float(theta), "pairs": "(2i, 2i+1)" if adjacent else "(i, i + R/2)",
-            "scaling": None if scaling is None else {"original_max_position_embeddings": max_position, **scaling}}
+            "scaling": {"original_max_position_embeddings": max_position, **scaling} if is_scaled(scaling) else None}
 
 
 class DecodeAttention:
@@ -232,8 +232,9 @@ class PagedAttention:
     PagedKVCache, all of them one page table.  Rows and the device arrays cu_q,
     kv_len and page_table: see bitnet_tt.paged_attention.  ``rotary_dim`` (a multiple
     of 16, default head_dim) rotates part of a head; ``rope_scaling`` is a model
-    config's dict (utils.rope.scaled_frequencies).  Without scaling the angles are those of
-    DecodeAttention.  ``scale`` as for DecodeAttention."""
+    config's dict (utils.rope.scaled_frequencies).  Without scaling the angles of the first 4096
+    positions are those of DecodeAttention; behind them, and with scaling, they are computed in
+    float64.  ``scale`` as for DecodeAttention."""
 
     def __init__(self, num_heads: int, num_kv_heads: int, head_dim: int, max_seq_len: int, device=None,
                  rope_theta: float = 500000.0, use_fused_rope: bool = False, scale: float | None = None,
@@ -242,7 +243,7 @@ class PagedAttention:
 
         import torch
 
-        from ..utils.rope import long_rope_tables, rope_tables
+        from ..utils.rope import paged_rope_tables
 
         rotary_dim = head_dim if rotary_dim is None else rotary_dim
         if head_dim not in (64, 128) or num_heads % num_kv_heads or num_heads // num_kv_heads > 64:
@@ -257,11 +258,8 @@ class PagedAttention:
         self.use_fused_rope = use_fused_rope
         self.scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
         self.rotation = _rotation(rotary_dim, rope_theta, use_fused_rope, rope_scaling, max_position)
-        if rope_scaling is None:
-            cos, sin = (torch.from_numpy(t) for t in rope_tables(rotary_dim, max_seq_len, rope_theta))
-        else:
-            cos, sin = long_rope_tables(rotary_dim, max_seq_len, rope_theta, rope_scaling, max_position, self.device)
-        self.rope_cos, self.rope_sin = cos.to(self.device), sin.to(self.device)
+        self.rope_cos, self.rope_sin = paged_rope_tables(rotary_dim, max_seq_len, rope_theta, rope_scaling,
+                                                         max_position, self.device)
 
     def new_cache(self, num_pages: int, page_size: int = 64, dtype: str = "bf16"):
         """A layer's page pools; dtype "bf16" or "fp8"."""

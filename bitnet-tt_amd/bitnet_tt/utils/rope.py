@@ -75,13 +75,40 @@ def scaled_frequencies(dim: int, theta: float = 10000.0, scaling: dict | None = 
     return freq * (1.0 - ramp) + freq / factor * ramp, 0.1 * np.log(factor) + 1.0 if attention is None else float(attention)
 
 
+def is_scaled(scaling: dict | None) -> bool:
+    """Whether a model config's ``scaling`` changes the plain frequencies."""
+    return scaling is not None and scaling.get("rope_type", scaling.get("type", "default")) != "default"
+
+
 def long_rope_tables(dim: int, max_seq_len: int, theta: float = 10000.0, scaling: dict | None = None,
-                     max_position: int = 4096, device="cpu"):
-    """(cos, sin) torch tensors [max_seq_len, dim/2] fp32 of scaled_frequencies,
-    angles in float64: at position 100000 a float32 angle is off by up to 0.004,
-    half a step of bf16; rope_tables keeps the reference's float32 angles."""
+                     max_position: int = 4096, device="cpu", first: int = 0):
+    """(cos, sin) torch tensors [max_seq_len - first, dim/2] fp32 of scaled_frequencies
+    at positions first, first + 1 .., angles in float64; rope_tables keeps the
+    reference's float32 angles."""
     import torch
 
     freq, factor = scaled_frequencies(dim, theta, scaling, max_position)
-    angle = torch.arange(max_seq_len, dtype=torch.float64, device=device)[:, None] * torch.from_numpy(freq).to(device)
+    pos = torch.arange(first, max_seq_len, dtype=torch.float64, device=device)
+    angle = pos[:, None] * torch.from_numpy(freq).to(device)
     return (angle.cos() * factor).float(), (angle.sin() * factor).float()
+
+
+# Positions whose float32 angles are as good as any: what they cost cos and sin (theta 5e5 and 1e4, up to
+# 2.4e-4 before position 4096, 0.004 at 65536, 0.008 at 131072) is a sixteenth of half a step of bf16 near one.
+FLOAT32_POSITIONS = 4096
+
+
+def paged_rope_tables(dim: int, max_seq_len: int, theta: float = 10000.0, scaling: dict | None = None,
+                      max_position: int = 4096, device="cpu"):
+    """(cos, sin) torch tensors [max_seq_len, dim/2] fp32 of a paged layer: without scaling the
+    rows of rope_tables before FLOAT32_POSITIONS, so that its keys are those of DecodeAttention
+    bit for bit, and angles in float64 behind them; with scaling long_rope_tables."""
+    import torch
+
+    if is_scaled(scaling):
+        return long_rope_tables(dim, max_seq_len, theta, scaling, max_position, device)
+    near = [torch.from_numpy(t).to(device) for t in rope_tables(dim, min(max_seq_len, FLOAT32_POSITIONS), theta)]
+    if max_seq_len <= FLOAT32_POSITIONS:
+        return tuple(near)
+    far = long_rope_tables(dim, max_seq_len, theta, device=device, first=FLOAT32_POSITIONS)
+    return tuple(torch.cat(t) for t in zip(near, far))

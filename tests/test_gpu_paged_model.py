@@ -171,7 +171,7 @@ def stepping(paged=(), attention=()):
     """A model of no layers on the host with both kinds of attention."""
     cfg = BitNetMiniConfig(num_attention_heads=2)
     step = BitLinearDecodeStep(cfg, torch.device("cpu"), batch=2)
-    step.alloc_attention(max_seq_len=64, **dict(attention))
+    step.alloc_attention(**{"max_seq_len": 64, **dict(attention)})
     step.paged = PagedAttention(cfg.num_attention_heads, cfg.num_kv_heads, cfg.head_dim,
                                 **{"max_seq_len": 64, "device": "cpu", "rope_theta": cfg.rope_theta, **dict(paged)})
     step.pages = []
@@ -212,6 +212,40 @@ def test_long_tables_without_scaling_are_the_plain_angles():
     far, _ = long_rope_tables(16, 100001, 10000.0)
     want = np.cos(100000.0 * 10000.0 ** (-np.arange(0, 16, 2) / 16.0))
     assert np.abs(far[100000].double().numpy() - want).max() <= 2.0 ** -24
+
+
+@pytest.mark.parametrize("theta,dim,rotary", [(500000.0, 128, None), (10000.0, 64, 32)])
+def test_the_layers_own_angles_at_far_positions(theta, dim, rotary):
+    """Float32 angles are off by up to 0.006 at position 100000; the layer's tables are rounded once. The first
+    4096 rows are DecodeAttention's."""
+    n, R = 100001, rotary or dim
+    for kw in ({}, {"rope_scaling": {"type": "default"}}):
+        att = PagedAttention(4, 2, dim, n, "cpu", rope_theta=theta, rotary_dim=rotary, **kw)
+        assert att.rope_cos.shape == att.rope_sin.shape == (n, R // 2) and att.rope_cos.dtype is torch.float32
+        c, s = rope_tables(R, 5000, theta)
+        assert np.array_equal(att.rope_cos[:4096], c[:4096]) and np.array_equal(att.rope_sin[:4096], s[:4096])
+        freq = theta ** (-np.arange(0, R, 2) / R)
+        for p in (4096, 4097, 65536, 100000):
+            # a 64-bit angle of up to 1e5: off by 1e5 x 2^-52
+            for got, f in ((att.rope_cos, np.cos), (att.rope_sin, np.sin)):
+                assert np.abs(got[p].double().numpy() - f(p * freq)).max() <= 2.0 ** -24 / 2 + 1e-10
+    for n in (1, 4095, 4096):
+        c, s = rope_tables(R, n, theta)
+        att = PagedAttention(4, 2, dim, n, "cpu", rope_theta=theta, rotary_dim=rotary)
+        assert np.array_equal(att.rope_cos, c) and np.array_equal(att.rope_sin, s)
+
+
+@pytest.mark.parametrize("paged,contiguous", [(5000, 5000), (6000, 5000), (5000, 6000), (4096, 5000), (4100, 64)])
+def test_the_step_takes_the_far_angles_of_the_cached_keys(paged, contiguous):
+    step = stepping({"max_seq_len": paged}, {"max_seq_len": contiguous})
+    before = step.attention.rope_cos.clone(), step.attention.rope_sin.clone()
+    where = step.attention.rope_cos.data_ptr()
+    step.load_contiguous(torch.zeros((2, 1), dtype=torch.int32), torch.tensor([5, 7], dtype=torch.int32))
+    n = min(paged, contiguous)
+    for got, own, old in ((step.attention.rope_cos, step.paged.rope_cos, before[0]),
+                          (step.attention.rope_sin, step.paged.rope_sin, before[1])):
+        assert got.shape[0] == contiguous and torch.equal(got[:n], own[:n]) and torch.equal(got[n:], old[n:])
+    assert step.attention.rope_cos.data_ptr() == where  # captured steps read them
 
 
 def test_linear_and_llama3_frequencies():
