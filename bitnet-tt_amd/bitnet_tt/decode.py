@@ -346,9 +346,12 @@ class BitLinearDecodeStep:
         if getattr(self, "paged", None) is None:
             raise RuntimeError("forward_rows needs alloc_paged() first")
         c = self.config
+        if hidden.dtype is not torch.bfloat16 or hidden.dim() != 2 or hidden.shape[1] != c.hidden_size:
+            raise ValueError(f"hidden must be bf16 [T, {c.hidden_size}]")
         T = hidden.shape[0]
         if T == 0:
             return hidden
+        N.require_cuda(hidden, "hidden")
         dev = hidden.device
         qkv = torch.empty((T, c.qkv_dim), dtype=torch.bfloat16, device=dev)
         attn = torch.empty((T, c.num_attention_heads * c.head_dim), dtype=torch.bfloat16, device=dev)

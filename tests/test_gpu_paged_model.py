@@ -178,6 +178,19 @@ def stepping(paged=(), attention=()):
     return step
 
 
+@pytest.mark.parametrize("hidden,match", [
+    (torch.zeros((3, 256)), "bf16"), (torch.zeros((3, 256), dtype=torch.int8), "bf16"),
+    (torch.zeros((3, 256), dtype=torch.float16), "bf16"), (torch.zeros((3, 128), dtype=torch.bfloat16), "bf16"),
+    (torch.zeros((1, 3, 256), dtype=torch.bfloat16), "bf16"), (torch.zeros(256, dtype=torch.bfloat16), "bf16"),
+    (torch.zeros((3, 256), dtype=torch.bfloat16), "ROCm GPU"),
+])
+def test_rows_that_forward_rows_refuses(hidden, match):
+    """Before anything reads them: rows of fewer bytes than bf16's would be read behind their end."""
+    i32 = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match=match):
+        stepping().forward_rows(hidden, i32[None], i32, i32[:1])
+
+
 @pytest.mark.parametrize("paged,attention", [
     ({"use_fused_rope": True}, {}), ({}, {"use_fused_rope": True}), ({"rope_theta": 10000.0}, {}), ({"rotary_dim": 64}, {}),
     ({"rope_scaling": {"type": "linear", "factor": 2.0}}, {}),
