@@ -339,7 +339,9 @@ class BitLinearDecodeStep:
         """The layers on any rows of any users: hidden bf16 [T, hidden], in place.
         Sequence b's rows are ``cu_q[b] .. cu_q[b + 1] - 1``, its newest tokens; their
         keys and values are cached, and kv_len counts them (bitnet_tt.paged_attention).
-        Whole prompts, chunks of them and single tokens may share a call.  Needs
+        Whole prompts, chunks of them and single tokens may share a call.  Rows of no
+        sequence (behind cu_q[B], say, in a captured call of fewer tokens) run through the
+        layers with zeros for their attention; nothing is cached for them.  Needs
         alloc_paged()."""
         import torch
 
@@ -354,7 +356,8 @@ class BitLinearDecodeStep:
         N.require_cuda(hidden, "hidden")
         dev = hidden.device
         qkv = torch.empty((T, c.qkv_dim), dtype=torch.bfloat16, device=dev)
-        attn = torch.empty((T, c.num_attention_heads * c.head_dim), dtype=torch.bfloat16, device=dev)
+        # (zeros: the attention leaves rows of no sequence as they were)
+        attn = torch.zeros((T, c.num_attention_heads * c.head_dim), dtype=torch.bfloat16, device=dev)
         ffn = torch.empty((T, c.intermediate_size), dtype=torch.bfloat16, device=dev)
         for w, pages in zip(self.layers, self.pages):
             ternary_matmul_into(hidden, w.qkv, qkv, norm_weight=w.input_layernorm, norm_epsilon=self.eps)

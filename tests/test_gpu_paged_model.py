@@ -108,6 +108,56 @@ def test_forward_rows_is_the_layers_chain():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("lead", [0, 2])
+def test_rows_of_no_sequence_meet_no_stale_memory(lead):
+    """A batch padded before and behind its rows, in memory that held other values: the padding's rows are what zeros for
+    their attention make of them, the others the unpadded call's; eager and replayed."""
+    cfg = BitNetMiniConfig()
+    step = BitLinearDecodeStep.random_init(cfg, dev(), seed=3, batch=2, num_layers=2)
+    step.alloc_paged(16, 256, page_size=32)
+    table = torch.arange(16, dtype=torch.int32, device=dev()).view(2, 8)
+    hidden = normal((40, cfg.hidden_size), 4).to(torch.bfloat16).to(dev())
+    cu, total = cu_of([20, 7]), ints([20, 7])
+    real = slice(lead, lead + 27)
+    alone = step.forward_rows(hidden[real].clone(), table, cu, total)
+    pad = torch.cat((hidden[:lead], hidden[lead + 27:]))
+    want = torch.empty_like(hidden)
+    want[real] = alone
+    h = pad.clone()
+    for w in step.layers:
+        a = torch.zeros((len(pad), cfg.num_attention_heads * cfg.head_dim), dtype=torch.bfloat16, device=dev())
+        h = ternary_matmul(a, w.o_proj, norm_weight=w.attn_sub_norm, norm_epsilon=step.eps, residual=h)
+        f = ternary_matmul(h, w.gate_up, norm_weight=w.post_attention_layernorm, norm_epsilon=step.eps,
+                           epilogue="relu2_mul")
+        h = ternary_matmul(f, w.down, norm_weight=w.ffn_sub_norm, norm_epsilon=step.eps, residual=h)
+    want[:lead], want[lead + 27:] = h[:lead], h[lead:]
+    padded = cu + lead
+
+    def stale():
+        return [torch.full((40, n), 3.0, dtype=torch.bfloat16, device=dev())
+                for n in (cfg.qkv_dim, cfg.hidden_size, cfg.intermediate_size) for _ in range(20)]
+
+    got = hidden.clone()
+    stale()  # (freed at once)
+    assert torch.equal(step.forward_rows(got, table, padded, total), want)
+    stream, rows = torch.cuda.Stream(), hidden.clone()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        step.forward_rows(rows, table, padded, total)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            step.forward_rows(rows, table, padded, total)
+    for _ in range(3):
+        rows.copy_(hidden)
+        stale()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(rows, want)
+    step.check()
+
+
+@pytest.mark.gpu
 def test_pages_to_the_contiguous_step():
     """A prompt over pages, then decode steps on the contiguous caches: the attention of the
     first step sees what the pages held."""
