@@ -161,6 +161,7 @@ EXPORTS = {
         _I,
     ),
     "btl_page_row": ([_I64, _I64, _I64, _I64, _I64, _I64], _I64),
+    "btl_page_run": ([_I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P], _I),
     "btl_clamp_seq": ([_I64, _I64, _I64, _I64, _I64, _P], _I),
     "btl_row_exponent": ([_F], _I),
     "btl_paged_attention_plan": ([_I64, _I64, _I64, _I64, _I64, _I64, _I64, _P], _I),

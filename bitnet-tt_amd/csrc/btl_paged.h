@@ -88,7 +88,7 @@ struct Run {
   int64_t row;
   uint32_t n;
 };
-__device__ __forceinline__ Run run_at(const Pages& pg, int hk, int at, int kv_end, int32_t page, int most, bool& bad) {
+__host__ __device__ __forceinline__ Run run_at(const Pages& pg, int hk, int at, int kv_end, int32_t page, int most, bool& bad) {
   const int left = clampi(kv_end - at, 0, most);
   const bool none = (uint32_t)page >= (uint32_t)pg.P;
   bad |= none & (left > 0);

@@ -198,8 +198,8 @@ __global__ __launch_bounds__(kRopeThreads) void k_rope_write(RopeArgs p) {
       *reinterpret_cast<uint4*>(d + o0) = o.a;
       *reinterpret_cast<uint4*>(d + o1) = o.b;
     }
-    if (page < 0) continue;
-    const int64_t at = ((int64_t)page * p.Hkv + hk) * p.pg.ps.d + s_row[t];
+    const int64_t at = page_row(page, p.pg.P, p.Hkv, hk, p.pg.ps.d, s_row[t]);
+    if (at < 0) continue;
     uint8_t* const pages = is_k ? p.pg.k : p.pg.v;
     if (!p.fp8) {
       uint16_t* d = reinterpret_cast<uint16_t*>(pages) + at * D;
@@ -323,6 +323,23 @@ int64_t btl_page_row(int64_t page, int64_t num_pages, int64_t num_kv_heads, int6
   const FastDiv f = fast_div((uint32_t)page_size);
   return page_row((int32_t)page, (int)num_pages, (int)num_kv_heads, (int)kv_head, (int)page_size,
                   (int)(position - (int64_t)div_by((uint32_t)position, f) * page_size));
+}
+
+int btl_page_run(int64_t page, int64_t num_pages, int64_t num_kv_heads, int64_t kv_head, int64_t page_size, int64_t position,
+                 int64_t end, int64_t most, int64_t* run) {
+  if (!run || page_size < 16 || page_size > kMaxPageSize || num_pages <= 0 || num_pages > INT32_MAX || page > INT32_MAX ||
+      page < INT32_MIN || num_kv_heads <= 0 || num_kv_heads > 1024 || kv_head < 0 || kv_head >= num_kv_heads || position < 0 ||
+      position > INT32_MAX || end < 0 || end > INT32_MAX || most < 0 || most > INT32_MAX)
+    return -1;
+  Pages pg{};
+  pg.P = (int)num_pages;
+  pg.Hkv = (int)num_kv_heads;
+  pg.ps = fast_div((uint32_t)page_size);
+  bool bad = false;
+  const Run r = run_at(pg, (int)kv_head, (int)position, (int)end, (int32_t)page, (int)most, bad);
+  run[0] = r.row;
+  run[1] = r.n;
+  return bad ? 1 : 0;
 }
 
 int btl_clamp_seq(int64_t lo, int64_t hi, int64_t len, int64_t T, int64_t cap, int64_t* seq) {

@@ -491,8 +491,10 @@ int btl_paged_attention(const uint16_t* q, int64_t ldq, int64_t T, int64_t H, co
                         int64_t B, float scale, int64_t max_q, int64_t max_kv, uint16_t* out, int64_t ldo,
                         void* scratch, size_t scratch_bytes, int32_t* error_word, btl_stream_t stream);
 
-/* Test hooks, host only: the functions that the kernels call.  btl_page_row:
- * the index of a position's (page, head, row), -1 for a page outside the pool.
+/* Test hooks, host only: the functions that the kernels call.  btl_page_row (writes and
+ * page reads): the index of a position's (page, head, row), -1 for a page outside the pool.
+ * btl_page_run (attention): {index of the first, rows} of the run of up to `most` rows from a position up
+ * to `end`, no rows for a page outside the pool; 1 where there should be some, -1 for bad arguments.
  * btl_clamp_seq: {first row, rows, positions} of a sequence (cu_q entries lo
  * and hi) after clamping; 1 if nothing had to be; cap < 0: no length is given, the
  * positions are the rows.  btl_row_exponent: e of an 8-bit
@@ -501,6 +503,8 @@ int btl_paged_attention(const uint16_t* q, int64_t ldq, int64_t T, int64_t H, co
  * that it refuses. */
 int64_t btl_page_row(int64_t page, int64_t num_pages, int64_t num_kv_heads, int64_t kv_head, int64_t page_size,
                      int64_t position);
+int btl_page_run(int64_t page, int64_t num_pages, int64_t num_kv_heads, int64_t kv_head, int64_t page_size, int64_t position,
+                 int64_t end, int64_t most, int64_t* run);
 int btl_clamp_seq(int64_t lo, int64_t hi, int64_t len, int64_t T, int64_t cap, int64_t* seq);
 int btl_row_exponent(float largest);
 int btl_paged_attention_plan(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t B, int64_t max_q, int64_t max_kv,

@@ -165,6 +165,32 @@ def test_page_of_a_position(L):
     assert L.btl_page_row(2 ** 31 - 2, 2 ** 31 - 1, 8, 7, 256, 255) == ((2 ** 31 - 2) * 8 + 7) * 256 + 255
 
 
+def test_run_of_positions(L):
+    """What attention places its rows with: as btl_page_row, whatever the pool's size."""
+    out = (ctypes.c_int64 * 2)()
+
+    def f(*a):
+        return L.btl_page_run(*a, out), tuple(out)
+
+    r = random.Random(3)
+    for _ in range(3000):
+        ps = 16 * r.choice([1, 2, 3, 4, 16, 63, 4096, 65536, r.randint(1, 65536)])
+        heads = r.choice([1, 2, 5, 8, 128, 1024])
+        P = r.choice([1, 9, 1 << 20, 2 ** 31 - 1])
+        page = r.choice([0, P - 1, r.randrange(P)])
+        hk, at = r.randrange(heads), 16 * r.randrange(2 ** 26)
+        most = r.choice([16, 32, 64])
+        end = min(2 ** 31 - 1, max(0, at + r.randint(-40, 80)))
+        left = max(0, min(most, end - at))
+        assert f(page, P, heads, hk, ps, at, end, most) == (0, ((page * heads + hk) * ps + at % ps, left))
+        assert L.btl_page_row(page, P, heads, hk, ps, at) == out[0]
+        for outside in (-1, P, 2 ** 31 - 1, -2 ** 31):
+            if outside != page and not 0 <= outside < P:
+                bad, (row, n) = f(outside, P, heads, hk, ps, at, end, most)
+                assert (bad, n) == (left > 0, 0) and 0 <= row < heads * ps
+    assert L.btl_page_run(0, 1, 1, 1, 16, 0, 1, 16, out) == -1 and L.btl_page_run(0, 1, 1, 0, 8, 0, 1, 16, out) == -1
+
+
 def test_clamped_sequences(L):
     out = (ctypes.c_int64 * 3)()
 
