@@ -339,7 +339,8 @@ class BitLinearDecodeStep:
         """The layers on any rows of any users: hidden bf16 [T, hidden], in place.
         Sequence b's rows are ``cu_q[b] .. cu_q[b + 1] - 1``, its newest tokens; their
         keys and values are cached, and kv_len counts them (bitnet_tt.paged_attention).
-        Whole prompts, chunks of them and single tokens may share a call.  Rows of no
+        Whole prompts, chunks of them and single tokens may share a call; all of them attend to
+        the pages, so with 8-bit pages a prompt's own keys and values are the rounded ones.  Rows of no
         sequence (behind cu_q[B], say, in a captured call of fewer tokens) run through the
         layers with zeros for their attention; nothing is cached for them.  Needs
         alloc_paged()."""

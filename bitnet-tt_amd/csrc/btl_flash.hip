@@ -22,7 +22,10 @@
 // factors that this puts on what has been summed are powers of two: exact.  p is
 // rounded to bf16 for the second product, the matrix units' operand type, and the
 // sum takes the same rounded values, so the weights that are used sum to one (few rows over bf16
-// pages: 16 bits of p).
+// pages: 16 bits of p).  Two bf16 values of p in the tiles as well, a second product on the same values,
+// measured: 4096 tokens 100 us, 136 so; 16001 415, 565; chunks of 4 users over up to 8000 139, 187; 67
+// tokens over 40067 8-bit positions 62, 73.  Against 64 bits the one value costs 0.0020-0.0022 of the
+// outputs' size where their own rounding has 0.0016.
 //
 // Rows of V behind the last position read as zero (whatever lies there), and a
 // value that is not finite at a position that some of the tile's rows may not see is added
@@ -648,15 +651,15 @@ __global__ __launch_bounds__(256, 2) void k_flash_tile(FlashArgs p) {
 // fetched a round ahead of that.  The waves' partials meet in LDS.
 //
 // Over bf16 pages p is two bf16 values, itself rounded and what that leaves, so 16 bits of it
-// are used: the matrix units have the time (one user at 131001 positions 66.0 us, 66.2 so; 128 users at 2048
-// 121 and 120).  The rests have a sum of their own (one sum for both: 0.3 us less at 512 positions, but infinite values
+// are used: the matrix units have the time (one user at 131001 positions 65.3 us, 65.7 so; 128 users at 2048
+// 126.6, 126.9; 32 at 2048 35.5, 35.9).  The rests have a sum of their own (in one sum with the rest an infinite value
 // that a row sees would become NaN), and the error against 64 bits is that of the output's own rounding.  8-bit
-// pages, whose values have 4 bits, cost 1 to 8% for it and have one.
+// pages, whose values have 4 bits, would pay 1 to 7% (128 users at 2048 70.2, 71.1; 32 at 2048 21.7, 23.3) and have one.
 //
-// 5 heads of 128: one user at 131001 positions 59 us (5.7 TB/s) and 5 of the merge, 128
-// users at 2048 124 us (5.4 TB/s); 8-bit pages 69 us (4.9).  8 / 4 / 2 waves a workgroup, each
-// at its best number of splits, 32 users of mixed lengths up to 4096, 8-bit pages: 38.5, 36.9,
-// 36.2 us; one user at 512 positions: 10.7, 9.7, 13.0.
+// 5 heads of 128: one user at 131001 positions 60 us (5.6 TB/s) and 5 of the merge, 128
+// users at 2048 127 us (5.3 TB/s); 8-bit pages 70 us (4.8).  8 / 4 / 2 waves a workgroup, each
+// at its best number of splits, in an early form of this kernel, 32 users of mixed lengths up to 4096,
+// 8-bit pages: 38.5, 36.9, 36.2 us; one user at 512 positions: 10.7, 9.7, 13.0.
 // ======================================================================
 constexpr int kFewRows = 16;
 constexpr int kFewWaves = 4;
@@ -1038,10 +1041,17 @@ struct FlashPlan {
 //    at n = sqrt(whole / part), and n = 1 is better where that saves less than it costs.
 //    Without this, with it: 2 x 512 rows at 512: 27.4, 17.8; 4 x 256 at 1024: 36.0, 26.8;
 //    1000 at 1000: 28.9, 26.6; 512 at 2048: 34.9, 31.0; 256 at 1024: 23.2, 24.2.
+//    The two rates are those of bf16 pages and D = 128; a step over 8-bit pages takes up to 1.4 times as long, one of
+//    D = 64 0.8 times.  What the rule takes against the best of 1, 2, 3, 4, 6, 8, 12, 16, 32 splits:
+//    67 rows at 40067 | 256 at 1024 | 512 at 2048 | 1000 at 9000 | 2047 of 4 up to 8000 | 2048 of 8 up to 7700,
+//    D = 128, bf16: 64.3, 59.6 | 22.5, 21.2 | 29.7, 29.7 | 116, 111 | 140, 140 | 189, 176;
+//    8-bit:         65.6, 61.5 | 25.6, 23.1 | 34.3, 33.8 | 122, 121 | 154, 154 | 206, 196;
+//    4 / 2 heads of 64, bf16: 24.4, 24.4 | 12.6, 12.6 | 14.3, 14.2 | 31.9, 30.0 | 38.3, 38.3 | 41.4, 41.0;
+//    8-bit:         26.5, 26.5 | 13.4, 13.3 | 14.9, 14.8 | 34.6, 32.0 | 41.7, 41.7 | 45.2, 44.7.
 //  - Few rows: bound by memory, which one workgroup a CU saturates: as many
 //    as there are CUs, from 1024 positions on.  bf16, 1 user at 16384, 16 / 25 / 51 / 102
-//    splits: 20.1, 17.8, 16.5, 20.6; 8 users at 4096, 3 / 6 / 8: 24.3, 21.2, 24.6; 32 users
-//    at 4096, 1 / 2 / 3: 60, 78, 70; 1 user at 1024, 1 / 4: 13.2, 11.2.
+//    splits: 20.1, 17.8, 16.5, 20.6; 8 users at 4096, 3 / 6 / 8: 24.3, 21.2, 24.6; 1 user at 1024,
+//    1 / 4: 13.2, 11.2.
 //    Up to 9/4 as many workgroups as CUs, some CUs have a long context more than others:
 //    four splits from 2560 positions on.  Contexts of unlike length up to 4000, 1 / 2 / 3 / 4 / 6:
 //    bf16, 36 users 53, 56, 49, 43, 49; 56: 100, 70, 65, 65, 66; 80: 107, 84, 85, 85, 87; 110: 125,
@@ -1049,6 +1059,11 @@ struct FlashPlan {
 //    bf16: 36: 69, 82, 82, 72, 76; 56: 138, 121, 117, 110, 110; 110: 227, 214, 209, 203, 207.  At 2048 positions,
 //    1 / 4, unlike or alike, the gain is gone: bf16, 32 users 25.7, 27.2 or 33.7, 37.5;
 //    140: 86, 86 or 134, 138.
+//    Below one workgroup a CU the gain is that of 8-bit pages, and of some lengths: 1 / 2 / 3 / 4 splits, unlike
+//    lengths up to 4096 (a quarter of it the least) or all of 4096, 32 users, bf16: 58, 65, 60, 59 or 65, 80, 71, 72;
+//    8-bit: 37, 32, 31, 34 or 42, 46, 42, 42; 48 users, bf16: 68, 73, 69, 69 or 92, 97, 98, 98; 8-bit: 39, 39, 39,
+//    37 or 50, 55, 56, 56; 80 users of 2 heads of 64, bf16: 28, 30, 27, 27 or 35, 43, 38, 38; 8-bit: 30, 25, 22, 19 or
+//    31, 25, 23, 23.  (What would serve both: positions shared out by the lengths on the device.)
 constexpr int64_t kMinChunk = 256;
 constexpr int64_t kMaxSplits = 256;
 // A hint behind this plans for as many positions as a page table may have room for: splits x
