@@ -426,6 +426,8 @@ int btl_decode_attention_split(const uint16_t* qkv, int64_t B, int64_t H, int64_
  * and nothing is written for them.  Rows outside [cu_q[0], cu_q[B]) are left
  * as they were.
  *
+ * Attention keeps scores as 32-bit floats: it is defined for |scale q.k| below 2^30.
+ *
  * error_word: a device int32 the caller owns, zero at first; a kernel that
  * meets a cu_q that decreases or leaves [0, T], a kv_len that is negative or
  * behind the page table's (or the angle tables') last position, or a page

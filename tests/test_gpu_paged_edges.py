@@ -212,3 +212,23 @@ def test_hints_of_the_c_entry_behind_the_table(kv, max_kv, new, max_q):
     want, tol = pb.reference()
     check_close(out, want, tol)
     assert int(word) == 0
+
+
+@pytest.mark.parametrize("power", [21, 29])
+def test_large_scores_that_are_equal(power):
+    """scale q.k of 2^power at every position: weights are equal whatever 32 bits make of the offset, so the
+    output is the value that all positions have."""
+    H, Hkv, D, n = 4, 2, 64, 40
+    side = 2.0 ** ((power + 3 - 6) // 2)  # D side^2 / 8
+    assert side * side * D / 8 == 2.0 ** power
+    q = torch.full((n, H, D), side, dtype=torch.bfloat16, device=dev())
+    k = torch.full((n, Hkv, D), side, dtype=torch.bfloat16, device=dev())
+    v = torch.full((n, Hkv, D), 3.0, dtype=torch.bfloat16, device=dev())
+    assert torch.equal(pa.prompt_attention(q, k, v, cu_of([n])), torch.full_like(q, 3.0))
+    cache = pa.PagedKVCache.allocate(3, Hkv, D, dev(), page_size=16)
+    cache.key_pages.fill_(side)
+    cache.value_pages.fill_(3.0)
+    table = torch.arange(3, dtype=torch.int32, device=dev())[None]
+    for max_q in (1, 40):
+        out = pa.paged_attention(q, cache, table, cu_of([n]), ints([n]), max_q=max_q)
+        assert torch.equal(out, torch.full_like(q, 3.0))

@@ -217,6 +217,61 @@ def test_the_step_goes_on_where_the_prompts_end():
     assert float((a - b).norm() / a.norm()) < 0.05
 
 
+@pytest.mark.gpu
+def test_captured_hand_over_to_the_one_launch_step():
+    """load_contiguous and the one-launch step in a graph: what the pages hold, positions and far angles follow at
+    every replay, and the step is the eager calls' bit for bit."""
+    from bitnet_tt.config import BitNetConfig
+
+    cfg = BitNetConfig(hidden_size=512, num_layers=2, num_attention_heads=4, num_key_value_heads=1,
+                       intermediate_size=1024, vocab_size=1000, max_position_embeddings=256)
+    S = 4160
+    step = BitLinearDecodeStep.random_init(cfg, dev(), seed=5, batch=2)
+    step.alloc_buffers().alloc_attention(max_seq_len=S).alloc_paged(2 * S // 64, S, page_size=64)
+    assert not torch.equal(step.attention.rope_cos[4096:], step.paged.rope_cos[4096:])
+    table = torch.arange(2 * S // 64, dtype=torch.int32, device=dev()).view(2, -1)
+    for pages, seed in zip(step.pages, (1, 2)):
+        pages.key_pages.copy_(normal(pages.shape, seed))
+        pages.value_pages.copy_(normal(pages.shape, seed + 2))
+    kv_len = ints([100, 4130])
+
+    def go():
+        step.reset_hidden()
+        step.load_contiguous(table, kv_len)
+        step.step_persistent_full()
+
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        go()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            go()
+    for lens in ([100, 4130], [0, 4159], [4100, 1], [64, 65]):
+        kv_len.copy_(ints(lens))
+        for kv in step.kv:
+            kv.key_cache.fill_(3.0)
+            kv.value_cache.fill_(3.0)
+        step.pos.fill_(0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        got, caches = step.hidden.clone(), [kv.key_cache.clone() for kv in step.kv]
+        assert step.pos.tolist() == lens
+        assert torch.equal(step.attention.rope_sin[4096:], step.paged.rope_sin[4096:])
+        for kv, pages in zip(step.kv, step.pages):
+            for b, n in enumerate(lens):
+                rows = pages.key_pages[table[b].long(), 0].flatten(0, 1)
+                assert torch.equal(kv.key_cache[b, 0, :n], rows[:n])
+                assert bool((kv.key_cache[b, 0, n + 1:] == 3.0).all())  # row n is the step's own
+        step.reset_hidden()
+        step.load_contiguous(table, kv_len)
+        step.step_full()
+        assert torch.equal(got, step.hidden)
+        assert all(torch.equal(a, kv.key_cache) for a, kv in zip(caches, step.kv))
+    step.check()
+
+
 def stepping(paged=(), attention=()):
     """A model of no layers on the host with both kinds of attention."""
     cfg = BitNetMiniConfig(num_attention_heads=2)
