@@ -349,7 +349,8 @@ class BitLinearDecodeStep:
         if getattr(self, "paged", None) is None:
             raise RuntimeError("forward_rows needs alloc_paged() first")
         c = self.config
-        if hidden.dtype is not torch.bfloat16 or hidden.dim() != 2 or hidden.shape[1] != c.hidden_size:
+        if (hidden.dtype is not torch.bfloat16 or hidden.dim() < 2
+                or hidden.numel() != hidden.shape[0] * c.hidden_size):  # [T, 1, hidden] is [T, hidden] too
             raise ValueError(f"hidden must be bf16 [T, {c.hidden_size}]")
         T = hidden.shape[0]
         if T == 0:

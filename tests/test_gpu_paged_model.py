@@ -287,7 +287,8 @@ def stepping(paged=(), attention=()):
     (torch.zeros((3, 256)), "bf16"), (torch.zeros((3, 256), dtype=torch.int8), "bf16"),
     (torch.zeros((3, 256), dtype=torch.float16), "bf16"), (torch.zeros((3, 128), dtype=torch.bfloat16), "bf16"),
     (torch.zeros((1, 3, 256), dtype=torch.bfloat16), "bf16"), (torch.zeros(256, dtype=torch.bfloat16), "bf16"),
-    (torch.zeros((3, 256), dtype=torch.bfloat16), "ROCm GPU"),
+    (torch.zeros((3, 256), dtype=torch.bfloat16), "ROCm GPU"), (torch.zeros((3, 1, 256), dtype=torch.bfloat16), "ROCm GPU"),
+    (torch.zeros((3, 2, 256), dtype=torch.bfloat16), "bf16"),
 ])
 def test_rows_that_forward_rows_refuses(hidden, match):
     """Before anything reads them: rows of fewer bytes than bf16's would be read behind their end."""
