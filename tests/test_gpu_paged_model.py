@@ -194,7 +194,7 @@ def test_pages_to_the_contiguous_step():
 
 @pytest.mark.gpu
 def test_the_step_goes_on_where_the_prompts_end():
-    """As the README has it: alloc_attention's own positions (the last) and random caches, prompts, load_contiguous,
+    """alloc_attention's own positions (the last) and random caches, prompts, load_contiguous,
     and a step: it attends to the prompts and its own token, not to what else the caches hold."""
     from bitnet_tt.config import BitNetConfig
 
