@@ -34,6 +34,7 @@ from . import _native as N
 _BF16 = torch.bfloat16
 _ERROR_BYTES = 256
 _ERROR_KIND = "paged"
+_FAR = 1 << 30  # no position is as far as that
 
 
 class PagedKVCache:
@@ -254,9 +255,24 @@ def read_pages(cache: PagedKVCache, page_table, kv_len, key_cache, value_cache) 
         N.check(rc, "btl_read_pages")
 
 
-def prompt_attention(q, k, v, cu_seqlens, scale: float | None = None, max_q: int | None = None, out=None):
+def _window(window, sinks):
+    """(window, sinks) of a call, window None where there is none."""
+    if window is None:
+        if sinks:
+            raise ValueError("sinks need a window")
+        return None, 0
+    window, sinks = int(window), int(sinks)
+    if window < 1 or sinks < 0:
+        raise ValueError(f"window {window} must be at least 1, sinks {sinks} at least 0")
+    return min(window, _FAR), min(sinks, _FAR)
+
+
+def prompt_attention(q, k, v, cu_seqlens, scale: float | None = None, max_q: int | None = None, out=None,
+                     window: int | None = None, sinks: int = 0):
     """Causal attention within packed sequences: row i attends to the rows up to
     itself of its own sequence, query head h to key-value head h // (H / Hkv).
+    With ``window``: of those to the last ``window``, itself among them, and to the
+    sequence's first ``sinks``.
 
     q bf16 [T, H, D], k and v [T, Hkv, D] (parts of a QKV row will do: rows may
     be strided); cu_seqlens int32 [B + 1]; scale, positive, defaults to 1/sqrt(D); max_q,
@@ -265,7 +281,9 @@ def prompt_attention(q, k, v, cu_seqlens, scale: float | None = None, max_q: int
     index = _gpu(q, "q")
     if index != torch.cuda.current_device():
         with torch.cuda.device(index):
-            return prompt_attention(q, k, v, cu_seqlens, scale, max_q, out)
+            return prompt_attention(q, k, v, cu_seqlens, scale, max_q, out, window, sinks)
+    if window is not None or sinks:
+        window, sinks = _window(window, sinks)
     if q.dim() != 3 or k.dim() != 3:
         raise ValueError("q must be [T, H, D], k and v [T, Hkv, D]")
     T, H, D = q.shape
@@ -281,19 +299,25 @@ def prompt_attention(q, k, v, cu_seqlens, scale: float | None = None, max_q: int
     else:
         ldo = _rows(out, T, H, D, "out", index)
     stream = N.raw_stream(index)
-    rc = N.lib().btl_prompt_attention(
-        q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, T, H, Hkv, D, cu_seqlens.data_ptr(), B,
-        1.0 / math.sqrt(D) if scale is None else scale, T if max_q is None else max_q, out.data_ptr(), ldo,
-        _error_word(index, stream), stream)
+    args = (q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, T, H, Hkv, D, cu_seqlens.data_ptr(), B,
+            1.0 / math.sqrt(D) if scale is None else scale, T if max_q is None else max_q)
+    if window is None:
+        rc = N.lib().btl_prompt_attention(*args, out.data_ptr(), ldo, _error_word(index, stream), stream)
+    else:
+        rc = N.lib().btl_prompt_attention_window(*args, window, sinks, out.data_ptr(), ldo, _error_word(index, stream),
+                                                 stream)
     if rc != N.BTL_OK:
         N.check(rc, "btl_prompt_attention")
     return out
 
 
 def paged_attention(q, cache: PagedKVCache, page_table, cu_q, kv_len, scale: float | None = None,
-                    max_q: int | None = None, max_kv: int | None = None, out=None):
+                    max_q: int | None = None, max_kv: int | None = None, out=None, window: int | None = None,
+                    sinks: int = 0):
     """Attention of each sequence's newest tokens over its pages: the row at
     position p attends to positions [0, p], which have been written before.
+    With ``window``: to those in (p - window, p] and [0, sinks).  Pages that hold no position
+    that a row of the call sees are not looked up: their entries of the page table may be anything.
 
     q bf16 [T, H, D], rotated.  max_q and max_kv, where known, are the most new
     tokens and the longest kv_len of any sequence: they choose the kernel and how
@@ -303,7 +327,9 @@ def paged_attention(q, cache: PagedKVCache, page_table, cu_q, kv_len, scale: flo
     index = cache.index
     if index != torch.cuda.current_device():
         with torch.cuda.device(index):
-            return paged_attention(q, cache, page_table, cu_q, kv_len, scale, max_q, max_kv, out)
+            return paged_attention(q, cache, page_table, cu_q, kv_len, scale, max_q, max_kv, out, window, sinks)
+    if window is not None or sinks:
+        window, sinks = _window(window, sinks)
     if q.dim() != 3:
         raise ValueError("q must be [T, H, D]")
     T, H, D = q.shape
@@ -326,14 +352,22 @@ def paged_attention(q, cache: PagedKVCache, page_table, cu_q, kv_len, scale: flo
         return out
     if max_q < 1 or max_kv < 1:
         raise ValueError(f"max_q {max_q} and max_kv {max_kv} must be at least 1")
+    if window is not None and window >= most:  # every row sees all of its context
+        window = None
     stream = N.raw_stream(index)
-    nbytes = _scratch_bytes(index, T, H, Hkv, D, B, max_q, max_kv)
+    if window is None:
+        nbytes = _scratch_bytes(index, T, H, Hkv, D, B, max_q, max_kv)
+    else:
+        nbytes = _window_scratch_bytes(index, T, H, Hkv, D, B, max_q, max_kv, window, sinks)
     # the call's own, from the stream-ordered allocator: calls that overlap share nothing
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    rc = N.lib().btl_paged_attention(
-        q.data_ptr(), ldq, T, H, cache._pages, page_table.data_ptr(), max_pages, cu_q.data_ptr(), kv_len.data_ptr(), B,
-        1.0 / math.sqrt(D) if scale is None else scale, max_q, max_kv, out.data_ptr(), ldo,
-        None if scratch is None else scratch.data_ptr(), nbytes, _error_word(index, stream), stream)
+    args = (q.data_ptr(), ldq, T, H, cache._pages, page_table.data_ptr(), max_pages, cu_q.data_ptr(), kv_len.data_ptr(), B,
+            1.0 / math.sqrt(D) if scale is None else scale, max_q, max_kv)
+    into = (out.data_ptr(), ldo, None if scratch is None else scratch.data_ptr(), nbytes, _error_word(index, stream), stream)
+    if window is None:
+        rc = N.lib().btl_paged_attention(*args, *into)
+    else:
+        rc = N.lib().btl_paged_attention_window(*args, window, sinks, *into)
     if rc != N.BTL_OK:
         N.check(rc, "btl_paged_attention")
     return out
@@ -342,6 +376,12 @@ def paged_attention(q, cache: PagedKVCache, page_table, cu_q, kv_len, scale: flo
 @functools.lru_cache(maxsize=4096)
 def _scratch_bytes(index: int, T: int, H: int, Hkv: int, D: int, B: int, max_q: int, max_kv: int) -> int:
     return int(N.lib().btl_paged_attention_scratch_bytes(T, H, Hkv, D, B, max_q, max_kv))
+
+
+@functools.lru_cache(maxsize=4096)
+def _window_scratch_bytes(index: int, T: int, H: int, Hkv: int, D: int, B: int, max_q: int, max_kv: int, window: int,
+                          sinks: int) -> int:
+    return int(N.lib().btl_paged_attention_window_scratch_bytes(T, H, Hkv, D, B, max_q, max_kv, window, sinks))
 
 
 def check(device=None) -> None:

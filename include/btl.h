@@ -493,6 +493,22 @@ int btl_paged_attention(const uint16_t* q, int64_t ldq, int64_t T, int64_t H, co
                         int64_t B, float scale, int64_t max_q, int64_t max_kv, uint16_t* out, int64_t ldo,
                         void* scratch, size_t scratch_bytes, int32_t* error_word, btl_stream_t stream);
 
+/* Both with a window (at least 1) and sinks (at least 0): the row at position p attends to
+ * the positions in (p - window, p] and, up to p, in [0, sinks).  Over pages, those
+ * that hold no position that a row of the call sees are not looked up: their entries of the page table may be anything.
+ * The scratch is that of btl_paged_attention_window_scratch_bytes. */
+int btl_prompt_attention_window(const uint16_t* q, int64_t ldq, const uint16_t* k, int64_t ldk, const uint16_t* v,
+                                int64_t ldv, int64_t T, int64_t H, int64_t Hkv, int64_t D, const int32_t* cu_q, int64_t B,
+                                float scale, int64_t max_q, int64_t window, int64_t sinks, uint16_t* out, int64_t ldo,
+                                int32_t* error_word, btl_stream_t stream);
+int64_t btl_paged_attention_window_scratch_bytes(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t B, int64_t max_q,
+                                                 int64_t max_kv, int64_t window, int64_t sinks);
+int btl_paged_attention_window(const uint16_t* q, int64_t ldq, int64_t T, int64_t H, const btl_pages_t* pages,
+                               const int32_t* page_table, int64_t max_pages, const int32_t* cu_q, const int32_t* kv_len,
+                               int64_t B, float scale, int64_t max_q, int64_t max_kv, int64_t window, int64_t sinks,
+                               uint16_t* out, int64_t ldo, void* scratch, size_t scratch_bytes, int32_t* error_word,
+                               btl_stream_t stream);
+
 /* Test hooks, host only: the functions that the kernels call.  btl_page_row (writes and
  * page reads): the index of a position's (page, head, row), -1 for a page outside the pool.
  * btl_page_run (attention): {index of the first, rows} of the run of up to `most` rows from a position up
@@ -501,8 +517,8 @@ int btl_paged_attention(const uint16_t* q, int64_t ldq, int64_t T, int64_t H, co
  * and hi) after clamping; 1 if nothing had to be; cap < 0: no length is given, the
  * positions are the rows.  btl_row_exponent: e of an 8-bit
  * row whose largest magnitude is given.  btl_paged_attention_plan: {1 where the kernel of
- * few rows runs, splits, positions of a split} of btl_paged_attention; 1, or 0 for sizes
- * that it refuses. */
+ * few rows runs, splits, positions of a split} of btl_paged_attention (_window_plan: of
+ * btl_paged_attention_window); 1, or 0 for sizes that it refuses. */
 int64_t btl_page_row(int64_t page, int64_t num_pages, int64_t num_kv_heads, int64_t kv_head, int64_t page_size,
                      int64_t position);
 int btl_page_run(int64_t page, int64_t num_pages, int64_t num_kv_heads, int64_t kv_head, int64_t page_size, int64_t position,
@@ -511,6 +527,8 @@ int btl_clamp_seq(int64_t lo, int64_t hi, int64_t len, int64_t T, int64_t cap, i
 int btl_row_exponent(float largest);
 int btl_paged_attention_plan(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t B, int64_t max_q, int64_t max_kv,
                              int64_t* plan);
+int btl_paged_attention_window_plan(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t B, int64_t max_q, int64_t max_kv,
+                                    int64_t window, int64_t sinks, int64_t* plan);
 
 #ifdef __cplusplus
 }
