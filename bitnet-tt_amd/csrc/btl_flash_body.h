@@ -96,13 +96,13 @@ struct FlashArgs {
 struct Span {
   int lo, sinks, end;  // positions: end is behind the last
   int turn, gap;       // the axis leaves the sinks at `turn`
-  // align: what a step's first position must be a multiple of
+  // align: what a step's first position must be a multiple of; step and align are powers of two
   __device__ __forceinline__ void init(const FlashArgs& p, int first_row, int end_, int step, int align) {
-    lo = max(0, first_row - p.window + 1);
+    lo = uni(max(0, first_row - p.window + 1));
     sinks = p.sinks;
     end = end_;
-    turn = (int)(((uint32_t)sinks + step - 1) / step * step);
-    gap = max(0, lo / align * align - turn);
+    turn = (sinks + step - 1) & -step;
+    gap = uni(max(0, (lo & -align) - turn));
   }
   __device__ __forceinline__ int pos(int u) const { return u < turn ? u : u + gap; }
   // Where the positions that are to be loaded end, of n from `at`.
@@ -435,14 +435,30 @@ __device__ __forceinline__ void tile_scores(const lds8* ks, TileKeys& a, const T
     }
 }
 
+// The lowest n bits (n <= 0: none, n >= 32: all).
+__device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? ~0u : (1u << max(n, 0)) - 1u; }
+
 template <int D, int MODE>
 __device__ __forceinline__ void tile_mask(const FlashArgs& p, const TileState<D>& s, int kv, v16f (&sc)[2]) {
   const int h = __lane_id() >> 5;
+  if (MODE == kWindow) {  // a bit a position: three conditions a score would want more scalar registers than there are
+    const int at = max(s.limit - kv - 4 * h, -1), sink = p.sinks - kv - 4 * h;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const uint32_t see = low_bits(at + 1 - 32 * t) & (~low_bits(at + 1 - p.window - 32 * t) | low_bits(sink - 32 * t));
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int keep = __builtin_amdgcn_sbfe((int)see, c_row(r, 0), 1);
+        sc[t][r] = __int_as_float((keep & __float_as_int(sc[t][r])) | (~keep & __float_as_int(kNegInf)));
+      }
+    }
+    return;
+  }
 #pragma unroll
   for (int t = 0; t < 2; ++t)
 #pragma unroll
     for (int r = 0; r < 16; ++r)
-      if (!sees<MODE>(p, s.limit, kv + 32 * t + c_row(r, h))) sc[t][r] = kNegInf;
+      if (kv + 32 * t + c_row(r, h) > s.limit) sc[t][r] = kNegInf;
 }
 
 // Raises the offset where the scores of the next step need it.
@@ -530,6 +546,28 @@ __device__ __forceinline__ void add_not_finite(const FlashArgs& p, const lds8* v
         }
       }
   }
+}
+
+// The tile's part of it: whether there are such values is asked by all waves together.
+template <int D, int MODE>
+__device__ __forceinline__ void tile_not_finite(const FlashArgs& p, lds8* vs, int* s_flag, TileState<D>& s, int pos, bool mine) {
+  const int tid = threadIdx.x;
+  bool nf = false;
+#pragma unroll
+  for (int i = 0; i < Tile<D>::kLoads; ++i) nf |= any_not_finite(lds_ld128(vs + (i * 256 + tid) * 16));
+  const bool any = __any(nf);
+  if ((tid & 63) == 0) s_flag[uni(tid >> 6)] = any;
+  lds_barrier();
+  if (!(s_flag[0] | s_flag[1] | s_flag[2] | s_flag[3])) return;
+  if (mine) add_not_finite<D, MODE>(p, vs, s, pos);
+  lds_barrier();
+#pragma unroll
+  for (int i = 0; i < Tile<D>::kLoads; ++i) {
+    lds8* const piece = vs + (i * 256 + tid) * 16;
+    const uint4 x = lds_ld128(piece);
+    lds_st128(piece, make_uint4(drop_not_finite(x.x), drop_not_finite(x.y), drop_not_finite(x.z), drop_not_finite(x.w)));
+  }
+  lds_barrier();
 }
 
 // LDS: keys in stages 0 and 1, values in 2 and 3; a flag per wave.  (One LDS object: the
@@ -652,19 +690,6 @@ __device__ __forceinline__ void tile_item(const FlashArgs& p, uint8_t* smem, int
       store_ahead(k_free, v_free);
       kv += kStep;
     };
-    // (kWindow: from the first steps' loop, with the parity that they leave; a wave without rows does those steps there)
-    auto hot_steps = [&] {
-      while (kv + 2 * kStep <= whole_end) {
-        hot(sm + kB, sm + 2 * kB, sm, sm + 3 * kB, sa, sb);
-        if (kv + 2 * kStep > whole_end) {
-          at = 1;
-#pragma unroll
-          for (int t = 0; t < 2; ++t) sa[t] = sb[t];
-          break;
-        }
-        hot(sm, sm + 3 * kB, sm + kB, sm + 2 * kB, sb, sa);
-      }
-    };
     if (MODE != kWindow && wr >= rows) {  // a wave without rows only loads (67 tokens at 40000 positions: 68.5 us, 65.5 so)
       for (; kv + 2 * kStep <= whole_end; kv += kStep, at ^= 1) {
         arrived();
@@ -672,9 +697,8 @@ __device__ __forceinline__ void tile_item(const FlashArgs& p, uint8_t* smem, int
         store_ahead(sm + at * kB, sm + (3 - at) * kB);
       }
     }
-    if (MODE != kWindow) hot_steps();
-    for (; kv < kv_end; kv += kStep, at ^= 1) {
-      if (MODE == kWindow && at == 0 && wr < rows && kv >= whole_from) hot_steps();
+    // any step, of the wave's rows those that see some of it
+    auto edge = [&] {
       const lds8* const ks = sm + (at ^ 1) * kB;
       lds8* const vs = sm + (2 + at) * kB;
       lds8 *const k_free = sm + at * kB, *const v_free = sm + (2 + (at ^ 1)) * kB;
@@ -683,28 +707,8 @@ __device__ __forceinline__ void tile_item(const FlashArgs& p, uint8_t* smem, int
       const int pos = src.pos(kv), pos2 = src.pos(kv + kStep);
       const bool mine = some_see<MODE>(p, s.lo, s.hi, pos, kStep);  // some of the wave's rows see some of it
       const bool next = kv + kStep < kv_end && some_see<MODE>(p, s.lo, s.hi, pos2, kStep);
-      bool special = false;
-      if (!all_see<MODE>(p, wg_lo, wg_hi, pos, kStep)) {  // some of the tile's rows do not see all of it
-        bool nf = false;
-#pragma unroll
-        for (int i = 0; i < Tile<D>::kLoads; ++i) nf |= any_not_finite(lds_ld128(vs + (i * 256 + tid) * 16));
-        const bool any = __any(nf);
-        if (lane == 0) s_flag[wv] = any;
-        lds_barrier();
-        special = s_flag[0] | s_flag[1] | s_flag[2] | s_flag[3];
-      }
-      if (special) {
-        if (mine) add_not_finite<D, MODE>(p, vs, s, pos);
-        lds_barrier();
-#pragma unroll
-        for (int i = 0; i < Tile<D>::kLoads; ++i) {
-          lds8* const piece = vs + (i * 256 + tid) * 16;
-          const uint4 x = lds_ld128(piece);
-          lds_st128(piece, make_uint4(drop_not_finite(x.x), drop_not_finite(x.y), drop_not_finite(x.z),
-                                      drop_not_finite(x.w)));
-        }
-        lds_barrier();
-      }
+      if (!all_see<MODE>(p, wg_lo, wg_hi, pos, kStep))  // some of the tile's rows do not see all of it
+        tile_not_finite<D, MODE>(p, vs, s_flag, s, pos, mine);
       if (mine) {
         v8bf pb[4];
         tile_exp<D>(s, p.c, sa, pb);
@@ -717,7 +721,22 @@ __device__ __forceinline__ void tile_item(const FlashArgs& p, uint8_t* smem, int
         tile_raise<D>(s, p.c, sa);
       }
       store_ahead(k_free, v_free);
+      kv += kStep;
+      at ^= 1;
+    };
+    if constexpr (MODE == kWindow)  // those that some rows do not see from their beginning, and on to where the stages are in order
+      while (kv < kv_end && (at == 1 || kv < whole_from)) edge();
+    while (kv + 2 * kStep <= whole_end) {
+      hot(sm + kB, sm + 2 * kB, sm, sm + 3 * kB, sa, sb);
+      if (kv + 2 * kStep > whole_end) {
+        at = 1;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) sa[t] = sb[t];
+        break;
+      }
+      hot(sm, sm + 3 * kB, sm + kB, sm + 2 * kB, sb, sa);
     }
+    while (kv < kv_end) edge();
     if (KV != kDense && src.bad) flag_error(p.error);
   }
 
