@@ -170,6 +170,12 @@ EXPORTS = {
         _I,
     ),
     "btl_paged_attention_window_plan": ([_I64] * 9 + [_P], _I),
+    "btl_shared_prefix_attention_scratch_bytes": ([_I64] * 8, _I64),
+    "btl_shared_prefix_attention": (
+        [_P, _I64, _I64, _I64, _PGP, _P, _I64, _P, _P, _P, _I64, _F, _I64, _I64, _I64, _P, _I64, _P, _SZ, _P, _P],
+        _I,
+    ),
+    "btl_shared_prefix_attention_plan": ([_I64] * 8 + [_P], _I),
     "btl_page_row": ([_I64, _I64, _I64, _I64, _I64, _I64], _I64),
     "btl_page_run": ([_I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P], _I),
     "btl_clamp_seq": ([_I64, _I64, _I64, _I64, _I64, _P], _I),

@@ -373,6 +373,58 @@ def paged_attention(q, cache: PagedKVCache, page_table, cu_q, kv_len, scale: flo
     return out
 
 
+def shared_prefix_attention(q, cache: PagedKVCache, page_table, cu_q, kv_len, shared_pages, scale: float | None = None,
+                            max_q: int | None = None, max_kv: int | None = None, max_shared: int | None = None, out=None):
+    """As :func:`paged_attention`, of a batch whose sequences all begin with the same
+    pages: a system prompt, a document.  They are read once for all of them.
+
+    shared_pages int32 [1] on the device: how many whole pages, those that ``page_table[0]``
+    begins with (what the other rows of the table have there is not read).  Every row's
+    position must be behind them, but for padding; kv_len counts them.  max_shared,
+    where known, is the most shared pages (a hint, as max_q and max_kv).  Several
+    groups with a prefix each: a call each, on slices of page_table, cu_q and kv_len."""
+    index = cache.index
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return shared_prefix_attention(q, cache, page_table, cu_q, kv_len, shared_pages, scale, max_q, max_kv, max_shared,
+                                           out)
+    if q.dim() != 3:
+        raise ValueError("q must be [T, H, D]")
+    T, H, D = q.shape
+    _, Hkv, page_size, dim = cache.shape
+    ldq = _rows(q, T, H, dim, "q", index)
+    if H < 1 or H % Hkv:
+        raise ValueError(f"{H} query heads over {Hkv} key-value heads")
+    B = _sequences(cu_q, index)
+    _int32(kv_len, index, (B,), "kv_len")
+    _int32(shared_pages, index, (1,), "shared_pages")
+    max_pages = _table(page_table, index, B)
+    most = max_pages * page_size
+    max_q = T if max_q is None or max_q > T else max_q
+    max_kv = most if max_kv is None or max_kv > most else max_kv
+    max_shared = max_pages if max_shared is None or max_shared > max_pages else max_shared
+    if out is None:
+        out = q.new_empty(T, H, D)
+        ldo = H * D
+    else:
+        ldo = _rows(out, T, H, D, "out", index)
+    if T == 0:
+        return out
+    if max_q < 1 or max_kv < 1 or max_shared < 0:
+        raise ValueError(f"max_q {max_q} and max_kv {max_kv} must be at least 1, max_shared {max_shared} at least 0")
+    stream = N.raw_stream(index)
+    max_shared *= page_size
+    nbytes = _shared_scratch_bytes(index, T, H, Hkv, D, B, max_q, max_kv, max_shared)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device)  # the call's own
+    rc = N.lib().btl_shared_prefix_attention(
+        q.data_ptr(), ldq, T, H, cache._pages, page_table.data_ptr(), max_pages, cu_q.data_ptr(), kv_len.data_ptr(),
+        shared_pages.data_ptr(), B, 1.0 / math.sqrt(D) if scale is None else scale, max_q, max_kv, max_shared,
+        out.data_ptr(), ldo, scratch.data_ptr(), nbytes, _error_word(index, stream), stream)
+    if rc != N.BTL_OK:
+        N.check(rc, "btl_shared_prefix_attention")
+    return out
+
+
 @functools.lru_cache(maxsize=4096)
 def _scratch_bytes(index: int, T: int, H: int, Hkv: int, D: int, B: int, max_q: int, max_kv: int) -> int:
     return int(N.lib().btl_paged_attention_scratch_bytes(T, H, Hkv, D, B, max_q, max_kv))
@@ -382,6 +434,12 @@ def _scratch_bytes(index: int, T: int, H: int, Hkv: int, D: int, B: int, max_q: 
 def _window_scratch_bytes(index: int, T: int, H: int, Hkv: int, D: int, B: int, max_q: int, max_kv: int, window: int,
                           sinks: int) -> int:
     return int(N.lib().btl_paged_attention_window_scratch_bytes(T, H, Hkv, D, B, max_q, max_kv, window, sinks))
+
+
+@functools.lru_cache(maxsize=4096)
+def _shared_scratch_bytes(index: int, T: int, H: int, Hkv: int, D: int, B: int, max_q: int, max_kv: int,
+                          max_shared: int) -> int:
+    return int(N.lib().btl_shared_prefix_attention_scratch_bytes(T, H, Hkv, D, B, max_q, max_kv, max_shared))
 
 
 def check(device=None) -> None:

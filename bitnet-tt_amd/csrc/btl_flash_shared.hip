@@ -1,0 +1,145 @@
+// Attention of a batch whose sequences begin with the same pages: the entry points.
+//
+//   out_i = (e_p o_p + sum_z e_z o_z) / (e_p l_p + sum_z e_z l_z),   e = 2^(m - max m)
+//
+// where (m, l, o) are maximum, sum and product of a part of the positions that row i sees.  The rows
+// of all sequences together (their G query heads of a key-value head) attend to the shared positions,
+// so that those are read once for 128 rows and not once for each sequence; each sequence's rows attend to
+// its own positions as everywhere else.  Both are workgroups of one launch, the shared ones
+// first; the merge is a second one.
+#include <type_traits>
+
+#include "btl_flash_plan.h"
+
+namespace btl {
+
+// FEW: the kernel of few rows for a part, else tiles of 128 rows.
+template <int D, int KV, bool SHARED_FEW, bool OWN_FEW>
+__global__ __launch_bounds__(256, 2) void k_flash_shared(FlashArgs p, int shared_items, int own_items) {
+  constexpr int kFewBytes = (int)sizeof(FewShared<D>);
+  constexpr int kBytes = SHARED_FEW && OWN_FEW ? kFewBytes : kFewBytes > kTileShared<D> ? kFewBytes : kTileShared<D>;
+  __shared__ __attribute__((aligned(16))) uint8_t smem[kBytes];
+  const int shared = shared_items * p.Hkv * p.shared_splits;
+  int x = blockIdx.x;
+  if (x < shared) {
+    const int hk = uni(x % p.Hkv), y = x / p.Hkv, item = uni(y % shared_items), split = uni(y / shared_items);
+    if constexpr (SHARED_FEW)
+      few_item<D, KV, kShared>(p, *reinterpret_cast<FewShared<D>*>(smem), hk, 0, split);
+    else
+      tile_item<D, KV, kShared>(p, smem, hk, item, split);
+  } else {
+    x -= shared;
+    const int hk = uni(x % p.Hkv), y = x / p.Hkv, item = uni(y % own_items), split = uni(y / own_items);
+    if constexpr (OWN_FEW)
+      few_item<D, KV, kOwn>(p, *reinterpret_cast<FewShared<D>*>(smem), hk, item, split);
+    else
+      tile_item<D, KV, kOwn>(p, smem, hk, item, split);
+  }
+}
+
+struct SharedPlan {
+  bool shared_few;
+  int64_t shared_items, own_items;  // of a key-value head
+  int shared_splits, shared_chunk;
+  FlashPlan own;
+};
+
+// max_kv: positions of the longest sequence, max_shared of them shared.
+inline SharedPlan shared_plan(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t B, int64_t max_q, int64_t max_kv,
+                              int64_t max_shared) {
+  SharedPlan s{};
+  const int64_t G = H / Hkv;
+  // (both parts' ends together stay below 2^31)
+  max_shared = std::min(max_shared, kMaxPositions);
+  const int64_t own = std::min(std::max(max_kv - max_shared, (int64_t)1), kMaxPositions / 2);
+  s.own = flash_plan(T, H, Hkv, D, B, max_q, own, true);
+  s.own_items = s.own.few ? B : s.own.tiles / Hkv;
+  s.shared_few = T * G <= kFewRows && s.own.few;
+  const FlashPlan f = flash_plan(T, H, Hkv, D, 1, s.shared_few ? 1 : T, std::max(max_shared, (int64_t)1), true);
+  s.shared_items = s.shared_few ? 1 : (T * G + kTileRows - 1) / kTileRows;
+  s.shared_splits = f.splits;
+  s.shared_chunk = f.chunk;
+  return s;
+}
+
+inline int64_t shared_scratch(const SharedPlan& s, int64_t T, int64_t H, int64_t D) {
+  return (int64_t)(s.shared_splits + s.own.splits) * T * H * (D + 2) * 4;
+}
+
+inline bool shared_sizes(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t B, int64_t max_q, int64_t max_kv,
+                         int64_t max_shared) {
+  return flash_sizes(T, H, Hkv, D, B, max_q, max_kv) && max_shared >= 0;
+}
+
+}  // namespace btl
+
+using namespace btl;
+
+extern "C" {
+
+int64_t btl_shared_prefix_attention_scratch_bytes(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t B, int64_t max_q,
+                                                  int64_t max_kv, int64_t max_shared) {
+  if (!shared_sizes(T, H, Hkv, D, B, max_q, max_kv, max_shared)) return 0;
+  return shared_scratch(shared_plan(T, H, Hkv, D, B, max_q, max_kv, max_shared), T, H, D);
+}
+
+int btl_shared_prefix_attention_plan(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t B, int64_t max_q, int64_t max_kv,
+                                     int64_t max_shared, int64_t* plan) {
+  if (!plan || !shared_sizes(T, H, Hkv, D, B, max_q, max_kv, max_shared)) return 0;
+  const SharedPlan s = shared_plan(T, H, Hkv, D, B, max_q, max_kv, max_shared);
+  plan[0] = s.shared_few;
+  plan[1] = s.shared_splits;
+  plan[2] = s.shared_chunk;
+  plan[3] = s.own.few;
+  plan[4] = s.own.splits;
+  plan[5] = s.own.chunk;
+  return 1;
+}
+
+int btl_shared_prefix_attention(const uint16_t* q, int64_t ldq, int64_t T, int64_t H, const btl_pages_t* pages,
+                                const int32_t* page_table, int64_t max_pages, const int32_t* cu_q, const int32_t* kv_len,
+                                const int32_t* shared_pages, int64_t B, float scale, int64_t max_q, int64_t max_kv,
+                                int64_t max_shared, uint16_t* out, int64_t ldo, void* scratch, size_t scratch_bytes,
+                                int32_t* error_word, btl_stream_t stream) {
+  const char* who = "btl_shared_prefix_attention";
+  clear_error();
+  FlashArgs a{};
+  int rc = paged_args(who, q, ldq, T, H, pages, page_table, max_pages, cu_q, kv_len, B, scale, max_q, max_kv, out, ldo,
+                      error_word, &a);
+  if (rc != BTL_OK) return rc;
+  if (max_shared < 0) return set_error(BTL_ERR_SHAPE, "%s: max_shared=%lld", who, (long long)max_shared);
+  if (T == 0) return BTL_OK;
+  if (!shared_pages) return set_error(BTL_ERR_NULL, "%s: NULL pointer", who);
+  if (!aligned(shared_pages, 4)) return set_error(BTL_ERR_ALIGN, "%s: misaligned shared_pages", who);
+  const int64_t Hkv = a.Hkv, D = pages->head_dim;
+  const bool fp8 = pages->k_exp != nullptr;
+  const SharedPlan s = shared_plan(T, H, Hkv, D, B, max_q, max_kv, max_shared);
+  const int parts = s.shared_splits + s.own.splits;
+  const int64_t groups = (s.shared_items * s.shared_splits + s.own_items * s.own.splits) * Hkv;
+  if (groups > INT32_MAX) return set_error(BTL_ERR_SHAPE, "%s: T=%lld B=%lld", who, (long long)T, (long long)B);
+  rc = partials(who, scratch, scratch_bytes, shared_scratch(s, T, H, D), (int64_t)parts * T * H * D, &a);
+  if (rc != BTL_OK) return rc;
+  a.shared = shared_pages;
+  a.shared_splits = s.shared_splits;
+  a.shared_chunk = s.shared_chunk;
+  a.splits = s.own.splits;
+  a.chunk = s.own.chunk;
+  auto pick = [&](auto d, auto kv) {
+    constexpr int kD = decltype(d)::value, kKV = decltype(kv)::value;
+    return s.shared_few ? k_flash_shared<kD, kKV, true, true>
+           : s.own.few  ? k_flash_shared<kD, kKV, false, true>
+                        : k_flash_shared<kD, kKV, false, false>;
+  };
+  using std::integral_constant;
+  auto* kern = D == 128 ? (fp8 ? pick(integral_constant<int, 128>(), integral_constant<int, kPagedFp8>())
+                               : pick(integral_constant<int, 128>(), integral_constant<int, kPagedBf16>()))
+                        : (fp8 ? pick(integral_constant<int, 64>(), integral_constant<int, kPagedFp8>())
+                               : pick(integral_constant<int, 64>(), integral_constant<int, kPagedBf16>()));
+  hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream, a, (int)s.shared_items,
+                     (int)s.own_items);
+  rc = check_launch("shared prefix attention");
+  if (rc != BTL_OK) return rc;
+  return launch_merge("shared prefix attention", a, T, H, D, true, parts, (hipStream_t)stream);
+}
+
+}  // extern "C"

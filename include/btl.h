@@ -509,6 +509,21 @@ int btl_paged_attention_window(const uint16_t* q, int64_t ldq, int64_t T, int64_
                                uint16_t* out, int64_t ldo, void* scratch, size_t scratch_bytes, int32_t* error_word,
                                btl_stream_t stream);
 
+/* Attention of the newest tokens over the pages, as btl_paged_attention, for a batch whose sequences all begin
+ * with the same pages: shared_pages (device, one int32) of them, those that
+ * page_table[0] begins with, whole.  Their positions are read once for the rows of all sequences; of the
+ * other sequences' tables the first shared_pages entries are not read.  A row before the end of the shared
+ * positions (but for rows with a negative position: zeros), or a shared_pages outside [0, max_pages],
+ * sets the error word.  max_kv: as there; max_shared: an upper bound of the shared positions where known, a hint
+ * too.  scratch: always, of btl_shared_prefix_attention_scratch_bytes with the same arguments. */
+int64_t btl_shared_prefix_attention_scratch_bytes(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t B, int64_t max_q,
+                                                  int64_t max_kv, int64_t max_shared);
+int btl_shared_prefix_attention(const uint16_t* q, int64_t ldq, int64_t T, int64_t H, const btl_pages_t* pages,
+                                const int32_t* page_table, int64_t max_pages, const int32_t* cu_q, const int32_t* kv_len,
+                                const int32_t* shared_pages, int64_t B, float scale, int64_t max_q, int64_t max_kv,
+                                int64_t max_shared, uint16_t* out, int64_t ldo, void* scratch, size_t scratch_bytes,
+                                int32_t* error_word, btl_stream_t stream);
+
 /* Test hooks, host only: the functions that the kernels call.  btl_page_row (writes and
  * page reads): the index of a position's (page, head, row), -1 for a page outside the pool.
  * btl_page_run (attention): {index of the first, rows} of the run of up to `most` rows from a position up
@@ -529,6 +544,9 @@ int btl_paged_attention_plan(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64
                              int64_t* plan);
 int btl_paged_attention_window_plan(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t B, int64_t max_q, int64_t max_kv,
                                     int64_t window, int64_t sinks, int64_t* plan);
+/* {few rows kernel, splits, positions of a split} of the shared positions, then of each sequence's own. */
+int btl_shared_prefix_attention_plan(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t B, int64_t max_q, int64_t max_kv,
+                                     int64_t max_shared, int64_t* plan);
 
 #ifdef __cplusplus
 }

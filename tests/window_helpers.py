@@ -73,3 +73,41 @@ class WindowBatch(PagedBatch):
             tol.append(t)
             at += n
         return torch.cat(o), torch.cat(tol)
+
+
+class SharedBatch(PagedBatch):
+    """Sequences that begin with the same ``shared`` pages, then ``own`` positions each (the new ones among
+    them); what the tables of all but the first sequence have for the shared pages is no page."""
+
+    def __init__(self, new, own, shared, H, Hkv, D, page, kv, **kw):
+        super().__init__([0] + list(new), [shared * page] + list(own), H, Hkv, D, page, kv, **kw)
+        self.shared = shared
+        both = self.table_host
+        width = max(shared + max(-(-n // page) for n in own), 1)
+        table = torch.full((len(new), width), -7, dtype=torch.int32)
+        self.full_tables = []
+        for b in range(len(new)):
+            table[b, shared:] = both[b + 1, : width - shared]
+            self.full_tables.append(torch.cat((both[0, :shared], both[b + 1])))
+        table[0, :shared] = both[0, :shared]
+        self.table_host = table
+        self.new = list(new)
+        self.total = [shared * page + n if n else 0 for n in own]  # an empty slot has no prefix either
+        device = self.table.device
+        self.table = table.to(device)
+        self.cu, self.len = self.cu[1:], torch.tensor(self.total, dtype=torch.int32, device=device)
+        self.pages = torch.tensor([shared], dtype=torch.int32, device=device)
+
+    def rows(self, pool64, b):
+        n = self.total[b]
+        ids = self.full_tables[b][: -(-n // self.page)].long()
+        return pool64[ids].transpose(0, 1).reshape(self.Hkv, -1, self.D)[:, :n]
+
+    def reference(self, scale=None):
+        o, tol, at = [], [], 0
+        for b, n in enumerate(self.new):
+            x, t = attend_window64(self.q[at:at + n].double(), self.rows(self.k64, b), self.rows(self.v64, b), scale=scale)
+            o.append(x)
+            tol.append(t)
+            at += n
+        return torch.cat(o), torch.cat(tol)
