@@ -1,0 +1,385 @@
+// Products of 8-bit integers with a scale for each row (token) and each column (channel):
+//
+//   out[m, n] = (sum_k a[m, k] w[n, k]) sa[m] sw[n]
+//
+// The sum is exact in 32 bits (K up to 16384: below 2^28); it becomes fp32 (one rounding from 2^24 on),
+// is multiplied by the row's scale and then the column's, each rounded to fp32, and rounded to
+// bf16 where that is the output.
+//
+// Weights are laid out once: blocks of 16 columns x 64 k, 1 KiB, [ceil(N/16)][ceil(K/64)], a
+// lane's 16 bytes being those that v_mfma_i32_16x16x64_i8 takes from it (column lane % 16, k
+// 16 (lane / 16) ..), zeros behind N and K.  A wave's operand is one coalesced load, from
+// memory to registers or to LDS.  Weights are the MFMA's first operand, so that a lane holds four
+// neighbouring columns of one row.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "btl.h"
+#include "btl_act_row.h"
+#include "btl_common.h"
+#include "btl_mfma.h"
+
+namespace btl {
+
+typedef __attribute__((address_space(3))) uint8_t lds8;
+
+struct Int8Args {
+  const int8_t* a;
+  int64_t lda;
+  const float* sa;
+  const uint8_t* w;
+  const float* sw;
+  int M, K, N, KB, NT;  // KB, NT: blocks of 64 k, of 16 columns
+  void* out;
+  int64_t ldo;
+  int f32;
+};
+
+__device__ __forceinline__ int uni8(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// A buffer resource at a scalar address; a piece behind its `bytes` reads as zeros and costs no traffic.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc8(const void* p, uint32_t bytes) {
+  const uint64_t at = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = (uint32_t)uni8((int)(uint32_t)at), hi = (uint32_t)uni8((int)(at >> 32));
+  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(((uint64_t)hi << 32) | lo), (short)0,
+                                           uni8((int)bytes), 0x00020000);
+}
+__device__ __forceinline__ v4i buf128(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+  return __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(r, (int)off, 0, 0));
+}
+
+__device__ __forceinline__ float scaled(int acc, float sa, float sw) { return (float)acc * sa * sw; }
+
+// ======================================================================
+// Few rows: a stream of weights.  A workgroup takes groups of CT column blocks, its 8 waves the
+// blocks of 64 k in turn (wave w: w, w + 8, ...); the waves' sums meet in LDS.  A wave has two sets of U x CT
+// loads: while it works on one, the other's are on their way, across the sums of a group as well.
+// ======================================================================
+constexpr int kI8Waves = 8;
+
+template <int RB, int CT, int U>
+__global__ __launch_bounds__(64 * kI8Waves, 1) void k_int8_stream(Int8Args p, int groups) {
+  __shared__ int red[kI8Waves][RB][CT][4][64];
+  const int tid = threadIdx.x, lane = tid & 63, wv = uni8(tid >> 6);
+  const int m0 = blockIdx.y * 16 * RB;
+  const int rounds = ((p.KB + kI8Waves - 1) / kI8Waves + U - 1) / U;
+  const int mine = (groups - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
+  const int chunks = mine * rounds;
+
+  // rows behind M: the last one's values, never written; k behind K: any values, the weights are zero there
+  const auto ra = rsrc8(p.a + (int64_t)m0 * p.lda, 0x7fffffff);
+  uint32_t row_off[RB];
+#pragma unroll
+  for (int r = 0; r < RB; ++r) row_off[r] = (uint32_t)(min(16 * r + (lane & 15), p.M - 1 - m0) * p.lda);
+
+  v4i b[2][U][CT], a[2][U][RB];
+  auto issue = [&](int set, int c) {
+    const int g = blockIdx.x + min(c / rounds, mine - 1) * gridDim.x, k0 = (c % rounds) * U * kI8Waves + wv;
+#pragma unroll
+    for (int t = 0; t < CT; ++t) {
+      const int nt = min(g * CT + t, p.NT - 1);
+      const auto rw = rsrc8(p.w + (int64_t)nt * p.KB * 1024, c < chunks ? p.KB * 1024 : 0);
+#pragma unroll
+      for (int u = 0; u < U; ++u) b[set][u][t] = buf128(rw, (k0 + kI8Waves * u) * 1024 + lane * 16);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int r = 0; r < RB; ++r)
+        a[set][u][r] = buf128(ra, row_off[r] + min((k0 + kI8Waves * u) * 64 + 16 * (lane >> 4), p.K - 16));
+  };
+  v4i acc[RB][CT];
+  auto clear = [&] {
+#pragma unroll
+    for (int r = 0; r < RB; ++r)
+#pragma unroll
+      for (int t = 0; t < CT; ++t) acc[r][t] = (v4i){0, 0, 0, 0};
+  };
+  auto consume = [&](int set) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int r = 0; r < RB; ++r)
+#pragma unroll
+        for (int t = 0; t < CT; ++t)
+          acc[r][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b[set][u][t], a[set][u][r], acc[r][t], 0, 0, 0);
+  };
+  auto finish = [&](int c) {  // the group of chunk c is complete
+    const int g = blockIdx.x + c / rounds * gridDim.x;
+#pragma unroll
+    for (int r = 0; r < RB; ++r)
+#pragma unroll
+      for (int t = 0; t < CT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) red[wv][r][t][i][lane] = acc[r][t][i];
+    __syncthreads();
+    for (int e = tid; e < RB * CT * 256; e += 64 * kI8Waves) {
+      const int n = e % (16 * CT), m = e / (16 * CT);
+      const int l = 16 * ((n & 15) >> 2) + (m & 15);
+      int s = 0;
+#pragma unroll
+      for (int w = 0; w < kI8Waves; ++w) s += red[w][m >> 4][n >> 4][n & 3][l];
+      const int row = m0 + m, col = g * 16 * CT + n;
+      if (row < p.M && col < p.N) {
+        const float y = scaled(s, p.sa[row], p.sw[col]);
+        if (p.f32)
+          static_cast<float*>(p.out)[row * p.ldo + col] = y;
+        else
+          static_cast<uint16_t*>(p.out)[row * p.ldo + col] = f2bf(y);
+      }
+    }
+    __syncthreads();
+    clear();
+  };
+
+  clear();
+  issue(0, 0);
+  for (int c = 0; c < chunks; c += 2) {
+    issue(1, c + 1);
+    consume(0);
+    if ((c + 1) % rounds == 0) finish(c);
+    if (c + 1 >= chunks) break;
+    issue(0, c + 2);
+    consume(1);
+    if ((c + 2) % rounds == 0) finish(c + 1);
+  }
+}
+
+// ======================================================================
+// Many rows: tiles of BM x BN, the workgroup's waves WM x WN of them; S stages of 64 k in LDS, filled without registers.
+// ======================================================================
+template <int BM, int BN, int WM, int WN, int S>
+__global__ __launch_bounds__(64 * WM * WN, 1) void k_int8_tile(Int8Args p, int ngm, int ngn) {
+  constexpr int kWaves = WM * WN, kA = BM / 16, kB = BN / 16;  // KiB of a stage
+  constexpr int kLoads = (kA + kB) / kWaves;
+  constexpr int TM = BM / WM / 16, TN = BN / WN / 16;  // a wave's blocks
+  static_assert((kA + kB) % kWaves == 0 && kA % kWaves == 0, "loads of a wave");
+  __shared__ __attribute__((aligned(16))) uint8_t smem[S * (kA + kB) * 1024];
+  lds8* const sm = (lds8*)smem;
+  const int tid = threadIdx.x, lane = tid & 63, wv = uni8(tid >> 6);
+  const int gm = uni8(blockIdx.x % ngm), gn = uni8(blockIdx.x / ngm);
+  const int m0 = gm * BM, nt0 = gn * kB;
+
+  // this wave's blocks of a stage: kLoads of them, the first kA / kWaves of the rows
+  constexpr int kLa = kA / kWaves;
+  const auto ra = rsrc8(p.a + (int64_t)m0 * p.lda, 0x7fffffff);
+  uint32_t off_a[kLa];
+#pragma unroll
+  for (int i = 0; i < kLa; ++i)
+    off_a[i] = (uint32_t)(min((wv + kWaves * i) * 16 + (lane & 15), p.M - 1 - m0) * p.lda);
+  const auto rw = rsrc8(p.w + (int64_t)nt0 * p.KB * 1024, (uint32_t)min(kB, p.NT - nt0) * p.KB * 1024);
+  auto issue = [&](int step, lds8* at) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      lds8* const dst = at + (wv + kWaves * i) * 1024;
+      if (i < kLa)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, dst, 16, (int)(off_a[i] + min(step * 64 + 16 * (lane >> 4), p.K - 16)),
+                                                 0, 0, 0);
+      else
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            rw, dst, 16, ((wv + kWaves * i - kA) * p.KB + min(step, p.KB - 1)) * 1024 + lane * 16, 0, 0, 0);
+    }
+  };
+  const int wm = wv % WM, wn = wv / WM;
+  v4i acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = (v4i){0, 0, 0, 0};
+
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s) issue(s, sm + s * (kA + kB) * 1024);
+  int at = 0;
+  for (int step = 0; step < p.KB; ++step) {
+    constexpr int kLeft = (S - 2) * kLoads;  // loads that may still be on their way
+    __builtin_amdgcn_s_waitcnt(0x0f70 | (kLeft & 15) | ((kLeft >> 4) << 14));
+    lds_barrier();
+    issue(step + S - 1, sm + (at + S - 1 >= S ? at - 1 : at + S - 1) * (kA + kB) * 1024);
+    const lds8* const as = sm + at * (kA + kB) * 1024 + wm * TM * 1024 + lane * 16;
+    const lds8* const bs = sm + at * (kA + kB) * 1024 + (kA + wn * TN) * 1024 + lane * 16;
+    v4i x[TM], y[TN];
+#pragma unroll
+    for (int j = 0; j < TN; ++j) y[j] = *(const __attribute__((address_space(3))) v4i*)(bs + j * 1024);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) x[i] = *(const __attribute__((address_space(3))) v4i*)(as + i * 1024);
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(y[j], x[i], acc[i][j], 0, 0, 0);
+    at = at + 1 == S ? 0 : at + 1;
+  }
+
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // nothing may land in LDS after the workgroup's end
+
+  // element i of a block: row lane % 16, column 4 (lane / 16) + i
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+    const int row = m0 + (wm * TM + i) * 16 + (lane & 15);
+    if (row >= p.M) continue;
+    const float sa = p.sa[row];
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const int col = (nt0 + wn * TN + j) * 16 + 4 * (lane >> 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (col + e < p.N) {
+          const float v = scaled(acc[i][j][e], sa, p.sw[col + e]);
+          if (p.f32)
+            static_cast<float*>(p.out)[row * p.ldo + col + e] = v;
+          else
+            static_cast<uint16_t*>(p.out)[row * p.ldo + col + e] = f2bf(v);
+        }
+    }
+  }
+}
+
+// ---- weights ---------------------------------------------------------------
+__global__ void k_int8_layout(const int8_t* w, int64_t ldw, int N, int K, int KB, int64_t total, uint4* out) {
+  const int64_t g = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (g >= total) return;
+  const int lane = (int)(g & 63);
+  const int64_t blk = g >> 6;
+  const int64_t n = blk / KB * 16 + (lane & 15);
+  const int k = (int)(blk % KB) * 64 + 16 * (lane >> 4);
+  uint4 v = make_uint4(0u, 0u, 0u, 0u);
+  if (n < N && k < K) v = *reinterpret_cast<const uint4*>(w + n * ldw + k);
+  out[g] = v;
+}
+
+// Channel n of float weights: scale = max|w| / 127 (1 where that is 0), codes round(w / scale) to even, on a wave.  The
+// quotient is the correctly rounded one, so a code is off by half a step and 127 is reached, never passed.
+template <typename T>
+__device__ __forceinline__ float weight_at(const T* w, int64_t i);
+template <>
+__device__ __forceinline__ float weight_at<float>(const float* w, int64_t i) { return w[i]; }
+template <>
+__device__ __forceinline__ float weight_at<uint16_t>(const uint16_t* w, int64_t i) { return bf2f(w[i]); }
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_int8_quantise(const T* w, int64_t ldw, int N, int K, int KB, uint8_t* out, float* scale) {
+  const int lane = threadIdx.x & 63;
+  const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);  // up to the end of the last block
+  if (n >= (int64_t)(N + 15) / 16 * 16) return;
+  const T* const row = w + n * ldw;
+  float m = 0.0f;
+  bool bad = false;
+  if (n < N)
+    for (int k = lane; k < K; k += 64) {
+      const float x = weight_at(row, k);
+      bad |= !__builtin_isfinite(x);
+      m = fmaxf(m, fabsf(x));
+    }
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+  bad = __any(bad);
+  // a tiny row's m / 127 could be a subnormal of few bits, and w / scale pass 127: below it the codes are zero
+  const bool none = m < 0x1p-119f;
+  const float s = none ? 1.0f : m / 127.0f;
+  if (n < N && lane == 0) scale[n] = bad ? __builtin_nanf("") : s;
+  uint8_t* const col = out + n / 16 * KB * 1024 + (n & 15) * 16;
+  for (int k = lane; k < KB * 64; k += 64) {
+    int q = 0;
+    if (n < N && k < K && !bad && !none) q = min(127, max(-127, (int)__builtin_rintf(weight_at(row, k) / s)));
+    col[(int64_t)(k >> 6) * 1024 + ((k & 63) >> 4) * 256 + (k & 15)] = (uint8_t)(int8_t)q;
+  }
+}
+
+// ---- host ------------------------------------------------------------------
+inline int check_int8_shape(const char* who, int64_t N, int64_t K) {
+  if (N <= 0 || N > (1 << 24)) return set_error(BTL_ERR_SHAPE, "%s: N=%lld", who, (long long)N);
+  if (K <= 0 || K % 16 || K > BTL_MAX_K)
+    return set_error(BTL_ERR_SHAPE, "%s: K=%lld (a multiple of 16 up to %d)", who, (long long)K, BTL_MAX_K);
+  return BTL_OK;
+}
+inline int64_t int8_kb(int64_t K) { return (K + 63) / 64; }
+inline int64_t int8_nt(int64_t N) { return (N + 15) / 16; }
+
+template <int RB, int CT>
+static void launch_stream(const Int8Args& a, int groups, dim3 grid, hipStream_t s) {
+  const int each = (a.KB + kI8Waves - 1) / kI8Waves;
+  if (each <= 2)
+    hipLaunchKernelGGL((k_int8_stream<RB, CT, 2>), grid, dim3(64 * kI8Waves), 0, s, a, groups);
+  else
+    hipLaunchKernelGGL((k_int8_stream<RB, CT, 5>), grid, dim3(64 * kI8Waves), 0, s, a, groups);
+}
+
+}  // namespace btl
+
+using namespace btl;
+
+extern "C" {
+
+int64_t btl_int8_weight_bytes(int64_t N, int64_t K) {
+  if (N <= 0 || N > (1 << 24) || K <= 0 || K % 16 || K > BTL_MAX_K) return 0;
+  return int8_nt(N) * int8_kb(K) * 1024;
+}
+
+int btl_int8_weight_layout(const int8_t* w, int64_t ldw, int64_t N, int64_t K, uint8_t* wdev, btl_stream_t stream) {
+  const char* who = "btl_int8_weight_layout";
+  clear_error();
+  const int rc = check_int8_shape(who, N, K);
+  if (rc != BTL_OK) return rc;
+  if (!w || !wdev) return set_error(BTL_ERR_NULL, "%s: NULL pointer", who);
+  if (ldw < K) return set_error(BTL_ERR_SHAPE, "%s: row stride smaller than a row", who);
+  if (!aligned(w, 16) || !aligned(wdev, 16) || ldw % 16) return set_error(BTL_ERR_ALIGN, "%s: 16-byte alignment", who);
+  const int64_t total = int8_nt(N) * int8_kb(K) * 64;
+  hipLaunchKernelGGL(k_int8_layout, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, (hipStream_t)stream, w, ldw, (int)N,
+                     (int)K, (int)int8_kb(K), total, reinterpret_cast<uint4*>(wdev));
+  return check_launch(who);
+}
+
+int btl_int8_weight_quantise(const void* w, int bf16, int64_t ldw, int64_t N, int64_t K, uint8_t* wdev, float* scale,
+                             btl_stream_t stream) {
+  const char* who = "btl_int8_weight_quantise";
+  clear_error();
+  const int rc = check_int8_shape(who, N, K);
+  if (rc != BTL_OK) return rc;
+  if (!w || !wdev || !scale) return set_error(BTL_ERR_NULL, "%s: NULL pointer", who);
+  if (ldw < K) return set_error(BTL_ERR_SHAPE, "%s: row stride smaller than a row", who);
+  if (!aligned(w, bf16 ? 2 : 4) || !aligned(wdev, 16) || !aligned(scale, 4))
+    return set_error(BTL_ERR_ALIGN, "%s: misaligned buffer", who);
+  const dim3 grid((unsigned)(int8_nt(N) * 4));
+  if (bf16)
+    hipLaunchKernelGGL(k_int8_quantise<uint16_t>, grid, dim3(256), 0, (hipStream_t)stream, static_cast<const uint16_t*>(w), ldw,
+                       (int)N, (int)K, (int)int8_kb(K), wdev, scale);
+  else
+    hipLaunchKernelGGL(k_int8_quantise<float>, grid, dim3(256), 0, (hipStream_t)stream, static_cast<const float*>(w), ldw,
+                       (int)N, (int)K, (int)int8_kb(K), wdev, scale);
+  return check_launch(who);
+}
+
+int btl_int8_matmul(const int8_t* a, int64_t lda, const float* a_scale, int64_t M, int64_t K, int64_t N, const uint8_t* wdev,
+                    const float* w_scale, void* out, int64_t ldo, int out_f32, btl_stream_t stream) {
+  const char* who = "btl_int8_matmul";
+  clear_error();
+  const int rc = check_int8_shape(who, N, K);
+  if (rc != BTL_OK) return rc;
+  if (M < 0 || M > (1 << 24)) return set_error(BTL_ERR_SHAPE, "%s: M=%lld", who, (long long)M);
+  if (lda < K || lda > (1 << 22) || ldo < N) return set_error(BTL_ERR_SHAPE, "%s: lda=%lld ldo=%lld", who, (long long)lda,
+                                                             (long long)ldo);
+  if (M == 0) return BTL_OK;
+  if (!a || !a_scale || !wdev || !w_scale || !out) return set_error(BTL_ERR_NULL, "%s: NULL pointer", who);
+  if (!aligned(a, 16) || lda % 16 || !aligned(wdev, 16) || !aligned(a_scale, 4) || !aligned(w_scale, 4) ||
+      !aligned(out, out_f32 ? 4 : 2))
+    return set_error(BTL_ERR_ALIGN, "%s: misaligned buffer or row stride", who);
+  Int8Args p{a, lda, a_scale, wdev, w_scale, (int)M, (int)K, (int)N, (int)int8_kb(K), (int)int8_nt(N), out, ldo, out_f32 != 0};
+  hipStream_t s = (hipStream_t)stream;
+  if (M <= 64) {
+    const int cus = device_cus();
+    const int ct = p.NT > cus ? 2 : 1, groups = (p.NT + ct - 1) / ct;
+    const int rb = M <= 16 ? 1 : 2, ny = (int)((M + 16 * rb - 1) / (16 * rb));
+    const dim3 grid((unsigned)std::min(groups, cus), (unsigned)ny);
+    if (rb == 1)
+      ct == 1 ? launch_stream<1, 1>(p, groups, grid, s) : launch_stream<1, 2>(p, groups, grid, s);
+    else
+      ct == 1 ? launch_stream<2, 1>(p, groups, grid, s) : launch_stream<2, 2>(p, groups, grid, s);
+    return check_launch(who);
+  }
+  const int ngm = (int)((M + 255) / 256), ngn = (p.NT + 15) / 16;
+  if ((int64_t)ngm * ngn > INT32_MAX) return set_error(BTL_ERR_SHAPE, "%s: M=%lld N=%lld", who, (long long)M, (long long)N);
+  hipLaunchKernelGGL((k_int8_tile<256, 256, 2, 4, 4>), dim3((unsigned)(ngm * ngn)), dim3(512), 0, s, p, ngm, ngn);
+  return check_launch(who);
+}
+
+}  // extern "C"

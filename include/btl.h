@@ -369,6 +369,31 @@ int btl_lm_head_repack(const uint16_t* w, int64_t V, int64_t K, uint16_t* wdev, 
 int btl_lm_head(const uint16_t* xn, int64_t M, int64_t K, int64_t V, const uint16_t* wdev, float* logits,
                 int32_t* tokens, void* workspace, size_t workspace_bytes, btl_stream_t stream);
 
+/* ---- products of 8-bit integers ----------------------------------------
+ * out[m, n] = (sum_k a[m, k] w[n, k]) a_scale[m] w_scale[n]: the sum exact in
+ * int32, then fp32 (one rounding where it is 2^24 or more), the row's scale, the
+ * column's scale, each product rounded to fp32, and bf16 unless out_f32.  K a
+ * multiple of 16 up to BTL_MAX_K.  (The reference's other weight dtypes are
+ * Tensix block formats: src/bitnet_tt/layers/bitlinear.py:153-197.)
+ *
+ * btl_int8_weight_bytes: bytes of an [N, K] weight in the device layout
+ *   (16 columns x 64 k per KiB in MFMA operand order, zeros behind N and K; 0
+ *   for unsupported shapes).
+ * btl_int8_weight_layout: codes w [N, K], row stride ldw (a multiple of 16),
+ *   16-byte aligned -> the device layout.
+ * btl_int8_weight_quantise: a float weight [N, K] (fp32, or bf16 when bf16 is
+ *   non-zero) -> codes round(w / scale) in the device layout, scale[n] =
+ *   max|w[n]| / 127 (1 for rows of zeros or below 2^-119; NaN, and codes 0, for a row with a
+ *   value that is not finite).
+ * btl_int8_matmul: a [M, K] int8, row stride lda (a multiple of 16 up to 2^22),
+ *   16-byte aligned; out [M, N] fp32 or bf16, row stride ldo, any alignment. */
+int64_t btl_int8_weight_bytes(int64_t N, int64_t K);
+int btl_int8_weight_layout(const int8_t* w, int64_t ldw, int64_t N, int64_t K, uint8_t* wdev, btl_stream_t stream);
+int btl_int8_weight_quantise(const void* w, int bf16, int64_t ldw, int64_t N, int64_t K, uint8_t* wdev, float* scale,
+                             btl_stream_t stream);
+int btl_int8_matmul(const int8_t* a, int64_t lda, const float* a_scale, int64_t M, int64_t K, int64_t N,
+                    const uint8_t* wdev, const float* w_scale, void* out, int64_t ldo, int out_f32, btl_stream_t stream);
+
 /* ---- decode attention between QKV and o_proj --------------------------
  * Replaces the decode attention of src/bitnet_tt/layers/attention.py:
  * 1040-1262 (nlp_create_qkv_heads_decode, rotary_embedding_llama,
