@@ -33,7 +33,7 @@ struct Int8Args {
   int M, K, N, KB, NT;  // KB, NT: blocks of 64 k, of 16 columns
   void* out;
   int64_t ldo;
-  int f32;
+  int f32, vec;  // vec: rows of out are 16-byte aligned
 };
 
 __device__ __forceinline__ int uni8(int x) { return __builtin_amdgcn_readfirstlane(x); }
@@ -54,16 +54,18 @@ __device__ __forceinline__ float scaled(int acc, float sa, float sw) { return (f
 // ======================================================================
 // Few rows: a stream of weights.  A workgroup takes groups of CT column blocks, its 8 waves the
 // blocks of 64 k in turn (wave w: w, w + 8, ...); the waves' sums meet in LDS.  A wave has two sets of U x CT
-// loads: while it works on one, the other's are on their way, across the sums of a group as well.
+// loads: while it works on one, the other's are on their way, across the sums of a group as well.  ONCE: a
+// wave's blocks are one set (K <= 512 U), so that its rows stay in registers for all groups.
 // ======================================================================
 constexpr int kI8Waves = 8;
 
-template <int RB, int CT, int U>
-__global__ __launch_bounds__(64 * kI8Waves, 1) void k_int8_stream(Int8Args p, int groups) {
-  __shared__ int red[kI8Waves][RB][CT][4][64];
+template <int RB, int CT, int U, bool ONCE>
+__global__ __launch_bounds__(64 * kI8Waves, 2) void k_int8_stream(Int8Args p, int groups) {
+  constexpr int kPart = 4 * 68;  // words of a block's sums: 16 rows of four columns, four times, and what keeps those in other banks
+  __shared__ __attribute__((aligned(16))) int red[kI8Waves][RB][CT][kPart];
   const int tid = threadIdx.x, lane = tid & 63, wv = uni8(tid >> 6);
   const int m0 = blockIdx.y * 16 * RB;
-  const int rounds = ((p.KB + kI8Waves - 1) / kI8Waves + U - 1) / U;
+  const int rounds = ONCE ? 1 : ((p.KB + kI8Waves - 1) / kI8Waves + U - 1) / U;
   const int mine = (groups - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
   const int chunks = mine * rounds;
 
@@ -73,9 +75,16 @@ __global__ __launch_bounds__(64 * kI8Waves, 1) void k_int8_stream(Int8Args p, in
 #pragma unroll
   for (int r = 0; r < RB; ++r) row_off[r] = (uint32_t)(min(16 * r + (lane & 15), p.M - 1 - m0) * p.lda);
 
-  v4i b[2][U][CT], a[2][U][RB];
+  v4i b[2][U][CT], a[ONCE ? 1 : 2][U][RB];
+  auto issue_rows = [&](int set, int k0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int r = 0; r < RB; ++r)
+        a[set][u][r] = buf128(ra, row_off[r] + min((k0 + kI8Waves * u) * 64 + 16 * (lane >> 4), p.K - 16));
+  };
   auto issue = [&](int set, int c) {
-    const int g = blockIdx.x + min(c / rounds, mine - 1) * gridDim.x, k0 = (c % rounds) * U * kI8Waves + wv;
+    const int g = blockIdx.x + min(c / rounds, mine - 1) * gridDim.x, k0 = c % rounds * U * kI8Waves + wv;
 #pragma unroll
     for (int t = 0; t < CT; ++t) {
       const int nt = min(g * CT + t, p.NT - 1);
@@ -83,11 +92,7 @@ __global__ __launch_bounds__(64 * kI8Waves, 1) void k_int8_stream(Int8Args p, in
 #pragma unroll
       for (int u = 0; u < U; ++u) b[set][u][t] = buf128(rw, (k0 + kI8Waves * u) * 1024 + lane * 16);
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int r = 0; r < RB; ++r)
-        a[set][u][r] = buf128(ra, row_off[r] + min((k0 + kI8Waves * u) * 64 + 16 * (lane >> 4), p.K - 16));
+    if (!ONCE) issue_rows(set, k0);
   };
   v4i acc[RB][CT];
   auto clear = [&] {
@@ -103,85 +108,151 @@ __global__ __launch_bounds__(64 * kI8Waves, 1) void k_int8_stream(Int8Args p, in
       for (int r = 0; r < RB; ++r)
 #pragma unroll
         for (int t = 0; t < CT; ++t)
-          acc[r][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b[set][u][t], a[set][u][r], acc[r][t], 0, 0, 0);
+          acc[r][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b[set][u][t], a[ONCE ? 0 : set][u][r], acc[r][t], 0, 0, 0);
   };
   auto finish = [&](int c) {  // the group of chunk c is complete
     const int g = blockIdx.x + c / rounds * gridDim.x;
 #pragma unroll
     for (int r = 0; r < RB; ++r)
 #pragma unroll
-      for (int t = 0; t < CT; ++t)
+      for (int t = 0; t < CT; ++t) *reinterpret_cast<v4i*>(&red[wv][r][t][4 * lane + 4 * (lane >> 4)]) = acc[r][t];
+    lds_barrier();
+    // a thread's four columns of a row
+    for (int e = tid; e < RB * CT * 64; e += 64 * kI8Waves) {
+      const int q = e % (4 * CT), m = e / (4 * CT), at = 4 * (16 * (q & 3) + (m & 15)) + 4 * (q & 3);
+      v4i sum = (v4i){0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) red[wv][r][t][i][lane] = acc[r][t][i];
-    __syncthreads();
-    for (int e = tid; e < RB * CT * 256; e += 64 * kI8Waves) {
-      const int n = e % (16 * CT), m = e / (16 * CT);
-      const int l = 16 * ((n & 15) >> 2) + (m & 15);
-      int s = 0;
+      for (int w = 0; w < kI8Waves; ++w) sum += *reinterpret_cast<const v4i*>(&red[w][m >> 4][q >> 2][at]);
+      const int row = m0 + m, col = g * 16 * CT + 4 * q;
+      if (row >= p.M) continue;
+      const float sa = p.sa[row];
+      float y[4];
 #pragma unroll
-      for (int w = 0; w < kI8Waves; ++w) s += red[w][m >> 4][n >> 4][n & 3][l];
-      const int row = m0 + m, col = g * 16 * CT + n;
-      if (row < p.M && col < p.N) {
-        const float y = scaled(s, p.sa[row], p.sw[col]);
-        if (p.f32)
-          static_cast<float*>(p.out)[row * p.ldo + col] = y;
+      for (int i = 0; i < 4; ++i) y[i] = scaled(sum[i], sa, p.sw[min(col + i, p.N - 1)]);
+      if (p.f32) {
+        float* const o = static_cast<float*>(p.out) + row * p.ldo + col;
+        if (p.vec && col + 4 <= p.N)
+          *reinterpret_cast<float4*>(o) = make_float4(y[0], y[1], y[2], y[3]);
         else
-          static_cast<uint16_t*>(p.out)[row * p.ldo + col] = f2bf(y);
+          for (int i = 0; i < 4; ++i)
+            if (col + i < p.N) o[i] = y[i];
+      } else {
+        uint16_t* const o = static_cast<uint16_t*>(p.out) + row * p.ldo + col;
+        if (p.vec && col + 4 <= p.N)
+          *reinterpret_cast<uint2*>(o) = make_uint2(f2bf_pair(y[0], y[1]), f2bf_pair(y[2], y[3]));
+        else
+          for (int i = 0; i < 4; ++i)
+            if (col + i < p.N) o[i] = f2bf(y[i]);
       }
     }
-    __syncthreads();
+    lds_barrier();
     clear();
   };
 
   clear();
   issue(0, 0);
+  if (ONCE) issue_rows(0, wv);
+  issue(1, 1);
   for (int c = 0; c < chunks; c += 2) {
-    issue(1, c + 1);
     consume(0);
-    if ((c + 1) % rounds == 0) finish(c);
-    if (c + 1 >= chunks) break;
     issue(0, c + 2);
+    if (ONCE || (c + 1) % rounds == 0) finish(c);
+    if (c + 1 >= chunks) break;
     consume(1);
-    if ((c + 2) % rounds == 0) finish(c + 1);
+    issue(1, c + 3);
+    if (ONCE || (c + 2) % rounds == 0) finish(c + 1);
   }
 }
 
 // ======================================================================
-// Many rows: tiles of BM x BN, the workgroup's waves WM x WN of them; S stages of 64 k in LDS, filled without registers.
+// Many rows: tiles of BM x BN, S stages of KG x 64 k in LDS, filled without registers.  The waves are KG groups
+// of WM x WN; a group takes its 64 k of every stage, and the groups' sums meet in LDS.
 // ======================================================================
-template <int BM, int BN, int WM, int WN, int S>
-__global__ __launch_bounds__(64 * WM * WN, 1) void k_int8_tile(Int8Args p, int ngm, int ngn) {
-  constexpr int kWaves = WM * WN, kA = BM / 16, kB = BN / 16;  // KiB of a stage
-  constexpr int kLoads = (kA + kB) / kWaves;
+// 16 rows of a wave's TN blocks through its own LDS, so that they leave in whole lines: a lane has four columns
+// (4 (lane / 16) ..) of one row (lane % 16) of each block.
+template <typename T>
+__device__ __forceinline__ void put4(T* at, const float* y);
+template <>
+__device__ __forceinline__ void put4<float>(float* at, const float* y) {
+  *reinterpret_cast<float4*>(at) = make_float4(y[0], y[1], y[2], y[3]);
+}
+template <>
+__device__ __forceinline__ void put4<uint16_t>(uint16_t* at, const float* y) {
+  *reinterpret_cast<uint2*>(at) = make_uint2(f2bf_pair(y[0], y[1]), f2bf_pair(y[2], y[3]));
+}
+template <int TN, typename T>
+__device__ __forceinline__ void store_block(const Int8Args& p, const v4i (&acc)[TN], float sa, const float (&sw)[TN][4], T* mine,
+                                            int row0, int col0) {
+  constexpr int kCols = 16 * TN, kLd = kCols + 16 / (int)sizeof(T);  // elements of a row in LDS
+  const int lane = threadIdx.x & 63;
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int j = 0; j < TN; ++j) {
+    float y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = scaled(acc[j][e], sa, sw[j][e]);
+    put4(mine + (lane & 15) * kLd + 16 * j + 4 * (lane >> 4), y);
+  }
+  __builtin_amdgcn_wave_barrier();
+  T* const out = static_cast<T*>(p.out) + (int64_t)row0 * p.ldo + col0;
+  const int rows = min(16, p.M - row0), cols = min(kCols, p.N - col0);
+  if (p.vec && cols == kCols) {
+    constexpr int kPiece = 16 / (int)sizeof(T), kPer = kCols / kPiece;  // pieces of a row
+#pragma unroll
+    for (int q = 0; q < 16 * kPer / 64; ++q) {
+      const int piece = q * 64 + lane, r = piece / kPer, c = piece % kPer * kPiece;
+      const uint4 v = *reinterpret_cast<const uint4*>(mine + r * kLd + c);
+      if (r < rows) *reinterpret_cast<uint4*>(out + r * p.ldo + c) = v;
+    }
+  } else {
+    for (int r = 0; r < rows; ++r)
+      for (int c = lane; c < cols; c += 64) out[r * p.ldo + c] = mine[r * kLd + c];
+  }
+}
+
+template <int BM, int BN, int WM, int WN, int KG, int SUB, int S, int PER_CU>
+__global__ __launch_bounds__(64 * WM * WN * KG, PER_CU) void k_int8_tile(Int8Args p, int ngm, int ngn) {
+  constexpr int kWaves = WM * WN * KG, kB = BN / 16, kK = KG * SUB;  // kK: blocks of 64 k of a stage
+  constexpr int kRowKiB = kK * BM / 16, kStage = kRowKiB + kK * kB;  // KiB of a stage: the rows', all
+  constexpr int kLoads = kStage / kWaves;
   constexpr int TM = BM / WM / 16, TN = BN / WN / 16;  // a wave's blocks
-  static_assert((kA + kB) % kWaves == 0 && kA % kWaves == 0, "loads of a wave");
-  __shared__ __attribute__((aligned(16))) uint8_t smem[S * (kA + kB) * 1024];
+  constexpr int kOutBytes = 16 * (TN * 16 + 4) * 4, kSums = KG > 1 ? BM * BN * 4 * (KG - 1) : 0;
+  static_assert(kK % 2 == 0 && kStage % kWaves == 0 && kRowKiB % kWaves == 0 && TM % KG == 0, "loads and sums of a wave");
+  constexpr int kBytes = std::max(S * kStage * 1024, std::max(kWaves * kOutBytes, kSums));
+  __shared__ __attribute__((aligned(16))) uint8_t smem[kBytes];
   lds8* const sm = (lds8*)smem;
   const int tid = threadIdx.x, lane = tid & 63, wv = uni8(tid >> 6);
   const int gm = uni8(blockIdx.x % ngm), gn = uni8(blockIdx.x / ngm);
   const int m0 = gm * BM, nt0 = gn * kB;
+  const int steps = (p.KB + kK - 1) / kK;
 
-  // this wave's blocks of a stage: kLoads of them, the first kA / kWaves of the rows
-  constexpr int kLa = kA / kWaves;
+  // Rows: 8 of them x 128 k a KiB, so that whole lines of memory are asked for; 16-byte pieces of a row are at piece ^ row % 8,
+  // for the banks that 8 lanes read at once.  Columns: their blocks as they lie in memory.
   const auto ra = rsrc8(p.a + (int64_t)m0 * p.lda, 0x7fffffff);
-  uint32_t off_a[kLa];
-#pragma unroll
-  for (int i = 0; i < kLa; ++i)
-    off_a[i] = (uint32_t)(min((wv + kWaves * i) * 16 + (lane & 15), p.M - 1 - m0) * p.lda);
   const auto rw = rsrc8(p.w + (int64_t)nt0 * p.KB * 1024, (uint32_t)min(kB, p.NT - nt0) * p.KB * 1024);
+  constexpr int kLa = kRowKiB / kWaves;  // a wave's loads of rows, then those of columns
+  uint32_t off[kLoads];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int x = wv + kWaves * i;
+    off[i] = i < kLa ? (uint32_t)(min(x % (BM / 8) * 8 + (lane >> 3), p.M - 1 - m0) * p.lda)
+                     : (uint32_t)((x - kRowKiB) % kB) * p.KB * 1024 + lane * 16;
+  }
   auto issue = [&](int step, lds8* at) {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      lds8* const dst = at + (wv + kWaves * i) * 1024;
-      if (i < kLa)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, dst, 16, (int)(off_a[i] + min(step * 64 + 16 * (lane >> 4), p.K - 16)),
-                                                 0, 0, 0);
-      else
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            rw, dst, 16, ((wv + kWaves * i - kA) * p.KB + min(step, p.KB - 1)) * 1024 + lane * 16, 0, 0, 0);
+      const int x = wv + kWaves * i;
+      lds8* const dst = at + x * 1024;
+      if (i < kLa) {  // k behind K: any values of the row, the weights are zero there
+        const int k = step * kK * 64 + x / (BM / 8) * 128 + 16 * ((lane & 7) ^ (lane >> 3));
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, dst, 16, (int)(off[i] + min(k, p.K - 16)), 0, 0, 0);
+      } else {  // blocks behind the last read as zeros
+        const int kb = step * kK + (x - kRowKiB) / kB;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, dst, 16, kb < p.KB ? (int)(off[i] + kb * 1024) : -1, 0, 0, 0);
+      }
     }
   };
-  const int wm = wv % WM, wn = wv / WM;
+  const int kg = wv / (WM * WN), wm = wv % WM, wn = wv / WM % WN;
   v4i acc[TM][TN];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
@@ -189,48 +260,80 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_int8_tile(Int8Args p, int n
     for (int j = 0; j < TN; ++j) acc[i][j] = (v4i){0, 0, 0, 0};
 
 #pragma unroll
-  for (int s = 0; s < S - 1; ++s) issue(s, sm + s * (kA + kB) * 1024);
+  for (int s = 0; s < S - 1; ++s) issue(s, sm + s * kStage * 1024);
   int at = 0;
-  for (int step = 0; step < p.KB; ++step) {
+  for (int step = 0; step < steps; ++step) {
     constexpr int kLeft = (S - 2) * kLoads;  // loads that may still be on their way
     __builtin_amdgcn_s_waitcnt(0x0f70 | (kLeft & 15) | ((kLeft >> 4) << 14));
     lds_barrier();
-    issue(step + S - 1, sm + (at + S - 1 >= S ? at - 1 : at + S - 1) * (kA + kB) * 1024);
-    const lds8* const as = sm + at * (kA + kB) * 1024 + wm * TM * 1024 + lane * 16;
-    const lds8* const bs = sm + at * (kA + kB) * 1024 + (kA + wn * TN) * 1024 + lane * 16;
-    v4i x[TM], y[TN];
+    issue(step + S - 1, sm + (at == 0 ? S - 1 : at - 1) * kStage * 1024);
 #pragma unroll
-    for (int j = 0; j < TN; ++j) y[j] = *(const __attribute__((address_space(3))) v4i*)(bs + j * 1024);
+    for (int u = 0; u < SUB; ++u) {
+      const int kb = kg * SUB + u;
+      const lds8* const as = sm + at * kStage * 1024 + kb / 2 * BM * 128 + (wm * TM * 16 + (lane & 15)) * 128 +
+                             16 * ((4 * (kb & 1) + (lane >> 4)) ^ (lane & 7));
+      const lds8* const bs = sm + (at * kStage + kRowKiB + kb * kB + wn * TN) * 1024 + lane * 16;
+      v4i x[TM], y[TN];
 #pragma unroll
-    for (int i = 0; i < TM; ++i) x[i] = *(const __attribute__((address_space(3))) v4i*)(as + i * 1024);
+      for (int j = 0; j < TN; ++j) y[j] = *(const __attribute__((address_space(3))) v4i*)(bs + j * 1024);
 #pragma unroll
-    for (int i = 0; i < TM; ++i)
+      for (int i = 0; i < TM; ++i) x[i] = *(const __attribute__((address_space(3))) v4i*)(as + i * 2048);
 #pragma unroll
-      for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(y[j], x[i], acc[i][j], 0, 0, 0);
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(y[j], x[i], acc[i][j], 0, 0, 0);
+    }
     at = at + 1 == S ? 0 : at + 1;
   }
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // nothing may land in LDS any more
+  lds_barrier();                       // every wave is done with the stages: their place takes sums and outputs
 
-  __builtin_amdgcn_s_waitcnt(0x0f70);  // nothing may land in LDS after the workgroup's end
-
-  // element i of a block: row lane % 16, column 4 (lane / 16) + i
+  constexpr int kRows = TM / KG;  // of a wave's row blocks, those that it finishes
+  if (KG > 1) {
+    v4i* const sums = reinterpret_cast<v4i*>(smem);
+    // place of (owner, which of the others, row block, column block) of this wave's part of the tile
+    auto place = [&](int owner, int other, int i, int j) {
+      return ((((owner * (KG - 1) + other) * kRows + i) * TN + j) * (WM * WN) + wv % (WM * WN)) * 64 + lane;
+    };
 #pragma unroll
-  for (int i = 0; i < TM; ++i) {
-    const int row = m0 + (wm * TM + i) * 16 + (lane & 15);
-    if (row >= p.M) continue;
-    const float sa = p.sa[row];
+    for (int o = 0; o < KG; ++o)
+      if (o != kg)
 #pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      const int col = (nt0 + wn * TN + j) * 16 + 4 * (lane >> 4);
+        for (int i = 0; i < kRows; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (col + e < p.N) {
-          const float v = scaled(acc[i][j][e], sa, p.sw[col + e]);
-          if (p.f32)
-            static_cast<float*>(p.out)[row * p.ldo + col + e] = v;
-          else
-            static_cast<uint16_t*>(p.out)[row * p.ldo + col + e] = f2bf(v);
-        }
-    }
+          for (int j = 0; j < TN; ++j) sums[place(o, kg - (kg > o), i, j)] = acc[o * kRows + i][j];
+    lds_barrier();
+#pragma unroll
+    for (int o = 0; o < KG; ++o)
+      if (o == kg)
+#pragma unroll
+        for (int i = 0; i < kRows; ++i)
+#pragma unroll
+          for (int j = 0; j < TN; ++j) {
+            v4i v = acc[o * kRows + i][j];
+#pragma unroll
+            for (int x = 0; x < KG - 1; ++x) v += sums[place(o, x, i, j)];
+            acc[i][j] = v;
+          }
+    lds_barrier();
+  }
+  uint8_t* const mine = smem + wv * kOutBytes;
+  const int col0 = (nt0 + wn * TN) * 16;
+  if (col0 >= p.N) return;
+  float sw[TN][4];
+#pragma unroll
+  for (int j = 0; j < TN; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sw[j][e] = p.sw[min(col0 + 16 * j + 4 * (lane >> 4) + e, p.N - 1)];
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const int row0 = m0 + (wm * TM + kg * kRows + i) * 16;
+    if (row0 >= p.M) break;
+    const float sa = p.sa[min(row0 + (lane & 15), p.M - 1)];
+    if (p.f32)
+      store_block<TN, float>(p, acc[i], sa, sw, reinterpret_cast<float*>(mine), row0, col0);
+    else
+      store_block<TN, uint16_t>(p, acc[i], sa, sw, reinterpret_cast<uint16_t*>(mine), row0, col0);
   }
 }
 
@@ -299,9 +402,21 @@ template <int RB, int CT>
 static void launch_stream(const Int8Args& a, int groups, dim3 grid, hipStream_t s) {
   const int each = (a.KB + kI8Waves - 1) / kI8Waves;
   if (each <= 2)
-    hipLaunchKernelGGL((k_int8_stream<RB, CT, 2>), grid, dim3(64 * kI8Waves), 0, s, a, groups);
+    hipLaunchKernelGGL((k_int8_stream<RB, CT, 2, true>), grid, dim3(64 * kI8Waves), 0, s, a, groups);
+  else if (each <= 5)
+    hipLaunchKernelGGL((k_int8_stream<RB, CT, 5, true>), grid, dim3(64 * kI8Waves), 0, s, a, groups);
   else
-    hipLaunchKernelGGL((k_int8_stream<RB, CT, 5>), grid, dim3(64 * kI8Waves), 0, s, a, groups);
+    hipLaunchKernelGGL((k_int8_stream<RB, CT, RB == 4 ? 2 : 4, false>), grid, dim3(64 * kI8Waves), 0, s, a, groups);
+}
+
+template <int BM, int BN, int WM, int WN, int KG, int SUB, int S, int PER_CU>
+static void launch_tile(const Int8Args& a, hipStream_t s) {
+  const int ngm = (a.M + BM - 1) / BM, ngn = (a.NT * 16 + BN - 1) / BN;
+  hipLaunchKernelGGL((k_int8_tile<BM, BN, WM, WN, KG, SUB, S, PER_CU>), dim3((unsigned)(ngm * ngn)), dim3(64 * WM * WN * KG), 0, s, a, ngm, ngn);
+}
+
+static int tile_choice(int64_t M, int64_t N, int64_t K) {
+  return 0;
 }
 
 }  // namespace btl
@@ -363,22 +478,35 @@ int btl_int8_matmul(const int8_t* a, int64_t lda, const float* a_scale, int64_t 
   if (!aligned(a, 16) || lda % 16 || !aligned(wdev, 16) || !aligned(a_scale, 4) || !aligned(w_scale, 4) ||
       !aligned(out, out_f32 ? 4 : 2))
     return set_error(BTL_ERR_ALIGN, "%s: misaligned buffer or row stride", who);
-  Int8Args p{a, lda, a_scale, wdev, w_scale, (int)M, (int)K, (int)N, (int)int8_kb(K), (int)int8_nt(N), out, ldo, out_f32 != 0};
+  Int8Args p{a, lda, a_scale, wdev, w_scale, (int)M, (int)K, (int)N, (int)int8_kb(K), (int)int8_nt(N), out, ldo, out_f32 != 0,
+             aligned(out, 16) && ldo % (out_f32 ? 4 : 8) == 0};
   hipStream_t s = (hipStream_t)stream;
+  const int cus = device_cus();
   if (M <= 64) {
-    const int cus = device_cus();
     const int ct = p.NT > cus ? 2 : 1, groups = (p.NT + ct - 1) / ct;
-    const int rb = M <= 16 ? 1 : 2, ny = (int)((M + 16 * rb - 1) / (16 * rb));
-    const dim3 grid((unsigned)std::min(groups, cus), (unsigned)ny);
-    if (rb == 1)
+    const dim3 grid((unsigned)std::min(groups, cus));
+    if (M <= 16)
       ct == 1 ? launch_stream<1, 1>(p, groups, grid, s) : launch_stream<1, 2>(p, groups, grid, s);
-    else
+    else if (M <= 32)
       ct == 1 ? launch_stream<2, 1>(p, groups, grid, s) : launch_stream<2, 2>(p, groups, grid, s);
+    else
+      ct == 1 ? launch_stream<4, 1>(p, groups, grid, s) : launch_stream<4, 2>(p, groups, grid, s);
     return check_launch(who);
   }
-  const int ngm = (int)((M + 255) / 256), ngn = (p.NT + 15) / 16;
-  if ((int64_t)ngm * ngn > INT32_MAX) return set_error(BTL_ERR_SHAPE, "%s: M=%lld N=%lld", who, (long long)M, (long long)N);
-  hipLaunchKernelGGL((k_int8_tile<256, 256, 2, 4, 4>), dim3((unsigned)(ngm * ngn)), dim3(512), 0, s, p, ngm, ngn);
+  if ((M + 63) / 64 * ((N + 63) / 64) > INT32_MAX)
+    return set_error(BTL_ERR_SHAPE, "%s: M=%lld N=%lld", who, (long long)M, (long long)N);
+  switch (tile_choice(M, N, K)) {
+    case 0: launch_tile<256, 256, 2, 4, 1, 2, 2, 1>(p, s); break;
+    case 1: launch_tile<128, 256, 2, 4, 1, 2, 3, 1>(p, s); break;
+    case 2: launch_tile<128, 128, 2, 2, 2, 1, 4, 1>(p, s); break;
+    case 3: launch_tile<128, 128, 2, 2, 2, 1, 2, 2>(p, s); break;
+    case 4: launch_tile<128, 64, 2, 2, 2, 1, 6, 1>(p, s); break;
+    case 5: launch_tile<64, 64, 2, 2, 2, 1, 8, 1>(p, s); break;
+    case 6: launch_tile<64, 64, 2, 2, 2, 1, 4, 2>(p, s); break;
+    case 7: launch_tile<256, 128, 4, 2, 1, 2, 3, 1>(p, s); break;
+    case 8: launch_tile<64, 128, 1, 4, 2, 1, 6, 1>(p, s); break;
+    case 9: launch_tile<64, 64, 1, 2, 4, 1, 4, 1>(p, s); break;
+  }
   return check_launch(who);
 }
 
