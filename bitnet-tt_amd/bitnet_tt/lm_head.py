@@ -7,31 +7,48 @@ takes ``ttnn.argmax`` over the vocabulary (:1170-1174).  Here the head stays
 bf16 (the checkpoint's dtype; the reference's bfp8 is a Tensix block format)
 in an MFMA operand layout made once at load time, and one launch streams it
 for up to 32 rows, writing fp32 logits (optional) and the token ids.
+
+``weight_dtype="int8"`` keeps 8-bit integers with a scale for each vocabulary row
+instead, half the bytes: the normed rows are quantised as the ternary layers quantise
+theirs, and any number of rows is taken (a prompt's, to score it).
 """
 
 from __future__ import annotations
+
+import math
 
 import numpy as np
 
 from . import _native as N
 
 
-class LMHead:
-    """``norm`` + head + argmax; API pieces of bitnet.py:139-215."""
+_ROWS = 1024  # of a pass without logits over many rows
+_MAX_ROWS = 65535
 
-    def __init__(self, hidden_size: int, vocab_size: int, device=None, eps: float = 1e-5) -> None:
+
+class LMHead:
+    """``norm`` + head + argmax; API pieces of bitnet.py:139-215.  ``weight_dtype``: "bf16", or
+    "int8" (hidden_size a multiple of 32)."""
+
+    def __init__(self, hidden_size: int, vocab_size: int, device=None, eps: float = 1e-5,
+                 weight_dtype: str = "bf16") -> None:
         import torch
 
+        if weight_dtype not in ("bf16", "int8"):
+            raise ValueError(f"weight_dtype {weight_dtype!r}: 'bf16' or 'int8'")
+        if weight_dtype == "int8" and (hidden_size % 32 or hidden_size > N.MAX_K):
+            raise ValueError(f"hidden size {hidden_size}: the 8-bit head takes multiples of 32 up to {N.MAX_K}")
+        self.weight_dtype = weight_dtype
         self.hidden_size = hidden_size
         self.vocab_size = vocab_size
         self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         self.eps = eps
         self.norm_weight = None
-        self.weight = None  # device layout (uint8 bytes)
+        self.weight = None  # device layout (uint8 bytes; int8: an Int8Weight)
 
     def load_final_weights(self, norm_weight, lm_head_weight) -> None:
         """Final norm gain [hidden] and head [vocab, hidden] (numpy or tensor,
-        any float dtype; stored as bf16)."""
+        any float dtype; stored as bf16, or quantised from bf16 or fp32)."""
         import torch
 
         H, V = self.hidden_size, self.vocab_size
@@ -44,6 +61,12 @@ class LMHead:
             np.ascontiguousarray(np.asarray(lm_head_weight, dtype=np.float32)))
         if tuple(w.shape) != (V, H):
             raise ValueError(f"head weight is {tuple(w.shape)}, expected ({V}, {H})")
+        if self.weight_dtype == "int8":
+            from .int8_matmul import Int8Weight
+
+            self.weight = Int8Weight.quantize(w.to(self.device))
+            self.norm_weight = g
+            return
         w = w.to(device=self.device, dtype=torch.bfloat16).contiguous()
         L = N.lib()
         nbytes = int(L.btl_lm_head_weight_bytes(V, H))
@@ -55,7 +78,7 @@ class LMHead:
         self.weight = dev
 
     def __call__(self, hidden, return_logits: bool = True, normed_out=None, logits_out=None, tokens_out=None):
-        """bf16 hidden [M, hidden] (M <= 32) -> (fp32 logits [M, vocab] or None,
+        """bf16 hidden [M, hidden] (M <= 32; int8: up to 65535) -> (fp32 logits [M, vocab] or None,
         int32 token ids [M]).  The ``*_out`` tensors, when given, are written
         in place (no allocation: the call can then be captured in a graph
         after one eager call on the same stream)."""
@@ -68,6 +91,8 @@ class LMHead:
         if hidden.dtype != torch.bfloat16 or hidden.shape[-1] != H:
             raise ValueError("hidden must be bf16 [..., hidden_size]")
         M = hidden.numel() // H
+        if self.weight_dtype == "int8":
+            return self._int8(hidden.reshape(M, H), return_logits, normed_out, logits_out, tokens_out)
         if M > 32:
             raise ValueError(f"{M} rows: the head launch takes up to 32")
         x = hidden.reshape(M, H)
@@ -89,6 +114,53 @@ class LMHead:
                               ws_bytes, stream), "btl_lm_head")
         return logits, tokens
 
+    def _int8(self, x, return_logits, normed_out, logits_out, tokens_out):
+        """The 8-bit head on x [M, hidden]."""
+        import torch
+
+        M, H = x.shape
+        V, dev = self.vocab_size, x.device
+        if M > _MAX_ROWS:
+            raise ValueError(f"{M} rows: a call takes up to {_MAX_ROWS}")
+        for t, shape, dtype, name in ((normed_out, (M, H), torch.bfloat16, "normed_out"),
+                                      (logits_out, (M, V), torch.float32, "logits_out"),
+                                      (tokens_out, (M,), torch.int32, "tokens_out")):
+            if t is not None and (t.dtype is not dtype or t.numel() != math.prod(shape) or not t.is_contiguous()
+                                  or t.device != dev):
+                raise ValueError(f"{name} must be contiguous {dtype} {list(shape)} on {dev}")
+        if self.weight.device != dev:
+            raise ValueError(f"hidden is on {dev}, the head on {self.weight.device}")
+        with torch.cuda.device(dev):
+            logits = logits_out if logits_out is not None else (
+                torch.empty((M, V), dtype=torch.float32, device=dev) if return_logits else None)
+            tokens = tokens_out if tokens_out is not None else torch.empty(M, dtype=torch.int32, device=dev)
+            if M == 0:
+                return logits, tokens
+            L, stream, index = N.lib(), N.raw_stream(dev.index), dev.index
+            nbytes = int(L.btl_int8_head_workspace_bytes(M))
+            if torch.cuda.is_current_stream_capturing() and not N.has_workspace(dev, nbytes, "int8_head"):
+                raise RuntimeError("run one eager head call on this stream before capturing it in a graph")
+            ws, ws_bytes, _ = N.workspace_ptr(index, nbytes, "int8_head", None, stream)
+            codes = torch.empty((M, H), dtype=torch.int8, device=dev)
+            blocked = torch.empty(int(L.btl_act_bytes(M, H)), dtype=torch.int8, device=dev)
+            scale = torch.empty((M + 31) // 32 * 32, dtype=torch.float32, device=dev)
+            N.check(L.btl_quant_absmax(x.data_ptr(), M, H, H, N.ptr(self.norm_weight), float(self.eps), blocked.data_ptr(),
+                                       scale.data_ptr(), None, None, codes.data_ptr(), N.ptr(normed_out), stream),
+                    "btl_quant_absmax")
+            # without logits up to 64 rows need none; more go in passes that share a buffer
+            rows = M if logits is not None or M <= 64 else _ROWS
+            part = logits
+            if logits is None and M > 64:
+                part = torch.empty((min(M, rows), V), dtype=torch.float32, device=dev)
+            for lo in range(0, M, rows):
+                n = min(rows, M - lo)
+                N.check(L.btl_int8_head(codes.data_ptr() + lo * H, H, scale.data_ptr() + 4 * lo, n, H, V,
+                                        self.weight.data.data_ptr(), self.weight.scale.data_ptr(), N.ptr(part), V,
+                                        tokens.data_ptr() + 4 * lo, ws, ws_bytes, stream), "btl_int8_head")
+        return logits, tokens
+
     def weight_bytes(self) -> int:
-        """Compulsory HBM bytes of one head call's weights (bf16 vocab x hidden)."""
+        """Compulsory HBM bytes of one head call's weights (vocab x hidden, bf16, or int8 and the scales)."""
+        if self.weight_dtype == "int8":
+            return self.vocab_size * (self.hidden_size + 4)
         return 2 * self.vocab_size * self.hidden_size

@@ -34,7 +34,20 @@ struct Int8Args {
   void* out;
   int64_t ldo;
   int f32, vec;  // vec: rows of out are 16-byte aligned
+  // few rows, the head: out may be missing; the first index of each row's largest output
+  int32_t* tokens;
+  uint64_t* keys;   // [M], zero between calls
+  uint32_t* count;  // workgroups that are done, zero between calls
 };
+
+// An output's place in the order (value, then the lower index); 0: a NaN.
+__device__ __forceinline__ uint64_t arg_key(float y, int col) {
+  const uint32_t u = __float_as_uint(y + 0.0f);  // (both zeros alike)
+  const uint32_t order = (u & 0x80000000u) ? ~u : u | 0x80000000u;
+  return y == y ? ((uint64_t)order << 32) | (0xffffffffu - (uint32_t)col) : 0u;
+}
+__device__ __forceinline__ uint64_t arg_max(uint64_t a, uint64_t b) { return a > b ? a : b; }
+__device__ __forceinline__ int32_t arg_col(uint64_t key) { return key ? (int32_t)(0xffffffffu - (uint32_t)key) : -1; }
 
 __device__ __forceinline__ int uni8(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
@@ -110,6 +123,8 @@ __global__ __launch_bounds__(64 * kI8Waves, 2) void k_int8_stream(Int8Args p, in
         for (int t = 0; t < CT; ++t)
           acc[r][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b[set][u][t], a[ONCE ? 0 : set][u][r], acc[r][t], 0, 0, 0);
   };
+  static_assert(RB * CT * 64 <= 64 * kI8Waves, "a thread has the same row in every group");
+  uint64_t best = 0;
   auto finish = [&](int c) {  // the group of chunk c is complete
     const int g = blockIdx.x + c / rounds * gridDim.x;
 #pragma unroll
@@ -118,7 +133,7 @@ __global__ __launch_bounds__(64 * kI8Waves, 2) void k_int8_stream(Int8Args p, in
       for (int t = 0; t < CT; ++t) *reinterpret_cast<v4i*>(&red[wv][r][t][4 * lane + 4 * (lane >> 4)]) = acc[r][t];
     lds_barrier();
     // a thread's four columns of a row
-    for (int e = tid; e < RB * CT * 64; e += 64 * kI8Waves) {
+    for (int e = tid; e < RB * CT * 64; e += 64 * kI8Waves) {  // (once)
       const int q = e % (4 * CT), m = e / (4 * CT), at = 4 * (16 * (q & 3) + (m & 15)) + 4 * (q & 3);
       v4i sum = (v4i){0, 0, 0, 0};
 #pragma unroll
@@ -129,6 +144,11 @@ __global__ __launch_bounds__(64 * kI8Waves, 2) void k_int8_stream(Int8Args p, in
       float y[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) y[i] = scaled(sum[i], sa, p.sw[min(col + i, p.N - 1)]);
+      if (p.tokens)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (col + i < p.N) best = arg_max(best, arg_key(y[i], col + i));
+      if (!p.out) continue;
       if (p.f32) {
         float* const o = static_cast<float*>(p.out) + row * p.ldo + col;
         if (p.vec && col + 4 <= p.N)
@@ -162,6 +182,47 @@ __global__ __launch_bounds__(64 * kI8Waves, 2) void k_int8_stream(Int8Args p, in
     issue(1, c + 3);
     if (ONCE || (c + 2) % rounds == 0) finish(c + 1);
   }
+  if (!p.tokens) return;
+
+  // the best of a row: over the 4 CT threads that have its columns here, then over the workgroups; the last of
+  // those to end writes the indexes
+#pragma unroll
+  for (int off = 1; off < 4 * CT; off <<= 1) best = arg_max(best, __shfl_xor(best, off, 64));
+  const int row = m0 + tid / (4 * CT);
+  if (tid < RB * CT * 64 && tid % (4 * CT) == 0 && row < p.M && best)
+    __hip_atomic_fetch_max(p.keys + row, best, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  wait_memory();  // this workgroup's maxima are performed before it counts itself done
+  int* const last = &red[0][0][0][0];
+  lds_barrier();
+  if (tid == 0) *last = atomicAdd(p.count, 1u) + 1u == gridDim.x;
+  lds_barrier();
+  if (!*last) return;
+  if (tid < p.M) {
+    p.tokens[tid] = arg_col(ld_coherent(p.keys + tid));
+    st_coherent(p.keys + tid, (uint64_t)0);
+  }
+  if (tid == 0) st_coherent(p.count, 0u);
+}
+
+// Row blockIdx.y of outputs: the best of a part of it, then as above; count [M], one a row.
+__global__ __launch_bounds__(256) void k_int8_argmax(const float* y, int64_t ldo, int N, int each, Int8Args p) {
+  __shared__ uint64_t s_best[4];
+  const int row = blockIdx.y, end = min(N, ((int)blockIdx.x + 1) * each);
+  const float* const at = y + (int64_t)row * ldo;
+  uint64_t best = 0;
+  for (int c = blockIdx.x * each + threadIdx.x; c < end; c += 256) best = arg_max(best, arg_key(at[c], c));
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) best = arg_max(best, __shfl_xor(best, off, 64));
+  if ((threadIdx.x & 63) == 0) s_best[threadIdx.x >> 6] = best;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  best = arg_max(arg_max(s_best[0], s_best[1]), arg_max(s_best[2], s_best[3]));
+  if (best) __hip_atomic_fetch_max(p.keys + row, best, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  wait_memory();
+  if (atomicAdd(p.count + row, 1u) + 1u != gridDim.x) return;
+  p.tokens[row] = arg_col(ld_coherent(p.keys + row));
+  st_coherent(p.keys + row, (uint64_t)0);
+  st_coherent(p.count + row, 0u);
 }
 
 // ======================================================================
@@ -210,20 +271,25 @@ __device__ __forceinline__ void store_block(const Int8Args& p, const v4i (&acc)[
   }
 }
 
-template <int BM, int BN, int WM, int WN, int KG, int SUB, int S, int PER_CU>
-__global__ __launch_bounds__(64 * WM * WN * KG, PER_CU) void k_int8_tile(Int8Args p, int ngm, int ngn) {
-  constexpr int kWaves = WM * WN * KG, kB = BN / 16, kK = KG * SUB;  // kK: blocks of 64 k of a stage
-  constexpr int kRowKiB = kK * BM / 16, kStage = kRowKiB + kK * kB;  // KiB of a stage: the rows', all
+template <int BM, int BN, int WM, int WN, int KG, int SUB, int S>
+struct TileShape {
+  static constexpr int kWaves = WM * WN * KG, kB = BN / 16, kK = KG * SUB;  // kK: blocks of 64 k of a stage
+  static constexpr int kRowKiB = kK * BM / 16, kStage = kRowKiB + kK * kB;  // KiB of a stage: the rows', all
+  static constexpr int TM = BM / WM / 16, TN = BN / WN / 16;                // a wave's blocks
+  static constexpr int kOutBytes = 16 * (TN * 16 + 4) * 4, kSums = KG > 1 ? BM * BN * 4 * (KG - 1) : 0;
+  static constexpr int kBytes = std::max(S * kStage * 1024, std::max(kWaves * kOutBytes, kSums));
+};
+
+// The tile whose first row is m0 and first block of columns nt0.
+template <int BM, int BN, int WM, int WN, int KG, int SUB, int S>
+__device__ __forceinline__ void int8_tile(const Int8Args& p, uint8_t* smem, int m0, int nt0) {
+  using Shape = TileShape<BM, BN, WM, WN, KG, SUB, S>;
+  constexpr int kWaves = Shape::kWaves, kB = Shape::kB, kK = Shape::kK, kRowKiB = Shape::kRowKiB, kStage = Shape::kStage;
+  constexpr int TM = Shape::TM, TN = Shape::TN, kOutBytes = Shape::kOutBytes;
   constexpr int kLoads = kStage / kWaves;
-  constexpr int TM = BM / WM / 16, TN = BN / WN / 16;  // a wave's blocks
-  constexpr int kOutBytes = 16 * (TN * 16 + 4) * 4, kSums = KG > 1 ? BM * BN * 4 * (KG - 1) : 0;
   static_assert(kK % 2 == 0 && kStage % kWaves == 0 && kRowKiB % kWaves == 0 && TM % KG == 0, "loads and sums of a wave");
-  constexpr int kBytes = std::max(S * kStage * 1024, std::max(kWaves * kOutBytes, kSums));
-  __shared__ __attribute__((aligned(16))) uint8_t smem[kBytes];
   lds8* const sm = (lds8*)smem;
   const int tid = threadIdx.x, lane = tid & 63, wv = uni8(tid >> 6);
-  const int gm = uni8(blockIdx.x % ngm), gn = uni8(blockIdx.x / ngm);
-  const int m0 = gm * BM, nt0 = gn * kB;
   const int steps = (p.KB + kK - 1) / kK;
 
   // Rows: 8 of them x 128 k a KiB, so that whole lines of memory are asked for; 16-byte pieces of a row are at piece ^ row % 8,
@@ -337,6 +403,26 @@ __global__ __launch_bounds__(64 * WM * WN * KG, PER_CU) void k_int8_tile(Int8Arg
   }
 }
 
+template <int BM, int BN, int WM, int WN, int KG, int SUB, int S, int PER_CU>
+__global__ __launch_bounds__(64 * WM * WN * KG, PER_CU) void k_int8_tile(Int8Args p, int ngm) {
+  __shared__ __attribute__((aligned(16))) uint8_t smem[TileShape<BM, BN, WM, WN, KG, SUB, S>::kBytes];
+  int8_tile<BM, BN, WM, WN, KG, SUB, S>(p, smem, uni8(blockIdx.x % ngm) * BM, uni8(blockIdx.x / ngm) * (BN / 16));
+}
+
+// Tiles of 256 x 256, the last ones (from `full` on) as two of 128 rows each: they fill the CUs once more where
+// whole tiles would fill half of them for twice as long.
+__global__ __launch_bounds__(512, 1) void k_int8_large(Int8Args p, int ngm, int full) {
+  constexpr int kBytes = std::max(TileShape<256, 256, 2, 4, 1, 2, 2>::kBytes, TileShape<128, 256, 2, 4, 1, 2, 3>::kBytes);
+  __shared__ __attribute__((aligned(16))) uint8_t smem[kBytes];
+  const int x = blockIdx.x;
+  if (x < full) {
+    int8_tile<256, 256, 2, 4, 1, 2, 2>(p, smem, uni8(x % ngm) * 256, uni8(x / ngm) * 16);
+  } else {
+    const int t = full + (x - full) / 2, m0 = uni8(t % ngm) * 256 + uni8((x - full) & 1) * 128;
+    if (m0 < p.M) int8_tile<128, 256, 2, 4, 1, 2, 3>(p, smem, m0, uni8(t / ngm) * 16);
+  }
+}
+
 // ---- weights ---------------------------------------------------------------
 __global__ void k_int8_layout(const int8_t* w, int64_t ldw, int N, int K, int KB, int64_t total, uint4* out) {
   const int64_t g = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
@@ -412,11 +498,87 @@ static void launch_stream(const Int8Args& a, int groups, dim3 grid, hipStream_t 
 template <int BM, int BN, int WM, int WN, int KG, int SUB, int S, int PER_CU>
 static void launch_tile(const Int8Args& a, hipStream_t s) {
   const int ngm = (a.M + BM - 1) / BM, ngn = (a.NT * 16 + BN - 1) / BN;
-  hipLaunchKernelGGL((k_int8_tile<BM, BN, WM, WN, KG, SUB, S, PER_CU>), dim3((unsigned)(ngm * ngn)), dim3(64 * WM * WN * KG), 0, s, a, ngm, ngn);
+  hipLaunchKernelGGL((k_int8_tile<BM, BN, WM, WN, KG, SUB, S, PER_CU>), dim3((unsigned)(ngm * ngn)), dim3(64 * WM * WN * KG), 0, s,
+                     a, ngm);
 }
 
-static int tile_choice(int64_t M, int64_t N, int64_t K) {
-  return 0;
+static void launch_large(const Int8Args& a, int cus, hipStream_t s) {
+  const int ngm = (a.M + 255) / 256, tiles = ngm * ((a.NT + 15) / 16);
+  const int rest = tiles % cus, halves = tiles > cus && 2 * rest <= cus ? rest : 0;
+  hipLaunchKernelGGL(k_int8_large, dim3((unsigned)(tiles + halves)), dim3(512), 0, s, a, ngm, tiles - halves);
+}
+
+// The tile of the least time, us: rounds of workgroups over the CUs x what a workgroup takes, before its first and
+// behind its last step and for each 128 k.
+struct TileCost {
+  int bm, bn, per_cu;
+  double start, step;
+};
+constexpr TileCost kTiles[] = {
+    {256, 256, 1, 4.0, 1.66}, {128, 256, 1, 3.5, 0.90}, {128, 128, 2, 3.0, 1.02},
+    {128, 128, 1, 3.0, 0.47}, {128, 64, 1, 2.5, 0.31},  {64, 64, 2, 2.0, 0.62}, {64, 64, 1, 2.0, 0.21},
+};
+static int tile_choice(int64_t M, int64_t N, int64_t K, int cus) {
+  const double steps = (double)((K + 127) / 128);
+  int best = 0;
+  double least = 0;
+  for (int i = 0; i < (int)(sizeof(kTiles) / sizeof(kTiles[0])); ++i) {
+    const TileCost& t = kTiles[i];
+    const int64_t tiles = (M + t.bm - 1) / t.bm * ((N + t.bn - 1) / t.bn), slots = (int64_t)cus * t.per_cu;
+    double rounds = (double)((tiles + slots - 1) / slots);
+    if (i == 0 && tiles > cus && 2 * (tiles % cus) <= cus && tiles % cus) rounds -= 0.25;  // halves
+    const double us = rounds * (t.start + t.step * steps);
+    if (i == 0 || us < least) best = i, least = us;
+  }
+  return best;
+}
+
+constexpr int kFewRows8 = 64;     // of the weight stream
+constexpr int kHeadRows = 65535;  // a grid's second dimension
+
+// Checks that the entry points share; fills what they share.
+static int int8_args(const char* who, const int8_t* a, int64_t lda, const float* a_scale, int64_t M, int64_t K, int64_t N,
+                     const uint8_t* wdev, const float* w_scale, void* out, int64_t ldo, int out_f32, Int8Args* p) {
+  const int rc = check_int8_shape(who, N, K);
+  if (rc != BTL_OK) return rc;
+  if (M < 0 || M > (1 << 24)) return set_error(BTL_ERR_SHAPE, "%s: M=%lld", who, (long long)M);
+  if (lda < K || lda > (1 << 22) || (out && ldo < N))
+    return set_error(BTL_ERR_SHAPE, "%s: lda=%lld ldo=%lld", who, (long long)lda, (long long)ldo);
+  if (M == 0) return BTL_OK;
+  if (!a || !a_scale || !wdev || !w_scale) return set_error(BTL_ERR_NULL, "%s: NULL pointer", who);
+  if (!aligned(a, 16) || lda % 16 || !aligned(wdev, 16) || !aligned(a_scale, 4) || !aligned(w_scale, 4) ||
+      !aligned(out, out_f32 ? 4 : 2))
+    return set_error(BTL_ERR_ALIGN, "%s: misaligned buffer or row stride", who);
+  if ((M + 63) / 64 * ((N + 63) / 64) > INT32_MAX)
+    return set_error(BTL_ERR_SHAPE, "%s: M=%lld N=%lld", who, (long long)M, (long long)N);
+  *p = Int8Args{a, lda, a_scale, wdev, w_scale, (int)M, (int)K, (int)N, (int)int8_kb(K), (int)int8_nt(N), out, ldo, out_f32 != 0,
+                aligned(out, 16) && ldo % (out_f32 ? 4 : 8) == 0, nullptr, nullptr, nullptr};
+  return BTL_OK;
+}
+
+static int int8_launch(const char* who, const Int8Args& p, hipStream_t s) {
+  const int cus = device_cus();
+  if (p.M <= kFewRows8) {
+    const int ct = p.NT > cus ? 2 : 1, groups = (p.NT + ct - 1) / ct;
+    const dim3 grid((unsigned)std::min(groups, cus));
+    if (p.M <= 16)
+      ct == 1 ? launch_stream<1, 1>(p, groups, grid, s) : launch_stream<1, 2>(p, groups, grid, s);
+    else if (p.M <= 32)
+      ct == 1 ? launch_stream<2, 1>(p, groups, grid, s) : launch_stream<2, 2>(p, groups, grid, s);
+    else
+      ct == 1 ? launch_stream<4, 1>(p, groups, grid, s) : launch_stream<4, 2>(p, groups, grid, s);
+    return check_launch(who);
+  }
+  switch (tile_choice(p.M, p.N, p.K, cus)) {
+    case 0: launch_large(p, cus, s); break;
+    case 1: launch_tile<128, 256, 2, 4, 1, 2, 3, 1>(p, s); break;
+    case 2: launch_tile<128, 128, 2, 2, 2, 1, 2, 2>(p, s); break;
+    case 3: launch_tile<128, 128, 2, 2, 2, 1, 4, 1>(p, s); break;
+    case 4: launch_tile<128, 64, 2, 2, 2, 1, 6, 1>(p, s); break;
+    case 5: launch_tile<64, 64, 2, 2, 2, 1, 4, 2>(p, s); break;
+    default: launch_tile<64, 64, 2, 2, 2, 1, 8, 1>(p, s); break;
+  }
+  return check_launch(who);
 }
 
 }  // namespace btl
@@ -468,45 +630,40 @@ int btl_int8_matmul(const int8_t* a, int64_t lda, const float* a_scale, int64_t 
                     const float* w_scale, void* out, int64_t ldo, int out_f32, btl_stream_t stream) {
   const char* who = "btl_int8_matmul";
   clear_error();
-  const int rc = check_int8_shape(who, N, K);
-  if (rc != BTL_OK) return rc;
-  if (M < 0 || M > (1 << 24)) return set_error(BTL_ERR_SHAPE, "%s: M=%lld", who, (long long)M);
-  if (lda < K || lda > (1 << 22) || ldo < N) return set_error(BTL_ERR_SHAPE, "%s: lda=%lld ldo=%lld", who, (long long)lda,
-                                                             (long long)ldo);
-  if (M == 0) return BTL_OK;
-  if (!a || !a_scale || !wdev || !w_scale || !out) return set_error(BTL_ERR_NULL, "%s: NULL pointer", who);
-  if (!aligned(a, 16) || lda % 16 || !aligned(wdev, 16) || !aligned(a_scale, 4) || !aligned(w_scale, 4) ||
-      !aligned(out, out_f32 ? 4 : 2))
-    return set_error(BTL_ERR_ALIGN, "%s: misaligned buffer or row stride", who);
-  Int8Args p{a, lda, a_scale, wdev, w_scale, (int)M, (int)K, (int)N, (int)int8_kb(K), (int)int8_nt(N), out, ldo, out_f32 != 0,
-             aligned(out, 16) && ldo % (out_f32 ? 4 : 8) == 0};
-  hipStream_t s = (hipStream_t)stream;
-  const int cus = device_cus();
-  if (M <= 64) {
-    const int ct = p.NT > cus ? 2 : 1, groups = (p.NT + ct - 1) / ct;
-    const dim3 grid((unsigned)std::min(groups, cus));
-    if (M <= 16)
-      ct == 1 ? launch_stream<1, 1>(p, groups, grid, s) : launch_stream<1, 2>(p, groups, grid, s);
-    else if (M <= 32)
-      ct == 1 ? launch_stream<2, 1>(p, groups, grid, s) : launch_stream<2, 2>(p, groups, grid, s);
-    else
-      ct == 1 ? launch_stream<4, 1>(p, groups, grid, s) : launch_stream<4, 2>(p, groups, grid, s);
-    return check_launch(who);
-  }
-  if ((M + 63) / 64 * ((N + 63) / 64) > INT32_MAX)
-    return set_error(BTL_ERR_SHAPE, "%s: M=%lld N=%lld", who, (long long)M, (long long)N);
-  switch (tile_choice(M, N, K)) {
-    case 0: launch_tile<256, 256, 2, 4, 1, 2, 2, 1>(p, s); break;
-    case 1: launch_tile<128, 256, 2, 4, 1, 2, 3, 1>(p, s); break;
-    case 2: launch_tile<128, 128, 2, 2, 2, 1, 4, 1>(p, s); break;
-    case 3: launch_tile<128, 128, 2, 2, 2, 1, 2, 2>(p, s); break;
-    case 4: launch_tile<128, 64, 2, 2, 2, 1, 6, 1>(p, s); break;
-    case 5: launch_tile<64, 64, 2, 2, 2, 1, 8, 1>(p, s); break;
-    case 6: launch_tile<64, 64, 2, 2, 2, 1, 4, 2>(p, s); break;
-    case 7: launch_tile<256, 128, 4, 2, 1, 2, 3, 1>(p, s); break;
-    case 8: launch_tile<64, 128, 1, 4, 2, 1, 6, 1>(p, s); break;
-    case 9: launch_tile<64, 64, 1, 2, 4, 1, 4, 1>(p, s); break;
-  }
+  Int8Args p{};
+  const int rc = int8_args(who, a, lda, a_scale, M, K, N, wdev, w_scale, out, ldo, out_f32, &p);
+  if (rc != BTL_OK || M == 0) return rc;
+  if (!out) return set_error(BTL_ERR_NULL, "%s: NULL pointer", who);
+  return int8_launch(who, p, (hipStream_t)stream);
+}
+
+int64_t btl_int8_head_workspace_bytes(int64_t M) { return M > 0 && M <= kHeadRows ? round_up(M, 64) * 12 : 0; }
+
+int btl_int8_head(const int8_t* a, int64_t lda, const float* a_scale, int64_t M, int64_t K, int64_t N, const uint8_t* wdev,
+                  const float* w_scale, float* logits, int64_t ldo, int32_t* tokens, void* workspace, size_t workspace_bytes,
+                  btl_stream_t stream) {
+  const char* who = "btl_int8_head";
+  clear_error();
+  Int8Args p{};
+  const int rc = int8_args(who, a, lda, a_scale, M, K, N, wdev, w_scale, logits, ldo, 1, &p);
+  if (rc != BTL_OK || M == 0) return rc;
+  if (M > kHeadRows) return set_error(BTL_ERR_SHAPE, "%s: M=%lld (up to %d)", who, (long long)M, kHeadRows);
+  if (!tokens || !workspace || (!logits && M > kFewRows8)) return set_error(BTL_ERR_NULL, "%s: NULL pointer", who);
+  if (!aligned(tokens, 4) || !aligned(workspace, 256)) return set_error(BTL_ERR_ALIGN, "%s: misaligned buffer", who);
+  if ((int64_t)workspace_bytes < btl_int8_head_workspace_bytes(M))
+    return set_error(BTL_ERR_WORKSPACE, "%s: workspace %zu < %lld bytes", who, workspace_bytes,
+                     (long long)btl_int8_head_workspace_bytes(M));
+  p.count = reinterpret_cast<uint32_t*>(static_cast<char*>(workspace));
+  p.keys = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + round_up(M, 64) * 4);
+  if (M <= kFewRows8) p.tokens = tokens;
+  const int launched = int8_launch(who, p, (hipStream_t)stream);
+  if (launched != BTL_OK || M <= kFewRows8) return launched;
+  p.tokens = tokens;
+  // parts of a row, about four workgroups a CU
+  const int64_t parts = std::max((int64_t)1, std::min((4 * (int64_t)device_cus() + M - 1) / M, (N + 2047) / 2048));
+  const int each = (int)((N + parts - 1) / parts);
+  hipLaunchKernelGGL(k_int8_argmax, dim3((unsigned)((N + each - 1) / each), (unsigned)M), dim3(256), 0, (hipStream_t)stream, logits,
+                     ldo, (int)N, each, p);
   return check_launch(who);
 }
 
