@@ -15,6 +15,7 @@ theirs, and any number of rows is taken (a prompt's, to score it).
 
 from __future__ import annotations
 
+import functools
 import math
 
 import numpy as np
@@ -24,6 +25,12 @@ from . import _native as N
 
 _ROWS = 1024  # of a pass without logits over many rows
 _MAX_ROWS = 65535
+
+
+@functools.lru_cache(maxsize=4096)
+def _scratch_bytes(index: int, m: int, k: int, v: int) -> int:
+    """Of an 8-bit head's call on device ``index``."""
+    return int(N.lib().btl_int8_head_scratch_bytes(m, k, v))
 
 
 class LMHead:
@@ -136,27 +143,22 @@ class LMHead:
             tokens = tokens_out if tokens_out is not None else torch.empty(M, dtype=torch.int32, device=dev)
             if M == 0:
                 return logits, tokens
-            L, stream, index = N.lib(), N.raw_stream(dev.index), dev.index
-            nbytes = int(L.btl_int8_head_workspace_bytes(M))
-            if torch.cuda.is_current_stream_capturing() and not N.has_workspace(dev, nbytes, "int8_head"):
-                raise RuntimeError("run one eager head call on this stream before capturing it in a graph")
-            ws, ws_bytes, _ = N.workspace_ptr(index, nbytes, "int8_head", None, stream)
-            codes = torch.empty((M, H), dtype=torch.int8, device=dev)
-            blocked = torch.empty(int(L.btl_act_bytes(M, H)), dtype=torch.int8, device=dev)
-            scale = torch.empty((M + 31) // 32 * 32, dtype=torch.float32, device=dev)
-            N.check(L.btl_quant_absmax(x.data_ptr(), M, H, H, N.ptr(self.norm_weight), float(self.eps), blocked.data_ptr(),
-                                       scale.data_ptr(), None, None, codes.data_ptr(), N.ptr(normed_out), stream),
-                    "btl_quant_absmax")
+            L, stream = N.lib(), N.raw_stream(dev.index)
             # without logits up to 64 rows need none; more go in passes that share a buffer
-            rows = M if logits is not None or M <= 64 else _ROWS
+            rows = M if logits is not None or M <= 64 else min(M, _ROWS)
             part = logits
             if logits is None and M > 64:
-                part = torch.empty((min(M, rows), V), dtype=torch.float32, device=dev)
+                part = torch.empty((rows, V), dtype=torch.float32, device=dev)
+            nbytes = max(_scratch_bytes(dev.index, rows, H, V), _scratch_bytes(dev.index, M % rows or rows, H, V))
+            # the call's own: calls that overlap share nothing
+            scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            w = self.weight
             for lo in range(0, M, rows):
                 n = min(rows, M - lo)
-                N.check(L.btl_int8_head(codes.data_ptr() + lo * H, H, scale.data_ptr() + 4 * lo, n, H, V,
-                                        self.weight.data.data_ptr(), self.weight.scale.data_ptr(), N.ptr(part), V,
-                                        tokens.data_ptr() + 4 * lo, ws, ws_bytes, stream), "btl_int8_head")
+                at = None if normed_out is None else normed_out.data_ptr() + 2 * lo * H
+                N.check(L.btl_int8_head(x.data_ptr() + 2 * lo * H, n, H, V, self.norm_weight.data_ptr(), float(self.eps),
+                                        w.data.data_ptr(), w.scale.data_ptr(), at, N.ptr(part), tokens.data_ptr() + 4 * lo,
+                                        scratch.data_ptr(), nbytes, stream), "btl_int8_head")
         return logits, tokens
 
     def weight_bytes(self) -> int:

@@ -36,8 +36,8 @@ struct Int8Args {
   int f32, vec;  // vec: rows of out are 16-byte aligned
   // few rows, the head: out may be missing; the first index of each row's largest output
   int32_t* tokens;
-  uint64_t* keys;   // [M], zero between calls
-  uint32_t* count;  // workgroups that are done, zero between calls
+  uint64_t* keys;   // [M], zero at first
+  uint32_t* count;  // workgroups that are done, zero at first
 };
 
 // An output's place in the order (value, then the lower index); 0: a NaN.
@@ -197,15 +197,11 @@ __global__ __launch_bounds__(64 * kI8Waves, 2) void k_int8_stream(Int8Args p, in
   if (tid == 0) *last = atomicAdd(p.count, 1u) + 1u == gridDim.x;
   lds_barrier();
   if (!*last) return;
-  if (tid < p.M) {
-    p.tokens[tid] = arg_col(ld_coherent(p.keys + tid));
-    st_coherent(p.keys + tid, (uint64_t)0);
-  }
-  if (tid == 0) st_coherent(p.count, 0u);
+  if (tid < p.M) p.tokens[tid] = arg_col(ld_coherent(p.keys + tid));
 }
 
-// Row blockIdx.y of outputs: the best of a part of it, then as above; count [M], one a row.
-__global__ __launch_bounds__(256) void k_int8_argmax(const float* y, int64_t ldo, int N, int each, Int8Args p) {
+// The best of part blockIdx.x of row blockIdx.y; a row of one part is done.
+__global__ __launch_bounds__(256) void k_int8_argmax(const float* y, int64_t ldo, int N, int each, uint64_t* keys, int32_t* tokens) {
   __shared__ uint64_t s_best[4];
   const int row = blockIdx.y, end = min(N, ((int)blockIdx.x + 1) * each);
   const float* const at = y + (int64_t)row * ldo;
@@ -217,12 +213,18 @@ __global__ __launch_bounds__(256) void k_int8_argmax(const float* y, int64_t ldo
   __syncthreads();
   if (threadIdx.x != 0) return;
   best = arg_max(arg_max(s_best[0], s_best[1]), arg_max(s_best[2], s_best[3]));
-  if (best) __hip_atomic_fetch_max(p.keys + row, best, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  wait_memory();
-  if (atomicAdd(p.count + row, 1u) + 1u != gridDim.x) return;
-  p.tokens[row] = arg_col(ld_coherent(p.keys + row));
-  st_coherent(p.keys + row, (uint64_t)0);
-  st_coherent(p.count + row, 0u);
+  if (gridDim.x == 1)
+    tokens[row] = arg_col(best);
+  else
+    keys[(int64_t)row * gridDim.x + blockIdx.x] = best;
+}
+
+__global__ __launch_bounds__(64) void k_int8_argmax_parts(const uint64_t* keys, int parts, int32_t* tokens) {
+  uint64_t best = 0;
+  for (int i = threadIdx.x; i < parts; i += 64) best = arg_max(best, keys[(int64_t)blockIdx.x * parts + i]);
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) best = arg_max(best, __shfl_xor(best, off, 64));
+  if (threadIdx.x == 0) tokens[blockIdx.x] = arg_col(best);
 }
 
 // ======================================================================
@@ -475,6 +477,12 @@ __global__ __launch_bounds__(256) void k_int8_quantise(const T* w, int64_t ldw, 
 }
 
 // ---- host ------------------------------------------------------------------
+// btl_act.hip
+int launch_act(const uint16_t* x, int64_t M, int64_t K, int64_t ldx, const uint16_t* gamma, float norm_eps,
+               int8_t* xa, float* a_dq, int32_t* rowsum, float* act_scale, int8_t* xq_rm, uint16_t* y_rm,
+               uint32_t* zero_words, int n_zero_words, hipStream_t stream);
+int check_act_args(const char* who, const uint16_t* x, int64_t M, int64_t K, int64_t ldx, const uint16_t* gamma);
+
 inline int check_int8_shape(const char* who, int64_t N, int64_t K) {
   if (N <= 0 || N > (1 << 24)) return set_error(BTL_ERR_SHAPE, "%s: N=%lld", who, (long long)N);
   if (K <= 0 || K % 16 || K > BTL_MAX_K)
@@ -535,6 +543,23 @@ static int tile_choice(int64_t M, int64_t N, int64_t K, int cus) {
 
 constexpr int kFewRows8 = 64;     // of the weight stream
 constexpr int kHeadRows = 65535;  // a grid's second dimension
+constexpr int kHeadWords = kFewRows8 * 2 + 1;  // few rows: keys and count, which the quantisation clears
+
+// A head call's scratch: byte offsets (few rows: the cleared words first), parts of a row for its argmax.
+struct HeadScratch {
+  int64_t codes, blocked, scale, keys, total, parts;
+};
+static HeadScratch head_scratch(int64_t M, int64_t K, int64_t N) {
+  HeadScratch h;
+  h.codes = 1024;
+  h.blocked = round_up(h.codes + M * K, 256);
+  h.scale = round_up(h.blocked + btl_act_bytes(M, K), 256);
+  h.keys = round_up(h.scale + round_up(M, 32) * 4, 256);
+  // about four workgroups a CU
+  h.parts = M <= kFewRows8 ? 1 : std::max((int64_t)1, std::min((4 * (int64_t)device_cus() + M - 1) / M, (N + 2047) / 2048));
+  h.total = h.keys + (h.parts > 1 ? M * h.parts * 8 : 0);
+  return h;
+}
 
 // Checks that the entry points share; fills what they share.
 static int int8_args(const char* who, const int8_t* a, int64_t lda, const float* a_scale, int64_t M, int64_t K, int64_t N,
@@ -637,33 +662,55 @@ int btl_int8_matmul(const int8_t* a, int64_t lda, const float* a_scale, int64_t 
   return int8_launch(who, p, (hipStream_t)stream);
 }
 
-int64_t btl_int8_head_workspace_bytes(int64_t M) { return M > 0 && M <= kHeadRows ? round_up(M, 64) * 12 : 0; }
+int64_t btl_int8_head_scratch_bytes(int64_t M, int64_t K, int64_t N) {
+  if (M <= 0 || M > kHeadRows || K <= 0 || K % 32 || K > BTL_MAX_K || N <= 0 || N > (1 << 24)) return 0;
+  return head_scratch(M, K, N).total;
+}
 
-int btl_int8_head(const int8_t* a, int64_t lda, const float* a_scale, int64_t M, int64_t K, int64_t N, const uint8_t* wdev,
-                  const float* w_scale, float* logits, int64_t ldo, int32_t* tokens, void* workspace, size_t workspace_bytes,
+int btl_int8_head(const uint16_t* x, int64_t M, int64_t K, int64_t N, const uint16_t* gamma, float norm_eps, const uint8_t* wdev,
+                  const float* w_scale, uint16_t* normed, float* logits, int32_t* tokens, void* scratch, size_t scratch_bytes,
                   btl_stream_t stream) {
   const char* who = "btl_int8_head";
   clear_error();
-  Int8Args p{};
-  const int rc = int8_args(who, a, lda, a_scale, M, K, N, wdev, w_scale, logits, ldo, 1, &p);
+  if (M < 0 || M > kHeadRows) return set_error(BTL_ERR_SHAPE, "%s: M=%lld (up to %d)", who, (long long)M, kHeadRows);
+  int rc = check_int8_shape(who, N, K);
   if (rc != BTL_OK || M == 0) return rc;
-  if (M > kHeadRows) return set_error(BTL_ERR_SHAPE, "%s: M=%lld (up to %d)", who, (long long)M, kHeadRows);
-  if (!tokens || !workspace || (!logits && M > kFewRows8)) return set_error(BTL_ERR_NULL, "%s: NULL pointer", who);
-  if (!aligned(tokens, 4) || !aligned(workspace, 256)) return set_error(BTL_ERR_ALIGN, "%s: misaligned buffer", who);
-  if ((int64_t)workspace_bytes < btl_int8_head_workspace_bytes(M))
-    return set_error(BTL_ERR_WORKSPACE, "%s: workspace %zu < %lld bytes", who, workspace_bytes,
-                     (long long)btl_int8_head_workspace_bytes(M));
-  p.count = reinterpret_cast<uint32_t*>(static_cast<char*>(workspace));
-  p.keys = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + round_up(M, 64) * 4);
-  if (M <= kFewRows8) p.tokens = tokens;
-  const int launched = int8_launch(who, p, (hipStream_t)stream);
-  if (launched != BTL_OK || M <= kFewRows8) return launched;
-  p.tokens = tokens;
-  // parts of a row, about four workgroups a CU
-  const int64_t parts = std::max((int64_t)1, std::min((4 * (int64_t)device_cus() + M - 1) / M, (N + 2047) / 2048));
-  const int each = (int)((N + parts - 1) / parts);
-  hipLaunchKernelGGL(k_int8_argmax, dim3((unsigned)((N + each - 1) / each), (unsigned)M), dim3(256), 0, (hipStream_t)stream, logits,
-                     ldo, (int)N, each, p);
+  rc = check_act_args(who, x, M, K, K, gamma);
+  if (rc != BTL_OK) return rc;
+  if (!gamma || !wdev || !w_scale || !tokens || !scratch || (!logits && M > kFewRows8))
+    return set_error(BTL_ERR_NULL, "%s: NULL pointer", who);
+  if (!aligned(tokens, 4) || !aligned(normed, 16) || !aligned(scratch, 256))
+    return set_error(BTL_ERR_ALIGN, "%s: misaligned buffer", who);
+  const HeadScratch h = head_scratch(M, K, N);
+  if ((int64_t)scratch_bytes < h.total)
+    return set_error(BTL_ERR_WORKSPACE, "%s: scratch %zu < %lld bytes", who, scratch_bytes, (long long)h.total);
+  char* const at = static_cast<char*>(scratch);
+  int8_t* const codes = reinterpret_cast<int8_t*>(at + h.codes);
+  float* const a_scale = reinterpret_cast<float*>(at + h.scale);
+  Int8Args p{};
+  rc = int8_args(who, codes, K, a_scale, M, K, N, wdev, w_scale, logits, N, 1, &p);
+  if (rc != BTL_OK) return rc;
+  const bool few = M <= kFewRows8;
+  hipStream_t s = (hipStream_t)stream;
+  rc = launch_act(x, M, K, K, gamma, norm_eps, reinterpret_cast<int8_t*>(at + h.blocked), a_scale, nullptr, nullptr, codes, normed,
+                  reinterpret_cast<uint32_t*>(at), few ? kHeadWords : 0, s);
+  if (rc != BTL_OK) return rc;
+  if (few) {
+    p.tokens = tokens;
+    p.keys = reinterpret_cast<uint64_t*>(at);
+    p.count = reinterpret_cast<uint32_t*>(at + kFewRows8 * 8);
+    return int8_launch(who, p, s);
+  }
+  rc = int8_launch(who, p, s);
+  if (rc != BTL_OK) return rc;
+  uint64_t* const keys = reinterpret_cast<uint64_t*>(at + h.keys);
+  const int each = (int)((N + h.parts - 1) / h.parts), parts = (int)((N + each - 1) / each);
+  hipLaunchKernelGGL(k_int8_argmax, dim3((unsigned)parts, (unsigned)M), dim3(256), 0, s, logits, N, (int)N, each, keys, tokens);
+  if (parts > 1) {
+    rc = check_launch(who);
+    if (rc != BTL_OK) return rc;
+    hipLaunchKernelGGL(k_int8_argmax_parts, dim3((unsigned)M), dim3(64), 0, s, keys, parts, tokens);
+  }
   return check_launch(who);
 }
 

@@ -394,14 +394,16 @@ int btl_int8_weight_quantise(const void* w, int bf16, int64_t ldw, int64_t N, in
 int btl_int8_matmul(const int8_t* a, int64_t lda, const float* a_scale, int64_t M, int64_t K, int64_t N,
                     const uint8_t* wdev, const float* w_scale, void* out, int64_t ldo, int out_f32, btl_stream_t stream);
 
-/* The LM head of 8-bit integers: the product as logits [M, N] fp32 (row stride ldo; may be NULL for M <= 64)
- * and tokens [M], the first index of each row's largest logit (NaNs ignored; -1 where there is nothing else).
- * M up to 65535.  workspace: btl_int8_head_workspace_bytes(M) bytes, 256-byte aligned, zero before its
- * first call; every completed call leaves it zero.  Calls that may run at once need one each. */
-int64_t btl_int8_head_workspace_bytes(int64_t M);
-int btl_int8_head(const int8_t* a, int64_t lda, const float* a_scale, int64_t M, int64_t K, int64_t N,
-                  const uint8_t* wdev, const float* w_scale, float* logits, int64_t ldo, int32_t* tokens,
-                  void* workspace, size_t workspace_bytes, btl_stream_t stream);
+/* The LM head of 8-bit integers: x [M, K] bf16 normed by gamma (btl_rmsnorm) and quantised per row
+ * (btl_quant_absmax), the product as logits [M, N] fp32 (may be NULL for M <= 64), and tokens [M], the first
+ * index of each row's largest logit (NaNs ignored; -1 where there is nothing else).  normed [M, K] bf16: the
+ * normed rows, if wanted.  K a multiple of 32, M up to 65535.  scratch: btl_int8_head_scratch_bytes
+ * bytes, 256-byte aligned, on the same device; its content is neither read nor kept, and calls that may run at
+ * once need one each. */
+int64_t btl_int8_head_scratch_bytes(int64_t M, int64_t K, int64_t N);
+int btl_int8_head(const uint16_t* x, int64_t M, int64_t K, int64_t N, const uint16_t* gamma, float norm_eps,
+                  const uint8_t* wdev, const float* w_scale, uint16_t* normed, float* logits, int32_t* tokens,
+                  void* scratch, size_t scratch_bytes, btl_stream_t stream);
 
 /* ---- decode attention between QKV and o_proj --------------------------
  * Replaces the decode attention of src/bitnet_tt/layers/attention.py:

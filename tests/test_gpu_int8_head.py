@@ -9,7 +9,6 @@ import torch
 
 from paged_helpers import dev, gen, normal
 
-from bitnet_tt import _native as N
 from bitnet_tt.int8_matmul import int8_matmul, quantize_rows
 from bitnet_tt.lm_head import LMHead
 
@@ -47,6 +46,19 @@ def test_logits_and_tokens(M, K, V):
     assert torch.equal(q, q2) and torch.equal(s, s2)
     none, again = head(x, return_logits=False)
     assert none is None and torch.equal(again, tokens)
+
+
+@pytest.mark.parametrize("M", [1023, 1024, 1025, 1090, 2047, 2112])
+def test_many_rows_without_logits(M):
+    """Passes over the rows that share a buffer, the last one short."""
+    head = head_of(32, 9000)
+    x = normal((M, 32), 3).to(torch.bfloat16).to(dev())
+    normed = torch.zeros_like(x)
+    _, tokens = head(x, return_logits=False, normed_out=normed)
+    all_normed = torch.zeros_like(x)
+    logits, want = head(x, normed_out=all_normed)
+    assert torch.equal(tokens, want) and torch.equal(normed, all_normed)
+    assert tokens.tolist() == first_max(logits)
 
 
 @pytest.mark.parametrize("M", [2, 100])
@@ -98,46 +110,35 @@ def test_columns_that_are_not_numbers(M):
     assert tokens.tolist() == first_max(logits)
 
 
-def test_captured_replays_and_a_clean_workspace():
-    """One workspace for calls of different numbers of rows; it is zero after each."""
+def test_two_graphs_at_once():
+    """Captured on one stream, replayed on two: each call has its own scratch.  Eager calls between."""
     K, V = 512, 5000
     head = head_of(K, V)
-    xs = {M: normal((M, K), 20 + M).to(torch.bfloat16).to(dev()) for M in (32, 5, 200)}
+    runs = []
     stream = torch.cuda.Stream()
     stream.wait_stream(torch.cuda.current_stream())
-    graphs = {}
     with torch.cuda.stream(stream):
-        for M, x in xs.items():
-            head(x)
-        for M, x in xs.items():
+        for M in (32, 31, 200, 199):
+            x = normal((M, K), 20 + M).to(torch.bfloat16).to(dev())
             g = torch.cuda.CUDAGraph()
             with torch.cuda.graph(g, stream=stream):
-                graphs[M] = (g, head(x))
-    want = {M: head(x) for M, x in xs.items()}
-    for _ in range(3):
-        for M, (g, (logits, tokens)) in graphs.items():
+                out = head(x)
+            runs.append((x, g, out, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    want = [head(x) for x, _, _, _ in runs]
+    for _ in range(4):
+        for _, _, (logits, tokens), _ in runs:
             logits.fill_(-7)
             tokens.fill_(-7)
-            torch.cuda.synchronize()
-            with torch.cuda.stream(stream):
+        torch.cuda.synchronize()
+        for _, g, _, s in runs:
+            with torch.cuda.stream(s):
                 g.replay()
-            torch.cuda.synchronize()
-            assert torch.equal(logits, want[M][0]) and torch.equal(tokens, want[M][1])
-    for key, ws in N._workspaces.items():
-        if key[0] == "int8_head":
-            assert not bool(ws.any())
-
-
-def test_a_capture_needs_a_workspace():
-    head = head_of(64, 100)
-    x = normal((4, 64), 3).to(torch.bfloat16).to(dev())
-    stream = torch.cuda.Stream()
-    stream.wait_stream(torch.cuda.current_stream())
-    with torch.cuda.stream(stream):
-        g = torch.cuda.CUDAGraph()
-        with pytest.raises(RuntimeError, match="eager head call"):
-            with torch.cuda.graph(g, stream=stream):
-                head(x)
+        again = head(runs[0][0])
+        torch.cuda.synchronize()
+        assert torch.equal(again[1], want[0][1])
+        for (_, _, (logits, tokens), _), (l, t) in zip(runs, want):
+            assert torch.equal(logits, l) and torch.equal(tokens, t)
 
 
 def test_full_vocabulary():

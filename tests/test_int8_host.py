@@ -24,30 +24,31 @@ def matmul(L, **kw):
 
 
 def head(L, **kw):
-    a = dict(a=FAKE, lda=64, sa=FAKE, M=4, K=64, N=10, w=FAKE, sw=FAKE, out=FAKE, ldo=10, tokens=FAKE, ws=FAKE, nbytes=1 << 20,
-             stream=None)
+    a = dict(x=FAKE, M=4, K=64, N=10, gamma=FAKE, eps=1e-5, w=FAKE, sw=FAKE, normed=None, out=FAKE, tokens=FAKE, scratch=FAKE,
+             nbytes=1 << 40, stream=None)
     a.update(kw)
     return L.btl_int8_head(*a.values())
 
 
-SHARED = [
+@pytest.mark.parametrize("want,kw", [
     (SHAPE, dict(K=0)), (SHAPE, dict(K=24)), (SHAPE, dict(K=16400, lda=16400)), (SHAPE, dict(N=0)), (SHAPE, dict(N=(1 << 24) + 1)),
     (SHAPE, dict(M=-1)), (SHAPE, dict(M=(1 << 24) + 1)), (SHAPE, dict(lda=48)), (SHAPE, dict(lda=(1 << 22) + 16)),
     (SHAPE, dict(ldo=9)), (ALIGN, dict(lda=72)), (ALIGN, dict(a=FAKE + 8)), (ALIGN, dict(w=FAKE + 8)), (ALIGN, dict(out=FAKE + 2)),
     (ALIGN, dict(sa=FAKE + 1)), (ALIGN, dict(sw=FAKE + 2)), (NULL, dict(a=None)), (NULL, dict(sa=None)), (NULL, dict(w=None)),
     (NULL, dict(sw=None)), (SHAPE, dict(M=1 << 24, N=1 << 24, ldo=1 << 24)),
-]
-
-
-@pytest.mark.parametrize("want,kw", SHARED + [(NULL, dict(out=None)), (ALIGN, dict(out=FAKE + 1, f32=0))])
+    (NULL, dict(out=None)), (ALIGN, dict(out=FAKE + 1, f32=0)),
+])
 def test_matmul_refuses(L, want, kw):
     assert matmul(L, **kw) == want
     assert b"btl_int8_matmul" in L.btl_last_error()
 
 
-@pytest.mark.parametrize("want,kw", SHARED + [
-    (SHAPE, dict(M=65536)), (NULL, dict(tokens=None)), (NULL, dict(ws=None)), (NULL, dict(out=None, M=65)),
-    (ALIGN, dict(ws=FAKE + 64)), (ALIGN, dict(tokens=FAKE + 2)), (WORKSPACE, dict(nbytes=767)),
+@pytest.mark.parametrize("want,kw", [
+    (SHAPE, dict(M=65536)), (SHAPE, dict(M=-1)), (SHAPE, dict(K=0)), (SHAPE, dict(K=48)), (SHAPE, dict(K=16416)), (SHAPE, dict(N=0)),
+    (SHAPE, dict(N=(1 << 24) + 1)), (NULL, dict(x=None)), (NULL, dict(gamma=None)), (NULL, dict(w=None)), (NULL, dict(sw=None)),
+    (NULL, dict(tokens=None)), (NULL, dict(scratch=None)), (NULL, dict(out=None, M=65)), (ALIGN, dict(x=FAKE + 8)),
+    (ALIGN, dict(gamma=FAKE + 2)), (ALIGN, dict(normed=FAKE + 8)), (ALIGN, dict(scratch=FAKE + 64)), (ALIGN, dict(tokens=FAKE + 2)),
+    (ALIGN, dict(w=FAKE + 8)), (ALIGN, dict(sw=FAKE + 2)), (ALIGN, dict(out=FAKE + 2)), (WORKSPACE, dict(nbytes=1024)),
 ])
 def test_head_refuses(L, want, kw):
     assert head(L, **kw) == want
@@ -55,15 +56,18 @@ def test_head_refuses(L, want, kw):
 
 
 def test_no_rows_is_no_launch(L):
-    assert matmul(L, M=0, a=None, out=None) == 0 and head(L, M=0, a=None) == 0
+    assert matmul(L, M=0, a=None, out=None) == 0 and head(L, M=0, x=None) == 0
 
 
 def test_sizes(L):
     f = L.btl_int8_weight_bytes
     assert f(128256, 2560) == 128256 * 2560 and f(1, 16) == 1024 and f(17, 80) == 2 * 2 * 1024
     assert f(10, 8) == 0 and f(10, 16400) == 0 and f(0, 64) == 0 and f(-5, 64) == 0 and f((1 << 24) + 1, 64) == 0
-    g = L.btl_int8_head_workspace_bytes
-    assert g(1) == g(64) == 768 and g(65) == 1536 and g(0) == 0 and g(65536) == 0 and g(65535) == 65536 * 12
+    g = L.btl_int8_head_scratch_bytes
+    for bad in ((0, 64, 10), (65536, 64, 10), (4, 48, 10), (4, 16416, 10), (4, 64, 0), (-1, 64, 10), (4, 64, (1 << 24) + 1)):
+        assert g(*bad) == 0
+    for M in (1, 64, 65, 1000, 65535):  # the cleared words, codes twice, scales
+        assert g(M, 2560, 128256) >= 1024 + M * 2560 + L.btl_act_bytes(M, 2560) + 4 * M
 
 
 @pytest.mark.parametrize("want,kw", [
