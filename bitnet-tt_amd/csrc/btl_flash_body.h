@@ -768,10 +768,33 @@ __device__ __forceinline__ void tile_item(const FlashArgs& p, uint8_t* smem, int
                      f2bf_pair(s.o[t][4 * i + 2] * inv, s.o[t][4 * i + 3] * inv));
 }
 
+// Workgroup x of units of `each` items that read the same keys and values: those are x's of one remainder by 8, which
+// share an L2 (a workgroup's XCD is its number's remainder), close to one another in time.
+constexpr int kXcds = 8;
+struct UnitItem {
+  int unit, item;
+};
+__device__ __forceinline__ UnitItem unit_item(int x, int each) {
+  const int i = x / kXcds;
+  return {uni(i / each * kXcds + x % kXcds), uni(i % each)};
+}
+inline int64_t unit_groups(int64_t units, int64_t each) { return (units + kXcds - 1) / kXcds * kXcds * each; }
+
+// kWindow: neighbouring tiles of a head see mostly the same positions.
+constexpr int kNeighbours = 16;
+
 template <int D, int KV, int MODE>
 __global__ __launch_bounds__(256, 2) void k_flash_tile(FlashArgs p) {
   __shared__ __attribute__((aligned(16))) uint8_t smem[kTileShared<D>];
-  tile_item<D, KV, MODE>(p, smem, uni(blockIdx.x % p.Hkv), blockIdx.x / p.Hkv, blockIdx.y);
+  if (MODE == kWindow) {
+    const UnitItem u = unit_item(blockIdx.x, kNeighbours);
+    tile_item<D, KV, MODE>(p, smem, uni(u.unit % p.Hkv), u.unit / p.Hkv * kNeighbours + u.item, blockIdx.y);
+  } else {
+    tile_item<D, KV, MODE>(p, smem, uni(blockIdx.x % p.Hkv), blockIdx.x / p.Hkv, blockIdx.y);
+  }
+}
+inline int64_t window_groups(int64_t tiles, int64_t Hkv) {  // tiles: of all heads
+  return unit_groups((tiles / Hkv + kNeighbours - 1) / kNeighbours * Hkv, kNeighbours);
 }
 
 // ======================================================================

@@ -188,7 +188,7 @@ inline int partials(const char* who, void* scratch, size_t bytes, int64_t need, 
 
 template <int MODE>
 inline int launch_prompt(const char* what, const FlashArgs& a, int64_t tiles, int64_t D, hipStream_t stream) {
-  const dim3 grid((unsigned)tiles);
+  const dim3 grid((unsigned)(MODE == kWindow ? window_groups(tiles, a.Hkv) : tiles));
   if (D == 128)
     hipLaunchKernelGGL((k_flash_tile<128, kDense, MODE>), grid, dim3(256), 0, stream, a);
   else
@@ -212,7 +212,7 @@ inline int launch_paged(const char* who, const char* what, const FlashPlan& f, F
                           : (fp8 ? k_flash_few<64, kPagedFp8, MODE> : k_flash_few<64, kPagedBf16, MODE>);
     hipLaunchKernelGGL(kern, grid, dim3(64 * kFewWaves), 0, stream, *a);
   } else {
-    const dim3 grid((unsigned)f.tiles, (unsigned)f.splits);
+    const dim3 grid((unsigned)(MODE == kWindow ? window_groups(f.tiles, a->Hkv) : f.tiles), (unsigned)f.splits);
     auto* kern = D == 128 ? (fp8 ? k_flash_tile<128, kPagedFp8, MODE> : k_flash_tile<128, kPagedBf16, MODE>)
                           : (fp8 ? k_flash_tile<64, kPagedFp8, MODE> : k_flash_tile<64, kPagedBf16, MODE>);
     hipLaunchKernelGGL(kern, grid, dim3(256), 0, stream, *a);

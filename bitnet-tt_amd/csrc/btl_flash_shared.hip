@@ -19,10 +19,13 @@ __global__ __launch_bounds__(256, 2) void k_flash_shared(FlashArgs p, int shared
   constexpr int kFewBytes = (int)sizeof(FewShared<D>);
   constexpr int kBytes = SHARED_FEW && OWN_FEW ? kFewBytes : kFewBytes > kTileShared<D> ? kFewBytes : kTileShared<D>;
   __shared__ __attribute__((aligned(16))) uint8_t smem[kBytes];
-  const int shared = shared_items * p.Hkv * p.shared_splits;
+  const int units = p.Hkv * p.shared_splits, shared = (units + kXcds - 1) / kXcds * kXcds * shared_items;
   int x = blockIdx.x;
   if (x < shared) {
-    const int hk = uni(x % p.Hkv), y = x / p.Hkv, item = uni(y % shared_items), split = uni(y / shared_items);
+    // the tiles of a head's split read the same pages
+    const UnitItem u = unit_item(x, shared_items);
+    if (u.unit >= units) return;
+    const int hk = uni(u.unit % p.Hkv), split = uni(u.unit / p.Hkv), item = u.item;
     if constexpr (SHARED_FEW)
       few_item<D, KV, kShared>(p, *reinterpret_cast<FewShared<D>*>(smem), hk, 0, split);
     else
@@ -115,7 +118,7 @@ int btl_shared_prefix_attention(const uint16_t* q, int64_t ldq, int64_t T, int64
   const bool fp8 = pages->k_exp != nullptr;
   const SharedPlan s = shared_plan(T, H, Hkv, D, B, max_q, max_kv, max_shared);
   const int parts = s.shared_splits + s.own.splits;
-  const int64_t groups = (s.shared_items * s.shared_splits + s.own_items * s.own.splits) * Hkv;
+  const int64_t groups = unit_groups(s.shared_splits * Hkv, s.shared_items) + s.own_items * s.own.splits * Hkv;
   if (groups > INT32_MAX) return set_error(BTL_ERR_SHAPE, "%s: T=%lld B=%lld", who, (long long)T, (long long)B);
   rc = partials(who, scratch, scratch_bytes, shared_scratch(s, T, H, D), (int64_t)parts * T * H * D, &a);
   if (rc != BTL_OK) return rc;
