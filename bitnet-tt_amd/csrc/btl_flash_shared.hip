@@ -48,20 +48,46 @@ struct SharedPlan {
 };
 
 // max_kv: positions of the longest sequence, max_shared of them shared.
+//  - The shared positions in tiles: up to one workgroup a CU (a call has the sequences' own workgroups besides), unless
+//    the tiles alone are more; of these the split that costs least, P steps of a / n us and n partials of T H D 8 bytes:
+//    n = sqrt(a P / part) with a = 0.0085 us, a fitted constant, as what a step takes depends on the workgroups
+//    beside it.  20 / 5 heads of 128, bf16, us at about half of n / n / double: 32 users, 8192 positions (n = 23):
+//    27, 23, 25; 64, 16384 (23): 44, 42, 43; 64, 4096 (11): 24, 22, 22; 16, 8192 (32): 22, 23, 23; 48, 30000 (25): 66, 54, 69;
+//    16 x 5 rows, 16000 (17): 39, 41, 42; 32 x 4, 4096 (8): 27, 25, 29; 10 x 12, 2000 (5): 24, 24, 27.  8-bit pages, 32
+//    users, 8192 (23): 28, 25, 24; 64, 16384 (23): 45, 37, 43; 64, 65536 (25): 125, 93, 97.  A chunk is at least two steps.
+//  - Few rows in all: as for a call without a prefix.
+//  - Their own positions: the merge's launch is paid in any case, so that splits that fill two workgroups a CU pay from 512
+//    positions on: 16 users of 8192 + 1000, n = 1 / 2: 21.7, 19.5; 16 x 5 rows of 16000 + 1000, 1 / 2 / 4: 41, 39, 34.
 inline SharedPlan shared_plan(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t B, int64_t max_q, int64_t max_kv,
                               int64_t max_shared) {
   SharedPlan s{};
-  const int64_t G = H / Hkv;
+  const int64_t G = H / Hkv, cus = device_cus();
   // (both parts' ends together stay below 2^31)
-  max_shared = std::min(max_shared, kMaxPositions);
+  max_shared = std::max(std::min(max_shared, kMaxPositions), (int64_t)1);
   const int64_t own = std::min(std::max(max_kv - max_shared, (int64_t)1), kMaxPositions / 2);
   s.own = flash_plan(T, H, Hkv, D, B, max_q, own, true);
   s.own_items = s.own.few ? B : s.own.tiles / Hkv;
   s.shared_few = T * G <= kFewRows && s.own.few;
-  const FlashPlan f = flash_plan(T, H, Hkv, D, 1, s.shared_few ? 1 : T, std::max(max_shared, (int64_t)1), true);
   s.shared_items = s.shared_few ? 1 : (T * G + kTileRows - 1) / kTileRows;
-  s.shared_splits = f.splits;
-  s.shared_chunk = f.chunk;
+  const int64_t tiles = s.shared_items * Hkv;
+  if (s.shared_few) {
+    const FlashPlan f = flash_plan(T, H, Hkv, D, 1, 1, max_shared, true);
+    s.shared_splits = f.splits;
+    s.shared_chunk = f.chunk;
+  } else {
+    const double part = 1.67e-6 * (double)(T * H * D);
+    int64_t n = (int64_t)(std::sqrt(0.0085 * (double)max_shared / part) + 0.5);
+    n = std::min(n, 2 * tiles <= cus ? cus / tiles : (4 * cus + tiles) / (2 * tiles));
+    n = std::max((int64_t)1, std::min(n, std::min(max_shared / (2 * kStep), kMaxSplits)));
+    s.shared_chunk = (int)round_up((max_shared + n - 1) / n, kStep);
+    s.shared_splits = (int)((max_shared + s.shared_chunk - 1) / s.shared_chunk);
+  }
+  const int64_t rest = (2 * cus - tiles * s.shared_splits) / (s.own_items * Hkv);
+  const int64_t n = std::min(rest, std::min(own / kMinChunk, kMaxSplits));
+  if (n > s.own.splits) {
+    s.own.chunk = (int)round_up((own + n - 1) / n, kMinChunk);
+    s.own.splits = (int)((own + s.own.chunk - 1) / s.own.chunk);
+  }
   return s;
 }
 

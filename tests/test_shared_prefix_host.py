@@ -62,7 +62,7 @@ def test_plan_of_any_hint(L, T, B, max_q, D):
         for max_shared in (0, 16, 1000, 65536, 2 ** 30, 2 ** 31, 2 ** 63 - 1):
             sizes = (T, 20, 5, D, B, max_q, max_kv, max_shared)
             few, n, chunk, own_few, own_n, own_chunk = plan(L, *sizes)
-            assert 1 <= n <= 256 and 256 <= chunk and n * chunk < 2 ** 31
+            assert 1 <= n <= 256 and 64 <= chunk and n * chunk < 2 ** 31
             assert 1 <= own_n <= 256 and 256 <= own_chunk and 2 ** 30 + own_n * own_chunk < 2 ** 31
             assert n * chunk >= min(max_shared, 2 ** 30 - 1)
             assert own_few == (min(max_q, T) * 4 <= 16) and few == (T * 4 <= 16 and own_few)
