@@ -162,7 +162,10 @@ def prepare(case, seed):
         s = {"case": case, "a": a, "a_scale": 0.01 + 0.02 * normal(M).abs(), "w": w,
              "w_scale": 0.0005 + 0.0002 * normal(N).abs()}
         if own:
-            s["weight"] = _package("int8_matmul").Int8Weight.from_codes(w, s["w_scale"])
+            _package()
+            from bitnet_tt.int8_matmul import Int8Weight
+
+            s["weight"] = Int8Weight.from_codes(w, s["w_scale"])
         return s
     H, Hkv, D = case["heads"], case["kv_heads"], case["dim"]
     new, total = _sizes(case)
@@ -316,21 +319,22 @@ def _int8(s):
     return y if s["case"]["out"] == "fp32" else y.to(torch.bfloat16)
 
 
-def _package(name):
+def _package():
     if _PKG not in sys.path:
         sys.path.insert(0, _PKG)
-    import importlib
-
-    return importlib.import_module("bitnet_tt." + name)
 
 
 def _own(s):
     """The calls of the package."""
+    _package()
     c = s["case"]
     if c["op"] == "int8":
+        from bitnet_tt.int8_matmul import int8_matmul
+
         out = torch.float32 if c["out"] == "fp32" else torch.bfloat16
-        return _package("int8_matmul").int8_matmul(s["a"], s["a_scale"], s["weight"], out_dtype=out)
-    pa = _package("paged_attention")
+        return int8_matmul(s["a"], s["a_scale"], s["weight"], out_dtype=out)
+    from bitnet_tt import paged_attention as pa
+
     if c["op"] == "win_prompt":
         q, k, v = _split(s)
         return pa.prompt_attention(q, k, v, s["cu_q"], scale=s["scale"], max_q=s["max_q"], window=c["window"],
