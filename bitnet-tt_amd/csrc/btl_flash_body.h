@@ -90,13 +90,13 @@ struct FlashArgs {
   int shared_splits, shared_chunk;
 };
 
-// What some of a tile's rows see through their windows, as one axis of whole steps: the
-// sinks' steps, then from `lo`, the first position of the first row's window, on.  `gap` positions that no
+// What some of a tile's rows see through their windows, as one axis: the sinks (over pages, in whole
+// steps), then from `lo`, the first position of the first row's window, on.  `gap` positions that no
 // row sees lie between the two; they are not loaded, nor are their pages looked up.
 struct Span {
   int lo, sinks, end;  // positions: end is behind the last
   int turn, gap;       // the axis leaves the sinks at `turn`
-  // align: what a step's first position must be a multiple of; step and align are powers of two
+  // step: what `turn`, and align: what a step's first position must be a multiple of; powers of two
   __device__ __forceinline__ void init(const FlashArgs& p, int first_row, int end_, int step, int align) {
     lo = uni(max(0, first_row - p.window + 1));
     sinks = p.sinks;
@@ -105,6 +105,8 @@ struct Span {
     gap = uni(max(0, (lo & -align) - turn));
   }
   __device__ __forceinline__ int pos(int u) const { return u < turn ? u : u + gap; }
+  // Whether a step has both sinks and positions of the windows (rows that are packed: any of them).
+  __device__ __forceinline__ bool mixed(int u, int n) const { return gap > 0 && u < turn && u + n > turn; }
   // Where the positions that are to be loaded end, of n from `at`.
   __device__ __forceinline__ int end_of(int at, int n) const { return at + n <= lo ? sinks : end; }
 };
@@ -332,6 +334,20 @@ struct Source {
     const int kv = pos(u);
     if (KV == kDense) {
       const uint32_t ld = (uint32_t)(VAL ? ldv : ldk);
+      if (MODE == kWindow && span.mixed(u, kStep)) {
+        const uint8_t* const rows = (VAL ? v : k) + u * (VAL ? ldv : ldk);
+        const int sinks = span.turn - u;  // rows of the step
+        const auto s = buf_rsrc(rows, (uint32_t)sinks * ld);
+        const auto w = buf_rsrc(rows + span.gap * (VAL ? ldv : ldk), (uint32_t)min(span.end - span.gap - u, kStep) * ld);
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+          if (i * kRpl + my_row < sinks)
+            piece<VAL>(s, i, dst);
+          else
+            piece<VAL>(w, i, dst);
+        }
+        return;
+      }
       const int n = MODE == kWindow ? clampi(end_of(kv, kStep) - kv, 0, kStep) : min(kv_end - kv, kStep);
       const auto r = buf_rsrc((VAL ? v : k) + kv * (VAL ? ldv : ldk), (uint32_t)n * ld);
 #pragma unroll
@@ -438,14 +454,18 @@ __device__ __forceinline__ void tile_scores(const lds8* ks, TileKeys& a, const T
 // The lowest n bits (n <= 0: none, n >= 32: all).
 __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? ~0u : (1u << max(n, 0)) - 1u; }
 
+// (kWindow: kv is a place on the axis.)
 template <int D, int MODE>
-__device__ __forceinline__ void tile_mask(const FlashArgs& p, const TileState<D>& s, int kv, v16f (&sc)[2]) {
+__device__ __forceinline__ void tile_mask(const FlashArgs& p, const Span& span, const TileState<D>& s, int kv, v16f (&sc)[2]) {
   const int h = __lane_id() >> 5;
   if (MODE == kWindow) {  // a bit a position: three conditions a score would want more scalar registers than there are
-    const int at = max(s.limit - kv - 4 * h, -1), sink = p.sinks - kv - 4 * h;
+    const int from = (span.gap > 0 ? span.turn : span.sinks) - kv - 4 * h;  // the windows' part of the axis
+    const int sink = min(s.limit + 1, span.sinks) - kv - 4 * h;
+    const int end = max(s.limit + 1 - span.gap - kv - 4 * h, 0);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const uint32_t see = low_bits(at + 1 - 32 * t) & (~low_bits(at + 1 - p.window - 32 * t) | low_bits(sink - 32 * t));
+      const uint32_t see = low_bits(sink - 32 * t) |
+                           (low_bits(end - 32 * t) & ~low_bits(end - p.window - 32 * t) & ~low_bits(from - 32 * t));
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int keep = __builtin_amdgcn_sbfe((int)see, c_row(r, 0), 1);
@@ -526,11 +546,11 @@ __device__ __forceinline__ void tile_values(const lds8* __restrict__ vs, TileSta
 // values that are not finite: those are added to the rows that see them, and
 // then cleared for the product.
 template <int D, int MODE>
-__device__ __forceinline__ void add_not_finite(const FlashArgs& p, const lds8* vs, TileState<D>& s, int kv) {
+__device__ __forceinline__ void add_not_finite(const FlashArgs& p, const Span& span, const lds8* vs, TileState<D>& s, int kv) {
   const int h = __lane_id() >> 5;
 #pragma unroll 1
   for (int j = 0; j < kStep; ++j) {
-    const bool seen = sees<MODE>(p, s.limit, kv + j);
+    const bool seen = sees<MODE>(p, s.limit, MODE == kWindow ? span.pos(kv + j) : kv + j);
 #pragma unroll
     for (int t = 0; t < D / 32; ++t)
 #pragma unroll
@@ -550,7 +570,8 @@ __device__ __forceinline__ void add_not_finite(const FlashArgs& p, const lds8* v
 
 // The tile's part of it: whether there are such values is asked by all waves together.
 template <int D, int MODE>
-__device__ __forceinline__ void tile_not_finite(const FlashArgs& p, lds8* vs, int* s_flag, TileState<D>& s, int pos, bool mine) {
+__device__ __forceinline__ void tile_not_finite(const FlashArgs& p, const Span& span, lds8* vs, int* s_flag, TileState<D>& s,
+                                                int kv, bool mine) {
   const int tid = threadIdx.x;
   bool nf = false;
 #pragma unroll
@@ -559,7 +580,7 @@ __device__ __forceinline__ void tile_not_finite(const FlashArgs& p, lds8* vs, in
   if ((tid & 63) == 0) s_flag[uni(tid >> 6)] = any;
   lds_barrier();
   if (!(s_flag[0] | s_flag[1] | s_flag[2] | s_flag[3])) return;
-  if (mine) add_not_finite<D, MODE>(p, vs, s, pos);
+  if (mine) add_not_finite<D, MODE>(p, span, vs, s, kv);
   lds_barrier();
 #pragma unroll
   for (int i = 0; i < Tile<D>::kLoads; ++i) {
@@ -620,7 +641,7 @@ __device__ __forceinline__ void tile_item(const FlashArgs& p, uint8_t* smem, int
   int kv0 = begin;
   Source<D, KV, MODE> src;
   if (MODE == kWindow) {  // from here on steps are counted along the axis of what is seen
-    src.span.init(p, first + uni(row_token(r0, p)), kv_end, kStep,
+    src.span.init(p, first + uni(row_token(r0, p)), kv_end, KV == kDense ? 1 : kStep,
                   KV == kDense ? 1 : p.pg.ps.d % kStep == 0 ? kStep : 16);
     kv_end = max(0, kv_end - src.span.gap);
   }
@@ -668,10 +689,17 @@ __device__ __forceinline__ void tile_item(const FlashArgs& p, uint8_t* smem, int
     arrived();
     TileKeys keys;
     v16f sa[2], sb[2];
-    if (some_see<MODE>(p, s.lo, s.hi, src.pos(kv0), kStep)) {
+    // of rows whose limits are in [lo, hi]: whether all see all of the step at u, or some may see some of it
+    auto all_of = [&](int lo, int hi, int u) {
+      return !(MODE == kWindow && src.span.mixed(u, kStep)) && all_see<MODE>(p, lo, hi, src.pos(u), kStep);
+    };
+    auto some_of = [&](int lo, int hi, int u) {
+      return (MODE == kWindow && src.span.mixed(u, kStep)) || some_see<MODE>(p, lo, hi, src.pos(u), kStep);
+    };
+    if (some_of(s.lo, s.hi, kv0)) {
       tile_keys<D>(sm, keys);
       tile_scores<D>(sm, keys, s, sa);
-      if (!all_see<MODE>(p, s.lo, s.hi, src.pos(kv0), kStep)) tile_mask<D, MODE>(p, s, src.pos(kv0), sa);
+      if (!all_of(s.lo, s.hi, kv0)) tile_mask<D, MODE>(p, src.span, s, kv0, sa);
       tile_raise<D>(s, p.c, sa);
     }
     lds_barrier();  // the first keys are read: their stage is free
@@ -704,11 +732,10 @@ __device__ __forceinline__ void tile_item(const FlashArgs& p, uint8_t* smem, int
       lds8 *const k_free = sm + at * kB, *const v_free = sm + (2 + (at ^ 1)) * kB;
       arrived();
       load_ahead(k_free, v_free);
-      const int pos = src.pos(kv), pos2 = src.pos(kv + kStep);
-      const bool mine = some_see<MODE>(p, s.lo, s.hi, pos, kStep);  // some of the wave's rows see some of it
-      const bool next = kv + kStep < kv_end && some_see<MODE>(p, s.lo, s.hi, pos2, kStep);
-      if (!all_see<MODE>(p, wg_lo, wg_hi, pos, kStep))  // some of the tile's rows do not see all of it
-        tile_not_finite<D, MODE>(p, vs, s_flag, s, pos, mine);
+      const bool mine = some_of(s.lo, s.hi, kv);  // some of the wave's rows see some of it
+      const bool next = kv + kStep < kv_end && some_of(s.lo, s.hi, kv + kStep);
+      if (!all_of(wg_lo, wg_hi, kv))  // some of the tile's rows do not see all of it
+        tile_not_finite<D, MODE>(p, src.span, vs, s_flag, s, kv, mine);
       if (mine) {
         v8bf pb[4];
         tile_exp<D>(s, p.c, sa, pb);
@@ -717,7 +744,7 @@ __device__ __forceinline__ void tile_item(const FlashArgs& p, uint8_t* smem, int
       if (next) {
         tile_keys<D>(ks, keys);
         tile_scores<D>(ks, keys, s, sa);
-        if (!all_see<MODE>(p, s.lo, s.hi, pos2, kStep)) tile_mask<D, MODE>(p, s, pos2, sa);
+        if (!all_of(s.lo, s.hi, kv + kStep)) tile_mask<D, MODE>(p, src.span, s, kv + kStep, sa);
         tile_raise<D>(s, p.c, sa);
       }
       store_ahead(k_free, v_free);
@@ -828,13 +855,13 @@ __device__ __forceinline__ int few_swz(int row) {
   return D == 128 ? (2 * row) & 15 : row & 6;
 }
 
-template <int D>
+template <int D, int NW = kFewWaves>
 struct FewShared {
   union {
-    uint8_t v[kFewWaves][32 * 2 * D];       // 32 value rows of a wave
-    float o[kFewWaves][kFewRows][D];        // after the last round
+    uint8_t v[NW][32 * 2 * D];       // 32 value rows of a wave
+    float o[NW][kFewRows][D];        // after the last round
   };
-  float ml[kFewWaves][kFewRows][2];
+  float ml[NW][kFewRows][2];
 };
 
 template <int D, int KV, int MODE>
@@ -953,10 +980,10 @@ __device__ __forceinline__ void few_not_finite(const FlashArgs& p, lds8* vs, v4f
 }
 
 // Sequence b (kShared: the batch as one) and key-value head hk.
-template <int D, int KV, int MODE>
-__device__ __forceinline__ void few_item(const FlashArgs& p, FewShared<D>& s, int hk, int b, int split) {
+template <int D, int KV, int MODE, int NW = kFewWaves>
+__device__ __forceinline__ void few_item(const FlashArgs& p, FewShared<D, NW>& s, int hk, int b, int split) {
   using F = Few<D, KV, MODE>;
-  constexpr int kRound = F::kPos * kFewWaves;
+  constexpr int kRound = F::kPos * NW;
   const int tid = threadIdx.x, wv = uni(tid >> 6), lane = tid & 63, r16 = lane & 15, grp = lane >> 4;
   const int32_t* const table = p.bt.table + (int64_t)b * p.bt.max_pages;
   const int splits = MODE == kShared ? p.shared_splits : p.splits, chunk = MODE == kShared ? p.shared_chunk : p.chunk;
@@ -1110,15 +1137,15 @@ __device__ __forceinline__ void few_item(const FlashArgs& p, FewShared<D>& s, in
         make_float4(o[t][0], o[t][1], o[t][2], o[t][3]);
     __syncthreads();
     const int live = min(kFewRows, rows - r0);
-    for (int i = tid; i < live * (D / 4); i += 64 * kFewWaves) {
+    for (int i = tid; i < live * (D / 4); i += 64 * NW) {
       const int x = i / (D / 4), d = 4 * (i % (D / 4));
       float M = kNegInf;
 #pragma unroll
-      for (int w = 0; w < kFewWaves; ++w) M = fmaxf(M, s.ml[w][x][0]);
+      for (int w = 0; w < NW; ++w) M = fmaxf(M, s.ml[w][x][0]);
       float L = 0.0f;
       v4f O = (v4f){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int w = 0; w < kFewWaves; ++w) {
+      for (int w = 0; w < NW; ++w) {
         const float mw = s.ml[w][x][0], lw = s.ml[w][x][1];
         const float4 ow = *reinterpret_cast<const float4*>(&s.o[w][x][d]);
         if (empty(mw, lw)) continue;
@@ -1151,6 +1178,14 @@ template <int D, int KV, int MODE>
 __global__ __launch_bounds__(64 * kFewWaves, KV == kPagedFp8 ? 3 : 2) void k_flash_few(FlashArgs p) {
   __shared__ __attribute__((aligned(16))) FewShared<D> s;
   few_item<D, KV, MODE>(p, s, blockIdx.x, blockIdx.y, blockIdx.z);
+}
+
+// kWindow, where the workgroups are no more than the CUs: 8 waves have twice the loads on their way.  Us with 4 / 8 waves:
+// FIGURES
+template <int D, int KV>
+__global__ __launch_bounds__(512, 2) void k_flash_few_wide(FlashArgs p) {
+  __shared__ __attribute__((aligned(16))) FewShared<D, 8> s;
+  few_item<D, KV, kWindow, 8>(p, s, blockIdx.x, blockIdx.y, blockIdx.z);
 }
 
 // The splits' partials of a row, in an order that the number of splits fixes:

@@ -196,6 +196,9 @@ inline int launch_prompt(const char* what, const FlashArgs& a, int64_t tiles, in
   return check_launch(what);
 }
 
+// Windows: whether the kernel of few rows has 8 waves.
+inline bool few_wide(const FlashPlan& f) { return f.tiles * f.splits <= device_cus() && f.chunk > 32 * kFewWaves; }
+
 // A planned call over pages, the merge included.
 template <int MODE>
 inline int launch_paged(const char* who, const char* what, const FlashPlan& f, FlashArgs* a, int64_t T, int64_t H, int64_t D,
@@ -210,7 +213,15 @@ inline int launch_paged(const char* who, const char* what, const FlashPlan& f, F
     const dim3 grid((unsigned)a->Hkv, (unsigned)B, (unsigned)f.splits);
     auto* kern = D == 128 ? (fp8 ? k_flash_few<128, kPagedFp8, MODE> : k_flash_few<128, kPagedBf16, MODE>)
                           : (fp8 ? k_flash_few<64, kPagedFp8, MODE> : k_flash_few<64, kPagedBf16, MODE>);
-    hipLaunchKernelGGL(kern, grid, dim3(64 * kFewWaves), 0, stream, *a);
+    int threads = 64 * kFewWaves;
+    if constexpr (MODE == kWindow) {
+      if (few_wide(f)) {
+        threads = 512;
+        kern = D == 128 ? (fp8 ? k_flash_few_wide<128, kPagedFp8> : k_flash_few_wide<128, kPagedBf16>)
+                        : (fp8 ? k_flash_few_wide<64, kPagedFp8> : k_flash_few_wide<64, kPagedBf16>);
+      }
+    }
+    hipLaunchKernelGGL(kern, grid, dim3(threads), 0, stream, *a);
   } else {
     const dim3 grid((unsigned)(MODE == kWindow ? window_groups(f.tiles, a->Hkv) : f.tiles), (unsigned)f.splits);
     auto* kern = D == 128 ? (fp8 ? k_flash_tile<128, kPagedFp8, MODE> : k_flash_tile<128, kPagedBf16, MODE>)
