@@ -323,27 +323,31 @@ class BitLinearDecodeStep:
 
     # -- prompts and chunks over a paged cache --------------------------------
     def alloc_paged(self, num_pages: int, max_seq_len: int, page_size: int = 64, dtype: str = "bf16",
-                    use_fused_rope: bool = False, rope_scaling: dict | None = None):
+                    use_fused_rope: bool = False, rope_scaling: dict | None = None, window: int | None = None,
+                    sinks: int = 0):
         """Page pools of every layer for ``forward_rows``: num_pages pages of
-        page_size rows, dtype "bf16" or "fp8", positions up to max_seq_len."""
+        page_size rows, dtype "bf16" or "fp8", positions up to max_seq_len.  ``window`` and ``sinks``:
+        every layer's attention sees the last ``window`` positions and the first ``sinks`` only."""
         from .layers.attention import PagedAttention
 
         c = self.config
         self.paged = PagedAttention(c.num_attention_heads, c.num_kv_heads, c.head_dim, max_seq_len, self.device,
                                     rope_theta=c.rope_theta, use_fused_rope=use_fused_rope, rope_scaling=rope_scaling,
-                                    max_position=c.max_position_embeddings)
+                                    max_position=c.max_position_embeddings, window=window, sinks=sinks)
         self.pages = [self.paged.new_cache(num_pages, page_size, dtype) for _ in self.layers]
         return self
 
-    def forward_rows(self, hidden, page_table, cu_q, kv_len, max_q: int | None = None, max_kv: int | None = None):
+    def forward_rows(self, hidden, page_table, cu_q, kv_len, max_q: int | None = None, max_kv: int | None = None,
+                     shared_pages=None, max_shared: int | None = None):
         """The layers on any rows of any users: hidden bf16 [T, hidden], in place.
         Sequence b's rows are ``cu_q[b] .. cu_q[b + 1] - 1``, its newest tokens; their
         keys and values are cached, and kv_len counts them (bitnet_tt.paged_attention).
         Whole prompts, chunks of them and single tokens may share a call; all of them attend to
         the pages, so with 8-bit pages a prompt's own keys and values are the rounded ones.  Rows of no
         sequence (behind cu_q[B], say, in a captured call of fewer tokens) run through the
-        layers with zeros for their attention; nothing is cached for them.  Needs
-        alloc_paged()."""
+        layers with zeros for their attention; nothing is cached for them.  ``shared_pages`` (int32 [1] on the
+        device): every sequence begins with that many pages of page_table[0], a prompt that has been cached once
+        for all of them, and the rows are behind it (PagedAttention).  Needs alloc_paged()."""
         import torch
 
         if getattr(self, "paged", None) is None:
@@ -363,7 +367,8 @@ class BitLinearDecodeStep:
         ffn = torch.empty((T, c.intermediate_size), dtype=torch.bfloat16, device=dev)
         for w, pages in zip(self.layers, self.pages):
             ternary_matmul_into(hidden, w.qkv, qkv, norm_weight=w.input_layernorm, norm_epsilon=self.eps)
-            self.paged(qkv, pages, page_table, cu_q, kv_len, max_q=max_q, max_kv=max_kv, out=attn)
+            self.paged(qkv, pages, page_table, cu_q, kv_len, max_q=max_q, max_kv=max_kv, out=attn, shared_pages=shared_pages,
+                       max_shared=max_shared)
             ternary_matmul_into(attn, w.o_proj, hidden, norm_weight=w.attn_sub_norm, norm_epsilon=self.eps,
                                 residual=hidden)
             ternary_matmul_into(hidden, w.gate_up, ffn, norm_weight=w.post_attention_layernorm, norm_epsilon=self.eps,
@@ -376,12 +381,15 @@ class BitLinearDecodeStep:
         (rows [0, kv_len[b]) of user b), and ``pos`` to kv_len, every user's next position: the
         decode steps go on from here.  Their queries are rotated as ``alloc_attention`` says, so
         ValueError where ``alloc_paged`` rotated the cached keys otherwise; from position 4096 on
-        the steps' angle tables get the rows that the cached keys were rotated by (float64 angles)."""
+        the steps' angle tables get the rows that the cached keys were rotated by (float64 angles).
+        Not from a cache with a window: the steps see all of their contexts."""
         from .paged_attention import read_pages
         from .utils.rope import FLOAT32_POSITIONS
 
         if getattr(self, "paged", None) is None or getattr(self, "kv", None) is None:
             raise RuntimeError("load_contiguous needs alloc_paged() and alloc_attention() first")
+        if self.paged.window is not None:
+            raise ValueError("the decode steps' attention has no window")
         if self.paged.rotation != self.attention.rotation:
             raise ValueError(f"the cached keys are rotated by {self.paged.rotation}, the queries of the decode steps by "
                              f"{self.attention.rotation}")

@@ -234,16 +234,22 @@ class PagedAttention:
     of 16, default head_dim) rotates part of a head; ``rope_scaling`` is a model
     config's dict (utils.rope.scaled_frequencies).  Without scaling the angles of the first 4096
     positions are those of DecodeAttention; behind them, and with scaling, they are computed in
-    float64.  ``scale`` as for DecodeAttention."""
+    float64.  ``scale`` as for DecodeAttention.  ``window`` and ``sinks``: a row sees the last ``window``
+    positions, its own among them, and the first ``sinks`` only; pages that no row will see any more may be
+    given away, their entries of the page table are not read."""
 
     def __init__(self, num_heads: int, num_kv_heads: int, head_dim: int, max_seq_len: int, device=None,
                  rope_theta: float = 500000.0, use_fused_rope: bool = False, scale: float | None = None,
-                 rotary_dim: int | None = None, rope_scaling: dict | None = None, max_position: int = 4096) -> None:
+                 rotary_dim: int | None = None, rope_scaling: dict | None = None, max_position: int = 4096,
+                 window: int | None = None, sinks: int = 0) -> None:
         import math
 
         import torch
 
+        from ..paged_attention import check_window
         from ..utils.rope import paged_rope_tables
+
+        self.window, self.sinks = check_window(window, sinks)
 
         rotary_dim = head_dim if rotary_dim is None else rotary_dim
         if head_dim not in (64, 128) or num_heads % num_kv_heads or num_heads // num_kv_heads > 64:
@@ -268,16 +274,25 @@ class PagedAttention:
         return PagedKVCache.allocate(num_pages, self.num_kv_heads, self.head_dim, self.device, page_size, dtype)
 
     def __call__(self, qkv, cache, page_table, cu_q, kv_len, max_q: int | None = None, max_kv: int | None = None,
-                 out=None):
+                 out=None, shared_pages=None, max_shared: int | None = None):
         """qkv bf16 [T, (H + 2 Hkv) D]: writes its keys and values to their pages,
-        then attends over everything cached; bf16 [T, H D]."""
-        from ..paged_attention import paged_attention, rope_write
+        then attends over everything cached; bf16 [T, H D].  ``shared_pages`` (int32 [1] on the
+        device, and its hint max_shared): the pages that every sequence begins with, which are read once for
+        all (paged_attention.shared_prefix_attention); not with a window."""
+        from ..paged_attention import paged_attention, rope_write, shared_prefix_attention
 
+        if shared_pages is not None and self.window is not None:
+            raise ValueError("shared pages and a window do not go together")
         H, D = self.num_heads, self.head_dim
         q = rope_write(qkv, self.rope_cos, self.rope_sin, cu_q, kv_len, H, self.num_kv_heads, cache=cache,
                        page_table=page_table, rope_adjacent=self.use_fused_rope)
-        o = paged_attention(q, cache, page_table, cu_q, kv_len, scale=self.scale, max_q=max_q, max_kv=max_kv,
-                            out=None if out is None else out.view(-1, H, D))
+        out = None if out is None else out.view(-1, H, D)
+        if shared_pages is not None:
+            o = shared_prefix_attention(q, cache, page_table, cu_q, kv_len, shared_pages, scale=self.scale, max_q=max_q,
+                                        max_kv=max_kv, max_shared=max_shared, out=out)
+        else:
+            o = paged_attention(q, cache, page_table, cu_q, kv_len, scale=self.scale, max_q=max_q, max_kv=max_kv, out=out,
+                                window=self.window, sinks=self.sinks)
         return o.view(-1, H * D)
 
     def prompt(self, qkv, cu_seqlens, cache=None, page_table=None, kv_len=None, max_q: int | None = None, out=None):
@@ -294,7 +309,7 @@ class PagedAttention:
                        page_table=page_table, rope_adjacent=self.use_fused_rope, k_out=k)
         v = qkv.view(-1, H + 2 * Hkv, D)[:, H + Hkv:]
         o = prompt_attention(q, k, v, cu_seqlens, scale=self.scale, max_q=max_q,
-                             out=None if out is None else out.view(-1, H, D))
+                             out=None if out is None else out.view(-1, H, D), window=self.window, sinks=self.sinks)
         return o.view(-1, H * D)
 
     def check(self) -> None:

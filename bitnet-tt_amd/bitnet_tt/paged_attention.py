@@ -255,8 +255,8 @@ def read_pages(cache: PagedKVCache, page_table, kv_len, key_cache, value_cache) 
         N.check(rc, "btl_read_pages")
 
 
-def _window(window, sinks):
-    """(window, sinks) of a call, window None where there is none."""
+def check_window(window, sinks):
+    """(window, sinks) of a call as whole numbers, window None where there is none."""
     if window is None:
         if sinks:
             raise ValueError("sinks need a window")
@@ -283,7 +283,7 @@ def prompt_attention(q, k, v, cu_seqlens, scale: float | None = None, max_q: int
         with torch.cuda.device(index):
             return prompt_attention(q, k, v, cu_seqlens, scale, max_q, out, window, sinks)
     if window is not None or sinks:
-        window, sinks = _window(window, sinks)
+        window, sinks = check_window(window, sinks)
     if q.dim() != 3 or k.dim() != 3:
         raise ValueError("q must be [T, H, D], k and v [T, Hkv, D]")
     T, H, D = q.shape
@@ -329,7 +329,7 @@ def paged_attention(q, cache: PagedKVCache, page_table, cu_q, kv_len, scale: flo
         with torch.cuda.device(index):
             return paged_attention(q, cache, page_table, cu_q, kv_len, scale, max_q, max_kv, out, window, sinks)
     if window is not None or sinks:
-        window, sinks = _window(window, sinks)
+        window, sinks = check_window(window, sinks)
     if q.dim() != 3:
         raise ValueError("q must be [T, H, D]")
     T, H, D = q.shape

@@ -106,8 +106,8 @@ def test_python_refuses():
     x = torch.zeros((4, 8, 64), dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="ROCm GPU"):
         pa.prompt_attention(x[:, :4], x[:, 4:6], x[:, 6:], torch.zeros(2, dtype=torch.int32), window=4)
-    assert pa._window(None, 0) == (None, 0) and pa._window(7, 2) == (7, 2)
-    assert pa._window(2 ** 63, 2 ** 70) == (2 ** 30, 2 ** 30)
+    assert pa.check_window(None, 0) == (None, 0) and pa.check_window(7, 2) == (7, 2)
+    assert pa.check_window(2 ** 63, 2 ** 70) == (2 ** 30, 2 ** 30)
     for bad in ((None, 3), (0, 0), (-1, 0), (5, -1)):
         with pytest.raises(ValueError):
-            pa._window(*bad)
+            pa.check_window(*bad)
