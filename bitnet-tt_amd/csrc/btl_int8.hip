@@ -321,6 +321,17 @@ __device__ __forceinline__ void int8_tile(const Int8Args& p, uint8_t* smem, int 
     }
   };
   const int kg = wv / (WM * WN), wm = wv % WM, wn = wv / WM % WN;
+  constexpr int kRows = TM / KG;  // of a wave's row blocks, those that it finishes
+  const int col0 = (nt0 + wn * TN) * 16, row0 = m0 + (wm * TM + kg * kRows) * 16;
+  // (now: a load between the stores of the outputs would wait for those)
+  float sa[kRows], sw[TN][4];
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) sa[i] = p.sa[min(row0 + 16 * i + (lane & 15), p.M - 1)];
+#pragma unroll
+  for (int j = 0; j < TN; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sw[j][e] = p.sw[min(col0 + 16 * j + 4 * (lane >> 4) + e, p.N - 1)];
+
   v4i acc[TM][TN];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
@@ -356,7 +367,6 @@ __device__ __forceinline__ void int8_tile(const Int8Args& p, uint8_t* smem, int 
   __builtin_amdgcn_s_waitcnt(0x0f70);  // nothing may land in LDS any more
   lds_barrier();                       // every wave is done with the stages: their place takes sums and outputs
 
-  constexpr int kRows = TM / KG;  // of a wave's row blocks, those that it finishes
   if (KG > 1) {
     v4i* const sums = reinterpret_cast<v4i*>(smem);
     // place of (owner, which of the others, row block, column block) of this wave's part of the tile
@@ -386,22 +396,14 @@ __device__ __forceinline__ void int8_tile(const Int8Args& p, uint8_t* smem, int 
     lds_barrier();
   }
   uint8_t* const mine = smem + wv * kOutBytes;
-  const int col0 = (nt0 + wn * TN) * 16;
   if (col0 >= p.N) return;
-  float sw[TN][4];
-#pragma unroll
-  for (int j = 0; j < TN; ++j)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) sw[j][e] = p.sw[min(col0 + 16 * j + 4 * (lane >> 4) + e, p.N - 1)];
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
-    const int row0 = m0 + (wm * TM + kg * kRows + i) * 16;
-    if (row0 >= p.M) break;
-    const float sa = p.sa[min(row0 + (lane & 15), p.M - 1)];
+    if (row0 + 16 * i >= p.M) break;
     if (p.f32)
-      store_block<TN, float>(p, acc[i], sa, sw, reinterpret_cast<float*>(mine), row0, col0);
+      store_block<TN, float>(p, acc[i], sa[i], sw, reinterpret_cast<float*>(mine), row0 + 16 * i, col0);
     else
-      store_block<TN, uint16_t>(p, acc[i], sa, sw, reinterpret_cast<uint16_t*>(mine), row0, col0);
+      store_block<TN, uint16_t>(p, acc[i], sa[i], sw, reinterpret_cast<uint16_t*>(mine), row0 + 16 * i, col0);
   }
 }
 
