@@ -77,16 +77,15 @@ __global__ __launch_bounds__(64 * kI8Waves, 2) void k_int8_stream(Int8Args p, in
   constexpr int kPart = 4 * 68;  // words of a block's sums: 16 rows of four columns, four times, and what keeps those in other banks
   __shared__ __attribute__((aligned(16))) int red[kI8Waves][RB][CT][kPart];
   const int tid = threadIdx.x, lane = tid & 63, wv = uni8(tid >> 6);
-  const int m0 = blockIdx.y * 16 * RB;
   const int rounds = ONCE ? 1 : ((p.KB + kI8Waves - 1) / kI8Waves + U - 1) / U;
   const int mine = (groups - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
   const int chunks = mine * rounds;
 
   // rows behind M: the last one's values, never written; k behind K: any values, the weights are zero there
-  const auto ra = rsrc8(p.a + (int64_t)m0 * p.lda, 0x7fffffff);
+  const auto ra = rsrc8(p.a, 0x7fffffff);
   uint32_t row_off[RB];
 #pragma unroll
-  for (int r = 0; r < RB; ++r) row_off[r] = (uint32_t)(min(16 * r + (lane & 15), p.M - 1 - m0) * p.lda);
+  for (int r = 0; r < RB; ++r) row_off[r] = (uint32_t)(min(16 * r + (lane & 15), p.M - 1) * p.lda);
 
   v4i b[2][U][CT], a[ONCE ? 1 : 2][U][RB];
   auto issue_rows = [&](int set, int k0) {
@@ -138,9 +137,9 @@ __global__ __launch_bounds__(64 * kI8Waves, 2) void k_int8_stream(Int8Args p, in
       v4i sum = (v4i){0, 0, 0, 0};
 #pragma unroll
       for (int w = 0; w < kI8Waves; ++w) sum += *reinterpret_cast<const v4i*>(&red[w][m >> 4][q >> 2][at]);
-      const int row = m0 + m, col = g * 16 * CT + 4 * q;
-      if (row >= p.M) continue;
-      const float sa = p.sa[row];
+      const int col = g * 16 * CT + 4 * q;
+      if (m >= p.M) continue;
+      const float sa = p.sa[m];
       float y[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) y[i] = scaled(sum[i], sa, p.sw[min(col + i, p.N - 1)]);
@@ -150,14 +149,14 @@ __global__ __launch_bounds__(64 * kI8Waves, 2) void k_int8_stream(Int8Args p, in
           if (col + i < p.N) best = arg_max(best, arg_key(y[i], col + i));
       if (!p.out) continue;
       if (p.f32) {
-        float* const o = static_cast<float*>(p.out) + row * p.ldo + col;
+        float* const o = static_cast<float*>(p.out) + m * p.ldo + col;
         if (p.vec && col + 4 <= p.N)
           *reinterpret_cast<float4*>(o) = make_float4(y[0], y[1], y[2], y[3]);
         else
           for (int i = 0; i < 4; ++i)
             if (col + i < p.N) o[i] = y[i];
       } else {
-        uint16_t* const o = static_cast<uint16_t*>(p.out) + row * p.ldo + col;
+        uint16_t* const o = static_cast<uint16_t*>(p.out) + m * p.ldo + col;
         if (p.vec && col + 4 <= p.N)
           *reinterpret_cast<uint2*>(o) = make_uint2(f2bf_pair(y[0], y[1]), f2bf_pair(y[2], y[3]));
         else
@@ -188,7 +187,7 @@ __global__ __launch_bounds__(64 * kI8Waves, 2) void k_int8_stream(Int8Args p, in
   // those to end writes the indexes
 #pragma unroll
   for (int off = 1; off < 4 * CT; off <<= 1) best = arg_max(best, __shfl_xor(best, off, 64));
-  const int row = m0 + tid / (4 * CT);
+  const int row = tid / (4 * CT);
   if (tid < RB * CT * 64 && tid % (4 * CT) == 0 && row < p.M && best)
     __hip_atomic_fetch_max(p.keys + row, best, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   wait_memory();  // this workgroup's maxima are performed before it counts itself done
@@ -512,21 +511,29 @@ static void launch_tile(const Int8Args& a, hipStream_t s) {
                      a, ngm);
 }
 
+// Of `tiles` large ones, how many go as halves: a last round that fills at most half of the CUs.  4096 x 2560 x 13824 (864 tiles)
+// 155 us, 146 so; 8192 x 2560 x 2560 (320) 84, 64.
+static int64_t large_halves(int64_t tiles, int64_t cus) { return tiles > cus && 2 * (tiles % cus) <= cus ? tiles % cus : 0; }
+
 static void launch_large(const Int8Args& a, int cus, hipStream_t s) {
-  const int ngm = (a.M + 255) / 256, tiles = ngm * ((a.NT + 15) / 16);
-  const int rest = tiles % cus, halves = tiles > cus && 2 * rest <= cus ? rest : 0;
+  const int ngm = (a.M + 255) / 256, tiles = ngm * ((a.NT + 15) / 16), halves = (int)large_halves(tiles, cus);
   hipLaunchKernelGGL(k_int8_large, dim3((unsigned)(tiles + halves)), dim3(512), 0, s, a, ngm, tiles - halves);
 }
 
-// The tile of the least time, us: rounds of workgroups over the CUs x what a workgroup takes, before its first and
-// behind its last step and for each 128 k.
+// The tile of the least time, us: rounds of workgroups over the CUs x what a workgroup takes, for a start (and an end) and for
+// each 128 k; alone on its CU, or beside another one.  Fitted to 70 shapes, 65-8192 rows, K 576-6912, 640-128256
+// columns: the rule takes the best of the five for 64 of them, within 2% of it for the others.  Us of each, in this order:
+// 4096 x 2560 x 13824: 146, 173, 230, 306, 285; 1024 x 2560 x 6912: 35, 28, 32, 39, 38; 256 x 2560 x 13824: 36, 25, 20, 27, 28;
+// 511 x 2560 x 3840: 34, 21, 13, 11, 14; 128 x 6912 x 2560: 77, 46, 27, 18, 13; 400 x 640 x 2560: 13, 9, 6.9, 5.9, 6.5.
+// (128 x 128 as two a CU is never more than 2% better, 64 x 64 as one of 8 stages never better.)
 struct TileCost {
   int bm, bn, per_cu;
-  double start, step;
+  double start, step;          // one on a CU
+  double start_two, step_two;  // per_cu 2
 };
 constexpr TileCost kTiles[] = {
-    {256, 256, 1, 4.0, 1.66}, {128, 256, 1, 3.5, 0.90}, {128, 128, 2, 3.0, 1.02},
-    {128, 128, 1, 3.0, 0.47}, {128, 64, 1, 2.5, 0.31},  {64, 64, 2, 2.0, 0.62}, {64, 64, 1, 2.0, 0.21},
+    {256, 256, 1, 8.0, 1.60, 0, 0}, {128, 256, 1, 5.5, 0.95, 0, 0},    {128, 128, 1, 4.2, 0.56, 0, 0},
+    {128, 64, 1, 3.0, 0.35, 0, 0},  {64, 64, 2, 2.8, 0.20, 3.5, 0.45},
 };
 static int tile_choice(int64_t M, int64_t N, int64_t K, int cus) {
   const double steps = (double)((K + 127) / 128);
@@ -535,15 +542,16 @@ static int tile_choice(int64_t M, int64_t N, int64_t K, int cus) {
   for (int i = 0; i < (int)(sizeof(kTiles) / sizeof(kTiles[0])); ++i) {
     const TileCost& t = kTiles[i];
     const int64_t tiles = (M + t.bm - 1) / t.bm * ((N + t.bn - 1) / t.bn), slots = (int64_t)cus * t.per_cu;
+    const bool two = t.per_cu == 2 && tiles > cus;
     double rounds = (double)((tiles + slots - 1) / slots);
-    if (i == 0 && tiles > cus && 2 * (tiles % cus) <= cus && tiles % cus) rounds -= 0.25;  // halves
-    const double us = rounds * (t.start + t.step * steps);
+    if (i == 0 && large_halves(tiles, cus)) rounds -= 0.5;
+    const double us = rounds * (two ? t.start_two + t.step_two * steps : t.start + t.step * steps);
     if (i == 0 || us < least) best = i, least = us;
   }
   return best;
 }
 
-constexpr int kFewRows8 = 64;     // of the weight stream
+constexpr int kFewRows8 = 64;     // that the weight stream can take
 constexpr int kHeadRows = 65535;  // a grid's second dimension
 constexpr int kHeadWords = kFewRows8 * 2 + 1;  // few rows: keys and count, which the quantisation clears
 
@@ -558,7 +566,7 @@ static HeadScratch head_scratch(int64_t M, int64_t K, int64_t N) {
   h.scale = round_up(h.blocked + btl_act_bytes(M, K), 256);
   h.keys = round_up(h.scale + round_up(M, 32) * 4, 256);
   // about four workgroups a CU
-  h.parts = M <= kFewRows8 ? 1 : std::max((int64_t)1, std::min((4 * (int64_t)device_cus() + M - 1) / M, (N + 2047) / 2048));
+  h.parts = std::max((int64_t)1, std::min((4 * (int64_t)device_cus() + M - 1) / M, (N + 2047) / 2048));
   h.total = h.keys + (h.parts > 1 ? M * h.parts * 8 : 0);
   return h;
 }
@@ -583,10 +591,23 @@ static int int8_args(const char* who, const int8_t* a, int64_t lda, const float*
   return BTL_OK;
 }
 
+// Whether the weight stream takes it, where a few rows' argmax is wanted without logits in any case.  Us of the stream / of tiles, K =
+// 2560, 16 rows: 640 columns 3.8 / 6.5, 3840: 4.6 / 7.0, 13824: 10.0 / 9.7, 128256: 66.7 / 72; 32 rows: 5.0 / 6.6, 5.7 / 7.1, 11.5 /
+// 11.0, 69.6 / 73; 64 rows: 7.3 / 6.7, 8.4 / 7.3, 15.5 / 12.3, 76.6 / 78.  K = 6912, where rows are loaded again for each group
+// of columns, 16 rows: 640: 8.9 / 12.7, 3840: 9.5 / 12.9, 13824: 27.6 / 20.8, 40000: 63 / 59; 32 rows: 14.0 / 12.8, 14.5 / 13.0,
+// 36 / 22, 80 / 61.
+static bool streams_once(const Int8Args& p) { return p.KB <= 5 * kI8Waves; }
+static bool few_rows(const Int8Args& p, int cus) {
+  if (p.tokens) return true;
+  return streams_once(p) ? p.M <= 32 : p.M <= 16 && p.NT <= cus;
+}
+
 static int int8_launch(const char* who, const Int8Args& p, hipStream_t s) {
   const int cus = device_cus();
-  if (p.M <= kFewRows8) {
-    const int ct = p.NT > cus ? 2 : 1, groups = (p.NT + ct - 1) / ct;
+  if (few_rows(p, cus)) {
+    // pairs of column blocks share the rows' registers and the sums' barriers: 128256 columns of 2560, 1 / 16 / 64 rows, alone 59 /
+    // 66 / 79 us, in pairs 57 / 62 / 74; 27648 columns 16.3 / 17.2 / 22.9, 16.9 / 17.5 / 23.8, as the last round is less even
+    const int ct = p.NT > 8 * cus ? 2 : 1, groups = (p.NT + ct - 1) / ct;
     const dim3 grid((unsigned)std::min(groups, cus));
     if (p.M <= 16)
       ct == 1 ? launch_stream<1, 1>(p, groups, grid, s) : launch_stream<1, 2>(p, groups, grid, s);
@@ -599,11 +620,9 @@ static int int8_launch(const char* who, const Int8Args& p, hipStream_t s) {
   switch (tile_choice(p.M, p.N, p.K, cus)) {
     case 0: launch_large(p, cus, s); break;
     case 1: launch_tile<128, 256, 2, 4, 1, 2, 3, 1>(p, s); break;
-    case 2: launch_tile<128, 128, 2, 2, 2, 1, 2, 2>(p, s); break;
-    case 3: launch_tile<128, 128, 2, 2, 2, 1, 4, 1>(p, s); break;
-    case 4: launch_tile<128, 64, 2, 2, 2, 1, 6, 1>(p, s); break;
-    case 5: launch_tile<64, 64, 2, 2, 2, 1, 4, 2>(p, s); break;
-    default: launch_tile<64, 64, 2, 2, 2, 1, 8, 1>(p, s); break;
+    case 2: launch_tile<128, 128, 2, 2, 2, 1, 4, 1>(p, s); break;
+    case 3: launch_tile<128, 64, 2, 2, 2, 1, 6, 1>(p, s); break;
+    default: launch_tile<64, 64, 2, 2, 2, 1, 4, 2>(p, s); break;
   }
   return check_launch(who);
 }
@@ -692,7 +711,8 @@ int btl_int8_head(const uint16_t* x, int64_t M, int64_t K, int64_t N, const uint
   Int8Args p{};
   rc = int8_args(who, codes, K, a_scale, M, K, N, wdev, w_scale, logits, N, 1, &p);
   if (rc != BTL_OK) return rc;
-  const bool few = M <= kFewRows8;
+  // (with logits: where rows are loaded again for each group of columns, tiles and the argmax behind them are faster)
+  const bool few = M <= kFewRows8 && (!logits || M <= 16 || streams_once(p));
   hipStream_t s = (hipStream_t)stream;
   rc = launch_act(x, M, K, K, gamma, norm_eps, reinterpret_cast<int8_t*>(at + h.blocked), a_scale, nullptr, nullptr, codes, normed,
                   reinterpret_cast<uint32_t*>(at), few ? kHeadWords : 0, s);
