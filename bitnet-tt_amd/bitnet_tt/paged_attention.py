@@ -26,6 +26,7 @@ from __future__ import annotations
 
 import functools
 import math
+import operator
 
 import torch
 
@@ -261,7 +262,7 @@ def check_window(window, sinks):
         if sinks:
             raise ValueError("sinks need a window")
         return None, 0
-    window, sinks = int(window), int(sinks)
+    window, sinks = operator.index(window), operator.index(sinks)
     if window < 1 or sinks < 0:
         raise ValueError(f"window {window} must be at least 1, sinks {sinks} at least 0")
     return min(window, _FAR), min(sinks, _FAR)

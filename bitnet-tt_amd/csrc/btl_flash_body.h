@@ -718,7 +718,9 @@ __device__ __forceinline__ void tile_item(const FlashArgs& p, uint8_t* smem, int
       store_ahead(k_free, v_free);
       kv += kStep;
     };
-    if (MODE != kWindow && wr >= rows) {  // a wave without rows only loads (67 tokens at 40000 positions: 68.5 us, 65.5 so)
+    // a wave without rows only loads (67 tokens at 40000 positions: 68.5 us, 65.5 so; windows, where this copy of the loads costs
+    // the hot loop its registers: 67 tokens 24.4, 26.1, prompts of 16001 190, 247)
+    if (MODE != kWindow && wr >= rows) {
       for (; kv + 2 * kStep <= whole_end; kv += kStep, at ^= 1) {
         arrived();
         load_ahead(sm + at * kB, sm + (3 - at) * kB);
@@ -807,8 +809,9 @@ __device__ __forceinline__ UnitItem unit_item(int x, int each) {
 }
 inline int64_t unit_groups(int64_t units, int64_t each) { return (units + kXcds - 1) / kXcds * kXcds * each; }
 
-// kWindow: neighbouring tiles of a head see mostly the same positions.
-constexpr int kNeighbours = 16;
+// kWindow: neighbouring tiles of a head see mostly the same positions.  16001 tokens of 20 / 5 heads of 128, window 1024, 1 / 8 / 16 of
+// them on an XCD, one after the other: 203, 189, 191 us; chunks of 4 users, window 2000: 75.9, 73, 74.
+constexpr int kNeighbours = 8;
 
 template <int D, int KV, int MODE>
 __global__ __launch_bounds__(256, 2) void k_flash_tile(FlashArgs p) {
@@ -1180,12 +1183,14 @@ __global__ __launch_bounds__(64 * kFewWaves, KV == kPagedFp8 ? 3 : 2) void k_fla
   few_item<D, KV, MODE>(p, s, blockIdx.x, blockIdx.y, blockIdx.z);
 }
 
-// kWindow, where the workgroups are no more than the CUs: 8 waves have twice the loads on their way.  Us with 4 / 8 waves:
-// FIGURES
-template <int D, int KV>
+// Windows over 8-bit pages, where the workgroups are no more than the CUs: 8 waves have twice the loads on their way, and the
+// conversions of twice the positions run at once.  20 / 5 heads of 128, us with 4 / 8 waves: 32 users, window 100 / 500 / 1024: 9.6,
+// 14.3, 19.4 / 9.1, 12.6, 15.3; 8 users, 4096: 18.3 / 17.1; one user, 4096: 14.8 / 14.0.  With more workgroups, 120 users, 1024: 44.9 / 51;
+// 256: 75 / 89.  bf16 pages, which need no conversion: 8 users 15.5 / 16.5, one user, 4096: 15.5 / 16.4, 64 users 45.6 / 49.5.
+template <int D>
 __global__ __launch_bounds__(512, 2) void k_flash_few_wide(FlashArgs p) {
   __shared__ __attribute__((aligned(16))) FewShared<D, 8> s;
-  few_item<D, KV, kWindow, 8>(p, s, blockIdx.x, blockIdx.y, blockIdx.z);
+  few_item<D, kPagedFp8, kWindow, 8>(p, s, blockIdx.x, blockIdx.y, blockIdx.z);
 }
 
 // The splits' partials of a row, in an order that the number of splits fixes:

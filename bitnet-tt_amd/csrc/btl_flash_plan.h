@@ -57,6 +57,9 @@ constexpr int64_t kMaxSplits = 256;
 // A hint behind this plans for as many positions as a page table may have room for: splits x
 // chunk stays below 2^31, the kernels' positions.
 constexpr int64_t kMaxPositions = INT32_MAX / 2;
+// Us, of the tiles' rule: all steps of the longest workgroup, the partials of a split.
+inline double split_whole(int64_t positions) { return 0.0117 * (double)positions; }
+inline double split_part(int64_t T, int64_t H, int64_t D) { return 1.67e-6 * (double)(T * H * D); }
 inline FlashPlan flash_plan(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t B, int64_t max_q, int64_t max_kv,
                             bool paged) {
   FlashPlan f{};
@@ -74,7 +77,7 @@ inline FlashPlan flash_plan(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_
     if (n <= 1 && 4 * f.tiles <= 9 * cus && max_kv >= 10 * kMinChunk) n = 4;
   } else {
     n = std::max((4 * cus + f.tiles) / (2 * f.tiles), (int64_t)(f.tiles <= 3 * cus ? 2 : 1));
-    const double whole = 0.0117 * (double)max_kv, part = 1.67e-6 * (double)(T * H * D);  // us
+    const double whole = split_whole(max_kv), part = split_part(T, H, D);
     n = std::min(n, (int64_t)(std::sqrt(whole / part) + 0.5));
     if (n > 1 && whole - whole / (double)n <= 4.0 + part * (double)n) n = 1;
   }
@@ -196,8 +199,8 @@ inline int launch_prompt(const char* what, const FlashArgs& a, int64_t tiles, in
   return check_launch(what);
 }
 
-// Windows: whether the kernel of few rows has 8 waves.
-inline bool few_wide(const FlashPlan& f) { return f.tiles * f.splits <= device_cus() && f.chunk > 32 * kFewWaves; }
+// Windows over 8-bit pages: whether the kernel of few rows has 8 waves.
+inline bool few_wide(const FlashPlan& f) { return f.tiles * f.splits <= device_cus(); }
 
 // A planned call over pages, the merge included.
 template <int MODE>
@@ -215,10 +218,9 @@ inline int launch_paged(const char* who, const char* what, const FlashPlan& f, F
                           : (fp8 ? k_flash_few<64, kPagedFp8, MODE> : k_flash_few<64, kPagedBf16, MODE>);
     int threads = 64 * kFewWaves;
     if constexpr (MODE == kWindow) {
-      if (few_wide(f)) {
+      if (fp8 && few_wide(f)) {
         threads = 512;
-        kern = D == 128 ? (fp8 ? k_flash_few_wide<128, kPagedFp8> : k_flash_few_wide<128, kPagedBf16>)
-                        : (fp8 ? k_flash_few_wide<64, kPagedFp8> : k_flash_few_wide<64, kPagedBf16>);
+        kern = D == 128 ? k_flash_few_wide<128> : k_flash_few_wide<64>;
       }
     }
     hipLaunchKernelGGL(kern, grid, dim3(threads), 0, stream, *a);

@@ -75,7 +75,7 @@ inline SharedPlan shared_plan(int64_t T, int64_t H, int64_t Hkv, int64_t D, int6
     s.shared_splits = f.splits;
     s.shared_chunk = f.chunk;
   } else {
-    const double part = 1.67e-6 * (double)(T * H * D);
+    const double part = split_part(T, H, D);
     int64_t n = (int64_t)(std::sqrt(0.0085 * (double)max_shared / part) + 0.5);
     n = std::min(n, 2 * tiles <= cus ? cus / tiles : (4 * cus + tiles) / (2 * tiles));
     n = std::max((int64_t)1, std::min(n, std::min(max_shared / (2 * kStep), kMaxSplits)));

@@ -4,14 +4,46 @@
 
 namespace btl {
 
-// Positions of the longest axis that a workgroup walks: those of its rows' windows (`tokens` of them
-// side by side), the sinks, and what both are rounded to.
+// The plan of a call over pages, by `seen`, the positions of the longest axis that a workgroup walks: those of its rows' windows
+// (`tokens` of them side by side), the sinks, and what both are rounded to.  Windows are alike in length, so that a split
+// only pays where the CUs are not full; measured on 256 of them, 20 / 5 heads of 128, us, chunks in positions:
+//  - Few rows: as many workgroups as CUs, a chunk at least a round of 4 waves, up to 36 of them (the merge).  One user, bf16, window
+//    4096, 128 / 256 / 512 / one: 12.3, 13.5, 15.6, 47.6; 8000: 16.8, 13.7, 15.1, 77.6; 4 users, 2000 (a CU each at
+//    256): 16.1, 13.8, 15.7, 27.4; 8 users, 8-bit, 1024 (256): 13.5, 12.4, 13.7, 14.3.  Where it shortens the longest workgroup
+//    by less than 576 positions the merge's launch costs more, 25 users, 1024, 640 / one: 8-bit 16.7, 14.8; bf16 20.0, 19.5.  From a
+//    workgroup on every other CU on: as without a window.
+//  - Tiles: what comes nearest to 1.4 workgroups a CU, by the rule on what a split costs (FlashPlan), a chunk not below 192.
+//    bf16, 1 / 2 / 3 / 4 / 5 / 6 / 8 splits: 500 rows of one user, 4096 (80 tiles of rows and heads): 85, 55, 50, 47, 57, 56, 60; 250, 4096 (40): -,
+//    53, 42, 36.2, 37.4, 36.6, 35.2; 1000, 4096 (160): -, 73, 83, 73, 75; 20 users of 10, 2000 (100): 49, 41, 34, 30, 38; 4 users' 2047
+//    rows, 2000 (340): 68, 69. 8-bit, 8 users of 1-10 rows, 1024 (40), chunks of 192 / 256 / 512: 20.4, 21.1, 27.1.
+constexpr int64_t kWindowSplits = 36;
+constexpr int64_t kWindowGain = 576;
+constexpr int64_t kWindowChunk = 192;
 inline FlashPlan window_plan(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t B, int64_t max_q, int64_t max_kv,
                              int64_t window, int64_t sinks) {
-  const int64_t G = H / Hkv;
+  const int64_t G = H / Hkv, cus = device_cus();
   const int64_t tokens = std::min(std::min(max_q, T), (int64_t)kTileRows / G + 2);
-  const int64_t seen = std::min(window, kMaxPositions) + tokens + kStep + round_up(std::min(sinks, kMaxPositions), kStep);
-  return flash_plan(T, H, Hkv, D, B, max_q, std::min(max_kv, seen), true);
+  const int64_t all = std::min(window, kMaxPositions) + tokens + kStep + round_up(std::min(sinks, kMaxPositions), kStep);
+  const int64_t seen = std::min(std::min(max_kv, all), kMaxPositions);
+  FlashPlan f = flash_plan(T, H, Hkv, D, B, max_q, 1, true);  // one split
+  f.chunk = (int)round_up(seen, kMinChunk);
+  int64_t n, chunk;
+  if (f.few) {
+    n = std::min(cus / f.tiles, kWindowSplits);
+    if (n <= 1) return flash_plan(T, H, Hkv, D, B, max_q, seen, true);
+    chunk = round_up((seen + n - 1) / n, 32 * kFewWaves);
+    if (seen - chunk < kWindowGain) return f;
+  } else {
+    const int64_t tiles = std::min(f.tiles, B * ((std::min(max_q, T) * G + kTileRows - 1) / kTileRows) * Hkv);  // (if the hint holds)
+    const double whole = split_whole(seen), part = split_part(T, H, D);
+    n = std::min((7 * cus / 5 + tiles / 2) / tiles, (int64_t)(std::sqrt(whole / part) + 0.5));
+    if (n <= 1 || whole - whole / (double)n <= 4.0 + part * (double)n) return f;
+    chunk = std::max(kWindowChunk, round_up((seen + n - 1) / n, kStep));
+    if (chunk >= seen) return f;
+  }
+  f.chunk = (int)chunk;
+  f.splits = (int)((seen + chunk - 1) / chunk);
+  return f;
 }
 
 static int check_window(const char* who, int64_t window, int64_t sinks, FlashArgs* a) {

@@ -80,7 +80,7 @@ def test_plan_of_any_window(L, T, B, max_q, D):
             for sinks in (0, 4, 700, 2 ** 31, 2 ** 63 - 1):
                 sizes = (T, 20, 5, D, B, max_q, max_kv, window, sinks)
                 few, splits, chunk = plan(L, *sizes)
-                assert 1 <= splits <= 256 and 256 <= chunk <= 2 ** 30 and splits * chunk < 2 ** 31
+                assert 1 <= splits <= 256 and 128 <= chunk <= 2 ** 30 and chunk % 64 == 0 and splits * chunk < 2 ** 31
                 assert splits * chunk >= min(max_kv, window, 2 ** 30 - 1)
                 assert L.btl_paged_attention_window_scratch_bytes(*sizes) == (
                     splits * T * 20 * (D + 2) * 4 if splits > 1 else 0)
@@ -110,4 +110,7 @@ def test_python_refuses():
     assert pa.check_window(2 ** 63, 2 ** 70) == (2 ** 30, 2 ** 30)
     for bad in ((None, 3), (0, 0), (-1, 0), (5, -1)):
         with pytest.raises(ValueError):
+            pa.check_window(*bad)
+    for bad in ((4.5, 0), (4, 1.0), ("4", 0)):  # no whole numbers
+        with pytest.raises(TypeError):
             pa.check_window(*bad)
