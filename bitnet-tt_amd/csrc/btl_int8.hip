@@ -69,6 +69,10 @@ __device__ __forceinline__ float scaled(int acc, float sa, float sw) { return (f
 // blocks of 64 k in turn (wave w: w, w + 8, ...); the waves' sums meet in LDS.  A wave has two sets of U x CT
 // loads: while it works on one, the other's are on their way, across the sums of a group as well.  ONCE: a
 // wave's blocks are one set (K <= 512 U), so that its rows stay in registers for all groups.
+//
+// Bound by the weights' bytes: 128256 columns of 2560 to bf16, 1 / 16 / 32 / 64 rows 57 / 62 / 66 / 74 us, 5.7 / 5.4 / 5.1 / 4.6
+// TB/s (a large copy reaches 5.2); rows loaded again for each group 64 / 82 / 108 / 144.  Few columns: by latency, 3840 of
+// 2560 4.1-5.7 us.
 // ======================================================================
 constexpr int kI8Waves = 8;
 
@@ -199,7 +203,8 @@ __global__ __launch_bounds__(64 * kI8Waves, 2) void k_int8_stream(Int8Args p, in
   if (tid < p.M) p.tokens[tid] = arg_col(ld_coherent(p.keys + tid));
 }
 
-// The best of part blockIdx.x of row blockIdx.y; a row of one part is done.
+// The best of part blockIdx.x of row blockIdx.y; a row of one part is done.  Parts of at least 2048 columns, four workgroups a CU:
+// bound by the logits' bytes.
 __global__ __launch_bounds__(256) void k_int8_argmax(const float* y, int64_t ldo, int N, int each, uint64_t* keys, int32_t* tokens) {
   __shared__ uint64_t s_best[4];
   const int row = blockIdx.y, end = min(N, ((int)blockIdx.x + 1) * each);
@@ -227,8 +232,15 @@ __global__ __launch_bounds__(64) void k_int8_argmax_parts(const uint64_t* keys, 
 }
 
 // ======================================================================
-// Many rows: tiles of BM x BN, S stages of KG x 64 k in LDS, filled without registers.  The waves are KG groups
-// of WM x WN; a group takes its 64 k of every stage, and the groups' sums meet in LDS.
+// Many rows: tiles of BM x BN, S stages of KG x SUB x 64 k in LDS, filled without registers.  The waves are KG groups
+// of WM x WN; a group takes its blocks of 64 k of every stage, and the groups' sums meet in LDS.
+//
+// Large tiles: the matrix units are busy 43% (K = 2560) to 54% (8192) of the cycles; what remains is a tile's first loads, its
+// outputs, and the wait for operands that 256 x 256 x 128 k take in (64 KiB a step through each CU).  8192^3: 474 us, 2.32
+// POP/s (a large library product 2.12); 4096 x 2560 x 13824: 146 us, 1.99.  Small tiles: bound by the operands that pass
+// through each CU, at 37-50 B/ns a CU, and by latency, so that they have several stages on their way and the waves of a
+// workgroup share a small tile's k (511 x 2560 x 3840: 11.0 us).  The next tile's first stage loaded before the outputs are
+// stored, by workgroups of several tiles each: 1-3% slower (474 -> 482).
 // ======================================================================
 // 16 rows of a wave's TN blocks through its own LDS, so that they leave in whole lines: a lane has four columns
 // (4 (lane / 16) ..) of one row (lane % 16) of each block.
@@ -426,7 +438,7 @@ __global__ __launch_bounds__(512, 1) void k_int8_large(Int8Args p, int ngm, int 
   }
 }
 
-// ---- weights ---------------------------------------------------------------
+// ---- weights (once, when they are loaded) ---------------------------------------------------------------
 __global__ void k_int8_layout(const int8_t* w, int64_t ldw, int N, int K, int KB, int64_t total, uint4* out) {
   const int64_t g = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (g >= total) return;

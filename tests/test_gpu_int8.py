@@ -56,6 +56,18 @@ def test_few_rows_of_many_columns(M, K, Nf):
     check(*case(M, K, Nf, seed=5))
 
 
+@pytest.mark.parametrize("M", [1, 16, 32])
+@pytest.mark.parametrize("K", [64, 592, 1600])
+def test_few_rows_of_pairs_of_column_blocks(M, K):
+    check(*case(M, K, 33001, seed=6))
+
+
+@pytest.mark.parametrize("M", [1, 16, 17, 40])
+@pytest.mark.parametrize("Nf", [4096, 4100])
+def test_few_rows_that_do_not_stay_in_registers(M, Nf):
+    check(*case(M, 2576, Nf, seed=7))
+
+
 @pytest.mark.parametrize("M", [65, 100, 128, 129, 255, 256, 257, 400, 513])
 @pytest.mark.parametrize("K,Nf", [(16, 3), (64, 64), (144, 255), (192, 257), (640, 130), (2560, 300)])
 def test_many_rows(M, K, Nf):

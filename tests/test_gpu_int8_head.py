@@ -22,6 +22,13 @@ def head_of(K, V, seed=1, w=None):
     return head
 
 
+def codes_of(weight):
+    """The codes of the device layout, in 64 bits: blocks of 16 columns x 64 k, a lane's 16 bytes of column lane % 16."""
+    n, k = weight.out_features, weight.in_features
+    w = weight.data.view(torch.int8).view(-(-n // 16), -(-k // 64), 4, 16, 16).permute(0, 3, 1, 2, 4)
+    return w.reshape(-(-n // 16) * 16, -1)[:n, :k].double()
+
+
 def first_max(logits):
     """The first index of each row's largest number; -1: none is one."""
     x = logits.double().cpu().numpy()
@@ -46,6 +53,20 @@ def test_logits_and_tokens(M, K, V):
     assert torch.equal(q, q2) and torch.equal(s, s2)
     none, again = head(x, return_logits=False)
     assert none is None and torch.equal(again, tokens)
+
+
+@pytest.mark.parametrize("M", [2, 16, 17, 40, 64])
+@pytest.mark.parametrize("K,V", [(64, 33001), (576, 33001), (2592, 3001), (2592, 33001)])
+def test_tokens_of_few_rows_by_either_way(M, K, V):
+    """With and without logits, pairs of column blocks, rows that stay in registers and rows that do not."""
+    head = head_of(K, V)
+    x = normal((M, K), 3).to(torch.bfloat16).to(dev())
+    logits, tokens = head(x)
+    q, s = quantize_rows(x, head.norm_weight, 1e-5)
+    acc = (q.double() @ codes_of(head.weight).t()).float()  # whole numbers below 2^53
+    assert torch.equal(logits, acc * s[:, None] * head.weight.scale)
+    assert tokens.tolist() == first_max(logits)
+    assert torch.equal(head(x, return_logits=False)[1], tokens)
 
 
 @pytest.mark.parametrize("M", [1023, 1024, 1025, 1090, 2047, 2112])

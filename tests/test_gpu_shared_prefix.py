@@ -84,6 +84,14 @@ def test_empty_slots(max_q):
     assert bool((got[1] == 0).all()) and bool((got[3:] == 0).all())
 
 
+@pytest.mark.parametrize("max_q", [1, None])
+def test_the_first_slot_is_empty(max_q):
+    """Its table still names the shared pages; its user is gone."""
+    sb = SharedBatch([2, 1, 1], [0, 9, 40], 6, 4, 2, 64, 16, "fp8")
+    got = case(sb, max_q=max_q)
+    assert bool((got[:2] == 0).all())
+
+
 def test_rows_of_no_sequence_stay():
     sb = SharedBatch([2, 5], [7, 30], 6, 4, 2, 64, 16, "bf16")
     q = torch.zeros((12, 4, 64), dtype=torch.bfloat16, device=dev())
