@@ -659,7 +659,8 @@ __device__ __forceinline__ void tile_item(const FlashArgs& p, uint8_t* smem, int
     const int gap = MODE == kWindow ? src.span.gap : 0;
     const int whole_from = MODE != kWindow ? kv0 : max(gap > 0 ? src.span.turn : 0, wg_hi - p.window + 1 - gap);
     const int whole_end = min(kv_end, wg_lo + 1 - gap);
-    int kv = kv0, at = 0;  // step j at position kv; at: j's parity
+    // step j at position kv; at: the parity of its stages, 0 where the whole steps begin
+    int kv = kv0, at = MODE == kWindow ? (max(0, whole_from - kv0) + kStep - 1) / kStep & 1 : 0;
     auto arrived = [&] {
       __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this thread's loads
       lds_barrier();                       // everyone's; and what the last step read is free
@@ -676,14 +677,14 @@ __device__ __forceinline__ void tile_item(const FlashArgs& p, uint8_t* smem, int
     };
 
     src.fetch_pages(p, kv0, src.page_k);
-    src.template load<false>(p, kv0, sm);
-    src.template store<false>(sm);
+    src.template load<false>(p, kv0, sm + at * kB);
+    src.template store<false>(sm + at * kB);
     src.turn_pages(p, kv0 + kStep);
-    src.template load<true>(p, kv0, sm + 2 * kB);
-    src.template store<true>(sm + 2 * kB);
+    src.template load<true>(p, kv0, sm + (2 + at) * kB);
+    src.template store<true>(sm + (2 + at) * kB);
     if (kv0 + kStep < kv_end) {
-      src.template load<false>(p, kv0 + kStep, sm + kB);
-      src.template store<false>(sm + kB);
+      src.template load<false>(p, kv0 + kStep, sm + (at ^ 1) * kB);
+      src.template store<false>(sm + (at ^ 1) * kB);
     }
     src.turn_pages(p, kv0 + 2 * kStep);
     arrived();
@@ -697,8 +698,8 @@ __device__ __forceinline__ void tile_item(const FlashArgs& p, uint8_t* smem, int
       return (MODE == kWindow && src.span.mixed(u, kStep)) || some_see<MODE>(p, lo, hi, src.pos(u), kStep);
     };
     if (some_of(s.lo, s.hi, kv0)) {
-      tile_keys<D>(sm, keys);
-      tile_scores<D>(sm, keys, s, sa);
+      tile_keys<D>(sm + at * kB, keys);
+      tile_scores<D>(sm + at * kB, keys, s, sa);
       if (!all_of(s.lo, s.hi, kv0)) tile_mask<D, MODE>(p, src.span, s, kv0, sa);
       tile_raise<D>(s, p.c, sa);
     }
@@ -753,8 +754,8 @@ __device__ __forceinline__ void tile_item(const FlashArgs& p, uint8_t* smem, int
       kv += kStep;
       at ^= 1;
     };
-    if constexpr (MODE == kWindow)  // those that some rows do not see from their beginning, and on to where the stages are in order
-      while (kv < kv_end && (at == 1 || kv < whole_from)) edge();
+    if constexpr (MODE == kWindow)  // those that some rows do not see from their beginning
+      while (kv < kv_end && kv < whole_from) edge();
     while (kv + 2 * kStep <= whole_end) {
       hot(sm + kB, sm + 2 * kB, sm, sm + 3 * kB, sa, sb);
       if (kv + 2 * kStep > whole_end) {
