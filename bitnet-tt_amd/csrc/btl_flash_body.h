@@ -210,6 +210,10 @@ __device__ __forceinline__ void lds_st128(lds8* p, uint4 x) {
   typedef uint32_t v4u __attribute__((ext_vector_type(4)));
   *(__attribute__((address_space(3))) v4u*)p = (v4u){x.x, x.y, x.z, x.w};
 }
+__device__ __forceinline__ void lds_st64(lds8* p, uint2 x) {
+  typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+  *(__attribute__((address_space(3))) v2u*)p = (v2u){x.x, x.y};
+}
 // ds_read_b64_tr_b16: in each group of 16 lanes, lane j receives, for r =
 // 0..3, element j % 4 of the four 16-bit values that lane 4 r + j / 4 addresses:
 // with lane 4 r + q at row r, columns 4 q .. 4 q + 3, lane j gets column j of rows 0..3.
@@ -771,10 +775,9 @@ __device__ __forceinline__ void tile_item(const FlashArgs& p, uint8_t* smem, int
   }
 
   const float l0 = s.l[0] + s.l[1], l = l0 + xor_partner<32>(l0);
-  if (r >= rows) return;
   const int64_t row = sq.row0 + tok;
-  if (whole && p.splits > 1 && h == 0) p.part_ml[row * p.H + head] = make_float2(0.0f, kWhole);
   if (!whole) {
+    if (r >= rows) return;
     const int64_t at = ((int64_t)(split + (MODE == kOwn ? p.shared_splits : 0)) * p.bt.T + row) * p.H + head;
     if (h == 0) p.part_ml[at] = MODE == kOwn && s.limit < 0 ? make_float2(0.0f, kNone) : make_float2(s.m, l);
     if (empty(s.m, l)) return;
@@ -787,15 +790,28 @@ __device__ __forceinline__ void tile_item(const FlashArgs& p, uint8_t* smem, int
             make_float4(s.o[t][4 * i], s.o[t][4 * i + 1], s.o[t][4 * i + 2], s.o[t][4 * i + 3]);
     return;
   }
+  if (p.splits > 1 && h == 0 && r < rows) p.part_ml[row * p.H + head] = make_float2(0.0f, kWhole);
   const float inv = empty(s.m, l) ? 0.0f : 1.0f / l;
-  uint16_t* o = p.out + row * p.ldo + head * D + 4 * h;
+  // A wave's rows go through the stages, which are read, to leave in whole lines (16001 tokens, window 1 / 1024: 61 / 195 us from the
+  // registers, 50 / 181 so; no window 396, 392).  Partials leave from the registers: their lines are shorter only by half,
+  // and tiles of few rows would wait for this (drafts of 8 users 19.4, 21.1).
+  lds_barrier();
+  lds8* const mine = (lds8*)smem + wv * 32 * 2 * D;
 #pragma unroll
   for (int t = 0; t < D / 32; ++t)
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      *reinterpret_cast<uint2*>(o + 32 * t + 8 * i) =
-          make_uint2(f2bf_pair(s.o[t][4 * i] * inv, s.o[t][4 * i + 1] * inv),
-                     f2bf_pair(s.o[t][4 * i + 2] * inv, s.o[t][4 * i + 3] * inv));
+      lds_st64(mine + (lane & 31) * 2 * D + ((4 * t + i) ^ Tile<D>::k_swz(lane & 31)) * 16 + 8 * h,
+               make_uint2(f2bf_pair(s.o[t][4 * i] * inv, s.o[t][4 * i + 1] * inv),
+                          f2bf_pair(s.o[t][4 * i + 2] * inv, s.o[t][4 * i + 3] * inv)));
+  __builtin_amdgcn_wave_barrier();
+  const int64_t at = r < rows ? row * p.ldo + head * D : -1;
+#pragma unroll
+  for (int j = 0; j < D / 16; ++j) {
+    const int x = 64 * j + lane, y = x / (D / 8), c = x % (D / 8);
+    const int64_t to = __shfl(at, y);
+    if (to >= 0) *reinterpret_cast<uint4*>(p.out + to + 8 * c) = lds_ld128(mine + y * 2 * D + (c ^ Tile<D>::k_swz(y)) * 16);
+  }
 }
 
 // Workgroup x of units of `each` items that read the same keys and values: those are x's of one remainder by 8, which
