@@ -827,7 +827,7 @@ __device__ __forceinline__ UnitItem unit_item(int x, int each) {
 inline int64_t unit_groups(int64_t units, int64_t each) { return (units + kXcds - 1) / kXcds * kXcds * each; }
 
 // kWindow: neighbouring tiles of a head see mostly the same positions.  16001 tokens of 20 / 5 heads of 128, window 1024, 1 / 8 / 16 of
-// them on an XCD, one after the other: 203, 189, 191 us; chunks of 4 users, window 2000: 75.9, 73, 74.
+// them on an XCD, one after the other: 195, 180, 189 us; chunks of 4 users, window 2000: 67.4, 66.8, 68.2.
 constexpr int kNeighbours = 8;
 
 template <int D, int KV, int MODE>
