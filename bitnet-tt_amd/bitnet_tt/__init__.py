@@ -10,6 +10,9 @@ that make up that path:
 * ``bitnet_tt.layers.attention``    fused RMSNorm->QKV projection builders
 * ``bitnet_tt.ternary_matmul``      the ``ternary_matmul`` op
 * ``bitnet_tt.decode``              BitLinear chain of a batch-32 decode step
+* ``bitnet_tt.paged_attention``     prompts and the paged cache; windows, shared prefixes
+* ``bitnet_tt.lm_head``             final norm, head and greedy tokens (bf16 or 8-bit)
+* ``bitnet_tt.int8_matmul``         products of 8-bit integers with scales
 
 Compute runs in hand-written HIP kernels (libbtl.so, C ABI in include/btl.h).
 """

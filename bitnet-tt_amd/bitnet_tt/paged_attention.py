@@ -1,6 +1,7 @@
 """Prompts and the paged key-value cache: rotation with page writes, page reads,
-attention within packed prompts and over the pages, on gfx950 (include/btl.h,
-"prompts and the paged key-value cache").
+attention within packed prompts and over the pages, causal, within a window or of a
+batch that shares its first pages, on gfx950 (include/btl.h, "prompts and the paged
+key-value cache").
 
 The reference's prompt path is src/bitnet_tt/layers/attention.py:1348-1507,
 its caches :115-458.  A *batch* here is T packed rows: sequence b's rows are
