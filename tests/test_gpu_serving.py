@@ -204,3 +204,46 @@ def test_what_does_not_go_together():
     step.kv = []  # (load_contiguous refuses before it reads any)
     with pytest.raises(ValueError, match="window"):
         step.load_contiguous(table, ints([17]))
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+def test_pages_far_into_a_pool(kv):
+    """Offsets that pass 32 bits: the same pages at the end of a large pool give the same bits."""
+    page, Hkv, D, H = 64, 2, 128, 4
+    each = Hkv * page * D * (2 if kv == "bf16" else 1)
+    P = 2 ** 32 // each + 40
+    n = 30  # pages of two users of one prefix
+    small = pa.PagedKVCache.allocate(n, Hkv, D, dev(), page, kv)
+    big = pa.PagedKVCache.allocate(P, Hkv, D, dev(), page, kv)
+    for a, b in ((small.key_pages, big.key_pages), (small.value_pages, big.value_pages)):
+        x = normal((n, Hkv, page, D), a.element_size() + (b is big.value_pages))
+        a.copy_(x.to(a.dtype).to(dev()))
+        b.view(torch.uint8)[P - n:] = a.view(torch.uint8)
+    if kv == "fp8":
+        for a, b in ((small.key_exp, big.key_exp), (small.value_exp, big.value_exp)):
+            a.fill_(127)
+            b[P - n:] = a
+    table = torch.arange(n, dtype=torch.int32).view(2, -1)
+    table[1, :4] = table[0, :4]
+    len_, one = ints([900, 700]), ints([4])
+    for rows in (1, 40):
+        q = normal((2 * rows, H, D), 5).to(torch.bfloat16).to(dev())
+        cu = ints([0, rows, 2 * rows])
+        for call in (lambda c, t: pa.paged_attention(q, c, t, cu, len_, max_q=rows, window=500, sinks=70),
+                     lambda c, t: pa.shared_prefix_attention(q, c, t, cu, len_, one, max_q=rows)):
+            want = call(small, table.to(dev()))
+            assert bool(torch.isfinite(want).all()) and float(want.abs().max()) > 0
+            assert torch.equal(call(big, (table + (P - n)).to(dev())), want)
+    pa.check("cuda:0")
+
+
+def test_products_of_more_than_2_to_the_31_outputs():
+    """Offsets of outputs that pass 32 bits: the last rows are those of a call of their own."""
+    M, K, V = 17000, 32, 128256
+    head = LMHead(K, V, dev(), weight_dtype="int8")
+    head.load_final_weights(1 + 0.1 * normal((K,), 1), normal((V, K), 2))
+    x = normal((M, K), 3).to(torch.bfloat16).to(dev())
+    logits, tokens = head(x)
+    few, last = head(x[-40:])
+    assert torch.equal(logits[-40:], few) and torch.equal(tokens[-40:], last)
+    assert torch.equal(logits[:40], head(x[:40])[0])

@@ -9,6 +9,7 @@ import torch
 from paged_helpers import check_close, cu_of, dev, ints, normal
 from window_helpers import WindowBatch, attend_window64
 
+from bitnet_tt import _native as N
 from bitnet_tt import paged_attention as pa
 
 pytestmark = pytest.mark.gpu
@@ -129,6 +130,36 @@ def test_windows_that_are_split(kv, new, H, Hkv, D, window, sinks):
     paged_case(wb, max_q=max(new), max_kv=1024)  # hints below what is there
     wb = WindowBatch(new, total, H, Hkv, D, 16, kv, window, sinks)
     paged_case(wb, max_q=max(new), max_kv=5000)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+@pytest.mark.parametrize("page", [16, 64, 80])
+@pytest.mark.parametrize("new,total", [([40, 1, 30, 2, 0], [4000, 1, 90, 0, 60]), ([1, 1, 1, 1], [4000, 1, 0, 700])])
+@pytest.mark.parametrize("window,sinks", [(1500, 4), (700, 500), (2000, 0)])
+def test_windows_that_are_split_beside_short_contexts(kv, page, new, total, window, sinks):
+    """Splits that end inside the sinks, in the gap and in the windows; contexts that one workgroup has alone, and none."""
+    wb = WindowBatch(new, total, 4, 2, 64, page, kv, window, sinks)
+    paged_case(wb, max_q=max(new), max_kv=max(total))
+    sizes = (sum(new), 4, 2, 64, len(new), max(new), max(total), window, sinks)
+    assert N.lib().btl_paged_attention_window_scratch_bytes(*sizes) > 0  # they are split
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+@pytest.mark.parametrize("new", [[1, 1], [40, 9]])
+def test_splits_with_values_that_are_not_finite(kv, new):
+    """Seen by some of the rows of a split only, in sinks, at the windows' beginnings and at their ends."""
+    total, window, sinks = [3000, 1700], 1400, 70
+    wb = WindowBatch(new, total, 4, 2, 64, 16, kv, window, sinks, release=False)
+    first = total[0] - window  # the last row's first position
+    for position in (3, first - 20, first + 1, 2400, 2999):
+        page, row = int(wb.full_table[0][position // 16]), position % 16
+        if kv == "fp8":
+            wb.cache.value_pages.view(torch.uint8)[page, 1, row, position % 64] = 0x7F
+            wb.v64[page, 1, row, position % 64] = math.nan
+        else:
+            wb.cache.value_pages[page, 1, row, position % 64] = math.inf
+            wb.v64[page, 1, row, position % 64] = math.inf
+    paged_case(wb, max_q=max(new))
 
 
 @pytest.mark.parametrize("kv", ["bf16", "fp8"])
