@@ -40,6 +40,8 @@ __global__ __launch_bounds__(256, 2) void k_flash_shared(FlashArgs p, int shared
   }
 }
 
+constexpr int64_t kSharedSplits = 64;  // of tiles
+
 struct SharedPlan {
   bool shared_few;
   int64_t shared_items, own_items;  // of a key-value head
@@ -48,13 +50,13 @@ struct SharedPlan {
 };
 
 // max_kv: positions of the longest sequence, max_shared of them shared.
-//  - The shared positions in tiles: up to one workgroup a CU (a call has the sequences' own workgroups besides), unless
-//    the tiles alone are more; of these the split that costs least, P steps of a / n us and n partials of T H D 8 bytes:
-//    n = sqrt(a P / part) with a = 0.0085 us, a fitted constant, as what a step takes depends on the workgroups
-//    beside it.  20 / 5 heads of 128, bf16, us at about half of n / n / double: 32 users, 8192 positions (n = 23):
-//    27, 23, 25; 64, 16384 (23): 44, 42, 43; 64, 4096 (11): 24, 22, 22; 16, 8192 (32): 22, 23, 23; 48, 30000 (25): 66, 54, 69;
-//    16 x 5 rows, 16000 (17): 39, 41, 42; 32 x 4, 4096 (8): 27, 25, 29; 10 x 12, 2000 (5): 24, 24, 27.  8-bit pages, 32
-//    users, 8192 (23): 28, 25, 24; 64, 16384 (23): 45, 37, 43; 64, 65536 (25): 125, 93, 97.  A chunk is at least two steps.
+//  - The shared positions in tiles: the split of the least time, in units of a step of a workgroup that has its CU alone (among
+//    the tiles): steps x 1, or 1.4 where two share a CU, by the workgroups of an XCD, which has a unit's all (unit_item), in
+//    rounds; and 2.4 times what a split's partials take, as the merge reads them with the rest.  Fitted to 23 shapes at 10 to
+//    17 splits each; it takes the best of them, or is 2% above it in the mean and 9% at most.  20 / 5 heads of 128, bf16, us
+//    by splits: 200 rows of 8 users behind 16000 (7 tiles a head): 5: 88, 6: 77, 7: 84, 10: 73, 13: 60, 16: 74; 400 of
+//    4 (13): 5: 118, 6: 105, 7: 138, 12: 105; 32 users behind 8192 (1): 11: 26, 22: 22.5, 32: 24.5, 64: 26.6; 64 of 65536, 8-bit (2):
+//    16: 125, 32: 93, 64: 99, 128: 119.  A chunk is at least two steps.
 //  - Few rows in all: as for a call without a prefix.
 //  - Their own positions: the merge's launch is paid in any case, so that splits that fill two workgroups a CU pay from 512
 //    positions on: 16 users of 8192 + 1000, n = 1 / 2: 21.7, 19.5; 16 x 5 rows of 16000 + 1000, 1 / 2 / 4: 41, 39, 34.
@@ -75,11 +77,18 @@ inline SharedPlan shared_plan(int64_t T, int64_t H, int64_t Hkv, int64_t D, int6
     s.shared_splits = f.splits;
     s.shared_chunk = f.chunk;
   } else {
-    const double part = split_part(T, H, D);
-    int64_t n = (int64_t)(std::sqrt(0.0085 * (double)max_shared / part) + 0.5);
-    n = std::min(n, 2 * tiles <= cus ? cus / tiles : (4 * cus + tiles) / (2 * tiles));
-    n = std::max((int64_t)1, std::min(n, std::min(max_shared / (2 * kStep), kMaxSplits)));
-    s.shared_chunk = (int)round_up((max_shared + n - 1) / n, kStep);
+    const double part = 2.4 * split_part(T, H, D);
+    const int64_t place = std::max(cus / kXcds, (int64_t)1);  // an XCD's CUs
+    double least = 0;
+    for (int64_t n = 1; n <= std::max((int64_t)1, std::min(max_shared / (2 * kStep), kSharedSplits)); ++n) {
+      const int64_t groups = (Hkv * n + kXcds - 1) / kXcds * s.shared_items, full = (groups - 1) / (2 * place);
+      const int64_t chunk = round_up((max_shared + n - 1) / n, kStep);
+      const double step = 1.4 * (double)full + (groups - full * 2 * place > place ? 1.4 : 1.0);
+      const double t = step * (double)(chunk / kStep) + part * (double)n;
+      if (n > 1 && t >= least) continue;
+      least = t;
+      s.shared_chunk = (int)chunk;
+    }
     s.shared_splits = (int)((max_shared + s.shared_chunk - 1) / s.shared_chunk);
   }
   const int64_t rest = (2 * cus - tiles * s.shared_splits) / (s.own_items * Hkv);
