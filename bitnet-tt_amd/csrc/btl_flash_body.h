@@ -84,6 +84,7 @@ struct FlashArgs {
   float2* part_ml;  // [splits][T][H]: exponents' offset, sum
   // kWindow: the row at position p sees (p - window, p] and, up to p, [0, sinks)
   int window, sinks;
+  int neighbours;  // tiles of a head that run on one XCD, one after the other
   // kShared, kOwn: pages of the shared prefix (device).  Every row has shared_splits partials of
   // the prefix, then `splits` of its own positions; the sum of a row that sees nothing is kNone there.
   const int32_t* shared;
@@ -826,22 +827,28 @@ __device__ __forceinline__ UnitItem unit_item(int x, int each) {
 }
 inline int64_t unit_groups(int64_t units, int64_t each) { return (units + kXcds - 1) / kXcds * kXcds * each; }
 
-// kWindow: neighbouring tiles of a head see mostly the same positions.  16001 tokens of 20 / 5 heads of 128, window 1024, 1 / 8 / 16 of
-// them on an XCD, one after the other: 195, 180, 189 us; chunks of 4 users, window 2000: 67.4, 66.8, 68.2.
-constexpr int kNeighbours = 8;
-
 template <int D, int KV, int MODE>
 __global__ __launch_bounds__(256, 2) void k_flash_tile(FlashArgs p) {
   __shared__ __attribute__((aligned(16))) uint8_t smem[kTileShared<D>];
   if (MODE == kWindow) {
-    const UnitItem u = unit_item(blockIdx.x, kNeighbours);
-    tile_item<D, KV, MODE>(p, smem, uni(u.unit % p.Hkv), u.unit / p.Hkv * kNeighbours + u.item, blockIdx.y);
+    const UnitItem u = unit_item(blockIdx.x, p.neighbours);
+    tile_item<D, KV, MODE>(p, smem, uni(u.unit % p.Hkv), u.unit / p.Hkv * p.neighbours + u.item, blockIdx.y);
   } else {
     tile_item<D, KV, MODE>(p, smem, uni(blockIdx.x % p.Hkv), blockIdx.x / p.Hkv, blockIdx.y);
   }
 }
-inline int64_t window_groups(int64_t tiles, int64_t Hkv) {  // tiles: of all heads
-  return unit_groups((tiles / Hkv + kNeighbours - 1) / kNeighbours * Hkv, kNeighbours);
+// kWindow: how many neighbouring tiles of a head, which see mostly the same positions, run on one XCD, one after the other: so
+// many that each XCD has several such groups, up to 8.  20 / 5 heads of 128, window 1024, us with 1 / 2 / 4 / 8 / 16: 16001 tokens
+// (2520 tiles of all heads) 198, 189, 186, 180, 188; 8000 (1270) 91.5, 85.5, 83.8, 86.6, 87.6; 4000 (640) 60.6, 57.9, 58.4, 60.6,
+// 62; 2000 (320) 30.5, 30.4, 30.5, 30.9, 31.0; over pages, chunks of 4000 (640), window 2000: 130, 117, 116, 116, 116.  Splits
+// read different positions, and want the XCDs evenly full: 500 rows at a window of 4096 in 4 (80 tiles), 1 / 8: 42, 46.
+inline int window_neighbours(int64_t tiles, int splits) {
+  int each = 1;
+  while (splits == 1 && each < 8 && 2 * each * 5 * device_cus() <= 8 * tiles) each *= 2;
+  return each;
+}
+inline int64_t window_groups(int64_t tiles, int64_t Hkv, int each) {
+  return unit_groups((tiles / Hkv + each - 1) / each * Hkv, each);
 }
 
 // ======================================================================

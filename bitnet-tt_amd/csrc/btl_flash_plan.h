@@ -190,8 +190,9 @@ inline int partials(const char* who, void* scratch, size_t bytes, int64_t need, 
 }
 
 template <int MODE>
-inline int launch_prompt(const char* what, const FlashArgs& a, int64_t tiles, int64_t D, hipStream_t stream) {
-  const dim3 grid((unsigned)(MODE == kWindow ? window_groups(tiles, a.Hkv) : tiles));
+inline int launch_prompt(const char* what, FlashArgs a, int64_t tiles, int64_t D, hipStream_t stream) {
+  a.neighbours = window_neighbours(tiles, 1);
+  const dim3 grid((unsigned)(MODE == kWindow ? window_groups(tiles, a.Hkv, a.neighbours) : tiles));
   if (D == 128)
     hipLaunchKernelGGL((k_flash_tile<128, kDense, MODE>), grid, dim3(256), 0, stream, a);
   else
@@ -225,7 +226,8 @@ inline int launch_paged(const char* who, const char* what, const FlashPlan& f, F
     }
     hipLaunchKernelGGL(kern, grid, dim3(threads), 0, stream, *a);
   } else {
-    const dim3 grid((unsigned)(MODE == kWindow ? window_groups(f.tiles, a->Hkv) : f.tiles), (unsigned)f.splits);
+    a->neighbours = window_neighbours(f.tiles, f.splits);
+    const dim3 grid((unsigned)(MODE == kWindow ? window_groups(f.tiles, a->Hkv, a->neighbours) : f.tiles), (unsigned)f.splits);
     auto* kern = D == 128 ? (fp8 ? k_flash_tile<128, kPagedFp8, MODE> : k_flash_tile<128, kPagedBf16, MODE>)
                           : (fp8 ? k_flash_tile<64, kPagedFp8, MODE> : k_flash_tile<64, kPagedBf16, MODE>);
     hipLaunchKernelGGL(kern, grid, dim3(256), 0, stream, *a);

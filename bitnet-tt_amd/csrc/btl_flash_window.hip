@@ -12,10 +12,11 @@ namespace btl {
 //    256): 16.1, 13.8, 15.7, 27.4; 8 users, 8-bit, 1024 (256): 13.5, 12.4, 13.7, 14.3.  Where it shortens the longest workgroup
 //    by less than 576 positions the merge's launch costs more, 25 users, 1024, 640 / one: 8-bit 16.7, 14.8; bf16 20.0, 19.5.  From a
 //    workgroup on every other CU on: as without a window.
-//  - Tiles: what comes nearest to 1.4 workgroups a CU, by the rule on what a split costs (FlashPlan), a chunk not below 192.
-//    bf16, 1 / 2 / 3 / 4 / 5 / 6 / 8 splits: 500 rows of one user, 4096 (80 tiles of rows and heads): 85, 55, 50, 47, 57, 56, 60; 250, 4096 (40): -,
-//    53, 42, 36.2, 37.4, 36.6, 35.2; 1000, 4096 (160): -, 73, 83, 73, 75; 20 users of 10, 2000 (100): 49, 41, 34, 30, 38; 4 users' 2047
-//    rows, 2000 (340): 68, 69. 8-bit, 8 users of 1-10 rows, 1024 (40), chunks of 192 / 256 / 512: 20.4, 21.1, 27.1.
+//  - Tiles: up to two workgroups a CU on every XCD, by the rule on what a split costs (FlashPlan), a chunk not below 192.
+//    bf16, 1 / 2 / 3 / 4 / 6 / 8 splits: 500 rows of one user, 4096 (80 tiles of rows and heads): -, 54, 43, 42, 44, 54; 250, 4096
+//    (40): -, 52, 40, 34, 29.5, 33; 1000, 4096 (160): -, 71, 67, 84, 78, 84; 20 users of 10, 2000 (100): 50, 36, 33, 30.5, 34;
+//    4 users' 2047 rows, 2000 (340): 68, 69.  8-bit, 8 users of 1-10 rows, 1024 (40), chunks of 192 / 256 / 512: 18.6, 19.1,
+//    24.2.
 constexpr int64_t kWindowSplits = 36;
 constexpr int64_t kWindowGain = 576;
 constexpr int64_t kWindowChunk = 192;
@@ -36,7 +37,7 @@ inline FlashPlan window_plan(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64
   } else {
     const int64_t tiles = std::min(f.tiles, B * ((std::min(max_q, T) * G + kTileRows - 1) / kTileRows) * Hkv);  // (if the hint holds)
     const double whole = split_whole(seen), part = split_part(T, H, D);
-    n = std::min((7 * cus / 5 + tiles / 2) / tiles, (int64_t)(std::sqrt(whole / part) + 0.5));
+    n = std::min(2 * cus / kXcds / ((tiles + kXcds - 1) / kXcds), (int64_t)(std::sqrt(whole / part) + 0.5));
     if (n <= 1 || whole - whole / (double)n <= 4.0 + part * (double)n) return f;
     chunk = std::max(kWindowChunk, round_up((seen + n - 1) / n, kStep));
     if (chunk >= seen) return f;
