@@ -52,11 +52,12 @@ struct SharedPlan {
 // max_kv: positions of the longest sequence, max_shared of them shared.
 //  - The shared positions in tiles: the split of the least time, in units of a step of a workgroup that has its CU alone (among
 //    the tiles): steps x 1, or 1.4 where two share a CU, by the workgroups of an XCD, which has a unit's all (unit_item), in
-//    rounds; and 2.4 times what a split's partials take, as the merge reads them with the rest.  Fitted to 23 shapes at 10 to
-//    17 splits each; it takes the best of them, or is 2% above it in the mean and 9% at most.  20 / 5 heads of 128, bf16, us
+//    rounds; and 2.4 times what a split's partials take, as the merge reads them with the rest.  Against the best of up to 27 splits
+//    in 26 shapes it is 3% above in the mean, 14% at most (128 users of up to 2000 behind 16384, 8-bit, whose own positions keep
+//    the CUs busy besides; their work in the rule gains nothing unless it knows the pages' type).  20 / 5 heads of 128, bf16, us
 //    by splits: 200 rows of 8 users behind 16000 (7 tiles a head): 5: 88, 6: 77, 7: 84, 10: 73, 13: 60, 16: 74; 400 of
-//    4 (13): 5: 118, 6: 105, 7: 138, 12: 105; 32 users behind 8192 (1): 11: 26, 22: 22.5, 32: 24.5, 64: 26.6; 64 of 65536, 8-bit (2):
-//    16: 125, 32: 93, 64: 99, 128: 119.  A chunk is at least two steps.
+//    4 (13): 5: 118, 6: 105, 7: 138, 12: 105; 32 users behind 8192 (1): 11: 26, 22: 22.5, 32: 24.5, 64: 26.6; 64 of 65536,
+//    8-bit (2): 16: 125, 25: 92, 32: 91, 36: 85, 64: 99.  A chunk is at least two steps.
 //  - Few rows in all: as for a call without a prefix.
 //  - Their own positions: the merge's launch is paid in any case, so that splits that fill two workgroups a CU pay from 512
 //    positions on: 16 users of 8192 + 1000, n = 1 / 2: 21.7, 19.5; 16 x 5 rows of 16000 + 1000, 1 / 2 / 4: 41, 39, 34.

@@ -236,10 +236,10 @@ __global__ __launch_bounds__(64) void k_int8_argmax_parts(const uint64_t* keys, 
 // of WM x WN; a group takes its blocks of 64 k of every stage, and the groups' sums meet in LDS.
 //
 // Large tiles: the matrix units are busy 43% (K = 2560) to 54% (8192) of the cycles; what remains is a tile's first loads, its
-// outputs, and the wait for operands that 256 x 256 x 128 k take in (64 KiB a step through each CU).  8192^3: 474 us, 2.32
-// POP/s (a large library product 2.12); 4096 x 2560 x 13824: 146 us, 1.99.  Small tiles: bound by the operands that pass
+// outputs, and the wait for operands that 256 x 256 x 128 k take in (64 KiB a step through each CU).  8192^3: 445 us, 2.47
+// POP/s (a large library product 2.12); 4096 x 2560 x 13824: 142-149 us, 1.95-2.04.  Small tiles: bound by the operands that pass
 // through each CU, at 37-50 B/ns a CU, and by latency, so that they have several stages on their way and the waves of a
-// workgroup share a small tile's k (511 x 2560 x 3840: 11.0 us).  The next tile's first stage loaded before the outputs are
+// workgroup share a small tile's k (511 x 2560 x 3840: 10.7 us).  The next tile's first stage loaded before the outputs are
 // stored, by workgroups of several tiles each: 1-3% slower (474 -> 482).
 // ======================================================================
 // 16 rows of a wave's TN blocks through its own LDS, so that they leave in whole lines: a lane has four columns
@@ -418,23 +418,50 @@ __device__ __forceinline__ void int8_tile(const Int8Args& p, uint8_t* smem, int 
   }
 }
 
+// Tiles in strips of `strip` rows of them, column by column; a workgroup's XCD is its number's remainder by 8, and takes a part of
+// that order, so that what it works on at a time is nearly square, and its L2 reads few rows and columns.  Numbers as they come,
+// down the rows / strips of 2 / 4 / 8 / 16: 4096 x 2560 x 13824 150, 152, 142, 143, 146 us; 1024 x 2560 x 6912 27.0, 24.0, 23.4, 24.6, 24.6;
+// 300 x 2560 x 128256 (fp32) 183, 182, 165, 160, 164; 511 x 2560 x 3840 11.1, 10.8, 10.7, 10.8, 10.8; 128 x 6912 x 2560, two rows of
+// tiles, 12.7, 13.2, 13.1, 13.1, 13.1.
+constexpr int kXcds8 = 8;
+struct TileAt {
+  int m, n;
+};
+__device__ __forceinline__ TileAt tile_at(int t, int ngm, int ngn, int strip) {
+  const int s = t / (strip * ngn), in = t - s * strip * ngn, h = min(strip, ngm - s * strip);
+  return {uni8(s * strip + in % h), uni8(in / h)};
+}
+// Workgroup x's place of `tiles`; -1: none.
+__device__ __forceinline__ int xcd_place(int x, int tiles) {
+  const int each = (tiles + kXcds8 - 1) / kXcds8, t = x % kXcds8 * each + x / kXcds8;
+  return x / kXcds8 < each && t < tiles ? t : -1;
+}
+inline int xcd_groups(int tiles) { return (tiles + kXcds8 - 1) / kXcds8 * kXcds8; }
+
 template <int BM, int BN, int WM, int WN, int KG, int SUB, int S, int PER_CU>
-__global__ __launch_bounds__(64 * WM * WN * KG, PER_CU) void k_int8_tile(Int8Args p, int ngm) {
+__global__ __launch_bounds__(64 * WM * WN * KG, PER_CU) void k_int8_tile(Int8Args p, int ngm, int ngn, int strip) {
   __shared__ __attribute__((aligned(16))) uint8_t smem[TileShape<BM, BN, WM, WN, KG, SUB, S>::kBytes];
-  int8_tile<BM, BN, WM, WN, KG, SUB, S>(p, smem, uni8(blockIdx.x % ngm) * BM, uni8(blockIdx.x / ngm) * (BN / 16));
+  const int t = xcd_place(blockIdx.x, ngm * ngn);
+  if (t < 0) return;
+  const TileAt at = tile_at(t, ngm, ngn, strip);
+  int8_tile<BM, BN, WM, WN, KG, SUB, S>(p, smem, at.m * BM, at.n * (BN / 16));
 }
 
 // Tiles of 256 x 256, the last ones (from `full` on) as two of 128 rows each: they fill the CUs once more where
 // whole tiles would fill half of them for twice as long.
-__global__ __launch_bounds__(512, 1) void k_int8_large(Int8Args p, int ngm, int full) {
+__global__ __launch_bounds__(512, 1) void k_int8_large(Int8Args p, int ngm, int ngn, int full, int strip) {
   constexpr int kBytes = std::max(TileShape<256, 256, 2, 4, 1, 2, 2>::kBytes, TileShape<128, 256, 2, 4, 1, 2, 3>::kBytes);
   __shared__ __attribute__((aligned(16))) uint8_t smem[kBytes];
-  const int x = blockIdx.x;
-  if (x < full) {
-    int8_tile<256, 256, 2, 4, 1, 2, 2>(p, smem, uni8(x % ngm) * 256, uni8(x / ngm) * 16);
+  const int whole = (full + kXcds8 - 1) / kXcds8 * kXcds8, x = (int)blockIdx.x - whole;
+  if (x < 0) {
+    const int t = xcd_place(blockIdx.x, full);
+    if (t < 0) return;
+    const TileAt at = tile_at(t, ngm, ngn, strip);
+    int8_tile<256, 256, 2, 4, 1, 2, 2>(p, smem, at.m * 256, at.n * 16);
   } else {
-    const int t = full + (x - full) / 2, m0 = uni8(t % ngm) * 256 + uni8((x - full) & 1) * 128;
-    if (m0 < p.M) int8_tile<128, 256, 2, 4, 1, 2, 3>(p, smem, m0, uni8(t / ngm) * 16);
+    const TileAt at = tile_at(full + x / 2, ngm, ngn, strip);
+    const int m0 = at.m * 256 + (x & 1) * 128;
+    if (m0 < p.M) int8_tile<128, 256, 2, 4, 1, 2, 3>(p, smem, m0, at.n * 16);
   }
 }
 
@@ -516,11 +543,13 @@ static void launch_stream(const Int8Args& a, int groups, dim3 grid, hipStream_t 
     hipLaunchKernelGGL((k_int8_stream<RB, CT, RB == 4 ? 2 : 4, false>), grid, dim3(64 * kI8Waves), 0, s, a, groups);
 }
 
+constexpr int kStrip = 4;  // rows of tiles
+
 template <int BM, int BN, int WM, int WN, int KG, int SUB, int S, int PER_CU>
 static void launch_tile(const Int8Args& a, hipStream_t s) {
   const int ngm = (a.M + BM - 1) / BM, ngn = (a.NT * 16 + BN - 1) / BN;
-  hipLaunchKernelGGL((k_int8_tile<BM, BN, WM, WN, KG, SUB, S, PER_CU>), dim3((unsigned)(ngm * ngn)), dim3(64 * WM * WN * KG), 0, s,
-                     a, ngm);
+  hipLaunchKernelGGL((k_int8_tile<BM, BN, WM, WN, KG, SUB, S, PER_CU>), dim3((unsigned)xcd_groups(ngm * ngn)),
+                     dim3(64 * WM * WN * KG), 0, s, a, ngm, ngn, kStrip);
 }
 
 // Of `tiles` large ones, how many go as halves: a last round that fills at most half of the CUs.  4096 x 2560 x 13824 (864 tiles)
@@ -528,16 +557,17 @@ static void launch_tile(const Int8Args& a, hipStream_t s) {
 static int64_t large_halves(int64_t tiles, int64_t cus) { return tiles > cus && 2 * (tiles % cus) <= cus ? tiles % cus : 0; }
 
 static void launch_large(const Int8Args& a, int cus, hipStream_t s) {
-  const int ngm = (a.M + 255) / 256, tiles = ngm * ((a.NT + 15) / 16), halves = (int)large_halves(tiles, cus);
-  hipLaunchKernelGGL(k_int8_large, dim3((unsigned)(tiles + halves)), dim3(512), 0, s, a, ngm, tiles - halves);
+  const int ngm = (a.M + 255) / 256, ngn = (a.NT + 15) / 16, tiles = ngm * ngn, halves = (int)large_halves(tiles, cus);
+  hipLaunchKernelGGL(k_int8_large, dim3((unsigned)(xcd_groups(tiles - halves) + 2 * halves)), dim3(512), 0, s, a, ngm, ngn,
+                     tiles - halves, kStrip);
 }
 
 // The tile of the least time, us: rounds of workgroups over the CUs x what a workgroup takes, for a start (and an end) and for
-// each 128 k; alone on its CU, or beside another one.  Fitted to 70 shapes, 65-8192 rows, K 576-6912, 640-128256
-// columns: the rule takes the best of the five for 64 of them, within 2% of it for the others.  Us of each, in this order:
-// 4096 x 2560 x 13824: 146, 173, 230, 306, 285; 1024 x 2560 x 6912: 35, 28, 32, 39, 38; 256 x 2560 x 13824: 36, 25, 20, 27, 28;
-// 511 x 2560 x 3840: 34, 21, 13, 11, 14; 128 x 6912 x 2560: 77, 46, 27, 18, 13; 400 x 640 x 2560: 13, 9, 6.9, 5.9, 6.5.
-// (128 x 128 as two a CU is never more than 2% better, 64 x 64 as one of 8 stages never better.)
+// each 128 k; alone on its CU, or beside another one.  Fitted to 69 shapes, 65-8192 rows, K 576-6912, 640-128256
+// columns: the rule takes the best of the five for 67 of them, and is 5 and 8% above it for the others.  Us of each, in this order:
+// 4096 x 2560 x 13824: 146, 173, 230, 306, 285 (in rows of tiles, not strips); 1024 x 2560 x 6912: 36, 25, 29, 38, 35; 256 x 2560 x
+// 13824: 36, 24, 19, 27, 26; 511 x 2560 x 3840: 34, 21, 14, 10.9, 11.8; 128 x 6912 x 2560: 77, 46, 28, 19, 13; 400 x 640 x 2560: 13,
+// 9, 7.0, 5.8, 6.0.  (128 x 128 as two a CU is never more than 2% better, 64 x 64 as one of 8 stages never better.)
 struct TileCost {
   int bm, bn, per_cu;
   double start, step;          // one on a CU
@@ -603,11 +633,11 @@ static int int8_args(const char* who, const int8_t* a, int64_t lda, const float*
   return BTL_OK;
 }
 
-// Whether the weight stream takes it, where a few rows' argmax is wanted without logits in any case.  Us of the stream / of tiles, K =
-// 2560, 16 rows: 640 columns 3.8 / 6.5, 3840: 4.6 / 7.0, 13824: 10.0 / 9.7, 128256: 66.7 / 72; 32 rows: 5.0 / 6.6, 5.7 / 7.1, 11.5 /
-// 11.0, 69.6 / 73; 64 rows: 7.3 / 6.7, 8.4 / 7.3, 15.5 / 12.3, 76.6 / 78.  K = 6912, where rows are loaded again for each group
-// of columns, 16 rows: 640: 8.9 / 12.7, 3840: 9.5 / 12.9, 13824: 27.6 / 20.8, 40000: 63 / 59; 32 rows: 14.0 / 12.8, 14.5 / 13.0,
-// 36 / 22, 80 / 61.
+// Whether the weight stream takes it, where a few rows' argmax is wanted without logits in any case.  Us of the stream / of tiles,
+// K = 2560, 16 rows: 640 columns 3.9 / 6.4, 3840: 4.7 / 7.1, 13824: 10.2 / 10.6, 128256: 66 / 71; 32 rows: 5.0 / 6.7, 5.8 / 7.1,
+// 11.9 / 11.1, 70 / 74; 64 rows: 7.3 / 6.9, 8.5 / 7.3, 14.7 / 11.7, 76 / 78.  K = 6912, where rows are loaded again for each group
+// of columns, 16 rows: 640: 8.9 / 12.9, 3840: 9.5 / 13.2, 13824: 34 / 21, 40000: 64 / 59; 32 rows: 14.1 / 12.8, 14.6 / 13.2, 48 / 22,
+// 80 / 59.
 static bool streams_once(const Int8Args& p) { return p.KB <= 5 * kI8Waves; }
 static bool few_rows(const Int8Args& p, int cus) {
   if (p.tokens) return true;
