@@ -240,7 +240,7 @@ __global__ __launch_bounds__(64) void k_int8_argmax_parts(const uint64_t* keys, 
 // POP/s (a large library product 2.12); 4096 x 2560 x 13824: 142-149 us, 1.95-2.04.  Small tiles: bound by the operands that pass
 // through each CU, at 37-50 B/ns a CU, and by latency, so that they have several stages on their way and the waves of a
 // workgroup share a small tile's k (511 x 2560 x 3840: 10.7 us).  The next tile's first stage loaded before the outputs are
-// stored, by workgroups of several tiles each: 1-3% slower (474 -> 482).
+// stored, by workgroups of several tiles each: 1-3% slower (474 -> 482); weights two steps ahead, in a third stage: no gain.
 // ======================================================================
 // 16 rows of a wave's TN blocks through its own LDS, so that they leave in whole lines: a lane has four columns
 // (4 (lane / 16) ..) of one row (lane % 16) of each block.
