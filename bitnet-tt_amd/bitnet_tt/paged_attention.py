@@ -383,7 +383,8 @@ def shared_prefix_attention(q, cache: PagedKVCache, page_table, cu_q, kv_len, sh
     shared_pages int32 [1] on the device: how many whole pages, those that ``page_table[0]``
     begins with (what the other rows of the table have there is not read).  Every row's
     position must be behind them, but for padding; kv_len counts them.  max_shared,
-    where known, is the most shared pages (a hint, as max_q and max_kv).  Several
+    where known, is the most shared pages (a hint, as max_q and max_kv; where it is not given, both
+    parts are split for contexts of max_kv).  Several
     groups with a prefix each: a call each, on slices of page_table, cu_q and kv_len."""
     index = cache.index
     if index != torch.cuda.current_device():
@@ -404,7 +405,6 @@ def shared_prefix_attention(q, cache: PagedKVCache, page_table, cu_q, kv_len, sh
     most = max_pages * page_size
     max_q = T if max_q is None or max_q > T else max_q
     max_kv = most if max_kv is None or max_kv > most else max_kv
-    max_shared = max_pages if max_shared is None or max_shared > max_pages else max_shared
     if out is None:
         out = q.new_empty(T, H, D)
         ldo = H * D
@@ -412,10 +412,10 @@ def shared_prefix_attention(q, cache: PagedKVCache, page_table, cu_q, kv_len, sh
         ldo = _rows(out, T, H, D, "out", index)
     if T == 0:
         return out
-    if max_q < 1 or max_kv < 1 or max_shared < 0:
+    if max_q < 1 or max_kv < 1 or (max_shared is not None and max_shared < 0):
         raise ValueError(f"max_q {max_q} and max_kv {max_kv} must be at least 1, max_shared {max_shared} at least 0")
     stream = N.raw_stream(index)
-    max_shared *= page_size
+    max_shared = _shared_positions(max_shared, page_size, max_kv)
     nbytes = _shared_scratch_bytes(index, T, H, Hkv, D, B, max_q, max_kv, max_shared)
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device)  # the call's own
     rc = N.lib().btl_shared_prefix_attention(
@@ -425,6 +425,11 @@ def shared_prefix_attention(q, cache: PagedKVCache, page_table, cu_q, kv_len, sh
     if rc != N.BTL_OK:
         N.check(rc, "btl_shared_prefix_attention")
     return out
+
+
+def _shared_positions(max_shared, page_size, max_kv):
+    """The hint in positions: no more than the longest sequence has, max_kv where it is not given."""
+    return max_kv if max_shared is None else min(max_shared * page_size, max_kv)
 
 
 @functools.lru_cache(maxsize=4096)

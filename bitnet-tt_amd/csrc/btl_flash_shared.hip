@@ -49,7 +49,7 @@ struct SharedPlan {
   FlashPlan own;
 };
 
-// max_kv: positions of the longest sequence, max_shared of them shared.
+// max_kv: positions of the longest sequence, max_shared of them shared (max_kv or more: not known).
 //  - The shared positions in tiles: the split of the least time, in units of a step of a workgroup that has its CU alone (among
 //    the tiles): steps x 1, or 1.4 where two share a CU, by the workgroups of an XCD, which has a unit's all (unit_item), in
 //    rounds; and 2.4 times what a split's partials take, as the merge reads them with the rest.  Against the best of up to 27 splits
@@ -61,13 +61,16 @@ struct SharedPlan {
 //  - Few rows in all: as for a call without a prefix.
 //  - Their own positions: the merge's launch is paid in any case, so that splits that fill two workgroups a CU pay from 512
 //    positions on: 16 users of 8192 + 1000, n = 1 / 2: 21.7, 19.5; 16 x 5 rows of 16000 + 1000, 1 / 2 / 4: 41, 39, 34.
+//    Where the shared positions are not known they are planned for all of max_kv: 4 users of 1024 + 16000 39 us (with one
+//    position of their own 147, known 34), 32 of 8192 + 500 23.6 (known 22.2), 16 of 2048 + 4000 30.5 (known 35).
 inline SharedPlan shared_plan(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t B, int64_t max_q, int64_t max_kv,
                               int64_t max_shared) {
   SharedPlan s{};
   const int64_t G = H / Hkv, cus = device_cus();
   // (both parts' ends together stay below 2^31)
   max_shared = std::max(std::min(max_shared, kMaxPositions), (int64_t)1);
-  const int64_t own = std::min(std::max(max_kv - max_shared, (int64_t)1), kMaxPositions / 2);
+  // a prefix as long as the sequences is no known length: their own positions may be all of theirs
+  const int64_t own = std::min(max_shared < max_kv ? max_kv - max_shared : max_kv, kMaxPositions / 2);
   s.own = flash_plan(T, H, Hkv, D, B, max_q, own, true);
   s.own_items = s.own.few ? B : s.own.tiles / Hkv;
   s.shared_few = T * G <= kFewRows && s.own.few;

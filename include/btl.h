@@ -550,8 +550,8 @@ int btl_paged_attention_window(const uint16_t* q, int64_t ldq, int64_t T, int64_
  * page_table[0] begins with, whole.  Their positions are read once for the rows of all sequences; of the
  * other sequences' tables the first shared_pages entries are not read.  A row before the end of the shared
  * positions (but for rows with a negative position: zeros), or a shared_pages outside [0, max_pages],
- * sets the error word.  max_kv: as there; max_shared: an upper bound of the shared positions where known, a hint
- * too.  scratch: always, of btl_shared_prefix_attention_scratch_bytes with the same arguments. */
+ * sets the error word.  max_kv: as there; max_shared: an upper bound of the shared positions where known, else
+ * max_kv (the sequences' own positions are then planned for max_kv as well): a hint too.  scratch: always, of btl_shared_prefix_attention_scratch_bytes with the same arguments. */
 int64_t btl_shared_prefix_attention_scratch_bytes(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t B, int64_t max_q,
                                                   int64_t max_kv, int64_t max_shared);
 int btl_shared_prefix_attention(const uint16_t* q, int64_t ldq, int64_t T, int64_t H, const btl_pages_t* pages,
