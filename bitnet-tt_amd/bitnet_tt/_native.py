@@ -144,6 +144,7 @@ EXPORTS = {
     "btl_int8_weight_layout": ([_P, _I64, _I64, _I64, _P, _P], _I),
     "btl_int8_weight_quantise": ([_P, _I, _I64, _I64, _I64, _P, _P, _P], _I),
     "btl_int8_matmul": ([_P, _I64, _P, _I64, _I64, _I64, _P, _P, _P, _I64, _I, _P], _I),
+    "btl_int8_matmul_plan": ([_I64, _I64, _I64, _P], _I),
     "btl_int8_head_scratch_bytes": ([_I64, _I64, _I64], _I64),
     "btl_int8_head": ([_P, _I64, _I64, _I64, _P, _F, _P, _P, _P, _P, _P, _P, _SZ, _P], _I),
     "btl_decode_attention_workspace_bytes": ([_I64, _I64, _I64, _I64], _I64),

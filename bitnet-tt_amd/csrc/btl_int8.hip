@@ -556,8 +556,8 @@ static void launch_tile(const Int8Args& a, hipStream_t s) {
 // 155 us, 146 so; 8192 x 2560 x 2560 (320) 84, 64.
 static int64_t large_halves(int64_t tiles, int64_t cus) { return tiles > cus && 2 * (tiles % cus) <= cus ? tiles % cus : 0; }
 
-static void launch_large(const Int8Args& a, int cus, hipStream_t s) {
-  const int ngm = (a.M + 255) / 256, ngn = (a.NT + 15) / 16, tiles = ngm * ngn, halves = (int)large_halves(tiles, cus);
+static void launch_large(const Int8Args& a, int halves, hipStream_t s) {
+  const int ngm = (a.M + 255) / 256, ngn = (a.NT + 15) / 16, tiles = ngm * ngn;
   hipLaunchKernelGGL(k_int8_large, dim3((unsigned)(xcd_groups(tiles - halves) + 2 * halves)), dim3(512), 0, s, a, ngm, ngn,
                      tiles - halves, kStrip);
 }
@@ -638,19 +638,31 @@ static int int8_args(const char* who, const int8_t* a, int64_t lda, const float*
 // 11.9 / 11.1, 70 / 74; 64 rows: 7.3 / 6.9, 8.5 / 7.3, 14.7 / 11.7, 76 / 78.  K = 6912, where rows are loaded again for each group
 // of columns, 16 rows: 640: 8.9 / 12.9, 3840: 9.5 / 13.2, 13824: 34 / 21, 40000: 64 / 59; 32 rows: 14.1 / 12.8, 14.6 / 13.2, 48 / 22,
 // 80 / 59.
-static bool streams_once(const Int8Args& p) { return p.KB <= 5 * kI8Waves; }
-static bool few_rows(const Int8Args& p, int cus) {
-  if (p.tokens) return true;
-  return streams_once(p) ? p.M <= 32 : p.M <= 16 && p.NT <= cus;
+static bool streams_once(int64_t K) { return int8_kb(K) <= 5 * kI8Waves; }
+static bool few_rows(int64_t M, int64_t N, int64_t K, bool tokens, int cus) {
+  if (tokens) return true;
+  return streams_once(K) ? M <= 32 : M <= 16 && int8_nt(N) <= cus;
+}
+
+// How a product is done: the weight stream in groups of `ct` column blocks (0: not so), or a tile of kTiles, of which `halves`
+// large ones go as two.
+struct Int8Plan {
+  int ct, tile, halves;
+};
+static Int8Plan int8_plan(int64_t M, int64_t N, int64_t K, bool tokens) {
+  const int cus = device_cus();
+  // pairs of column blocks share the rows' registers and the sums' barriers: 128256 columns of 2560, 1 / 16 / 64 rows, alone 59 /
+  // 66 / 79 us, in pairs 57 / 62 / 74; 27648 columns 16.3 / 17.2 / 22.9, 16.9 / 17.5 / 23.8, as the last round is less even
+  if (few_rows(M, N, K, tokens, cus)) return {int8_nt(N) > 8 * cus ? 2 : 1, 0, 0};
+  const int tile = tile_choice(M, N, K, cus);
+  return {0, tile, tile ? 0 : (int)large_halves((M + 255) / 256 * ((N + 255) / 256), cus)};
 }
 
 static int int8_launch(const char* who, const Int8Args& p, hipStream_t s) {
-  const int cus = device_cus();
-  if (few_rows(p, cus)) {
-    // pairs of column blocks share the rows' registers and the sums' barriers: 128256 columns of 2560, 1 / 16 / 64 rows, alone 59 /
-    // 66 / 79 us, in pairs 57 / 62 / 74; 27648 columns 16.3 / 17.2 / 22.9, 16.9 / 17.5 / 23.8, as the last round is less even
-    const int ct = p.NT > 8 * cus ? 2 : 1, groups = (p.NT + ct - 1) / ct;
-    const dim3 grid((unsigned)std::min(groups, cus));
+  const Int8Plan plan = int8_plan(p.M, p.N, p.K, p.tokens != nullptr);
+  if (plan.ct) {
+    const int ct = plan.ct, groups = (p.NT + ct - 1) / ct;
+    const dim3 grid((unsigned)std::min(groups, device_cus()));
     if (p.M <= 16)
       ct == 1 ? launch_stream<1, 1>(p, groups, grid, s) : launch_stream<1, 2>(p, groups, grid, s);
     else if (p.M <= 32)
@@ -659,8 +671,8 @@ static int int8_launch(const char* who, const Int8Args& p, hipStream_t s) {
       ct == 1 ? launch_stream<4, 1>(p, groups, grid, s) : launch_stream<4, 2>(p, groups, grid, s);
     return check_launch(who);
   }
-  switch (tile_choice(p.M, p.N, p.K, cus)) {
-    case 0: launch_large(p, cus, s); break;
+  switch (plan.tile) {
+    case 0: launch_large(p, plan.halves, s); break;
     case 1: launch_tile<128, 256, 2, 4, 1, 2, 3, 1>(p, s); break;
     case 2: launch_tile<128, 128, 2, 2, 2, 1, 4, 1>(p, s); break;
     case 3: launch_tile<128, 64, 2, 2, 2, 1, 6, 1>(p, s); break;
@@ -725,6 +737,18 @@ int btl_int8_matmul(const int8_t* a, int64_t lda, const float* a_scale, int64_t 
   return int8_launch(who, p, (hipStream_t)stream);
 }
 
+int btl_int8_matmul_plan(int64_t M, int64_t K, int64_t N, int64_t* plan) {
+  if (!plan || M <= 0 || M > (1 << 24) || N <= 0 || N > (1 << 24) || K <= 0 || K % 16 || K > BTL_MAX_K ||
+      (M + 63) / 64 * ((N + 63) / 64) > INT32_MAX)
+    return 0;
+  const Int8Plan f = int8_plan(M, N, K, false);
+  plan[0] = f.ct;
+  plan[1] = f.ct ? 0 : kTiles[f.tile].bm;
+  plan[2] = f.ct ? 0 : kTiles[f.tile].bn;
+  plan[3] = f.halves;
+  return 1;
+}
+
 int64_t btl_int8_head_scratch_bytes(int64_t M, int64_t K, int64_t N) {
   if (M <= 0 || M > kHeadRows || K <= 0 || K % 32 || K > BTL_MAX_K || N <= 0 || N > (1 << 24)) return 0;
   return head_scratch(M, K, N).total;
@@ -754,7 +778,7 @@ int btl_int8_head(const uint16_t* x, int64_t M, int64_t K, int64_t N, const uint
   rc = int8_args(who, codes, K, a_scale, M, K, N, wdev, w_scale, logits, N, 1, &p);
   if (rc != BTL_OK) return rc;
   // (with logits: where rows are loaded again for each group of columns, tiles and the argmax behind them are faster)
-  const bool few = M <= kFewRows8 && (!logits || M <= 16 || streams_once(p));
+  const bool few = M <= kFewRows8 && (!logits || M <= 16 || streams_once(K));
   hipStream_t s = (hipStream_t)stream;
   rc = launch_act(x, M, K, K, gamma, norm_eps, reinterpret_cast<int8_t*>(at + h.blocked), a_scale, nullptr, nullptr, codes, normed,
                   reinterpret_cast<uint32_t*>(at), few ? kHeadWords : 0, s);

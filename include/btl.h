@@ -569,7 +569,9 @@ int btl_shared_prefix_attention(const uint16_t* q, int64_t ldq, int64_t T, int64
  * positions are the rows.  btl_row_exponent: e of an 8-bit
  * row whose largest magnitude is given.  btl_paged_attention_plan: {1 where the kernel of
  * few rows runs, splits, positions of a split} of btl_paged_attention (_window_plan: of
- * btl_paged_attention_window); 1, or 0 for sizes that it refuses. */
+ * btl_paged_attention_window); 1, or 0 for sizes that it refuses.  btl_int8_matmul_plan: {column blocks that the weight
+ * stream takes at a time, 0 where tiles are used; rows and columns of a tile; how many tiles of 256 x 256 go as two halves}
+ * of btl_int8_matmul; 1, or 0. */
 int64_t btl_page_row(int64_t page, int64_t num_pages, int64_t num_kv_heads, int64_t kv_head, int64_t page_size,
                      int64_t position);
 int btl_page_run(int64_t page, int64_t num_pages, int64_t num_kv_heads, int64_t kv_head, int64_t page_size, int64_t position,
@@ -580,6 +582,7 @@ int btl_paged_attention_plan(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64
                              int64_t* plan);
 int btl_paged_attention_window_plan(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t B, int64_t max_q, int64_t max_kv,
                                     int64_t window, int64_t sinks, int64_t* plan);
+int btl_int8_matmul_plan(int64_t M, int64_t K, int64_t N, int64_t* plan);
 /* {few rows kernel, splits, positions of a split} of the shared positions, then of each sequence's own. */
 int btl_shared_prefix_attention_plan(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t B, int64_t max_q, int64_t max_kv,
                                      int64_t max_shared, int64_t* plan);
