@@ -177,6 +177,7 @@ EXPORTS = {
         _I,
     ),
     "btl_paged_attention_window_plan": ([_I64] * 9 + [_P], _I),
+    "btl_attention_window_tile": ([_I64] * 4 + [_P], _I64),
     "btl_shared_prefix_attention_scratch_bytes": ([_I64] * 8, _I64),
     "btl_shared_prefix_attention": (
         [_P, _I64, _I64, _I64, _PGP, _P, _I64, _P, _P, _P, _I64, _F, _I64, _I64, _I64, _P, _I64, _P, _SZ, _P, _P],

@@ -821,18 +821,27 @@ constexpr int kXcds = 8;
 struct UnitItem {
   int unit, item;
 };
-__device__ __forceinline__ UnitItem unit_item(int x, int each) {
+__host__ __device__ __forceinline__ UnitItem unit_item(int x, int each) {
   const int i = x / kXcds;
-  return {uni(i / each * kXcds + x % kXcds), uni(i % each)};
+  return {i / each * kXcds + x % kXcds, i % each};
 }
 inline int64_t unit_groups(int64_t units, int64_t each) { return (units + kXcds - 1) / kXcds * kXcds * each; }
+
+// kWindow: workgroup x's head and tile of it (any behind the last one), where units are `each` neighbouring tiles of a head.
+struct HeadTile {
+  int hk, x;
+};
+__host__ __device__ __forceinline__ HeadTile window_tile(int x, int Hkv, int each) {
+  const UnitItem u = unit_item(x, each);
+  return {u.unit % Hkv, u.unit / Hkv * each + u.item};
+}
 
 template <int D, int KV, int MODE>
 __global__ __launch_bounds__(256, 2) void k_flash_tile(FlashArgs p) {
   __shared__ __attribute__((aligned(16))) uint8_t smem[kTileShared<D>];
   if (MODE == kWindow) {
-    const UnitItem u = unit_item(blockIdx.x, p.neighbours);
-    tile_item<D, KV, MODE>(p, smem, uni(u.unit % p.Hkv), u.unit / p.Hkv * p.neighbours + u.item, blockIdx.y);
+    const HeadTile t = window_tile(blockIdx.x, p.Hkv, p.neighbours);
+    tile_item<D, KV, MODE>(p, smem, uni(t.hk), uni(t.x), blockIdx.y);
   } else {
     tile_item<D, KV, MODE>(p, smem, uni(blockIdx.x % p.Hkv), blockIdx.x / p.Hkv, blockIdx.y);
   }

@@ -25,7 +25,7 @@ __global__ __launch_bounds__(256, 2) void k_flash_shared(FlashArgs p, int shared
     // the tiles of a head's split read the same pages
     const UnitItem u = unit_item(x, shared_items);
     if (u.unit >= units) return;
-    const int hk = uni(u.unit % p.Hkv), split = uni(u.unit / p.Hkv), item = u.item;
+    const int hk = uni(u.unit % p.Hkv), split = uni(u.unit / p.Hkv), item = uni(u.item);
     if constexpr (SHARED_FEW)
       few_item<D, KV, kShared>(p, *reinterpret_cast<FewShared<D>*>(smem), hk, 0, split);
     else

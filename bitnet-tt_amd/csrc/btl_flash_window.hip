@@ -93,6 +93,18 @@ int btl_paged_attention_window_plan(int64_t T, int64_t H, int64_t Hkv, int64_t D
   return 1;
 }
 
+int64_t btl_attention_window_tile(int64_t tiles, int64_t splits, int64_t Hkv, int64_t x, int64_t* tile) {
+  if (!tile || Hkv <= 0 || Hkv > 1024 || tiles <= 0 || tiles > (1 << 26) || tiles % Hkv || splits <= 0) return 0;
+  const int each = window_neighbours(tiles, splits > 1 ? 2 : 1);
+  const int64_t groups = window_groups(tiles, Hkv, each);
+  if (x < 0 || x >= groups) return 0;
+  const HeadTile t = window_tile((int)x, (int)Hkv, each);
+  tile[0] = each;
+  tile[1] = t.hk;
+  tile[2] = t.x;
+  return groups;
+}
+
 int btl_paged_attention_window(const uint16_t* q, int64_t ldq, int64_t T, int64_t H, const btl_pages_t* pages,
                                const int32_t* page_table, int64_t max_pages, const int32_t* cu_q, const int32_t* kv_len,
                                int64_t B, float scale, int64_t max_q, int64_t max_kv, int64_t window, int64_t sinks,

@@ -571,7 +571,8 @@ int btl_shared_prefix_attention(const uint16_t* q, int64_t ldq, int64_t T, int64
  * few rows runs, splits, positions of a split} of btl_paged_attention (_window_plan: of
  * btl_paged_attention_window); 1, or 0 for sizes that it refuses.  btl_int8_matmul_plan: {column blocks that the weight
  * stream takes at a time, 0 where tiles are used; rows and columns of a tile; how many tiles of 256 x 256 go as two halves}
- * of btl_int8_matmul; 1, or 0. */
+ * of btl_int8_matmul; 1, or 0.  btl_attention_window_tile: {how many neighbouring tiles run on one XCD, the key-value head and the
+ * tile of it of workgroup x} of a windowed call of `tiles` tiles of all heads; the number of workgroups (of a split), or 0. */
 int64_t btl_page_row(int64_t page, int64_t num_pages, int64_t num_kv_heads, int64_t kv_head, int64_t page_size,
                      int64_t position);
 int btl_page_run(int64_t page, int64_t num_pages, int64_t num_kv_heads, int64_t kv_head, int64_t page_size, int64_t position,
@@ -583,6 +584,7 @@ int btl_paged_attention_plan(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64
 int btl_paged_attention_window_plan(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t B, int64_t max_q, int64_t max_kv,
                                     int64_t window, int64_t sinks, int64_t* plan);
 int btl_int8_matmul_plan(int64_t M, int64_t K, int64_t N, int64_t* plan);
+int64_t btl_attention_window_tile(int64_t tiles, int64_t splits, int64_t Hkv, int64_t x, int64_t* tile);
 /* {few rows kernel, splits, positions of a split} of the shared positions, then of each sequence's own. */
 int btl_shared_prefix_attention_plan(int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t B, int64_t max_q, int64_t max_kv,
                                      int64_t max_shared, int64_t* plan);
