@@ -347,7 +347,8 @@ class BitLinearDecodeStep:
         sequence (behind cu_q[B], say, in a captured call of fewer tokens) run through the
         layers with zeros for their attention; nothing is cached for them.  ``shared_pages`` (int32 [1] on the
         device): every sequence begins with that many pages of page_table[0], a prompt that has been cached once
-        for all of them, and the rows are behind it (PagedAttention).  Needs alloc_paged()."""
+        for all of them, and the rows are behind it (PagedAttention); single tokens over bf16 pages are then rounded as a
+        prompt's rows are (paged_attention.shared_prefix_attention).  Needs alloc_paged()."""
         import torch
 
         if getattr(self, "paged", None) is None:

@@ -278,7 +278,7 @@ class PagedAttention:
         """qkv bf16 [T, (H + 2 Hkv) D]: writes its keys and values to their pages,
         then attends over everything cached; bf16 [T, H D].  ``shared_pages`` (int32 [1] on the
         device, and its hint max_shared): the pages that every sequence begins with, which are read once for
-        all (paged_attention.shared_prefix_attention); not with a window."""
+        all (paged_attention.shared_prefix_attention, with its rounding of single tokens' weights); not with a window."""
         from ..paged_attention import paged_attention, rope_write, shared_prefix_attention
 
         if shared_pages is not None and self.window is not None:

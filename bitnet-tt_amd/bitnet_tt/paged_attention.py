@@ -385,7 +385,11 @@ def shared_prefix_attention(q, cache: PagedKVCache, page_table, cu_q, kv_len, sh
     position must be behind them, but for padding; kv_len counts them.  max_shared,
     where known, is the most shared pages (a hint, as max_q and max_kv; where it is not given, both
     parts are split for contexts of max_kv).  Several
-    groups with a prefix each: a call each, on slices of page_table, cu_q and kv_len."""
+    groups with a prefix each: a call each, on slices of page_table, cu_q and kv_len.
+
+    From more than 16 rows (T H / Hkv) on, the shared positions' softmax weights are rounded to bf16, as a
+    prompt's are.  For single tokens over bf16 pages :func:`paged_attention` keeps 16 bits of them: its outputs are
+    off by their own rounding, 0.0017 of their size, those behind a prefix by 0.0023."""
     index = cache.index
     if index != torch.cuda.current_device():
         with torch.cuda.device(index):

@@ -548,7 +548,9 @@ int btl_paged_attention_window(const uint16_t* q, int64_t ldq, int64_t T, int64_
 /* Attention of the newest tokens over the pages, as btl_paged_attention, for a batch whose sequences all begin
  * with the same pages: shared_pages (device, one int32) of them, those that
  * page_table[0] begins with, whole.  Their positions are read once for the rows of all sequences; of the
- * other sequences' tables the first shared_pages entries are not read.  A row before the end of the shared
+ * other sequences' tables the first shared_pages entries are not read.  The weights of the shared positions are
+ * rounded to bf16 where T H / Hkv is more than 16, also for single tokens over bf16 pages, for which btl_paged_attention keeps
+ * 16 bits of them: 0.0023 against 0.0017 of the outputs' size from 64 bits.  A row before the end of the shared
  * positions (but for rows with a negative position: zeros), or a shared_pages outside [0, max_pages],
  * sets the error word.  max_kv: as there; max_shared: an upper bound of the shared positions where known, else
  * max_kv (the sequences' own positions are then planned for max_kv as well): a hint too.  scratch: always, of btl_shared_prefix_attention_scratch_bytes with the same arguments. */
