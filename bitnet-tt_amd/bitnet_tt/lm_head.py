@@ -10,7 +10,7 @@ for up to 32 rows, writing fp32 logits (optional) and the token ids.
 
 ``weight_dtype="int8"`` keeps 8-bit integers with a scale for each vocabulary row
 instead, half the bytes: the normed rows are quantised as the ternary layers quantise
-theirs, and any number of rows is taken (a prompt's, to score it).
+theirs, and up to 65535 rows are taken in a call (a prompt's, to score it).
 """
 
 from __future__ import annotations
@@ -23,8 +23,15 @@ import numpy as np
 from . import _native as N
 
 
-_ROWS = 1024  # of a pass without logits over many rows
+_ROWS = 1024  # of a pass without logits over many rows, at most
+_BUFFER = 1 << 29  # bytes of such a pass's logits, for at least _FEW rows
+_FEW = 64  # rows that need no logits
 _MAX_ROWS = 65535
+
+
+def _pass_rows(m: int, v: int) -> int:
+    """Rows of a pass of the 8-bit head without logits."""
+    return min(m, max(_FEW, min(_ROWS, _BUFFER // (4 * v))))
 
 
 @functools.lru_cache(maxsize=4096)
@@ -87,8 +94,10 @@ class LMHead:
     def __call__(self, hidden, return_logits: bool = True, normed_out=None, logits_out=None, tokens_out=None):
         """bf16 hidden [M, hidden] (M <= 32; int8: up to 65535) -> (fp32 logits [M, vocab] or None,
         int32 token ids [M]).  The ``*_out`` tensors, when given, are written
-        in place (no allocation: the call can then be captured in a graph
-        after one eager call on the same stream)."""
+        in place.  The bf16 head then allocates nothing: it can be captured in a graph
+        after one eager call on the same stream.  The 8-bit head needs no eager call; each of its calls
+        allocates a scratch (about 2 M hidden bytes), and without logits for more than 64 rows
+        those of a pass of up to 1024 rows, at most 512 MiB or 64 rows of them.  A captured graph keeps both."""
         import torch
 
         if self.weight is None:
@@ -144,10 +153,10 @@ class LMHead:
             if M == 0:
                 return logits, tokens
             L, stream = N.lib(), N.raw_stream(dev.index)
-            # without logits up to 64 rows need none; more go in passes that share a buffer
-            rows = M if logits is not None or M <= 64 else min(M, _ROWS)
+            # without logits up to _FEW rows need none; more go in passes that share a buffer
+            rows = M if logits is not None else _pass_rows(M, V)
             part = logits
-            if logits is None and M > 64:
+            if logits is None and rows > _FEW:
                 part = torch.empty((rows, V), dtype=torch.float32, device=dev)
             nbytes = max(_scratch_bytes(dev.index, rows, H, V), _scratch_bytes(dev.index, M % rows or rows, H, V))
             # the call's own: calls that overlap share nothing
