@@ -203,8 +203,9 @@ __global__ __launch_bounds__(64 * kI8Waves, 2) void k_int8_stream(Int8Args p, in
   if (tid < p.M) p.tokens[tid] = arg_col(ld_coherent(p.keys + tid));
 }
 
-// The best of part blockIdx.x of row blockIdx.y; a row of one part is done.  Parts of at least 2048 columns, four workgroups a CU:
-// bound by the logits' bytes.
+// The best of part blockIdx.x of row blockIdx.y; a row of one part is done.  Parts of at least 2048 columns, about four workgroups a
+// CU.  Bound by latency, a thread having few loads of 4 bytes on their way: 128256 columns, 128 rows 28 us (2.4 TB/s) and 5 of the
+// join, 1024 rows 293 (1.8 TB/s), beside 74 and 356 of the product.
 __global__ __launch_bounds__(256) void k_int8_argmax(const float* y, int64_t ldo, int N, int each, uint64_t* keys, int32_t* tokens) {
   __shared__ uint64_t s_best[4];
   const int row = blockIdx.y, end = min(N, ((int)blockIdx.x + 1) * each);
@@ -235,9 +236,9 @@ __global__ __launch_bounds__(64) void k_int8_argmax_parts(const uint64_t* keys, 
 // Many rows: tiles of BM x BN, S stages of KG x SUB x 64 k in LDS, filled without registers.  The waves are KG groups
 // of WM x WN; a group takes its blocks of 64 k of every stage, and the groups' sums meet in LDS.
 //
-// Large tiles: the matrix units are busy 43% (K = 2560) to 54% (8192) of the cycles; what remains is a tile's first loads, its
-// outputs, and the wait for operands that 256 x 256 x 128 k take in (64 KiB a step through each CU).  8192^3: 445 us, 2.47
-// POP/s (a large library product 2.12); 4096 x 2560 x 13824: 142-149 us, 1.95-2.04.  Small tiles: bound by the operands that pass
+// Large tiles: the matrix units are busy 50% (K = 2560) to 59% (8192) of the cycles; what remains is a tile's first loads, its
+// outputs, and the wait for operands that 256 x 256 x 128 k take in (64 KiB a step through each CU).  8192^3: 445-468 us, 2.35-2.47
+// POP/s (a large library product 2.12); 4096 x 2560 x 13824: 142-151 us, 1.92-2.04.  Small tiles: bound by the operands that pass
 // through each CU, at 37-50 B/ns a CU, and by latency, so that they have several stages on their way and the waves of a
 // workgroup share a small tile's k (511 x 2560 x 3840: 10.7 us).  The next tile's first stage loaded before the outputs are
 // stored, by workgroups of several tiles each: 1-3% slower (474 -> 482); weights two steps ahead, in a third stage: no gain.
@@ -564,10 +565,11 @@ static void launch_large(const Int8Args& a, int halves, hipStream_t s) {
 
 // The tile of the least time, us: rounds of workgroups over the CUs x what a workgroup takes, for a start (and an end) and for
 // each 128 k; alone on its CU, or beside another one.  Fitted to 69 shapes, 65-8192 rows, K 576-6912, 640-128256
-// columns: the rule takes the best of the five for 67 of them, and is 5 and 8% above it for the others.  Us of each, in this order:
-// 4096 x 2560 x 13824: 146, 173, 230, 306, 285 (in rows of tiles, not strips); 1024 x 2560 x 6912: 36, 25, 29, 38, 35; 256 x 2560 x
-// 13824: 36, 24, 19, 27, 26; 511 x 2560 x 3840: 34, 21, 14, 10.9, 11.8; 128 x 6912 x 2560: 77, 46, 28, 19, 13; 400 x 640 x 2560: 13,
-// 9, 7.0, 5.8, 6.0.  (128 x 128 as two a CU is never more than 2% better, 64 x 64 as one of 8 stages never better.)
+// columns, with tiles in plain rows; in strips, as they are now, the rule takes the best of the five for 68 of them and 4% more for the
+// other, and for 46 others drawn at random (65-6000 rows, K 320-6912, 300-40000 columns) the best for 44, 5% and 0.2% more for two.  Us of
+// each, in this order: 4096 x 2560 x 13824: 148, 175, 232, 312, 270; 1024 x 2560 x 6912: 36, 26, 29, 36, 36; 256 x 2560 x
+// 13824: 36, 24, 19, 26, 26; 511 x 2560 x 3840: 34, 21, 14, 10.8, 12.3; 128 x 6912 x 2560: 78, 46, 28, 19, 13; 400 x 640 x 2560: 13,
+// 9, 7.0, 5.9, 6.0.  (128 x 128 as two a CU is never more than 2% better, 64 x 64 as one of 8 stages never better.)
 struct TileCost {
   int bm, bn, per_cu;
   double start, step;          // one on a CU
@@ -633,7 +635,9 @@ static int int8_args(const char* who, const int8_t* a, int64_t lda, const float*
   return BTL_OK;
 }
 
-// Whether the weight stream takes it, where a few rows' argmax is wanted without logits in any case.  Us of the stream / of tiles,
+// Whether the weight stream takes it; where a few rows' argmax is wanted without logits in any case, as tiles need them (whole head
+// calls, K = 6912, 40000 columns, 17 / 32 / 48 / 64 rows: 58 / 71 / 84 / 98 us so, with logits, in tiles from 17 rows on, 58 / 60 / 64 /
+// 69; 4096 x 128256, 17 / 32 / 64: 107 / 126 / 189, 108 / 112 / 128; 6912 x 3840: 19 / 24 / 29, 24 / 24 / 25).  Us of the stream / of tiles,
 // K = 2560, 16 rows: 640 columns 3.9 / 6.4, 3840: 4.7 / 7.1, 13824: 10.2 / 10.6, 128256: 66 / 71; 32 rows: 5.0 / 6.7, 5.8 / 7.1,
 // 11.9 / 11.1, 70 / 74; 64 rows: 7.3 / 6.9, 8.5 / 7.3, 14.7 / 11.7, 76 / 78.  K = 6912, where rows are loaded again for each group
 // of columns, 16 rows: 640: 8.9 / 12.9, 3840: 9.5 / 13.2, 13824: 34 / 21, 40000: 64 / 59; 32 rows: 14.1 / 12.8, 14.6 / 13.2, 48 / 22,
